@@ -16,7 +16,7 @@
  *   - One stream per call; calls that share a temp buffer must be ordered on one stream.
  *
  * Element-type suffixes: i32 int32_t, u32 uint32_t, f32 float, i64 int64_t, u64 uint64_t,
- * f64 double.  Value-size suffixes for SortPairs: v32 (any 4-byte value), v64 (any 8-byte value).
+ * f64 double; of attention rows bf16 and f16.  Value-size suffixes for SortPairs: v32 (any 4-byte value), v64 (any 8-byte value).
  */
 #ifndef LCPP_HIP_H_
 #define LCPP_HIP_H_
@@ -582,6 +582,110 @@ LCPP_HIP_DECLARE_SEGSORT(i64, int64_t)
 LCPP_HIP_DECLARE_SEGSORT(f64, double)
 #undef LCPP_HIP_DECLARE_SEGSORT
 #undef LCPP_HIP_DECLARE_SEGSORT_PAIRS
+
+/* ---------------------------------------------------------------------------------------------
+ * Attention over ragged batches, and a paged cache of its keys and values (no reference counterpart).
+ *
+ * A batch holds the rows of all its sequences one after another; offsets[b] .. offsets[b + 1] are those of
+ * sequence b (offsets in device memory, ascending, one more than there are sequences).  Rows that no sequence
+ * has are neither read nor written.  Types: bf16 and f16, in both directions; sums, maxima and the
+ * softmax are f32.  Head sizes: multiples of 8 up to 128 (others: LCPP_HIP_ERR_UNSUPPORTED).  `q_heads` is a
+ * multiple of `kv_heads`; query head h reads key head h / (q_heads / kv_heads).  Rows and pages start at
+ * multiples of 16 bytes, and their strides are multiples of 8 items.  `scale` (the products' factor, often
+ * 1 / sqrt(head_dim)) is positive.  lse is [q_heads][q_tokens] f32: the logarithm of the row's sum of exponentials.
+ * A row that sees no key has zeros for its output and -infinity for its lse, and passes no gradient.  Every
+ * result is a sum in one order: the same call gives the same bits.
+ * ------------------------------------------------------------------------------------------- */
+
+/* [tokens][heads][head_dim]: the last axis contiguous, strides of the others in items. */
+typedef struct lcpp_hip_rows {
+    void* data;
+    int64_t token_stride;
+    int64_t head_stride;
+} lcpp_hip_rows;
+
+/* [pages][page size][kv_heads][head_dim]: the last axis contiguous, the others in any order. */
+typedef struct lcpp_hip_pages {
+    void* data;
+    int64_t page_stride;
+    int64_t token_stride;
+    int64_t head_stride;
+} lcpp_hip_pages;
+
+/* Lays out one step of a batch: request r holds cached_lengths[r] tokens in its pages and brings new_lengths[r]
+ * more (negative lengths count as 0).  Pages that its row of the block table lacks are taken from `free_pages`, in
+ * request order: the table's entries from ceil(cached / page_size) to ceil((cached + new) / page_size) are written,
+ * the ones before are kept.  Outputs: query_offsets [requests + 1], the exclusive sum of the new lengths;
+ * kv_lengths [requests], cached + new; for each new token, its request, its position in it and its slot,
+ * page * page_size + place in the page; counts[0] new tokens and counts[1] pages taken.  Where the list holds
+ * fewer than counts[1] pages, the entries it cannot serve are -1 and the slots in them too, as are the
+ * slots of positions past table_width pages; such positions take no pages.  Token outputs hold max_tokens entries:
+ * past the last token, request and slot are -1 and the position is 0.  Tokens from max_tokens on, if counts[0] is
+ * larger, are left out, and so are the pages that begin with them.  All new tokens together, and every
+ * kv length, are below 2^31. */
+size_t lcpp_hip_page_plan_temp_bytes(uint32_t requests);
+int lcpp_hip_page_plan(void* temp, size_t temp_bytes, const int32_t* cached_lengths, const int32_t* new_lengths,
+                       uint32_t requests, uint32_t page_size, const int32_t* free_pages, uint32_t num_free,
+                       int32_t* block_table, uint64_t table_stride, uint32_t table_width, int32_t* query_offsets,
+                       int32_t* kv_lengths, int32_t* token_request, int32_t* token_position, int64_t* token_slot,
+                       uint64_t max_tokens, int32_t* counts, void* stream);
+
+/* Copies row t of `key` and `value` to slot slots[t] of the caches; slots that are negative or past the last page
+ * are left out.  No two rows share a slot. */
+#define LCPP_HIP_DECLARE_PAGED_WRITE(S)                                                                         \
+    int lcpp_hip_paged_write_##S(const lcpp_hip_rows* key, const lcpp_hip_rows* value, const int64_t* slots,    \
+                                 uint64_t tokens, const lcpp_hip_pages* key_cache,                              \
+                                 const lcpp_hip_pages* value_cache, uint32_t kv_heads, uint32_t head_dim,       \
+                                 uint32_t page_size, uint32_t pages, void* stream);
+LCPP_HIP_DECLARE_PAGED_WRITE(bf16)
+LCPP_HIP_DECLARE_PAGED_WRITE(f16)
+#undef LCPP_HIP_DECLARE_PAGED_WRITE
+
+/* Attention of packed rows to the packed keys of the same sequence.  Causal: row i of n sees key j of m where
+ * j <= i + m - n (the last row sees every key, so keys may have a head start, or fewer keys leave the first rows
+ * with none); otherwise every row sees every key.  lse may be null; the backward pass needs it.  The
+ * backward pass writes dq for the rows, dk and dv for the keys (sums over the query heads that share one). */
+size_t lcpp_hip_attention_packed_temp_bytes(uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads,
+                                            uint32_t kv_heads, uint32_t head_dim);
+size_t lcpp_hip_attention_packed_backward_temp_bytes(uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens,
+                                                     uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim);
+#define LCPP_HIP_DECLARE_ATTENTION(S)                                                                             \
+    int lcpp_hip_attention_packed_##S(void* temp, size_t temp_bytes, const lcpp_hip_rows* q,                      \
+                                      const lcpp_hip_rows* k, const lcpp_hip_rows* v, const int32_t* q_offsets,   \
+                                      const int32_t* k_offsets, const lcpp_hip_rows* out, float* lse,             \
+                                      uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads, \
+                                      uint32_t kv_heads, uint32_t head_dim, float scale, int causal,              \
+                                      void* stream);                                                              \
+    int lcpp_hip_attention_packed_backward_##S(                                                                   \
+        void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* v,    \
+        const lcpp_hip_rows* out, const float* lse, const lcpp_hip_rows* dout, const int32_t* q_offsets,          \
+        const int32_t* k_offsets, const lcpp_hip_rows* dq, const lcpp_hip_rows* dk, const lcpp_hip_rows* dv,      \
+        uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads, uint32_t kv_heads,            \
+        uint32_t head_dim, float scale, int causal, void* stream);
+LCPP_HIP_DECLARE_ATTENTION(bf16)
+LCPP_HIP_DECLARE_ATTENTION(f16)
+#undef LCPP_HIP_DECLARE_ATTENTION
+
+/* Attention of a step's new tokens to the paged cache, which holds their own keys and values already (page_plan,
+ * paged_write).  Request r has kv_lengths[r] keys, the last of them its new tokens' (q_offsets counts those).  New
+ * token i sees every key before them, and new key j where bit j of tree[i] is set: a tree of drafted tokens (at most
+ * 64 a request; keys from the 65th on are not seen).  Without a tree (null): j <= i.  A single new token a request
+ * is plain decoding.  Keys in pages outside [0, pages), or past table_width pages, are not seen.  max_kv_length is
+ * the longest request's length, or more: it decides how long requests are split and sizes temp; longer
+ * requests are right too, only slower. */
+size_t lcpp_hip_attention_paged_temp_bytes(uint32_t requests, uint64_t q_tokens, uint64_t max_kv_length, uint32_t q_heads,
+                                           uint32_t kv_heads, uint32_t head_dim);
+#define LCPP_HIP_DECLARE_ATTENTION_PAGED(S)                                                                      \
+    int lcpp_hip_attention_paged_##S(                                                                            \
+        void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_pages* key_cache,                  \
+        const lcpp_hip_pages* value_cache, const int32_t* block_table, uint32_t table_stride,                    \
+        uint32_t table_width, const int32_t* q_offsets, const int32_t* kv_lengths, const uint64_t* tree,         \
+        const lcpp_hip_rows* out, float* lse, uint32_t requests, uint64_t q_tokens, uint64_t max_kv_length,      \
+        uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t pages, float scale, \
+        void* stream);
+LCPP_HIP_DECLARE_ATTENTION_PAGED(bf16)
+LCPP_HIP_DECLARE_ATTENTION_PAGED(f16)
+#undef LCPP_HIP_DECLARE_ATTENTION_PAGED
 
 /* ---------------------------------------------------------------------------------------------
  * Seeded synthetic workloads for tests and benchmarks (no reference counterpart; the reference

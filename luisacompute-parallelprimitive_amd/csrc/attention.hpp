@@ -1,0 +1,198 @@
+// Building blocks of the attention kernels (packed and paged): 16-bit operand types and their matrix
+// instruction, staging of rows into LDS, fragment reads in both directions, and the map from a workgroup to its
+// tile of a ragged batch.
+//
+// Matrix instruction: 32x32x16, f32 accumulators.  Lane l = 32 h + c holds of the A operand row c, of the B
+// operand column c, at contraction indices 8 h .. 8 h + 7; of the result column c, rows acc_row(r, h), r < 16.
+// A contraction may run over its index in any order that both operands share.  Products are arranged so that
+// the softmax axis of a result lies in a lane's own registers and the result feeds the next product as its B
+// operand as it stands: step s of 16 contraction indices takes registers 8 s .. 8 s + 7, which are rows
+// 16 s + 4 h + {0..3} and 16 s + 8 + 4 h + {0..3}; the A operand is read in that order (read_columns).
+#pragma once
+
+#include "common.hpp"
+#include "../../include/lcpp_hip.h"
+
+namespace lcpp_hip {
+namespace attention {
+
+using F32x16 = float __attribute__((ext_vector_type(16)));
+using F32x4 = float __attribute__((ext_vector_type(4)));
+using F32x2 = float __attribute__((ext_vector_type(2)));
+using U32x4 = uint32_t __attribute__((ext_vector_type(4)));
+using U32x2 = uint32_t __attribute__((ext_vector_type(2)));
+using S16x4 = short __attribute__((ext_vector_type(4)));
+
+struct Bf16 {
+    using Item = __bf16;
+    using Vec2 = Item __attribute__((ext_vector_type(2)));
+    using Vec8 = Item __attribute__((ext_vector_type(8)));
+    __device__ static F32x16 mfma(U32x4 a, U32x4 b, F32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(Vec8, a), __builtin_bit_cast(Vec8, b), c, 0, 0, 0);
+    }
+};
+
+struct F16 {
+    using Item = _Float16;
+    using Vec2 = Item __attribute__((ext_vector_type(2)));
+    using Vec8 = Item __attribute__((ext_vector_type(8)));
+    __device__ static F32x16 mfma(U32x4 a, U32x4 b, F32x16 c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(Vec8, a), __builtin_bit_cast(Vec8, b), c, 0, 0, 0);
+    }
+};
+
+// Two floats rounded to nearest even, in one word.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const F32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, typename T::Vec2));
+}
+
+template <typename T>
+__device__ __forceinline__ float item_low(uint32_t w) {
+    return static_cast<float>(__builtin_bit_cast(typename T::Vec2, w)[0]);
+}
+template <typename T>
+__device__ __forceinline__ float item_high(uint32_t w) {
+    return static_cast<float>(__builtin_bit_cast(typename T::Vec2, w)[1]);
+}
+
+// Row of a 32x32 result that register r of a lane in half h holds.
+__device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
+
+// Registers 8 s .. 8 s + 7 of a result, rounded to 16 bits: the B operand of contraction step s.
+template <typename T>
+__device__ __forceinline__ U32x4 pack_step(const F32x16& p, int s) {
+    return U32x4{pack2<T>(p[8 * s + 0], p[8 * s + 1]), pack2<T>(p[8 * s + 2], p[8 * s + 3]),
+                 pack2<T>(p[8 * s + 4], p[8 * s + 5]), pack2<T>(p[8 * s + 6], p[8 * s + 7])};
+}
+
+// A value of this lane and of the lane 32 away: the lower lane's first.  (The two words are copied out before they are
+// reinterpreted: a bit cast of a vector's element would take its first.)
+struct Halves {
+    float low, high;
+};
+__device__ __forceinline__ Halves halves(float x) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, x), false, false);
+    const uint32_t low = r[0], high = r[1];
+    return {__builtin_bit_cast(float, low), __builtin_bit_cast(float, high)};
+}
+__device__ __forceinline__ float halves_max(float x) {
+    const Halves h = halves(x);
+    return fmaxf(h.low, h.high);
+}
+__device__ __forceinline__ float halves_sum(float x) {
+    const Halves h = halves(x);
+    return h.low + h.high;
+}
+
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// Rows of 16-bit items: one of a [tokens][heads][dim] array with the last axis contiguous.
+struct Rows {
+    char* data;
+    int64_t token_bytes;
+    int64_t head_bytes;
+    __device__ __forceinline__ char* at(int64_t token, int head) const {
+        return data + token * token_bytes + static_cast<int64_t>(head) * head_bytes;
+    }
+};
+
+// Rows of a paged cache: [pages][page size][heads][dim] in any order of the first three axes.
+struct Pages {
+    char* data;
+    int64_t page_bytes;
+    int64_t token_bytes;
+    int64_t head_bytes;
+    __device__ __forceinline__ char* at(int64_t page, int64_t slot, int head) const {
+        return data + page * page_bytes + slot * token_bytes + static_cast<int64_t>(head) * head_bytes;
+    }
+};
+
+// What the 16-byte loads and stores of rows need.
+inline bool usable(const lcpp_hip_rows* r) {
+    return r != nullptr && r->data != nullptr && reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->token_stride >= 0 &&
+           r->head_stride >= 0 && r->token_stride % 8 == 0 && r->head_stride % 8 == 0;
+}
+inline bool usable(const lcpp_hip_pages* c) {
+    return c != nullptr && c->data != nullptr && reinterpret_cast<uintptr_t>(c->data) % 16 == 0 && c->page_stride >= 0 &&
+           c->token_stride >= 0 && c->head_stride >= 0 && c->page_stride % 8 == 0 && c->token_stride % 8 == 0 &&
+           c->head_stride % 8 == 0;
+}
+inline int unusable(const char* what) {
+    return set_error(kInvalidArgument, "%s: rows must be there and 16-byte aligned, their strides multiples of 8 items", what);
+}
+inline Rows rows_of(const lcpp_hip_rows* r) { return {static_cast<char*>(r->data), r->token_stride * 2, r->head_stride * 2}; }
+inline Pages pages_of(const lcpp_hip_pages* c) {
+    return {static_cast<char*>(c->data), c->page_stride * 2, c->token_stride * 2, c->head_stride * 2};
+}
+
+// A tile of rows in LDS: DP items a row (the head size rounded up; zeros past it) and 16 bytes of padding.
+template <int DP>
+struct Tile {
+    static constexpr int kStride = DP * 2 + 16;  // bytes
+    static constexpr int bytes(int rows) { return rows * kStride; }
+};
+
+// Contraction step s of row c (A operand of 32 rows from `row0`): 8 items at 16 s + 8 h.
+template <int DP>
+__device__ __forceinline__ U32x4 read_rows(const char* tile, int row0, int s) {
+    const int lane = threadIdx.x % kWave;
+    return *reinterpret_cast<const U32x4*>(tile + (row0 + lane % 32) * Tile<DP>::kStride + s * 32 + (lane / 32) * 16);
+}
+
+// A operand of the transposed tile: 32 columns from `col0`, contraction over the 16 rows from `row0` in the order
+// of pack_step.  A transposed read hands each of 16 lanes the four items of its column from four rows.
+template <int DP>
+__device__ __forceinline__ U32x4 read_columns(const char* tile, int row0, int col0) {
+    using LdsPtr = __attribute__((address_space(3))) S16x4*;
+    const int lane = threadIdx.x % kWave;
+    const int row = row0 + 4 * (lane / 32) + lane % 16 / 4;
+    const int col = col0 + 16 * (lane / 16 % 2) + 4 * (lane % 4);
+    const char* p = tile + row * Tile<DP>::kStride + col * 2;
+    const S16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
+    const S16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 8 * Tile<DP>::kStride));
+    const U32x2 x = __builtin_bit_cast(U32x2, a), y = __builtin_bit_cast(U32x2, b);
+    return U32x4{x[0], x[1], y[0], y[1]};
+}
+
+// 16 bytes of a row, or zeros past the row's items or for a row that is not there.
+__device__ __forceinline__ U32x4 load_chunk(const char* row, int chunk, int dim, bool there) {
+    U32x4 v = {0u, 0u, 0u, 0u};
+    if (there && chunk * 8 < dim) v = *reinterpret_cast<const U32x4*>(row + chunk * 16);
+    return v;
+}
+
+// Places of a ragged batch's tiles.  Sequence b with rows [offsets[b], offsets[b + 1]) has its tiles of `size` rows
+// from number offsets[b] / size + b on: numbers never collide, because floor(x / size) + 1 more tiles than any
+// sequence of x rows needs are set aside, and there are at most total / size + count of them.  The tile's owner is
+// the last b whose first number is not above it; a number past its owner's rows has no tile.
+struct TilePlace {
+    int sequence;
+    int tile;
+};
+
+__device__ __forceinline__ TilePlace find_tile(const int32_t* offsets, int count, int scale, int size, int number) {
+    const int lane = threadIdx.x % kWave;
+    int low = 0, high = count;
+    while (high - low > 0) {
+        const int step = (high - low + kWave - 1) / kWave;
+        const int at = low + lane * step;
+        bool below = false;
+        if (at < high) below = static_cast<int64_t>(offsets[at]) * scale / size + at <= number;
+        const int passed = __popcll(wave_ballot(below));
+        if (passed == 0) return {-1, 0};
+        low += (passed - 1) * step;
+        if (step == 1) break;
+        high = low + step < high ? low + step : high;
+    }
+    low = __builtin_amdgcn_readfirstlane(low);
+    const int first = static_cast<int>(static_cast<int64_t>(offsets[low]) * scale / size) + low;
+    return {low, number - first};
+}
+
+}  // namespace attention
+}  // namespace lcpp_hip

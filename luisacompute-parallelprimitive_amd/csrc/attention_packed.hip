@@ -1,0 +1,478 @@
+// Causal or full attention over packed sequences with grouped heads, and its gradients.
+//
+//   S = scale q k^T,  row i of n sees key j of m where j <= i + m - n (causal) or any j,
+//   P = softmax(S),  O = P V,  lse = log sum exp S;  a row that sees nothing has O = 0 and lse = -inf.
+//   dV = P^T dO,  dP = dO V^T,  dS = P (dP - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q.
+#include "attention.hpp"
+
+namespace lcpp_hip {
+namespace attention {
+namespace {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / kWave;
+constexpr int kRowsPerWave = 32;
+constexpr int kRowTile = kWaves * kRowsPerWave;  // query rows of a workgroup
+constexpr int kKeyTile = 64;                     // keys staged at a time
+
+struct Shape {
+    int sequences;
+    int q_tokens;
+    int k_tokens;
+    int q_heads;
+    int kv_heads;
+    int dim;
+    float scale;
+    int causal;
+};
+
+struct Span {
+    int begin;
+    int size;
+};
+
+__device__ __forceinline__ Span span_of(const int32_t* offsets, int sequence, int tokens) {
+    int begin = offsets[sequence], end = offsets[sequence + 1];
+    begin = begin < 0 ? 0 : begin > tokens ? tokens : begin;
+    end = end < begin ? begin : end > tokens ? tokens : end;
+    return {begin, end - begin};
+}
+
+// Rows [row0, row0 + ROWS) of one head into LDS; zeros for rows from `rows` on.
+template <int DP, int ROWS>
+__device__ __forceinline__ void stage(char* tile, const Rows& src, int64_t token0, int head, int rows, int dim) {
+    constexpr int kChunks = DP / 8;
+#pragma unroll
+    for (int i = 0; i < ROWS * kChunks / kBlock; ++i) {
+        const int at = i * kBlock + threadIdx.x;
+        const int row = at / kChunks, chunk = at % kChunks;
+        const bool there = row < rows;
+        const U32x4 v = load_chunk(src.at(token0 + (there ? row : 0), head), chunk, dim, there);
+        *reinterpret_cast<U32x4*>(tile + row * Tile<DP>::kStride + chunk * 16) = v;
+    }
+}
+
+// The calling lane's row as a B operand: column lane % 32, all contraction steps.
+template <int DP>
+__device__ __forceinline__ void load_row(U32x4 (&f)[DP / 16], const Rows& src, int64_t token, int head, bool there, int dim) {
+    const char* row = src.at(there ? token : 0, head);
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) f[s] = load_chunk(row, 2 * s + threadIdx.x % kWave / 32, dim, there);
+}
+
+// Writes column `lane % 32` of a transposed result (rows are items of the head) times `factor`.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(const Rows& dst, int64_t token, int head, const F32x16 (&acc)[DP / 32], float factor,
+                                          int dim) {
+    const int half = threadIdx.x % kWave / 32;
+    char* row = dst.at(token, head);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = b * 32 + 8 * g + 4 * half;
+            if (d >= dim) continue;
+            const U32x2 v = {pack2<T>(acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor),
+                             pack2<T>(acc[b][4 * g + 2] * factor, acc[b][4 * g + 3] * factor)};
+            *reinterpret_cast<U32x2*>(row + d * 2) = v;
+        }
+    }
+}
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kBlock) void attention_packed_kernel(Rows q, Rows k, Rows v, Rows out, float* __restrict__ lse,
+                                                                  const int32_t* __restrict__ q_offsets,
+                                                                  const int32_t* __restrict__ k_offsets, Shape shape,
+                                                                  int tiles) {
+    __shared__ __attribute__((aligned(16))) char k_tile[Tile<DP>::bytes(kKeyTile)];
+    __shared__ __attribute__((aligned(16))) char v_tile[Tile<DP>::bytes(kKeyTile)];
+    const int head = blockIdx.x % shape.q_heads;
+    const int number = tiles - 1 - static_cast<int>(blockIdx.x / shape.q_heads);
+    const TilePlace place = find_tile(q_offsets, shape.sequences, 1, kRowTile, number);
+    if (place.sequence < 0) return;
+    const Span rows = span_of(q_offsets, place.sequence, shape.q_tokens);
+    const int row0 = place.tile * kRowTile;
+    if (row0 >= rows.size) return;
+    const Span keys = span_of(k_offsets, place.sequence, shape.k_tokens);
+    const int kv_head = head / (shape.q_heads / shape.kv_heads);
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int row = row0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
+    const bool there = row < rows.size;
+    const int shift = shape.causal ? keys.size - rows.size : keys.size;
+    // The last key that the row, and that any row of the workgroup, sees.
+    const int last = shape.causal ? row + shift : keys.size - 1;
+    const int tile_last = row0 + kRowTile < rows.size ? row0 + kRowTile - 1 : rows.size - 1;
+    int stop = shape.causal ? tile_last + shift + 1 : keys.size;
+    stop = stop < keys.size ? stop : keys.size;
+    const float c = shape.scale * kLog2e;
+
+    U32x4 qf[DP / 16];
+    load_row<DP>(qf, q, rows.begin + row, head, there, shape.dim);
+    F32x16 acc[DP / 32] = {};
+    float top = -INFINITY, total = 0.f;
+    for (int k0 = 0; k0 < stop; k0 += kKeyTile) {
+        __syncthreads();
+        stage<DP, kKeyTile>(k_tile, k, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
+        stage<DP, kKeyTile>(v_tile, v, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
+        __syncthreads();
+        F32x16 s[kKeyTile / 32] = {};
+#pragma unroll
+        for (int b = 0; b < kKeyTile / 32; ++b)
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) s[b] = T::mfma(read_rows<DP>(k_tile, b * 32, i), qf[i], s[b]);
+        const int limit = last < keys.size - 1 ? last : keys.size - 1;
+        float high = top;
+#pragma unroll
+        for (int b = 0; b < kKeyTile / 32; ++b)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                if (k0 + b * 32 + acc_row(r, half) > limit) s[b][r] = -INFINITY;
+                high = fmaxf(high, s[b][r]);
+            }
+        high = halves_max(high);
+        const float base = high == -INFINITY ? 0.f : high * c;
+        const float alpha = exp2_fast(top * c - base);
+        top = high;
+        total *= alpha;
+#pragma unroll
+        for (int b = 0; b < DP / 32; ++b) acc[b] *= alpha;
+#pragma unroll
+        for (int b = 0; b < kKeyTile / 32; ++b) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                s[b][r] = exp2_fast(s[b][r] * c - base);
+                total += s[b][r];
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const U32x4 p = pack_step<T>(s[b], i);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+                    acc[d] = T::mfma(read_columns<DP>(v_tile, b * 32 + i * 16, d * 32), p, acc[d]);
+            }
+        }
+    }
+    total = halves_sum(total);
+    if (!there) return;
+    store_row<T, DP>(out, rows.begin + row, head, acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
+    if (lse != nullptr && half == 0)
+        lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row] =
+            total == 0.f ? -INFINITY : top * shape.scale + __logf(total);
+}
+
+// ---- gradients ---------------------------------------------------------------------------------------------------
+
+// delta[h][t] = sum over the head's items of dO * O: 16 lanes a row.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void attention_delta_kernel(Rows out, Rows dout, float* __restrict__ delta, int q_tokens,
+                                                                 int q_heads, int dim) {
+    const int64_t item = static_cast<int64_t>(blockIdx.x) * (kBlock / 16) + threadIdx.x / 16;
+    if (item >= static_cast<int64_t>(q_tokens) * q_heads) return;
+    const int64_t token = item / q_heads;
+    const int head = static_cast<int>(item % q_heads), chunk = threadIdx.x % 16;
+    const U32x4 a = load_chunk(out.at(token, head), chunk, dim, true);
+    const U32x4 b = load_chunk(dout.at(token, head), chunk, dim, true);
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sum += item_low<T>(a[i]) * item_low<T>(b[i]);
+        sum += item_high<T>(a[i]) * item_high<T>(b[i]);
+    }
+#pragma unroll
+    for (int step = 8; step > 0; step /= 2) sum += __shfl_xor(sum, step);
+    if (chunk == 0) delta[static_cast<int64_t>(head) * q_tokens + token] = sum;
+}
+
+// dQ of a tile of query rows: the keys pass by as in the forward kernel.
+template <typename T, int DP>
+__global__ __launch_bounds__(kBlock) void attention_dq_kernel(Rows q, Rows k, Rows v, Rows dout, Rows dq,
+                                                              const float* __restrict__ lse, const float* __restrict__ delta,
+                                                              const int32_t* __restrict__ q_offsets,
+                                                              const int32_t* __restrict__ k_offsets, Shape shape, int tiles) {
+    __shared__ __attribute__((aligned(16))) char k_tile[Tile<DP>::bytes(kKeyTile)];
+    __shared__ __attribute__((aligned(16))) char v_tile[Tile<DP>::bytes(kKeyTile)];
+    const int head = blockIdx.x % shape.q_heads;
+    const int number = tiles - 1 - static_cast<int>(blockIdx.x / shape.q_heads);
+    const TilePlace place = find_tile(q_offsets, shape.sequences, 1, kRowTile, number);
+    if (place.sequence < 0) return;
+    const Span rows = span_of(q_offsets, place.sequence, shape.q_tokens);
+    const int row0 = place.tile * kRowTile;
+    if (row0 >= rows.size) return;
+    const Span keys = span_of(k_offsets, place.sequence, shape.k_tokens);
+    const int kv_head = head / (shape.q_heads / shape.kv_heads);
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int row = row0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
+    const bool there = row < rows.size;
+    const int shift = keys.size - rows.size;
+    const int tile_last = row0 + kRowTile < rows.size ? row0 + kRowTile - 1 : rows.size - 1;
+    int stop = shape.causal ? tile_last + shift + 1 : keys.size;
+    stop = stop < keys.size ? stop : keys.size;
+    int limit = shape.causal && row + shift < keys.size - 1 ? row + shift : keys.size - 1;
+    const float c = shape.scale * kLog2e;
+
+    U32x4 qf[DP / 16], of[DP / 16];
+    load_row<DP>(qf, q, rows.begin + row, head, there, shape.dim);
+    load_row<DP>(of, dout, rows.begin + row, head, there, shape.dim);
+    const int64_t stat = static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row;
+    const float row_lse = there ? lse[stat] : -INFINITY;
+    const float row_delta = there ? delta[stat] : 0.f;
+    if (row_lse == -INFINITY) limit = -1;
+    const float base = row_lse * kLog2e;
+    F32x16 acc[DP / 32] = {};
+    for (int k0 = 0; k0 < stop; k0 += kKeyTile) {
+        __syncthreads();
+        stage<DP, kKeyTile>(k_tile, k, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
+        stage<DP, kKeyTile>(v_tile, v, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
+        __syncthreads();
+#pragma unroll
+        for (int b = 0; b < kKeyTile / 32; ++b) {
+            F32x16 s = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                s = T::mfma(read_rows<DP>(k_tile, b * 32, i), qf[i], s);
+                dp = T::mfma(read_rows<DP>(v_tile, b * 32, i), of[i], dp);
+            }
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool seen = k0 + b * 32 + acc_row(r, half) <= limit;
+                s[r] = seen ? exp2_fast(s[r] * c - base) * (dp[r] - row_delta) : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const U32x4 ds = pack_step<T>(s, i);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d)
+                    acc[d] = T::mfma(read_columns<DP>(k_tile, b * 32 + i * 16, d * 32), ds, acc[d]);
+            }
+        }
+    }
+    if (there) store_row<T, DP>(dq, rows.begin + row, head, acc, shape.scale, shape.dim);
+}
+
+// dK and dV of a tile of keys of one key head: the rows of every query head of its group pass by, so that the sum
+// over the group is taken in registers and in one order.
+constexpr int kQueryTile = 32;
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, Rows v, Rows dout, Rows dk, Rows dv,
+                                                               const float* __restrict__ lse, const float* __restrict__ delta,
+                                                               const int32_t* __restrict__ q_offsets,
+                                                               const int32_t* __restrict__ k_offsets, Shape shape) {
+    __shared__ __attribute__((aligned(16))) char q_tile[Tile<DP>::bytes(kQueryTile)];
+    __shared__ __attribute__((aligned(16))) char o_tile[Tile<DP>::bytes(kQueryTile)];
+    __shared__ __attribute__((aligned(16))) float stats[2][kQueryTile];
+    const int kv_head = blockIdx.x % shape.kv_heads;
+    const TilePlace place = find_tile(k_offsets, shape.sequences, 1, kRowTile, static_cast<int>(blockIdx.x / shape.kv_heads));
+    if (place.sequence < 0) return;
+    const Span keys = span_of(k_offsets, place.sequence, shape.k_tokens);
+    const int key0 = place.tile * kRowTile;
+    if (key0 >= keys.size) return;
+    const Span rows = span_of(q_offsets, place.sequence, shape.q_tokens);
+    const int group = shape.q_heads / shape.kv_heads;
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int key = key0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
+    const bool there = key < keys.size;
+    const int shift = keys.size - rows.size;
+    // The first row that sees the key, and that sees any of the workgroup.
+    const int first = shape.causal && key - shift > 0 ? key - shift : 0;
+    int start = shape.causal && key0 - shift > 0 ? key0 - shift : 0;
+    start -= start % kQueryTile;
+    const float c = shape.scale * kLog2e;
+
+    U32x4 kf[DP / 16], vf[DP / 16];
+    load_row<DP>(kf, k, keys.begin + key, kv_head, there, shape.dim);
+    load_row<DP>(vf, v, keys.begin + key, kv_head, there, shape.dim);
+    F32x16 dk_acc[DP / 32] = {}, dv_acc[DP / 32] = {};
+    for (int g = 0; g < group; ++g) {
+        const int head = kv_head * group + g;
+        for (int r0 = start; r0 < rows.size; r0 += kQueryTile) {
+            __syncthreads();
+            stage<DP, kQueryTile>(q_tile, q, rows.begin + r0, head, rows.size - r0, shape.dim);
+            stage<DP, kQueryTile>(o_tile, dout, rows.begin + r0, head, rows.size - r0, shape.dim);
+            if (threadIdx.x < kQueryTile) {
+                const bool row_there = r0 + static_cast<int>(threadIdx.x) < rows.size;
+                const int64_t stat = static_cast<int64_t>(head) * shape.q_tokens + rows.begin + r0 + threadIdx.x;
+                const float l = row_there ? lse[stat] : -INFINITY;
+                // exp2(s c - inf) = 0: a row that is not there or sees nothing adds nothing.
+                stats[0][threadIdx.x] = l == -INFINITY ? INFINITY : l * kLog2e;
+                stats[1][threadIdx.x] = row_there ? delta[stat] : 0.f;
+            }
+            __syncthreads();
+            F32x16 s = {}, dp = {};
+#pragma unroll
+            for (int i = 0; i < DP / 16; ++i) {
+                s = T::mfma(read_rows<DP>(q_tile, 0, i), kf[i], s);
+                dp = T::mfma(read_rows<DP>(o_tile, 0, i), vf[i], dp);
+            }
+            F32x16 p;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const F32x4 l = *reinterpret_cast<const F32x4*>(&stats[0][acc_row(4 * j, half)]);
+                const F32x4 e = *reinterpret_cast<const F32x4*>(&stats[1][acc_row(4 * j, half)]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 4 * j + i;
+                    const bool seen = r0 + acc_row(r, half) >= first && there;
+                    p[r] = seen ? exp2_fast(s[r] * c - l[i]) : 0.f;
+                    s[r] = seen ? p[r] * (dp[r] - e[i]) : 0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const U32x4 pf = pack_step<T>(p, i), sf = pack_step<T>(s, i);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    dv_acc[d] = T::mfma(read_columns<DP>(o_tile, i * 16, d * 32), pf, dv_acc[d]);
+                    dk_acc[d] = T::mfma(read_columns<DP>(q_tile, i * 16, d * 32), sf, dk_acc[d]);
+                }
+            }
+        }
+    }
+    if (!there) return;
+    store_row<T, DP>(dk, keys.begin + key, kv_head, dk_acc, shape.scale, shape.dim);
+    store_row<T, DP>(dv, keys.begin + key, kv_head, dv_acc, 1.f, shape.dim);
+}
+
+// ---- host side ---------------------------------------------------------------------------------------------------
+
+
+int check_shape(const char* what, uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads,
+                uint32_t kv_heads, uint32_t dim, float scale) {
+    if (q_heads == 0 || kv_heads == 0 || q_heads % kv_heads != 0 || q_heads > 65535)
+        return set_error(kInvalidArgument, "%s: query heads must be a multiple of the key heads, and at most 65535", what);
+    if (dim == 0 || dim % 8 != 0 || dim > 128)
+        return set_error(kUnsupported, "%s: the head size must be a multiple of 8 up to 128", what);
+    if (q_tokens > 0x7FFFFFFFull || k_tokens > 0x7FFFFFFFull || sequences > 0x7FFFFFFu)
+        return set_error(kInvalidArgument, "%s: too many tokens or sequences", what);
+    if (!(scale > 0.f) || scale == INFINITY) return set_error(kInvalidArgument, "%s: the scale must be positive and finite", what);
+    return kOk;
+}
+
+// Tiles that a ragged batch may have, and the launch over (tile, head).
+int check_grid(const char* what, uint64_t tokens, uint32_t sequences, uint32_t heads, unsigned& tiles, unsigned& grid) {
+    const uint64_t t = tokens / kRowTile + sequences;
+    if (t * heads > 0x7FFFFFFFull / kBlock) return set_error(kInvalidArgument, "%s: too many tiles", what);
+    tiles = static_cast<unsigned>(t);
+    grid = static_cast<unsigned>(t * heads);
+    return kOk;
+}
+
+template <typename T>
+int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* v, const int32_t* q_offsets,
+           const int32_t* k_offsets, const lcpp_hip_rows* out, float* lse, uint32_t sequences, uint64_t q_tokens,
+           uint64_t k_tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t dim, float scale, int causal, void* stream_ptr) {
+    const char* what = "attention_packed";
+    hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+    if (int st = check_shape(what, sequences, q_tokens, k_tokens, q_heads, kv_heads, dim, scale); st != kOk) return st;
+    if (sequences == 0 || q_tokens == 0) return kOk;
+    if (!q_offsets || !k_offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
+    if (!usable(q) || !usable(out) || (k_tokens && (!usable(k) || !usable(v))))
+        return unusable(what);
+    unsigned tiles, grid;
+    if (int st = check_grid(what, q_tokens, sequences, q_heads, tiles, grid); st != kOk) return st;
+    const Shape shape{static_cast<int>(sequences), static_cast<int>(q_tokens), static_cast<int>(k_tokens),
+                      static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(dim), scale, causal != 0};
+    const Rows none{nullptr, 0, 0};
+    const Rows kr = k_tokens ? rows_of(k) : none, vr = k_tokens ? rows_of(v) : none;
+    LaunchScope scope("attention_packed", stream);
+    auto* kernel = dim <= 64 ? attention_packed_kernel<T, 64> : attention_packed_kernel<T, 128>;
+    kernel<<<grid, kBlock, 0, stream>>>(rows_of(q), kr, vr, rows_of(out), lse, q_offsets, k_offsets, shape, tiles);
+    return check_hip(hipGetLastError(), "attention_packed launch");
+}
+
+size_t backward_bytes(uint64_t q_tokens, uint32_t q_heads) { return align_up(q_tokens * q_heads * sizeof(float), kViewAlign); }
+
+template <typename T>
+int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* v,
+                    const lcpp_hip_rows* out, const float* lse, const lcpp_hip_rows* dout, const int32_t* q_offsets,
+                    const int32_t* k_offsets, const lcpp_hip_rows* dq, const lcpp_hip_rows* dk, const lcpp_hip_rows* dv,
+                    uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads, uint32_t kv_heads,
+                    uint32_t dim, float scale, int causal, void* stream_ptr) {
+    const char* what = "attention_packed_backward";
+    hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
+    if (int st = check_shape(what, sequences, q_tokens, k_tokens, q_heads, kv_heads, dim, scale); st != kOk) return st;
+    if (sequences == 0 || (q_tokens == 0 && k_tokens == 0)) return kOk;
+    if (!q_offsets || !k_offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
+    if (q_tokens && (!usable(q) || !usable(out) || !usable(dout) || !usable(dq) || !lse))
+        return unusable(what);
+    if (k_tokens && (!usable(k) || !usable(v) || !usable(dk) || !usable(dv)))
+        return unusable(what);
+    if (temp_bytes < backward_bytes(q_tokens, q_heads) || (q_tokens && !temp))
+        return set_error(kTempTooSmall, "%s: temp storage too small", what);
+    unsigned tiles, grid, key_tiles, key_grid;
+    if (int st = check_grid(what, q_tokens, sequences, q_heads, tiles, grid); st != kOk) return st;
+    if (int st = check_grid(what, k_tokens, sequences, kv_heads, key_tiles, key_grid); st != kOk) return st;
+    const Shape shape{static_cast<int>(sequences), static_cast<int>(q_tokens), static_cast<int>(k_tokens),
+                      static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(dim), scale, causal != 0};
+    float* delta = static_cast<float*>(temp);
+    const Rows none{nullptr, 0, 0};
+    const Rows qr = q_tokens ? rows_of(q) : none, dor = q_tokens ? rows_of(dout) : none;
+    const Rows kr = k_tokens ? rows_of(k) : none, vr = k_tokens ? rows_of(v) : none;
+    if (q_tokens) {
+        LaunchScope scope("attention_delta", stream);
+        const uint64_t blocks = ceil_div(q_tokens * q_heads, kBlock / 16);
+        if (blocks > 0x7FFFFFFFull / kBlock) return set_error(kInvalidArgument, "%s: too many rows", what);
+        attention_delta_kernel<T><<<static_cast<unsigned>(blocks), kBlock, 0, stream>>>(rows_of(out), dor, delta, shape.q_tokens,
+                                                                                        shape.q_heads, shape.dim);
+        if (int st = check_hip(hipGetLastError(), "attention_delta launch"); st != kOk) return st;
+    }
+    if (k_tokens) {
+        LaunchScope scope("attention_dkv", stream);
+        auto* kernel = dim <= 64 ? attention_dkv_kernel<T, 64> : attention_dkv_kernel<T, 128>;
+        kernel<<<key_grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dk), rows_of(dv), lse, delta, q_offsets, k_offsets, shape);
+        if (int st = check_hip(hipGetLastError(), "attention_dkv launch"); st != kOk) return st;
+    }
+    if (q_tokens) {
+        LaunchScope scope("attention_dq", stream);
+        auto* kernel = dim <= 64 ? attention_dq_kernel<T, 64> : attention_dq_kernel<T, 128>;
+        kernel<<<grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dq), lse, delta, q_offsets, k_offsets, shape, tiles);
+        return check_hip(hipGetLastError(), "attention_dq launch");
+    }
+    return kOk;
+}
+
+}  // namespace
+}  // namespace attention
+}  // namespace lcpp_hip
+
+using namespace lcpp_hip;
+
+extern "C" {
+
+size_t lcpp_hip_attention_packed_temp_bytes(uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads,
+                                            uint32_t kv_heads, uint32_t head_dim) {
+    (void)sequences, (void)q_tokens, (void)k_tokens, (void)q_heads, (void)kv_heads, (void)head_dim;
+    return 0;
+}
+
+size_t lcpp_hip_attention_packed_backward_temp_bytes(uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads,
+                                                     uint32_t kv_heads, uint32_t head_dim) {
+    (void)sequences, (void)k_tokens, (void)kv_heads, (void)head_dim;
+    return attention::backward_bytes(q_tokens, q_heads);
+}
+
+#define LCPP_HIP_DEFINE_ATTENTION(S, T)                                                                                     \
+    int lcpp_hip_attention_packed_##S(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_rows* k,        \
+                                      const lcpp_hip_rows* v, const int32_t* q_offsets, const int32_t* k_offsets,           \
+                                      const lcpp_hip_rows* out, float* lse, uint32_t sequences, uint64_t q_tokens,          \
+                                      uint64_t k_tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,            \
+                                      float scale, int causal, void* stream) {                                              \
+        (void)temp, (void)temp_bytes;                                                                                       \
+        return attention::packed<attention::T>(q, k, v, q_offsets, k_offsets, out, lse, sequences, q_tokens, k_tokens,      \
+                                               q_heads, kv_heads, head_dim, scale, causal, stream);                         \
+    }                                                                                                                       \
+    int lcpp_hip_attention_packed_backward_##S(                                                                             \
+        void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* v,              \
+        const lcpp_hip_rows* out, const float* lse, const lcpp_hip_rows* dout, const int32_t* q_offsets,                    \
+        const int32_t* k_offsets, const lcpp_hip_rows* dq, const lcpp_hip_rows* dk, const lcpp_hip_rows* dv,                \
+        uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,   \
+        float scale, int causal, void* stream) {                                                                            \
+        return attention::packed_backward<attention::T>(temp, temp_bytes, q, k, v, out, lse, dout, q_offsets, k_offsets,    \
+                                                        dq, dk, dv, sequences, q_tokens, k_tokens, q_heads, kv_heads,       \
+                                                        head_dim, scale, causal, stream);                                   \
+    }
+LCPP_HIP_DEFINE_ATTENTION(bf16, Bf16)
+LCPP_HIP_DEFINE_ATTENTION(f16, F16)
+#undef LCPP_HIP_DEFINE_ATTENTION
+
+}  // extern "C"

@@ -8,7 +8,9 @@ The operation names follow the reference API (``DeviceReduce::Sum``, ``DeviceSca
 ``DeviceRadixSort::SortKeys/SortPairs``, ``DeviceSpmv::CsrMV``, ``DeviceScan::*SumByKey``,
 ``DeviceReduce::ReduceByKey``, ``DeviceSelect``, ``DevicePartition``, ``DeviceRunLengthEncode``;
 src/lcpp/device/*.h) and the
-temp-storage queries return the reference's ``Get*TempStorageBytes`` values.
+temp-storage queries return the reference's ``Get*TempStorageBytes`` values.  Attention over ragged batches and its
+paged cache (:func:`page_plan`, :func:`paged_write`, :func:`attention_packed`, :func:`attention_paged`) have no
+counterpart there.
 """
 from __future__ import annotations
 
@@ -34,6 +36,7 @@ SORT_KEY_SUFFIXES = ("u32", "i32", "f32", "u64", "i64", "f64")
 SPMV_SUFFIXES = [(v, i) for v in ("f32", "f64", "i32", "u32") for i in ("i32", "u32")]
 BY_KEY_KEY_SUFFIXES = ("i32", "u32", "i64", "u64")
 BY_KEY_VALUE_SUFFIXES = SCALAR_SUFFIXES
+ATTENTION_SUFFIXES = ("bf16", "f16")
 FLAG_SUFFIXES = ("b8", "i32", "u32", "i64", "u64")
 
 # Predicate clause ops (include/lcpp_hip.h LCPP_HIP_PRED_*).
@@ -44,6 +47,16 @@ FLAG_SUFFIXES = ("b8", "i32", "u32", "i64", "u64")
 class Predicate(C.Structure):
     """lcpp_hip_predicate: two clauses that must both hold; operands are bits of the item type."""
     _fields_ = [("op", C.c_int32 * 2), ("a", C.c_uint64 * 2), ("b", C.c_uint64 * 2)]
+
+class Rows(C.Structure):
+    """lcpp_hip_rows: [tokens, heads, head_dim], strides of the first two axes in items."""
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Pages(C.Structure):
+    """lcpp_hip_pages: [pages, page size, kv heads, head_dim], strides of the first three axes in items."""
+    _fields_ = [("data", C.c_void_p), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
 
 _CTYPE = {
     "i32": C.c_int32, "u32": C.c_uint32, "f32": C.c_float,
@@ -173,6 +186,22 @@ def _declare(lib: C.CDLL) -> None:
             sig(f"lcpp_hip_partition_flagged_{t}_{f}", i32, vp, sz, vp, vp, vp, vp, u64, vp)
         for v in SCALAR_SUFFIXES:
             sig(f"lcpp_hip_select_unique_by_key_{t}_{v}", i32, vp, sz, vp, vp, vp, vp, vp, u64, u64, vp)
+
+
+    rp, gp, f32 = C.POINTER(Rows), C.POINTER(Pages), C.c_float
+    sig("lcpp_hip_page_plan_temp_bytes", sz, u32)
+    sig("lcpp_hip_page_plan", i32, vp, sz, vp, vp, u32, u32, vp, u32, vp, u64, u32, vp, vp, vp, vp, vp, u64, vp, vp)
+    sig("lcpp_hip_attention_packed_temp_bytes", sz, u32, u64, u64, u32, u32, u32)
+    sig("lcpp_hip_attention_packed_backward_temp_bytes", sz, u32, u64, u64, u32, u32, u32)
+    sig("lcpp_hip_attention_paged_temp_bytes", sz, u32, u64, u64, u32, u32, u32)
+    for t in ATTENTION_SUFFIXES:
+        sig(f"lcpp_hip_paged_write_{t}", i32, rp, rp, vp, u64, gp, gp, u32, u32, u32, u32, vp)
+        sig(f"lcpp_hip_attention_packed_{t}", i32, vp, sz, rp, rp, rp, vp, vp, rp, vp, u32, u64, u64, u32, u32, u32, f32,
+            i32, vp)
+        sig(f"lcpp_hip_attention_packed_backward_{t}", i32, vp, sz, rp, rp, rp, rp, vp, rp, vp, vp, rp, rp, rp, u32, u64,
+            u64, u32, u32, u32, f32, i32, vp)
+        sig(f"lcpp_hip_attention_paged_{t}", i32, vp, sz, rp, gp, gp, vp, u32, u32, vp, vp, vp, rp, vp, u32, u64, u64, u32,
+            u32, u32, u32, u32, f32, vp)
 
 
 def lib() -> C.CDLL:
@@ -630,3 +659,151 @@ def segmented_sort_db(key_suffix: str, keys0, keys1, selector: int, n: int, num_
              C.byref(ks), ptr(values0), ptr(values1), C.byref(vs), n, num_segments, ptr(begins), ptr(ends),
              begin_bit, end_bit, int(descending), int(value_order), stream_handle(stream))
     return ks.value, vs.value
+
+
+# ---- attention over ragged batches and a paged cache ----------------------------------------------
+_ROW_DTYPES = {"bf16": "torch.bfloat16", "f16": "torch.float16"}
+
+
+def _strides(suffix: str, name: str, t, axes: int, shape, written: bool) -> list:
+    """The strides of a tensor of `axes` axes of the suffix's type, its last axis contiguous; 0 along axes of one item."""
+    if str(t.dtype) != _ROW_DTYPES[suffix] or t.dim() != axes:
+        raise ValueError(f"{name}: {axes} axes of {_ROW_DTYPES[suffix]}, not {t.dim()} of {t.dtype}")
+    if shape is not None and t.shape != shape:
+        raise ValueError(f"{name}: {tuple(t.shape)} where {tuple(shape)} is needed")
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
+    if strides[-1] > 1:
+        raise ValueError(f"{name}: the last axis has to be contiguous")
+    if written and any(s == 0 and n > 1 for s, n in zip(strides, t.shape)):
+        raise ValueError(f"{name}: rows that are written share no memory")
+    return strides
+
+
+def _rows(suffix: str, name: str, t, shape=None, written: bool = False) -> Rows:
+    token, head, _ = _strides(suffix, name, t, 3, shape, written)
+    return Rows(t.data_ptr(), token, head)
+
+
+def _pages(suffix: str, name: str, t, shape=None, written: bool = False) -> Pages:
+    page, token, head, _ = _strides(suffix, name, t, 4, shape, written)
+    return Pages(t.data_ptr(), page, token, head)
+
+
+def _table(t, requests: int) -> tuple:
+    """Address, row stride and width of a block table."""
+    if str(t.dtype) != "torch.int32" or t.dim() != 2 or t.shape[0] < requests or (t.shape[1] > 1 and t.stride(1) != 1):
+        raise ValueError(f"block_table: [{requests}, width] of int32, its rows contiguous")
+    width = t.shape[1]
+    return t.data_ptr(), max(width, t.stride(0)), width
+
+
+def _array(name: str, t, dtype: str, count: int):
+    """Device address of a contiguous array of at least `count` items (None stays None)."""
+    if t is None:
+        return None
+    if str(t.dtype) != dtype or t.numel() < count or not t.is_contiguous():
+        raise ValueError(f"{name}: {count} contiguous items of {dtype} are needed")
+    return t.data_ptr()
+
+
+def page_plan_temp_bytes(requests: int) -> int:
+    return lib().lcpp_hip_page_plan_temp_bytes(requests)
+
+
+def page_plan(cached_lengths, new_lengths, page_size: int, free_pages, block_table, query_offsets, kv_lengths,
+              token_request, token_position, token_slot, counts, temp=None, stream=None) -> None:
+    """Lays out one step: offsets, lengths, and each new token's request, position and slot; pages that
+    block_table [requests, width] lacks come from free_pages.  All int32, token_slot int64."""
+    requests, tokens = cached_lengths.numel(), token_slot.numel()
+    i32, i64 = "torch.int32", "torch.int64"
+    table, table_stride, width = _table(block_table, requests)
+    if temp is None:
+        temp = _temp(page_plan_temp_bytes(requests), cached_lengths.device)
+    call("lcpp_hip_page_plan", ptr(temp), _tb(temp), _array("cached_lengths", cached_lengths, i32, requests),
+         _array("new_lengths", new_lengths, i32, requests), requests, page_size,
+         _array("free_pages", free_pages, i32, 0), free_pages.numel(), table, table_stride, width,
+         _array("query_offsets", query_offsets, i32, requests + 1),
+         _array("kv_lengths", kv_lengths, i32, requests), _array("token_request", token_request, i32, tokens),
+         _array("token_position", token_position, i32, tokens), _array("token_slot", token_slot, i64, tokens), tokens,
+         _array("counts", counts, i32, 2), stream_handle(stream))
+
+
+def paged_write(suffix: str, key, value, slots, key_cache, value_cache, stream=None) -> None:
+    """Rows [tokens, kv heads, head_dim] of key and value to their slots of the caches
+    [pages, page size, kv heads, head_dim]."""
+    pages, page_size, heads, dim = key_cache.shape
+    tokens = slots.numel()
+    shape = (tokens, heads, dim)
+    call(f"lcpp_hip_paged_write_{suffix}", _rows(suffix, "key", key, shape), _rows(suffix, "value", value, shape),
+         _array("slots", slots, "torch.int64", tokens), tokens, _pages(suffix, "key_cache", key_cache, None, True),
+         _pages(suffix, "value_cache", value_cache, key_cache.shape, True), heads, dim, page_size, pages, stream_handle(stream))
+
+
+def attention_packed_temp_bytes(sequences: int, q_tokens: int, k_tokens: int, q_heads: int, kv_heads: int,
+                                head_dim: int) -> int:
+    return lib().lcpp_hip_attention_packed_temp_bytes(sequences, q_tokens, k_tokens, q_heads, kv_heads, head_dim)
+
+
+def attention_packed_backward_temp_bytes(sequences: int, q_tokens: int, k_tokens: int, q_heads: int, kv_heads: int,
+                                         head_dim: int) -> int:
+    return lib().lcpp_hip_attention_packed_backward_temp_bytes(sequences, q_tokens, k_tokens, q_heads, kv_heads, head_dim)
+
+
+def attention_packed(suffix: str, q, k, v, q_offsets, k_offsets, out, lse=None, causal: bool = True, scale=None,
+                     temp=None, stream=None) -> None:
+    """Attention of the rows q [q tokens, q heads, head_dim] to k and v [k tokens, kv heads, head_dim] of the same
+    sequence into out; lse [q heads, q tokens] f32 if given.  `scale` defaults to 1 / sqrt(head_dim)."""
+    (tokens, heads, dim), (keys, kv_heads, _) = q.shape, k.shape
+    sequences = q_offsets.numel() - 1
+    if temp is None:
+        temp = _temp(attention_packed_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device)
+    shape = (keys, kv_heads, dim)
+    call(f"lcpp_hip_attention_packed_{suffix}", ptr(temp), _tb(temp), _rows(suffix, "q", q), _rows(suffix, "k", k, shape),
+         _rows(suffix, "v", v, shape), _array("q_offsets", q_offsets, "torch.int32", 1),
+         _array("k_offsets", k_offsets, "torch.int32", sequences + 1), _rows(suffix, "out", out, q.shape, True),
+         _array("lse", lse, "torch.float32", heads * tokens), sequences, tokens, keys, heads, kv_heads, dim,
+         dim ** -0.5 if scale is None else scale, int(causal), stream_handle(stream))
+
+
+def attention_packed_backward(suffix: str, q, k, v, out, lse, dout, q_offsets, k_offsets, dq, dk, dv,
+                              causal: bool = True, scale=None, temp=None, stream=None) -> None:
+    """Gradients of attention_packed: dq, dk and dv from dout, and from the out and lse that the forward call gave."""
+    (tokens, heads, dim), (keys, kv_heads, _) = q.shape, k.shape
+    sequences = q_offsets.numel() - 1
+    if temp is None:
+        temp = _temp(attention_packed_backward_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device)
+    shape = (keys, kv_heads, dim)
+    call(f"lcpp_hip_attention_packed_backward_{suffix}", ptr(temp), _tb(temp), _rows(suffix, "q", q),
+         _rows(suffix, "k", k, shape), _rows(suffix, "v", v, shape), _rows(suffix, "out", out, q.shape),
+         _array("lse", lse, "torch.float32", heads * tokens), _rows(suffix, "dout", dout, q.shape),
+         _array("q_offsets", q_offsets, "torch.int32", 1), _array("k_offsets", k_offsets, "torch.int32", sequences + 1),
+         _rows(suffix, "dq", dq, q.shape, True), _rows(suffix, "dk", dk, shape, True), _rows(suffix, "dv", dv, shape, True), sequences,
+         tokens, keys, heads, kv_heads, dim, dim ** -0.5 if scale is None else scale, int(causal), stream_handle(stream))
+
+
+def attention_paged_temp_bytes(requests: int, q_tokens: int, max_kv_length: int, q_heads: int, kv_heads: int,
+                               head_dim: int) -> int:
+    return lib().lcpp_hip_attention_paged_temp_bytes(requests, q_tokens, max_kv_length, q_heads, kv_heads, head_dim)
+
+
+def attention_paged(suffix: str, q, key_cache, value_cache, block_table, q_offsets, kv_lengths, out, lse=None, tree=None,
+                    max_kv_length=None, scale=None, temp=None, stream=None) -> None:
+    """Attention of each request's new rows q [q tokens, q heads, head_dim] to its pages of the caches
+    [pages, page size, kv heads, head_dim].  `tree` (int64, a word for each new token): bit j says whether the token
+    sees its request's j-th new token; without it, those up to itself.  `max_kv_length` defaults to what the block
+    table can hold."""
+    (tokens, heads, dim), (pages, page_size, kv_heads, _) = q.shape, key_cache.shape
+    requests = kv_lengths.numel()
+    table, table_stride, width = _table(block_table, requests)
+    if max_kv_length is None:
+        max_kv_length = width * page_size
+    if temp is None:
+        temp = _temp(attention_paged_temp_bytes(requests, tokens, max_kv_length, heads, kv_heads, dim), q.device)
+    call(f"lcpp_hip_attention_paged_{suffix}", ptr(temp), _tb(temp), _rows(suffix, "q", q),
+         _pages(suffix, "key_cache", key_cache, (pages, page_size, kv_heads, dim)),
+         _pages(suffix, "value_cache", value_cache, key_cache.shape), table, table_stride, width,
+         _array("q_offsets", q_offsets, "torch.int32", requests + 1),
+         _array("kv_lengths", kv_lengths, "torch.int32", requests), _array("tree", tree, "torch.int64", tokens),
+         _rows(suffix, "out", out, q.shape, True), _array("lse", lse, "torch.float32", heads * tokens), requests, tokens,
+         max_kv_length, heads, kv_heads, dim, page_size, pages, dim ** -0.5 if scale is None else scale,
+         stream_handle(stream))
