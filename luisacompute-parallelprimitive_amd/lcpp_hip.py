@@ -662,15 +662,20 @@ def segmented_sort_db(key_suffix: str, keys0, keys1, selector: int, n: int, num_
 
 
 # ---- attention over ragged batches and a paged cache ----------------------------------------------
-_ROW_DTYPES = {"bf16": "torch.bfloat16", "f16": "torch.float16"}
+_dtypes: dict = {}  # torch dtypes by suffix, filled at the first call (torch is imported by the calls that need it)
 
 
-def _strides(suffix: str, name: str, t, axes: int, shape, written: bool) -> list:
-    """The strides of a tensor of `axes` axes of the suffix's type, its last axis contiguous; 0 along axes of one item."""
-    if str(t.dtype) != _ROW_DTYPES[suffix] or t.dim() != axes:
-        raise ValueError(f"{name}: {axes} axes of {_ROW_DTYPES[suffix]}, not {t.dim()} of {t.dtype}")
-    if shape is not None and t.shape != shape:
-        raise ValueError(f"{name}: {tuple(t.shape)} where {tuple(shape)} is needed")
+def _row_types(suffix: str) -> tuple:
+    """The torch dtypes of rows of the suffix, and of f32, i32 and i64 arrays."""
+    if not _dtypes:
+        import torch
+        _dtypes.update({s: (t, torch.float32, torch.int32, torch.int64)
+                        for s, t in (("bf16", torch.bfloat16), ("f16", torch.float16))})
+    return _dtypes[suffix]
+
+
+def _strides(name: str, t, written: bool) -> list:
+    """The strides of a tensor whose last axis has to be contiguous; 0 along axes of one item."""
     strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
     if strides[-1] > 1:
         raise ValueError(f"{name}: the last axis has to be contiguous")
@@ -679,31 +684,51 @@ def _strides(suffix: str, name: str, t, axes: int, shape, written: bool) -> list
     return strides
 
 
-def _rows(suffix: str, name: str, t, shape=None, written: bool = False) -> Rows:
-    token, head, _ = _strides(suffix, name, t, 3, shape, written)
+def _refuse(name: str, t, dtype, shape):
+    if t.dtype is not dtype:
+        raise ValueError(f"{name}: {dtype} is needed, not {t.dtype}")
+    raise ValueError(f"{name}: {tuple(t.shape)} where {shape} is needed")
+
+
+def _rows(dtype, name: str, t, shape: tuple, written: bool = False) -> Rows:
+    if t.dtype is not dtype or t.shape != shape:
+        _refuse(name, t, dtype, shape)
+    token, head, item = t.stride()
+    if item != 1 or (token | head) & 7 or (written and not (token and head)):
+        token, head, _ = _strides(name, t, written)
     return Rows(t.data_ptr(), token, head)
 
 
-def _pages(suffix: str, name: str, t, shape=None, written: bool = False) -> Pages:
-    page, token, head, _ = _strides(suffix, name, t, 4, shape, written)
+def _pages(dtype, name: str, t, shape: tuple, written: bool = False) -> Pages:
+    if t.dtype is not dtype or t.shape != shape:
+        _refuse(name, t, dtype, shape)
+    page, token, head, item = t.stride()
+    if item != 1 or (page | token | head) & 7 or (written and not (page and token and head)):
+        page, token, head, _ = _strides(name, t, written)
     return Pages(t.data_ptr(), page, token, head)
 
 
-def _table(t, requests: int) -> tuple:
+def _table(i32, t, requests: int) -> tuple:
     """Address, row stride and width of a block table."""
-    if str(t.dtype) != "torch.int32" or t.dim() != 2 or t.shape[0] < requests or (t.shape[1] > 1 and t.stride(1) != 1):
+    if t.dtype is not i32 or t.dim() != 2 or t.shape[0] < requests or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"block_table: [{requests}, width] of int32, its rows contiguous")
     width = t.shape[1]
     return t.data_ptr(), max(width, t.stride(0)), width
 
 
-def _array(name: str, t, dtype: str, count: int):
+def _array(dtype, name: str, t, count: int):
     """Device address of a contiguous array of at least `count` items (None stays None)."""
     if t is None:
         return None
-    if str(t.dtype) != dtype or t.numel() < count or not t.is_contiguous():
+    if t.dtype is not dtype or t.numel() < count or not t.is_contiguous():
         raise ValueError(f"{name}: {count} contiguous items of {dtype} are needed")
     return t.data_ptr()
+
+
+def _axes(name: str, t, axes: int) -> tuple:
+    if t.dim() != axes:
+        raise ValueError(f"{name}: {axes} axes are needed, not {t.dim()}")
+    return tuple(t.shape)
 
 
 def page_plan_temp_bytes(requests: int) -> int:
@@ -715,28 +740,29 @@ def page_plan(cached_lengths, new_lengths, page_size: int, free_pages, block_tab
     """Lays out one step: offsets, lengths, and each new token's request, position and slot; pages that
     block_table [requests, width] lacks come from free_pages.  All int32, token_slot int64."""
     requests, tokens = cached_lengths.numel(), token_slot.numel()
-    i32, i64 = "torch.int32", "torch.int64"
-    table, table_stride, width = _table(block_table, requests)
+    _, _, i32, i64 = _row_types("bf16")
+    table, table_stride, width = _table(i32, block_table, requests)
     if temp is None:
         temp = _temp(page_plan_temp_bytes(requests), cached_lengths.device)
-    call("lcpp_hip_page_plan", ptr(temp), _tb(temp), _array("cached_lengths", cached_lengths, i32, requests),
-         _array("new_lengths", new_lengths, i32, requests), requests, page_size,
-         _array("free_pages", free_pages, i32, 0), free_pages.numel(), table, table_stride, width,
-         _array("query_offsets", query_offsets, i32, requests + 1),
-         _array("kv_lengths", kv_lengths, i32, requests), _array("token_request", token_request, i32, tokens),
-         _array("token_position", token_position, i32, tokens), _array("token_slot", token_slot, i64, tokens), tokens,
-         _array("counts", counts, i32, 2), stream_handle(stream))
+    call("lcpp_hip_page_plan", ptr(temp), _tb(temp), _array(i32, "cached_lengths", cached_lengths, requests),
+         _array(i32, "new_lengths", new_lengths, requests), requests, page_size,
+         _array(i32, "free_pages", free_pages, 0), free_pages.numel(), table, table_stride, width,
+         _array(i32, "query_offsets", query_offsets, requests + 1),
+         _array(i32, "kv_lengths", kv_lengths, requests), _array(i32, "token_request", token_request, tokens),
+         _array(i32, "token_position", token_position, tokens), _array(i64, "token_slot", token_slot, tokens), tokens,
+         _array(i32, "counts", counts, 2), stream_handle(stream))
 
 
 def paged_write(suffix: str, key, value, slots, key_cache, value_cache, stream=None) -> None:
     """Rows [tokens, kv heads, head_dim] of key and value to their slots of the caches
     [pages, page size, kv heads, head_dim]."""
-    pages, page_size, heads, dim = key_cache.shape
+    dt, _, _, i64 = _row_types(suffix)
+    pages, page_size, heads, dim = cache = _axes("key_cache", key_cache, 4)
     tokens = slots.numel()
     shape = (tokens, heads, dim)
-    call(f"lcpp_hip_paged_write_{suffix}", _rows(suffix, "key", key, shape), _rows(suffix, "value", value, shape),
-         _array("slots", slots, "torch.int64", tokens), tokens, _pages(suffix, "key_cache", key_cache, None, True),
-         _pages(suffix, "value_cache", value_cache, key_cache.shape, True), heads, dim, page_size, pages, stream_handle(stream))
+    call(f"lcpp_hip_paged_write_{suffix}", _rows(dt, "key", key, shape), _rows(dt, "value", value, shape),
+         _array(i64, "slots", slots, tokens), tokens, _pages(dt, "key_cache", key_cache, cache, True),
+         _pages(dt, "value_cache", value_cache, cache, True), heads, dim, page_size, pages, stream_handle(stream))
 
 
 def attention_packed_temp_bytes(sequences: int, q_tokens: int, k_tokens: int, q_heads: int, kv_heads: int,
@@ -753,31 +779,35 @@ def attention_packed(suffix: str, q, k, v, q_offsets, k_offsets, out, lse=None, 
                      temp=None, stream=None) -> None:
     """Attention of the rows q [q tokens, q heads, head_dim] to k and v [k tokens, kv heads, head_dim] of the same
     sequence into out; lse [q heads, q tokens] f32 if given.  `scale` defaults to 1 / sqrt(head_dim)."""
-    (tokens, heads, dim), (keys, kv_heads, _) = q.shape, k.shape
+    dt, f32, i32, _ = _row_types(suffix)
+    tokens, heads, dim = rows = _axes("q", q, 3)
+    keys, kv_heads, _ = _axes("k", k, 3)
     sequences = q_offsets.numel() - 1
     if temp is None:
         temp = _temp(attention_packed_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device)
     shape = (keys, kv_heads, dim)
-    call(f"lcpp_hip_attention_packed_{suffix}", ptr(temp), _tb(temp), _rows(suffix, "q", q), _rows(suffix, "k", k, shape),
-         _rows(suffix, "v", v, shape), _array("q_offsets", q_offsets, "torch.int32", 1),
-         _array("k_offsets", k_offsets, "torch.int32", sequences + 1), _rows(suffix, "out", out, q.shape, True),
-         _array("lse", lse, "torch.float32", heads * tokens), sequences, tokens, keys, heads, kv_heads, dim,
+    call(f"lcpp_hip_attention_packed_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows), _rows(dt, "k", k, shape),
+         _rows(dt, "v", v, shape), _array(i32, "q_offsets", q_offsets, 1),
+         _array(i32, "k_offsets", k_offsets, sequences + 1), _rows(dt, "out", out, rows, True),
+         _array(f32, "lse", lse, heads * tokens), sequences, tokens, keys, heads, kv_heads, dim,
          dim ** -0.5 if scale is None else scale, int(causal), stream_handle(stream))
 
 
 def attention_packed_backward(suffix: str, q, k, v, out, lse, dout, q_offsets, k_offsets, dq, dk, dv,
                               causal: bool = True, scale=None, temp=None, stream=None) -> None:
     """Gradients of attention_packed: dq, dk and dv from dout, and from the out and lse that the forward call gave."""
-    (tokens, heads, dim), (keys, kv_heads, _) = q.shape, k.shape
+    dt, f32, i32, _ = _row_types(suffix)
+    tokens, heads, dim = rows = _axes("q", q, 3)
+    keys, kv_heads, _ = _axes("k", k, 3)
     sequences = q_offsets.numel() - 1
     if temp is None:
         temp = _temp(attention_packed_backward_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device)
     shape = (keys, kv_heads, dim)
-    call(f"lcpp_hip_attention_packed_backward_{suffix}", ptr(temp), _tb(temp), _rows(suffix, "q", q),
-         _rows(suffix, "k", k, shape), _rows(suffix, "v", v, shape), _rows(suffix, "out", out, q.shape),
-         _array("lse", lse, "torch.float32", heads * tokens), _rows(suffix, "dout", dout, q.shape),
-         _array("q_offsets", q_offsets, "torch.int32", 1), _array("k_offsets", k_offsets, "torch.int32", sequences + 1),
-         _rows(suffix, "dq", dq, q.shape, True), _rows(suffix, "dk", dk, shape, True), _rows(suffix, "dv", dv, shape, True), sequences,
+    call(f"lcpp_hip_attention_packed_backward_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows),
+         _rows(dt, "k", k, shape), _rows(dt, "v", v, shape), _rows(dt, "out", out, rows),
+         _array(f32, "lse", lse, heads * tokens), _rows(dt, "dout", dout, rows),
+         _array(i32, "q_offsets", q_offsets, 1), _array(i32, "k_offsets", k_offsets, sequences + 1),
+         _rows(dt, "dq", dq, rows, True), _rows(dt, "dk", dk, shape, True), _rows(dt, "dv", dv, shape, True), sequences,
          tokens, keys, heads, kv_heads, dim, dim ** -0.5 if scale is None else scale, int(causal), stream_handle(stream))
 
 
@@ -792,18 +822,21 @@ def attention_paged(suffix: str, q, key_cache, value_cache, block_table, q_offse
     [pages, page size, kv heads, head_dim].  `tree` (int64, a word for each new token): bit j says whether the token
     sees its request's j-th new token; without it, those up to itself.  `max_kv_length` defaults to what the block
     table can hold."""
-    (tokens, heads, dim), (pages, page_size, kv_heads, _) = q.shape, key_cache.shape
+    dt, f32, i32, i64 = _row_types(suffix)
+    tokens, heads, dim = rows = _axes("q", q, 3)
+    pages, page_size, kv_heads, _ = _axes("key_cache", key_cache, 4)
+    cache = (pages, page_size, kv_heads, dim)
     requests = kv_lengths.numel()
-    table, table_stride, width = _table(block_table, requests)
+    table, table_stride, width = _table(i32, block_table, requests)
     if max_kv_length is None:
         max_kv_length = width * page_size
     if temp is None:
         temp = _temp(attention_paged_temp_bytes(requests, tokens, max_kv_length, heads, kv_heads, dim), q.device)
-    call(f"lcpp_hip_attention_paged_{suffix}", ptr(temp), _tb(temp), _rows(suffix, "q", q),
-         _pages(suffix, "key_cache", key_cache, (pages, page_size, kv_heads, dim)),
-         _pages(suffix, "value_cache", value_cache, key_cache.shape), table, table_stride, width,
-         _array("q_offsets", q_offsets, "torch.int32", requests + 1),
-         _array("kv_lengths", kv_lengths, "torch.int32", requests), _array("tree", tree, "torch.int64", tokens),
-         _rows(suffix, "out", out, q.shape, True), _array("lse", lse, "torch.float32", heads * tokens), requests, tokens,
+    call(f"lcpp_hip_attention_paged_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows),
+         _pages(dt, "key_cache", key_cache, cache),
+         _pages(dt, "value_cache", value_cache, cache), table, table_stride, width,
+         _array(i32, "q_offsets", q_offsets, requests + 1),
+         _array(i32, "kv_lengths", kv_lengths, requests), _array(i64, "tree", tree, tokens),
+         _rows(dt, "out", out, rows, True), _array(f32, "lse", lse, heads * tokens), requests, tokens,
          max_kv_length, heads, kv_heads, dim, page_size, pages, dim ** -0.5 if scale is None else scale,
          stream_handle(stream))
