@@ -1,0 +1,165 @@
+// The loop over keys that the packed forward kernel and the paged kernel for many rows share.
+//
+// A wave holds 32 query rows as B operands.  S^T = K Q^T leaves a row's scores in two lanes' registers (32 keys apart
+// in halves), so the running maximum and sum cost one lane exchange a tile, and the weights go into O^T = V^T P^T as
+// they stand.  Tiles of 64 keys are loaded straight into LDS, one ahead of the one in use.
+#pragma once
+
+#include "attention.hpp"
+
+namespace lcpp_hip {
+namespace attention {
+
+constexpr int kBlock = 256;
+constexpr int kWaves = kBlock / kWave;
+constexpr int kRowsPerWave = 32;
+constexpr int kRowTile = kWaves * kRowsPerWave;  // query rows of a workgroup
+constexpr int kKeyTile = 64;                     // keys in LDS at a time
+// The running maximum that scales the sums follows the true one only when a row has outgrown it by this (as an exponent
+// of 2): weights are then at most 2^8, within the 16-bit types, and the products are rescaled a few times a row at most.
+constexpr float kSlack = 8.f;
+
+// Direct loads of a tile: load i of a wave fills 1024 bytes in order, so a lane's row and chunk are fixed.
+template <int DP>
+struct TileLoads {
+    static constexpr int kPerWave = Tile<DP>::bytes(kKeyTile) / (kWaves * kWave * 16);
+    __device__ __forceinline__ static int item(int i) { return (i * kWaves + threadIdx.x / kWave) * kWave + threadIdx.x % kWave; }
+    __device__ __forceinline__ static int row(int i) { return item(i) / Tile<DP>::kChunks; }
+    __device__ __forceinline__ static int chunk(int i) { return item(i) % Tile<DP>::kChunks ^ Tile<DP>::swizzle(row(i)); }
+    __device__ __forceinline__ static char* place(char* tile, int i) {
+        return tile + (i * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * kWave * 16;
+    }
+};
+
+__device__ __forceinline__ void load_to_lds(const char* from, char* to) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(from),
+                                     (__attribute__((address_space(3))) uint32_t*)(to), 16, 0, 0);
+}
+
+// Zeros where a row of fewer items than DP has none; loads never touch those chunks.
+template <int DP>
+__device__ __forceinline__ void clear_past(char* tile, int dim) {
+    if (dim == DP) return;
+#pragma unroll
+    for (int i = 0; i < TileLoads<DP>::kPerWave; ++i)
+        if (TileLoads<DP>::chunk(i) * 8 >= dim) *reinterpret_cast<U32x4*>(tile + TileLoads<DP>::item(i) * 16) = U32x4{0u, 0u, 0u, 0u};
+}
+
+// Keys of a packed sequence: rows past its last are loaded as its last, and masked.
+template <int DP>
+struct PackedKeys {
+    const char* base;  // the sequence's first row of the head
+    int64_t token_bytes;
+    int size;
+    int dim;
+    __device__ __forceinline__ void load(char* tile, int k0) const {
+        const char* from = base + k0 * token_bytes;
+        const int last = size - 1 - k0;
+#pragma unroll
+        for (int i = 0; i < TileLoads<DP>::kPerWave; ++i) {
+            int row = TileLoads<DP>::row(i);
+            row = row < last ? row : last;
+            const int chunk = TileLoads<DP>::chunk(i);
+            if (DP == dim || chunk * 8 < dim) load_to_lds(from + row * token_bytes + chunk * 16, TileLoads<DP>::place(tile, i));
+        }
+    }
+};
+
+// What a lane has for its row.
+template <int DP>
+struct RowState {
+    F32x16 acc[DP / 32];
+    float top;    // the scale of acc and total: at most kSlack / c below the largest score so far
+    float total;  // of the lane's half of the keys
+};
+
+// Keys from k0 on that a row sees, when it sees the first `count` of its sequence.
+__device__ __forceinline__ uint32_t first_keys(int count, int k0) {
+    const int n = count - k0;
+    return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
+}
+
+// One tile of keys.  `seen(k0)`: the 32 keys from k0 on that the lane's row sees, as bits; `masked`: some row of the
+// workgroup does not see all of the tile.
+template <typename T, int DP, typename Seen>
+__device__ __forceinline__ void forward_tile(RowState<DP>& state, const char* k_tile, const char* v_tile, const U32x4 (&qf)[DP / 16],
+                                             float c, int k0, bool masked, Seen seen) {
+    constexpr int kBlocks = kKeyTile / 32;
+    const int half = threadIdx.x % kWave / 32;
+    F32x16 s[kBlocks] = {};
+#pragma unroll
+    for (int i = 0; i < DP / 16; ++i)
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) s[b] = T::mfma(read_rows<DP>(k_tile, b * 32, i), qf[i], s[b]);
+    if (masked) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) {
+            const uint32_t word = seen(k0 + 32 * b) >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[b][r] = word & (1u << acc_row(r, 0)) ? s[b][r] : -INFINITY;
+        }
+    }
+    float high = s[0][0];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) high = fmaxf(high, s[b][r]);
+    high = halves_max(high);
+    const bool outgrown = (high - state.top) * c > kSlack;  // (from -inf: yes, unless the row still sees nothing)
+    if (wave_ballot(outgrown) != 0) {
+        const float top = outgrown ? high : state.top;
+        const float alpha = outgrown ? exp2_fast((state.top - top) * c) : 1.f;
+        state.top = top;
+        state.total *= alpha;
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) state.acc[d] *= alpha;
+    }
+    const float base = state.top == -INFINITY ? 0.f : state.top * c;
+    float sum = 0.f;
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            s[b][r] = exp2_fast(s[b][r] * c - base);
+            sum += s[b][r];
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const U32x4 p = pack_step<T>(s[b], i);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d)
+                state.acc[d] = T::mfma(read_columns<DP>(v_tile, b * 32 + i * 16, d * 32), p, state.acc[d]);
+        }
+    }
+    state.total += sum;
+}
+
+// All keys in [begin, end), whose tiles the workgroup's waves load together.  Tiles from `full` on are masked.
+template <typename T, int DP, typename Keys, typename Seen>
+__device__ __forceinline__ void forward_keys(RowState<DP>& state, char* k_even, char* v_even, char* k_odd, char* v_odd, const Keys& keys,
+                                             const Keys& values, const U32x4 (&qf)[DP / 16], float c, int begin, int end, int full,
+                                             Seen seen) {
+    if (begin >= end) return;
+    keys.load(k_even, begin);
+    values.load(v_even, begin);
+    __syncthreads();
+    for (int k0 = begin;; k0 += 2 * kKeyTile) {
+        if (k0 + kKeyTile < end) {
+            keys.load(k_odd, k0 + kKeyTile);
+            values.load(v_odd, k0 + kKeyTile);
+        }
+        forward_tile<T, DP>(state, k_even, v_even, qf, c, k0, k0 + kKeyTile > full, seen);
+        if (k0 + kKeyTile >= end) break;
+        __syncthreads();
+        if (k0 + 2 * kKeyTile < end) {
+            keys.load(k_even, k0 + 2 * kKeyTile);
+            values.load(v_even, k0 + 2 * kKeyTile);
+        }
+        forward_tile<T, DP>(state, k_odd, v_odd, qf, c, k0 + kKeyTile, k0 + 2 * kKeyTile > full, seen);
+        if (k0 + 2 * kKeyTile >= end) break;
+        __syncthreads();
+    }
+}
+
+}  // namespace attention
+}  // namespace lcpp_hip

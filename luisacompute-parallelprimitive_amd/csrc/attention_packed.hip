@@ -3,17 +3,11 @@
 //   S = scale q k^T,  row i of n sees key j of m where j <= i + m - n (causal) or any j,
 //   P = softmax(S),  O = P V,  lse = log sum exp S;  a row that sees nothing has O = 0 and lse = -inf.
 //   dV = P^T dO,  dP = dO V^T,  dS = P (dP - rowsum(dO O)),  dQ = scale dS K,  dK = scale dS^T Q.
-#include "attention.hpp"
+#include "attention_forward.hpp"
 
 namespace lcpp_hip {
 namespace attention {
 namespace {
-
-constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / kWave;
-constexpr int kRowsPerWave = 32;
-constexpr int kRowTile = kWaves * kRowsPerWave;  // query rows of a workgroup
-constexpr int kKeyTile = 64;                     // keys staged at a time
 
 struct Shape {
     int sequences;
@@ -48,7 +42,7 @@ __device__ __forceinline__ void stage(char* tile, const Rows& src, int64_t token
         const int row = at / kChunks, chunk = at % kChunks;
         const bool there = row < rows;
         const U32x4 v = load_chunk(src.at(token0 + (there ? row : 0), head), chunk, dim, there);
-        *reinterpret_cast<U32x4*>(tile + row * Tile<DP>::kStride + chunk * 16) = v;
+        *reinterpret_cast<U32x4*>(tile + Tile<DP>::place(row, chunk)) = v;
     }
 }
 
@@ -80,13 +74,20 @@ __device__ __forceinline__ void store_row(const Rows& dst, int64_t token, int he
 }
 
 template <typename T, int DP>
-__global__ __launch_bounds__(kBlock) void attention_packed_kernel(Rows q, Rows k, Rows v, Rows out, float* __restrict__ lse,
-                                                                  const int32_t* __restrict__ q_offsets,
-                                                                  const int32_t* __restrict__ k_offsets, Shape shape,
-                                                                  int tiles) {
-    __shared__ __attribute__((aligned(16))) char k_tile[Tile<DP>::bytes(kKeyTile)];
-    __shared__ __attribute__((aligned(16))) char v_tile[Tile<DP>::bytes(kKeyTile)];
-    const int head = blockIdx.x % shape.q_heads;
+__global__ __launch_bounds__(kBlock, 2) void attention_packed_kernel(Rows q, Rows k, Rows v, Rows out, float* __restrict__ lse,
+                                                                     const int32_t* __restrict__ q_offsets,
+                                                                     const int32_t* __restrict__ k_offsets, Shape shape,
+                                                                     int tiles) {
+    constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);
+    __shared__ __attribute__((aligned(16))) char k_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char v_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char k_odd[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char v_odd[kTileBytes];
+    // Workgroups go to the 8 XCDs in turn: with the key head as the fastest number, those of a key head share an L2.
+    // Later tiles, which see more keys, come first.
+    const int group = shape.q_heads / shape.kv_heads;
+    const int kv_head = blockIdx.x % shape.kv_heads;
+    const int head = kv_head * group + blockIdx.x / shape.kv_heads % group;
     const int number = tiles - 1 - static_cast<int>(blockIdx.x / shape.q_heads);
     const TilePlace place = find_tile(q_offsets, shape.sequences, 1, kRowTile, number);
     if (place.sequence < 0) return;
@@ -94,70 +95,33 @@ __global__ __launch_bounds__(kBlock) void attention_packed_kernel(Rows q, Rows k
     const int row0 = place.tile * kRowTile;
     if (row0 >= rows.size) return;
     const Span keys = span_of(k_offsets, place.sequence, shape.k_tokens);
-    const int kv_head = head / (shape.q_heads / shape.kv_heads);
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int row = row0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
     const bool there = row < rows.size;
-    const int shift = shape.causal ? keys.size - rows.size : keys.size;
-    // The last key that the row, and that any row of the workgroup, sees.
-    const int last = shape.causal ? row + shift : keys.size - 1;
+    // Keys that the row, the workgroup's first row and its last row see.
+    const int shift = shape.causal ? keys.size - rows.size + 1 : keys.size;
+    const int count = shape.causal && row + shift < keys.size ? row + shift : keys.size;
+    int full = shape.causal && row0 + shift < keys.size ? row0 + shift : keys.size;
+    full = full < 0 ? 0 : full;
     const int tile_last = row0 + kRowTile < rows.size ? row0 + kRowTile - 1 : rows.size - 1;
-    int stop = shape.causal ? tile_last + shift + 1 : keys.size;
-    stop = stop < keys.size ? stop : keys.size;
+    const int end = shape.causal && tile_last + shift < keys.size ? tile_last + shift : keys.size;
     const float c = shape.scale * kLog2e;
 
     U32x4 qf[DP / 16];
     load_row<DP>(qf, q, rows.begin + row, head, there, shape.dim);
-    F32x16 acc[DP / 32] = {};
-    float top = -INFINITY, total = 0.f;
-    for (int k0 = 0; k0 < stop; k0 += kKeyTile) {
-        __syncthreads();
-        stage<DP, kKeyTile>(k_tile, k, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
-        stage<DP, kKeyTile>(v_tile, v, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
-        __syncthreads();
-        F32x16 s[kKeyTile / 32] = {};
-#pragma unroll
-        for (int b = 0; b < kKeyTile / 32; ++b)
-#pragma unroll
-            for (int i = 0; i < DP / 16; ++i) s[b] = T::mfma(read_rows<DP>(k_tile, b * 32, i), qf[i], s[b]);
-        const int limit = last < keys.size - 1 ? last : keys.size - 1;
-        float high = top;
-#pragma unroll
-        for (int b = 0; b < kKeyTile / 32; ++b)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                if (k0 + b * 32 + acc_row(r, half) > limit) s[b][r] = -INFINITY;
-                high = fmaxf(high, s[b][r]);
-            }
-        high = halves_max(high);
-        const float base = high == -INFINITY ? 0.f : high * c;
-        const float alpha = exp2_fast(top * c - base);
-        top = high;
-        total *= alpha;
-#pragma unroll
-        for (int b = 0; b < DP / 32; ++b) acc[b] *= alpha;
-#pragma unroll
-        for (int b = 0; b < kKeyTile / 32; ++b) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                s[b][r] = exp2_fast(s[b][r] * c - base);
-                total += s[b][r];
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const U32x4 p = pack_step<T>(s[b], i);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d)
-                    acc[d] = T::mfma(read_columns<DP>(v_tile, b * 32 + i * 16, d * 32), p, acc[d]);
-            }
-        }
-    }
-    total = halves_sum(total);
+    for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP>(tile, shape.dim);
+    RowState<DP> state = {};
+    state.top = -INFINITY;
+    forward_keys<T, DP>(state, k_even, v_even, k_odd, v_odd,
+                        PackedKeys<DP>{k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim},
+                        PackedKeys<DP>{v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim}, qf, c, 0, end, full,
+                        [&](int k0) { return first_keys(count, k0); });
+    const float total = halves_sum(state.total);
     if (!there) return;
-    store_row<T, DP>(out, rows.begin + row, head, acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
+    store_row<T, DP>(out, rows.begin + row, head, state.acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
     if (lse != nullptr && half == 0)
         lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row] =
-            total == 0.f ? -INFINITY : top * shape.scale + __logf(total);
+            total == 0.f ? -INFINITY : state.top * shape.scale + __logf(total);
 }
 
 // ---- gradients ---------------------------------------------------------------------------------------------------

@@ -92,8 +92,8 @@ __global__ __launch_bounds__(kBlock) void attention_paged_kernel(Rows q, Pages k
                                                                  const uint64_t* __restrict__ tree, Paged p) {
     constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);
     constexpr int kJoinStride = DP + 4;  // floats
-    static_assert(kWaves * kRowTile * kJoinStride * 4 <= kWaves * 2 * kTileBytes, "the join reuses the tiles");
-    __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * kTileBytes];
+    constexpr int kJoinBytes = kWaves * kRowTile * kJoinStride * 4;
+    __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * kTileBytes > kJoinBytes ? kWaves * 2 * kTileBytes : kJoinBytes];
     __shared__ float stats[2][kWaves][kRowTile];
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
@@ -140,8 +140,8 @@ __global__ __launch_bounds__(kBlock) void attention_paged_kernel(Rows q, Pages k
             const int64_t pg = here ? from_page : 0, sl = here ? from_slot : 0;
             const U32x4 kc = load_chunk(key_cache.at(pg, sl, kv_head), chunk, p.dim, here);
             const U32x4 vc = load_chunk(value_cache.at(pg, sl, kv_head), chunk, p.dim, here);
-            *reinterpret_cast<U32x4*>(k_tile + key * Tile<DP>::kStride + chunk * 16) = kc;
-            *reinterpret_cast<U32x4*>(v_tile + key * Tile<DP>::kStride + chunk * 16) = vc;
+            *reinterpret_cast<U32x4*>(k_tile + Tile<DP>::place(key, chunk)) = kc;
+            *reinterpret_cast<U32x4*>(v_tile + Tile<DP>::place(key, chunk)) = vc;
         }
         wave_lds_order();
         F32x16 s = {};
