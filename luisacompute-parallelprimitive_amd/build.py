@@ -33,6 +33,9 @@ HIP_FLAGS = [
     "-O3", "-std=c++20", f"--offload-arch={ARCH}", "-fPIC", "-fvisibility=hidden", "-Wall", "-Wno-unused-function",
     # Keep the compiler from forming packed-FP32 VALU instructions.
     "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops",
+    # Matrix products may have their results in any register, not in the accumulation registers alone (which the vector
+    # instructions between two products cannot read).
+    "-mllvm", "-amdgpu-mfma-vgpr-form=1",
     f"-I{REPO / 'include'}",
 ]
 HOST_FLAGS = ["-O2", "-std=c++20", "-fPIC", "-fvisibility=hidden", "-Wall", f"-I{REPO / 'include'}"]

@@ -131,35 +131,39 @@ inline Pages pages_of(const lcpp_hip_pages* c) {
 }
 
 // A tile of rows in LDS: DP items a row (the head size rounded up; zeros past it), in 16-byte chunks without padding, so
-// that a wave's direct loads fill it in order.  Chunk c of row r lies at place c ^ swizzle(r): eight rows in a row (a
-// read along them) and four rows' pairs of chunks (a transposed read) then lie in different banks.
+// that a wave's direct loads fill it in order.  LDS has 64 banks of 4 bytes: chunk c of row r lies at place
+// c ^ swizzle(r), so that the same chunk of 16 rows (a read along rows), and four chunks side by side of four rows (a
+// transposed read), fill all banks once.
 template <int DP>
 struct Tile {
     static constexpr int kChunks = DP / 8;
     static constexpr int kRowBytes = DP * 2;
     static constexpr int bytes(int rows) { return rows * kRowBytes; }
-    __device__ __forceinline__ static int swizzle(int row) { return 2 * (row % 4) + row / 4 % 2; }
+    __device__ __forceinline__ static int swizzle(int row) {
+        static_assert(DP == 64 || DP == 128, "two rows or one fill the banks");
+        return (DP == 128 ? 4 * (row % 4) : 4 * (row / 2 % 2)) + row / 4 % 4;
+    }
     __device__ __forceinline__ static int place(int row, int chunk) { return row * kRowBytes + (chunk ^ swizzle(row)) * 16; }
 };
 
-// Contraction step s of row c (A operand of 32 rows from `row0`, a multiple of 8): 8 items at 16 s + 8 h.
+// Contraction step s of row c (A operand of 32 rows from `row0`, a multiple of 16): 8 items at 16 s + 8 h.
 template <int DP>
 __device__ __forceinline__ U32x4 read_rows(const char* tile, int row0, int s) {
     const int lane = threadIdx.x % kWave;
     return *reinterpret_cast<const U32x4*>(tile + row0 * Tile<DP>::kRowBytes + Tile<DP>::place(lane % 32, 2 * s + lane / 32));
 }
 
-// A operand of the transposed tile: 32 columns from `col0`, contraction over the 16 rows from `row0` in the order
-// of pack_step.  A transposed read hands each of 16 lanes the four items of its column from four rows.
+// A operand of the transposed tile: 32 columns from `col0`, contraction over the 16 rows from `row0` (a multiple of 16)
+// in the order of pack_step.  A transposed read hands each of 16 lanes the four items of its column from four rows.
 template <int DP>
 __device__ __forceinline__ U32x4 read_columns(const char* tile, int row0, int col0) {
     using LdsPtr = __attribute__((address_space(3))) S16x4*;
     const int lane = threadIdx.x % kWave;
     const int row = 4 * (lane / 32) + lane % 16 / 4;
     const int chunk = col0 / 8 + 2 * (lane / 16 % 2) + lane % 4 / 2;
-    const char* p = tile + row0 * Tile<DP>::kRowBytes + Tile<DP>::place(row, chunk) + lane % 2 * 8;
-    const S16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
-    const S16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + 8 * Tile<DP>::kRowBytes));
+    const char* p = tile + row0 * Tile<DP>::kRowBytes + lane % 2 * 8;
+    const S16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + Tile<DP>::place(row, chunk)));
+    const S16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + Tile<DP>::place(row + 8, chunk)));
     const U32x2 x = __builtin_bit_cast(U32x2, a), y = __builtin_bit_cast(U32x2, b);
     return U32x4{x[0], x[1], y[0], y[1]};
 }

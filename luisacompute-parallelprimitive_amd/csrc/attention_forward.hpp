@@ -20,9 +20,9 @@ constexpr int kKeyTile = 64;                     // keys in LDS at a time
 constexpr float kSlack = 8.f;
 
 // Direct loads of a tile: load i of a wave fills 1024 bytes in order, so a lane's row and chunk are fixed.
-template <int DP>
+template <int DP, int ROWS>
 struct TileLoads {
-    static constexpr int kPerWave = Tile<DP>::bytes(kKeyTile) / (kWaves * kWave * 16);
+    static constexpr int kPerWave = Tile<DP>::bytes(ROWS) / (kWaves * kWave * 16);
     __device__ __forceinline__ static int item(int i) { return (i * kWaves + threadIdx.x / kWave) * kWave + threadIdx.x % kWave; }
     __device__ __forceinline__ static int row(int i) { return item(i) / Tile<DP>::kChunks; }
     __device__ __forceinline__ static int chunk(int i) { return item(i) % Tile<DP>::kChunks ^ Tile<DP>::swizzle(row(i)); }
@@ -37,30 +37,32 @@ __device__ __forceinline__ void load_to_lds(const char* from, char* to) {
 }
 
 // Zeros where a row of fewer items than DP has none; loads never touch those chunks.
-template <int DP>
+template <int DP, int ROWS>
 __device__ __forceinline__ void clear_past(char* tile, int dim) {
+    using Loads = TileLoads<DP, ROWS>;
     if (dim == DP) return;
 #pragma unroll
-    for (int i = 0; i < TileLoads<DP>::kPerWave; ++i)
-        if (TileLoads<DP>::chunk(i) * 8 >= dim) *reinterpret_cast<U32x4*>(tile + TileLoads<DP>::item(i) * 16) = U32x4{0u, 0u, 0u, 0u};
+    for (int i = 0; i < Loads::kPerWave; ++i)
+        if (Loads::chunk(i) * 8 >= dim) *reinterpret_cast<U32x4*>(tile + Loads::item(i) * 16) = U32x4{0u, 0u, 0u, 0u};
 }
 
-// Keys of a packed sequence: rows past its last are loaded as its last, and masked.
-template <int DP>
-struct PackedKeys {
+// Rows of a packed sequence: those past its last are loaded as its last, and masked.
+template <int DP, int ROWS>
+struct PackedRows {
     const char* base;  // the sequence's first row of the head
     int64_t token_bytes;
     int size;
     int dim;
-    __device__ __forceinline__ void load(char* tile, int k0) const {
-        const char* from = base + k0 * token_bytes;
-        const int last = size - 1 - k0;
+    __device__ __forceinline__ void load(char* tile, int row0) const {
+        using Loads = TileLoads<DP, ROWS>;
+        const char* from = base + row0 * token_bytes;
+        const int last = size - 1 - row0;
 #pragma unroll
-        for (int i = 0; i < TileLoads<DP>::kPerWave; ++i) {
-            int row = TileLoads<DP>::row(i);
+        for (int i = 0; i < Loads::kPerWave; ++i) {
+            int row = Loads::row(i);
             row = row < last ? row : last;
-            const int chunk = TileLoads<DP>::chunk(i);
-            if (DP == dim || chunk * 8 < dim) load_to_lds(from + row * token_bytes + chunk * 16, TileLoads<DP>::place(tile, i));
+            const int chunk = Loads::chunk(i);
+            if (DP == dim || chunk * 8 < dim) load_to_lds(from + row * token_bytes + chunk * 16, Loads::place(tile, i));
         }
     }
 };
@@ -134,31 +136,40 @@ __device__ __forceinline__ void forward_tile(RowState<DP>& state, const char* k_
     state.total += sum;
 }
 
-// All keys in [begin, end), whose tiles the workgroup's waves load together.  Tiles from `full` on are masked.
+// Runs the tiles from `begin` to `end`, SIZE apart, with two sets of buffers: while one is computed on, the other is loaded.
+// The sets are distinct arrays, so that reads of one do not wait for loads of the other.
+template <int SIZE, typename LoadEven, typename LoadOdd, typename StepEven, typename StepOdd>
+__device__ __forceinline__ void pass_tiles(int begin, int end, LoadEven load_even, LoadOdd load_odd, StepEven step_even,
+                                           StepOdd step_odd) {
+    if (begin >= end) return;
+    load_even(begin);
+    __syncthreads();
+    for (int at = begin;; at += 2 * SIZE) {
+        if (at + SIZE < end) load_odd(at + SIZE);
+        step_even(at);
+        if (at + SIZE >= end) break;
+        __syncthreads();
+        if (at + 2 * SIZE < end) load_even(at + 2 * SIZE);
+        step_odd(at + SIZE);
+        if (at + 2 * SIZE >= end) break;
+        __syncthreads();
+    }
+}
+
+// All keys in [begin, end), whose tiles the workgroup's waves load together.  Tiles that pass `full` are masked.
 template <typename T, int DP, typename Keys, typename Seen>
 __device__ __forceinline__ void forward_keys(RowState<DP>& state, char* k_even, char* v_even, char* k_odd, char* v_odd, const Keys& keys,
                                              const Keys& values, const U32x4 (&qf)[DP / 16], float c, int begin, int end, int full,
                                              Seen seen) {
-    if (begin >= end) return;
-    keys.load(k_even, begin);
-    values.load(v_even, begin);
-    __syncthreads();
-    for (int k0 = begin;; k0 += 2 * kKeyTile) {
-        if (k0 + kKeyTile < end) {
-            keys.load(k_odd, k0 + kKeyTile);
-            values.load(v_odd, k0 + kKeyTile);
-        }
-        forward_tile<T, DP>(state, k_even, v_even, qf, c, k0, k0 + kKeyTile > full, seen);
-        if (k0 + kKeyTile >= end) break;
-        __syncthreads();
-        if (k0 + 2 * kKeyTile < end) {
-            keys.load(k_even, k0 + 2 * kKeyTile);
-            values.load(v_even, k0 + 2 * kKeyTile);
-        }
-        forward_tile<T, DP>(state, k_odd, v_odd, qf, c, k0 + kKeyTile, k0 + 2 * kKeyTile > full, seen);
-        if (k0 + 2 * kKeyTile >= end) break;
-        __syncthreads();
-    }
+    const auto load = [&](char* k_tile, char* v_tile, int k0) {
+        keys.load(k_tile, k0);
+        values.load(v_tile, k0);
+    };
+    const auto step = [&](const char* k_tile, const char* v_tile, int k0) {
+        forward_tile<T, DP>(state, k_tile, v_tile, qf, c, k0, k0 + kKeyTile > full, seen);
+    };
+    pass_tiles<kKeyTile>(begin, end, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
+                         [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
 }
 
 }  // namespace attention

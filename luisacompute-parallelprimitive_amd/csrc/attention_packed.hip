@@ -73,6 +73,19 @@ __device__ __forceinline__ void store_row(const Rows& dst, int64_t token, int he
     }
 }
 
+// Keys that a row sees (the first `count`), that every row of its workgroup sees, and that any does.
+struct RowRange {
+    int count, full, end;
+    __device__ __forceinline__ RowRange(const Shape& shape, const Span& rows, const Span& keys, int row0, int row) {
+        const int shift = keys.size - rows.size + 1;
+        const int last = row0 + kRowTile < rows.size ? row0 + kRowTile - 1 : rows.size - 1;
+        const auto seen = [&](int r) { return !shape.causal || r + shift > keys.size ? keys.size : r + shift > 0 ? r + shift : 0; };
+        count = seen(row);
+        full = seen(row0);
+        end = seen(last);
+    }
+};
+
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock, 2) void attention_packed_kernel(Rows q, Rows k, Rows v, Rows out, float* __restrict__ lse,
                                                                      const int32_t* __restrict__ q_offsets,
@@ -98,24 +111,18 @@ __global__ __launch_bounds__(kBlock, 2) void attention_packed_kernel(Rows q, Row
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int row = row0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
     const bool there = row < rows.size;
-    // Keys that the row, the workgroup's first row and its last row see.
-    const int shift = shape.causal ? keys.size - rows.size + 1 : keys.size;
-    const int count = shape.causal && row + shift < keys.size ? row + shift : keys.size;
-    int full = shape.causal && row0 + shift < keys.size ? row0 + shift : keys.size;
-    full = full < 0 ? 0 : full;
-    const int tile_last = row0 + kRowTile < rows.size ? row0 + kRowTile - 1 : rows.size - 1;
-    const int end = shape.causal && tile_last + shift < keys.size ? tile_last + shift : keys.size;
+    const RowRange range(shape, rows, keys, row0, row);
     const float c = shape.scale * kLog2e;
 
     U32x4 qf[DP / 16];
     load_row<DP>(qf, q, rows.begin + row, head, there, shape.dim);
-    for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP>(tile, shape.dim);
+    for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile>(tile, shape.dim);
     RowState<DP> state = {};
     state.top = -INFINITY;
     forward_keys<T, DP>(state, k_even, v_even, k_odd, v_odd,
-                        PackedKeys<DP>{k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim},
-                        PackedKeys<DP>{v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim}, qf, c, 0, end, full,
-                        [&](int k0) { return first_keys(count, k0); });
+                        PackedRows<DP, kKeyTile>{k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim},
+                        PackedRows<DP, kKeyTile>{v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim}, qf, c, 0,
+                        range.end, range.full, [&](int k0) { return first_keys(range.count, k0); });
     const float total = halves_sum(state.total);
     if (!there) return;
     store_row<T, DP>(out, rows.begin + row, head, state.acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
@@ -126,12 +133,14 @@ __global__ __launch_bounds__(kBlock, 2) void attention_packed_kernel(Rows q, Row
 
 // ---- gradients ---------------------------------------------------------------------------------------------------
 
-// delta[h][t] = sum over the head's items of dO * O: 16 lanes a row.
+// What the gradients need of a row: stats[h][t] = lse in powers of 2 (infinity for a row that saw nothing: its weights
+// are then 2^-inf = 0), and behind all of those delta[h][t] = sum over the head's items of dO * O.  16 lanes a row.
 template <typename T>
-__global__ __launch_bounds__(kBlock) void attention_delta_kernel(Rows out, Rows dout, float* __restrict__ delta, int q_tokens,
-                                                                 int q_heads, int dim) {
+__global__ __launch_bounds__(kBlock) void attention_row_stats_kernel(Rows out, Rows dout, const float* __restrict__ lse,
+                                                                     float* __restrict__ stats, int q_tokens, int q_heads, int dim) {
     const int64_t item = static_cast<int64_t>(blockIdx.x) * (kBlock / 16) + threadIdx.x / 16;
-    if (item >= static_cast<int64_t>(q_tokens) * q_heads) return;
+    const int64_t rows = static_cast<int64_t>(q_tokens) * q_heads;
+    if (item >= rows) return;
     const int64_t token = item / q_heads;
     const int head = static_cast<int>(item % q_heads), chunk = threadIdx.x % 16;
     const U32x4 a = load_chunk(out.at(token, head), chunk, dim, true);
@@ -144,18 +153,28 @@ __global__ __launch_bounds__(kBlock) void attention_delta_kernel(Rows out, Rows 
     }
 #pragma unroll
     for (int step = 8; step > 0; step /= 2) sum += __shfl_xor(sum, step);
-    if (chunk == 0) delta[static_cast<int64_t>(head) * q_tokens + token] = sum;
+    if (chunk == 0) {
+        const int64_t at = static_cast<int64_t>(head) * q_tokens + token;
+        const float l = lse[at];
+        stats[at] = l == -INFINITY ? INFINITY : l * kLog2e;
+        stats[rows + at] = sum;
+    }
 }
 
 // dQ of a tile of query rows: the keys pass by as in the forward kernel.
 template <typename T, int DP>
-__global__ __launch_bounds__(kBlock) void attention_dq_kernel(Rows q, Rows k, Rows v, Rows dout, Rows dq,
-                                                              const float* __restrict__ lse, const float* __restrict__ delta,
-                                                              const int32_t* __restrict__ q_offsets,
-                                                              const int32_t* __restrict__ k_offsets, Shape shape, int tiles) {
-    __shared__ __attribute__((aligned(16))) char k_tile[Tile<DP>::bytes(kKeyTile)];
-    __shared__ __attribute__((aligned(16))) char v_tile[Tile<DP>::bytes(kKeyTile)];
-    const int head = blockIdx.x % shape.q_heads;
+__global__ __launch_bounds__(kBlock, 2) void attention_dq_kernel(Rows q, Rows k, Rows v, Rows dout, Rows dq,
+                                                                 const float* __restrict__ stats,
+                                                                 const int32_t* __restrict__ q_offsets,
+                                                                 const int32_t* __restrict__ k_offsets, Shape shape, int tiles) {
+    constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);
+    __shared__ __attribute__((aligned(16))) char k_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char v_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char k_odd[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char v_odd[kTileBytes];
+    const int group = shape.q_heads / shape.kv_heads;
+    const int kv_head = blockIdx.x % shape.kv_heads;
+    const int head = kv_head * group + blockIdx.x / shape.kv_heads % group;
     const int number = tiles - 1 - static_cast<int>(blockIdx.x / shape.q_heads);
     const TilePlace place = find_tile(q_offsets, shape.sequences, 1, kRowTile, number);
     if (place.sequence < 0) return;
@@ -163,31 +182,27 @@ __global__ __launch_bounds__(kBlock) void attention_dq_kernel(Rows q, Rows k, Ro
     const int row0 = place.tile * kRowTile;
     if (row0 >= rows.size) return;
     const Span keys = span_of(k_offsets, place.sequence, shape.k_tokens);
-    const int kv_head = head / (shape.q_heads / shape.kv_heads);
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int row = row0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
     const bool there = row < rows.size;
-    const int shift = keys.size - rows.size;
-    const int tile_last = row0 + kRowTile < rows.size ? row0 + kRowTile - 1 : rows.size - 1;
-    int stop = shape.causal ? tile_last + shift + 1 : keys.size;
-    stop = stop < keys.size ? stop : keys.size;
-    int limit = shape.causal && row + shift < keys.size - 1 ? row + shift : keys.size - 1;
+    const RowRange range(shape, rows, keys, row0, row);
     const float c = shape.scale * kLog2e;
 
     U32x4 qf[DP / 16], of[DP / 16];
     load_row<DP>(qf, q, rows.begin + row, head, there, shape.dim);
     load_row<DP>(of, dout, rows.begin + row, head, there, shape.dim);
     const int64_t stat = static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row;
-    const float row_lse = there ? lse[stat] : -INFINITY;
-    const float row_delta = there ? delta[stat] : 0.f;
-    if (row_lse == -INFINITY) limit = -1;
-    const float base = row_lse * kLog2e;
+    const float base = there ? stats[stat] : INFINITY;
+    const float delta = there ? stats[static_cast<int64_t>(shape.q_heads) * shape.q_tokens + stat] : 0.f;
+    for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile>(tile, shape.dim);
     F32x16 acc[DP / 32] = {};
-    for (int k0 = 0; k0 < stop; k0 += kKeyTile) {
-        __syncthreads();
-        stage<DP, kKeyTile>(k_tile, k, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
-        stage<DP, kKeyTile>(v_tile, v, keys.begin + k0, kv_head, keys.size - k0, shape.dim);
-        __syncthreads();
+    const PackedRows<DP, kKeyTile> key_rows{k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim};
+    const PackedRows<DP, kKeyTile> value_rows{v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim};
+    const auto load = [&](char* k_tile, char* v_tile, int k0) {
+        key_rows.load(k_tile, k0);
+        value_rows.load(v_tile, k0);
+    };
+    const auto step = [&](const char* k_tile, const char* v_tile, int k0) {
 #pragma unroll
         for (int b = 0; b < kKeyTile / 32; ++b) {
             F32x16 s = {}, dp = {};
@@ -197,9 +212,11 @@ __global__ __launch_bounds__(kBlock) void attention_dq_kernel(Rows q, Rows k, Ro
                 dp = T::mfma(read_rows<DP>(v_tile, b * 32, i), of[i], dp);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const bool seen = k0 + b * 32 + acc_row(r, half) <= limit;
-                s[r] = seen ? exp2_fast(s[r] * c - base) * (dp[r] - row_delta) : 0.f;
+            for (int r = 0; r < 16; ++r) s[r] = exp2_fast(s[r] * c - base) * (dp[r] - delta);
+            if (k0 + kKeyTile > range.full) {
+                const uint32_t word = first_keys(range.count, k0 + 32 * b) >> (4 * half);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = word & (1u << acc_row(r, 0)) ? s[r] : 0.f;
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -209,7 +226,9 @@ __global__ __launch_bounds__(kBlock) void attention_dq_kernel(Rows q, Rows k, Ro
                     acc[d] = T::mfma(read_columns<DP>(k_tile, b * 32 + i * 16, d * 32), ds, acc[d]);
             }
         }
-    }
+    };
+    pass_tiles<kKeyTile>(0, range.end, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
+                         [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
     if (there) store_row<T, DP>(dq, rows.begin + row, head, acc, shape.scale, shape.dim);
 }
 
@@ -219,12 +238,16 @@ constexpr int kQueryTile = 32;
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, Rows v, Rows dout, Rows dk, Rows dv,
-                                                               const float* __restrict__ lse, const float* __restrict__ delta,
-                                                               const int32_t* __restrict__ q_offsets,
-                                                               const int32_t* __restrict__ k_offsets, Shape shape) {
-    __shared__ __attribute__((aligned(16))) char q_tile[Tile<DP>::bytes(kQueryTile)];
-    __shared__ __attribute__((aligned(16))) char o_tile[Tile<DP>::bytes(kQueryTile)];
-    __shared__ __attribute__((aligned(16))) float stats[2][kQueryTile];
+                                                                  const float* __restrict__ stats,
+                                                                  const int32_t* __restrict__ q_offsets,
+                                                                  const int32_t* __restrict__ k_offsets, Shape shape) {
+    constexpr int kTileBytes = Tile<DP>::bytes(kQueryTile);
+    __shared__ __attribute__((aligned(16))) char q_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char o_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char q_odd[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char o_odd[kTileBytes];
+    __shared__ __attribute__((aligned(16))) float s_even[2 * kQueryTile];
+    __shared__ __attribute__((aligned(16))) float s_odd[2 * kQueryTile];
     const int kv_head = blockIdx.x % shape.kv_heads;
     const TilePlace place = find_tile(k_offsets, shape.sequences, 1, kRowTile, static_cast<int>(blockIdx.x / shape.kv_heads));
     if (place.sequence < 0) return;
@@ -233,65 +256,75 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, R
     if (key0 >= keys.size) return;
     const Span rows = span_of(q_offsets, place.sequence, shape.q_tokens);
     const int group = shape.q_heads / shape.kv_heads;
-    const int lane = threadIdx.x % kWave, half = lane / 32;
-    const int key = key0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
+    const int lane = threadIdx.x % kWave, half = lane / 32, wave = threadIdx.x / kWave;
+    const int key = key0 + wave * kRowsPerWave + lane % 32;
     const bool there = key < keys.size;
     const int shift = keys.size - rows.size;
-    // The first row that sees the key, and that sees any of the workgroup.
+    // The first row that sees the key, that sees any of the workgroup's, and from which on rows see all of them.
     const int first = shape.causal && key - shift > 0 ? key - shift : 0;
     int start = shape.causal && key0 - shift > 0 ? key0 - shift : 0;
     start -= start % kQueryTile;
+    const int full = shape.causal && key0 + kRowTile - 1 - shift > 0 ? key0 + kRowTile - 1 - shift : 0;
     const float c = shape.scale * kLog2e;
 
     U32x4 kf[DP / 16], vf[DP / 16];
     load_row<DP>(kf, k, keys.begin + key, kv_head, there, shape.dim);
     load_row<DP>(vf, v, keys.begin + key, kv_head, there, shape.dim);
+    for (char* tile : {q_even, o_even, q_odd, o_odd}) clear_past<DP, kQueryTile>(tile, shape.dim);
     F32x16 dk_acc[DP / 32] = {}, dv_acc[DP / 32] = {};
-    for (int g = 0; g < group; ++g) {
-        const int head = kv_head * group + g;
-        for (int r0 = start; r0 < rows.size; r0 += kQueryTile) {
-            __syncthreads();
-            stage<DP, kQueryTile>(q_tile, q, rows.begin + r0, head, rows.size - r0, shape.dim);
-            stage<DP, kQueryTile>(o_tile, dout, rows.begin + r0, head, rows.size - r0, shape.dim);
-            if (threadIdx.x < kQueryTile) {
-                const bool row_there = r0 + static_cast<int>(threadIdx.x) < rows.size;
-                const int64_t stat = static_cast<int64_t>(head) * shape.q_tokens + rows.begin + r0 + threadIdx.x;
-                const float l = row_there ? lse[stat] : -INFINITY;
-                // exp2(s c - inf) = 0: a row that is not there or sees nothing adds nothing.
-                stats[0][threadIdx.x] = l == -INFINITY ? INFINITY : l * kLog2e;
-                stats[1][threadIdx.x] = row_there ? delta[stat] : 0.f;
-            }
-            __syncthreads();
-            F32x16 s = {}, dp = {};
+    // The tiles of all heads of the group in one sequence: tile x is rows of head x / per.
+    const int per = rows.size > start ? (rows.size - start + kQueryTile - 1) / kQueryTile : 0;
+    const auto load = [&](char* q_tile, char* o_tile, float* s_tile, int x) {
+        const int head = kv_head * group + x / per, r0 = start + x % per * kQueryTile;
+        PackedRows<DP, kQueryTile>{q.at(rows.begin, head), q.token_bytes, rows.size, shape.dim}.load(q_tile, r0);
+        PackedRows<DP, kQueryTile>{dout.at(rows.begin, head), dout.token_bytes, rows.size, shape.dim}.load(o_tile, r0);
+        if (wave == 0) {
+            const int row = r0 + lane % 32 < rows.size ? r0 + lane % 32 : rows.size - 1;
+            const float* from = stats + (static_cast<int64_t>(half) * shape.q_heads + head) * shape.q_tokens + rows.begin + row;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(from),
+                                             (__attribute__((address_space(3))) uint32_t*)(s_tile), 4, 0, 0);
+        }
+    };
+    const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile, int x) {
+        const int r0 = start + x % per * kQueryTile;
+        F32x16 s = {}, dp = {};
 #pragma unroll
-            for (int i = 0; i < DP / 16; ++i) {
-                s = T::mfma(read_rows<DP>(q_tile, 0, i), kf[i], s);
-                dp = T::mfma(read_rows<DP>(o_tile, 0, i), vf[i], dp);
-            }
-            F32x16 p;
+        for (int i = 0; i < DP / 16; ++i) {
+            s = T::mfma(read_rows<DP>(q_tile, 0, i), kf[i], s);
+            dp = T::mfma(read_rows<DP>(o_tile, 0, i), vf[i], dp);
+        }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const F32x4 l = *reinterpret_cast<const F32x4*>(&stats[0][acc_row(4 * j, half)]);
-                const F32x4 e = *reinterpret_cast<const F32x4*>(&stats[1][acc_row(4 * j, half)]);
+        for (int j = 0; j < 4; ++j) {
+            const F32x4 l = *reinterpret_cast<const F32x4*>(&s_tile[acc_row(4 * j, half)]);
+            const F32x4 e = *reinterpret_cast<const F32x4*>(&s_tile[kQueryTile + acc_row(4 * j, half)]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int r = 4 * j + i;
-                    const bool seen = r0 + acc_row(r, half) >= first && there;
-                    p[r] = seen ? exp2_fast(s[r] * c - l[i]) : 0.f;
-                    s[r] = seen ? p[r] * (dp[r] - e[i]) : 0.f;
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const U32x4 pf = pack_step<T>(p, i), sf = pack_step<T>(s, i);
-#pragma unroll
-                for (int d = 0; d < DP / 32; ++d) {
-                    dv_acc[d] = T::mfma(read_columns<DP>(o_tile, i * 16, d * 32), pf, dv_acc[d]);
-                    dk_acc[d] = T::mfma(read_columns<DP>(q_tile, i * 16, d * 32), sf, dk_acc[d]);
-                }
+            for (int i = 0; i < 4; ++i) {
+                const int r = 4 * j + i;
+                s[r] = exp2_fast(s[r] * c - l[i]);
+                dp[r] = s[r] * (dp[r] - e[i]);
             }
         }
-    }
+        if (r0 < full || r0 + kQueryTile > rows.size) {
+            const uint32_t word = (first_keys(rows.size, r0) & ~first_keys(first, r0)) >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const bool seen = word & (1u << acc_row(r, 0));
+                s[r] = seen ? s[r] : 0.f;
+                dp[r] = seen ? dp[r] : 0.f;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const U32x4 pf = pack_step<T>(s, i), sf = pack_step<T>(dp, i);
+#pragma unroll
+            for (int d = 0; d < DP / 32; ++d) {
+                dv_acc[d] = T::mfma(read_columns<DP>(o_tile, i * 16, d * 32), pf, dv_acc[d]);
+                dk_acc[d] = T::mfma(read_columns<DP>(q_tile, i * 16, d * 32), sf, dk_acc[d]);
+            }
+        }
+    };
+    pass_tiles<1>(0, per * group, [&](int x) { load(q_even, o_even, s_even, x); }, [&](int x) { load(q_odd, o_odd, s_odd, x); },
+                  [&](int x) { step(q_even, o_even, s_even, x); }, [&](int x) { step(q_odd, o_odd, s_odd, x); });
     if (!there) return;
     store_row<T, DP>(dk, keys.begin + key, kv_head, dk_acc, shape.scale, shape.dim);
     store_row<T, DP>(dv, keys.begin + key, kv_head, dv_acc, 1.f, shape.dim);
@@ -344,7 +377,7 @@ int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* 
     return check_hip(hipGetLastError(), "attention_packed launch");
 }
 
-size_t backward_bytes(uint64_t q_tokens, uint32_t q_heads) { return align_up(q_tokens * q_heads * sizeof(float), kViewAlign); }
+size_t backward_bytes(uint64_t q_tokens, uint32_t q_heads) { return align_up(q_tokens * q_heads * 2 * sizeof(float), kViewAlign); }
 
 template <typename T>
 int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* v,
@@ -368,28 +401,28 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
     if (int st = check_grid(what, k_tokens, sequences, kv_heads, key_tiles, key_grid); st != kOk) return st;
     const Shape shape{static_cast<int>(sequences), static_cast<int>(q_tokens), static_cast<int>(k_tokens),
                       static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(dim), scale, causal != 0};
-    float* delta = static_cast<float*>(temp);
+    float* stats = static_cast<float*>(temp);
     const Rows none{nullptr, 0, 0};
     const Rows qr = q_tokens ? rows_of(q) : none, dor = q_tokens ? rows_of(dout) : none;
     const Rows kr = k_tokens ? rows_of(k) : none, vr = k_tokens ? rows_of(v) : none;
     if (q_tokens) {
-        LaunchScope scope("attention_delta", stream);
+        LaunchScope scope("attention_row_stats", stream);
         const uint64_t blocks = ceil_div(q_tokens * q_heads, kBlock / 16);
         if (blocks > 0x7FFFFFFFull / kBlock) return set_error(kInvalidArgument, "%s: too many rows", what);
-        attention_delta_kernel<T><<<static_cast<unsigned>(blocks), kBlock, 0, stream>>>(rows_of(out), dor, delta, shape.q_tokens,
-                                                                                        shape.q_heads, shape.dim);
-        if (int st = check_hip(hipGetLastError(), "attention_delta launch"); st != kOk) return st;
+        attention_row_stats_kernel<T><<<static_cast<unsigned>(blocks), kBlock, 0, stream>>>(
+            rows_of(out), dor, lse, stats, shape.q_tokens, shape.q_heads, shape.dim);
+        if (int st = check_hip(hipGetLastError(), "attention_row_stats launch"); st != kOk) return st;
     }
     if (k_tokens) {
         LaunchScope scope("attention_dkv", stream);
         auto* kernel = dim <= 64 ? attention_dkv_kernel<T, 64> : attention_dkv_kernel<T, 128>;
-        kernel<<<key_grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dk), rows_of(dv), lse, delta, q_offsets, k_offsets, shape);
+        kernel<<<key_grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dk), rows_of(dv), stats, q_offsets, k_offsets, shape);
         if (int st = check_hip(hipGetLastError(), "attention_dkv launch"); st != kOk) return st;
     }
     if (q_tokens) {
         LaunchScope scope("attention_dq", stream);
         auto* kernel = dim <= 64 ? attention_dq_kernel<T, 64> : attention_dq_kernel<T, 128>;
-        kernel<<<grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dq), lse, delta, q_offsets, k_offsets, shape, tiles);
+        kernel<<<grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dq), stats, q_offsets, k_offsets, shape, tiles);
         return check_hip(hipGetLastError(), "attention_dq launch");
     }
     return kOk;
