@@ -643,7 +643,8 @@ LCPP_HIP_DECLARE_PAGED_WRITE(f16)
 
 /* Attention of packed rows to the packed keys of the same sequence.  Causal: row i of n sees key j of m where
  * j <= i + m - n (the last row sees every key, so keys may have a head start, or fewer keys leave the first rows
- * with none); otherwise every row sees every key.  lse may be null; the backward pass needs it.  The
+ * with none); otherwise every row sees every key.  lse may be null; the backward pass needs it.  Token strides of k and
+ * v, and in the backward pass of q and dout, are below 2^24 items (others: LCPP_HIP_ERR_UNSUPPORTED).  The
  * backward pass writes dq for the rows, dk and dv for the keys (sums over the query heads that share one). */
 size_t lcpp_hip_attention_packed_temp_bytes(uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads,
                                             uint32_t kv_heads, uint32_t head_dim);

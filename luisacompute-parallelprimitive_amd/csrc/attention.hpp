@@ -130,27 +130,36 @@ inline Pages pages_of(const lcpp_hip_pages* c) {
     return {static_cast<char*>(c->data), c->page_stride * 2, c->token_stride * 2, c->head_stride * 2};
 }
 
-// A tile of rows in LDS: DP items a row (the head size rounded up; zeros past it), in 16-byte chunks without padding, so
-// that a wave's direct loads fill it in order.  LDS has 64 banks of 4 bytes: chunk c of row r lies at place
-// c ^ swizzle(r), so that the same chunk of 16 rows (a read along rows), and four chunks side by side of four rows (a
-// transposed read), fill all banks once.
+// A tile of rows in LDS: DP items a row (the head size rounded up; zeros past it), in chunks of 16 bytes, with room for 64
+// or 128 items.  A wave's direct load writes 64 chunks in lane order: 4 rows of 128 items, or 8 of 64.  Within these four chunks of a row lie side by side
+// (64 bytes that a load reads together), then the same four of the next row; and from one 4 rows to the next a chunk moves
+// by 16 bytes, by padding or by exchanging neighbours.  So the same chunk of 16 rows (a read along rows), and four chunks
+// of four rows (a transposed read), fill the 64 banks of 4 bytes once; and a lane's addresses in one tile differ by
+// constants.
 template <int DP>
 struct Tile {
-    static constexpr int kChunks = DP / 8;
-    static constexpr int kRowBytes = DP * 2;
-    static constexpr int bytes(int rows) { return rows * kRowBytes; }
-    __device__ __forceinline__ static int swizzle(int row) {
-        static_assert(DP == 64 || DP == 128, "two rows or one fill the banks");
-        return (DP == 128 ? 4 * (row % 4) : 4 * (row / 2 % 2)) + row / 4 % 4;
+    static_assert(DP % 32 == 0 && DP <= 128);
+    static constexpr bool kWide = DP > 64;
+    static constexpr int kBlockRows = kWide ? 4 : 8;
+    static constexpr int kBlockBytes = 1024 + (kWide ? 16 : 32);
+    static constexpr int bytes(int rows) { return rows / kBlockRows * kBlockBytes; }
+    __device__ __forceinline__ static int place(int row, int chunk) {
+        const int group = kWide ? 0 : row / 4 % 2;
+        return row / kBlockRows * kBlockBytes + group * 512 + chunk / 4 * 256 + row % 4 * 64 + (chunk % 4 ^ group) * 16;
     }
-    __device__ __forceinline__ static int place(int row, int chunk) { return row * kRowBytes + (chunk ^ swizzle(row)) * 16; }
+    // The row of its block and the chunk that a lane's direct load writes.
+    __device__ __forceinline__ static int lane_row(int lane) { return (kWide ? 0 : lane / 32 * 4) + lane % 16 / 4; }
+    __device__ __forceinline__ static int lane_chunk(int lane) {
+        return kWide ? lane / 16 * 4 + lane % 4 : lane / 16 % 2 * 4 + (lane % 4 ^ lane / 32);
+    }
 };
 
 // Contraction step s of row c (A operand of 32 rows from `row0`, a multiple of 16): 8 items at 16 s + 8 h.
 template <int DP>
 __device__ __forceinline__ U32x4 read_rows(const char* tile, int row0, int s) {
     const int lane = threadIdx.x % kWave;
-    return *reinterpret_cast<const U32x4*>(tile + row0 * Tile<DP>::kRowBytes + Tile<DP>::place(lane % 32, 2 * s + lane / 32));
+    const char* p = tile + Tile<DP>::place(lane % 32, lane / 32);
+    return *reinterpret_cast<const U32x4*>(p + Tile<DP>::bytes(row0) + s / 2 * 256 + s % 2 * 32);
 }
 
 // A operand of the transposed tile: 32 columns from `col0`, contraction over the 16 rows from `row0` (a multiple of 16)
@@ -159,11 +168,10 @@ template <int DP>
 __device__ __forceinline__ U32x4 read_columns(const char* tile, int row0, int col0) {
     using LdsPtr = __attribute__((address_space(3))) S16x4*;
     const int lane = threadIdx.x % kWave;
-    const int row = 4 * (lane / 32) + lane % 16 / 4;
-    const int chunk = col0 / 8 + 2 * (lane / 16 % 2) + lane % 4 / 2;
-    const char* p = tile + row0 * Tile<DP>::kRowBytes + lane % 2 * 8;
-    const S16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + Tile<DP>::place(row, chunk)));
-    const S16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + Tile<DP>::place(row + 8, chunk)));
+    const char* p = tile + Tile<DP>::place(4 * (lane / 32) + lane % 16 / 4, 2 * (lane / 16 % 2) + lane % 4 / 2) + lane % 2 * 8;
+    p += Tile<DP>::bytes(row0) + col0 / 32 * 256;
+    const S16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
+    const S16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + Tile<DP>::bytes(8)));
     const U32x2 x = __builtin_bit_cast(U32x2, a), y = __builtin_bit_cast(U32x2, b);
     return U32x4{x[0], x[1], y[0], y[1]};
 }

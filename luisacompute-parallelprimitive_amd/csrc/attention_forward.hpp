@@ -19,15 +19,18 @@ constexpr int kKeyTile = 64;                     // keys in LDS at a time
 // of 2): weights are then at most 2^8, within the 16-bit types, and the products are rescaled a few times a row at most.
 constexpr float kSlack = 8.f;
 
-// Direct loads of a tile: load i of a wave fills 1024 bytes in order, so a lane's row and chunk are fixed.
+// Direct loads of a tile, a block of rows each: a lane's chunk is the same in all of them, and its row goes up by kRowStep.
 template <int DP, int ROWS>
 struct TileLoads {
-    static constexpr int kPerWave = Tile<DP>::bytes(ROWS) / (kWaves * kWave * 16);
-    __device__ __forceinline__ static int item(int i) { return (i * kWaves + threadIdx.x / kWave) * kWave + threadIdx.x % kWave; }
-    __device__ __forceinline__ static int row(int i) { return item(i) / Tile<DP>::kChunks; }
-    __device__ __forceinline__ static int chunk(int i) { return item(i) % Tile<DP>::kChunks ^ Tile<DP>::swizzle(row(i)); }
+    static constexpr int kRowStep = kWaves * Tile<DP>::kBlockRows;
+    static constexpr int kPerWave = ROWS / kRowStep;
+    static_assert(kPerWave > 0 && ROWS % kRowStep == 0);
+    __device__ __forceinline__ static int row() {
+        return threadIdx.x / kWave * Tile<DP>::kBlockRows + Tile<DP>::lane_row(threadIdx.x % kWave);
+    }
+    __device__ __forceinline__ static int chunk() { return Tile<DP>::lane_chunk(threadIdx.x % kWave); }
     __device__ __forceinline__ static char* place(char* tile, int i) {
-        return tile + (i * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * kWave * 16;
+        return tile + (i * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * Tile<DP>::kBlockBytes;
     }
 };
 
@@ -40,29 +43,42 @@ __device__ __forceinline__ void load_to_lds(const char* from, char* to) {
 template <int DP, int ROWS>
 __device__ __forceinline__ void clear_past(char* tile, int dim) {
     using Loads = TileLoads<DP, ROWS>;
-    if (dim == DP) return;
+    if (Loads::chunk() * 8 < dim) return;
 #pragma unroll
     for (int i = 0; i < Loads::kPerWave; ++i)
-        if (Loads::chunk(i) * 8 >= dim) *reinterpret_cast<U32x4*>(tile + Loads::item(i) * 16) = U32x4{0u, 0u, 0u, 0u};
+        *reinterpret_cast<U32x4*>(Loads::place(tile, i) + threadIdx.x % kWave * 16) = U32x4{0u, 0u, 0u, 0u};
 }
 
-// Rows of a packed sequence: those past its last are loaded as its last, and masked.
+// Rows of a packed sequence: those past its last are loaded as its last, and masked.  Addresses are a scalar base and a
+// lane's offset of 32 bits, which stays the same from tile to tile (the host keeps a tile's bytes below 2^31).
 template <int DP, int ROWS>
 struct PackedRows {
+    using Loads = TileLoads<DP, ROWS>;
     const char* base;  // the sequence's first row of the head
     int64_t token_bytes;
     int size;
-    int dim;
+    uint32_t offset;
+    bool has;
+    __device__ __forceinline__ PackedRows(const char* first, int64_t bytes, int rows, int dim)
+        : base(first), token_bytes(bytes), size(rows),
+          offset(static_cast<uint32_t>(Loads::row()) * static_cast<uint32_t>(bytes) + Loads::chunk() * 16u),
+          has(Loads::chunk() * 8 < dim) {}
     __device__ __forceinline__ void load(char* tile, int row0) const {
-        using Loads = TileLoads<DP, ROWS>;
+        if (!has) return;
         const char* from = base + row0 * token_bytes;
-        const int last = size - 1 - row0;
+        if (row0 + ROWS <= size) {
 #pragma unroll
-        for (int i = 0; i < Loads::kPerWave; ++i) {
-            int row = Loads::row(i);
-            row = row < last ? row : last;
-            const int chunk = Loads::chunk(i);
-            if (DP == dim || chunk * 8 < dim) load_to_lds(from + row * token_bytes + chunk * 16, Loads::place(tile, i));
+            for (int i = 0; i < Loads::kPerWave; ++i)
+                load_to_lds(from + i * Loads::kRowStep * token_bytes + offset, Loads::place(tile, i));
+        } else {
+            const int last = size - 1 - row0;
+#pragma unroll
+            for (int i = 0; i < Loads::kPerWave; ++i) {
+                int row = Loads::row() + i * Loads::kRowStep;
+                row = row < last ? row : last;
+                const uint32_t at = static_cast<uint32_t>(row) * static_cast<uint32_t>(token_bytes) + Loads::chunk() * 16u;
+                load_to_lds(from + at, Loads::place(tile, i));
+            }
         }
     }
 };
@@ -156,17 +172,18 @@ __device__ __forceinline__ void pass_tiles(int begin, int end, LoadEven load_eve
     }
 }
 
-// All keys in [begin, end), whose tiles the workgroup's waves load together.  Tiles that pass `full` are masked.
+// All keys in [begin, end), whose tiles the workgroup's waves load together.  Tiles that pass `full` are masked; a wave
+// whose rows see nothing from `wave_end` on leaves the rest to the others.
 template <typename T, int DP, typename Keys, typename Seen>
 __device__ __forceinline__ void forward_keys(RowState<DP>& state, char* k_even, char* v_even, char* k_odd, char* v_odd, const Keys& keys,
-                                             const Keys& values, const U32x4 (&qf)[DP / 16], float c, int begin, int end, int full,
-                                             Seen seen) {
+                                             const Keys& values, const U32x4 (&qf)[DP / 16], float c, int begin, int end, int wave_end,
+                                             int full, Seen seen) {
     const auto load = [&](char* k_tile, char* v_tile, int k0) {
         keys.load(k_tile, k0);
         values.load(v_tile, k0);
     };
     const auto step = [&](const char* k_tile, const char* v_tile, int k0) {
-        forward_tile<T, DP>(state, k_tile, v_tile, qf, c, k0, k0 + kKeyTile > full, seen);
+        if (k0 < wave_end) forward_tile<T, DP>(state, k_tile, v_tile, qf, c, k0, k0 + kKeyTile > full, seen);
     };
     pass_tiles<kKeyTile>(begin, end, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
                          [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });

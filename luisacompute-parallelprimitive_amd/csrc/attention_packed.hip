@@ -73,9 +73,9 @@ __device__ __forceinline__ void store_row(const Rows& dst, int64_t token, int he
     }
 }
 
-// Keys that a row sees (the first `count`), that every row of its workgroup sees, and that any does.
+// Keys that a row sees (the first `count`), that every row of its workgroup sees, and that any does, or any of its wave.
 struct RowRange {
-    int count, full, end;
+    int count, full, end, wave_end;
     __device__ __forceinline__ RowRange(const Shape& shape, const Span& rows, const Span& keys, int row0, int row) {
         const int shift = keys.size - rows.size + 1;
         const int last = row0 + kRowTile < rows.size ? row0 + kRowTile - 1 : rows.size - 1;
@@ -83,6 +83,9 @@ struct RowRange {
         count = seen(row);
         full = seen(row0);
         end = seen(last);
+        const int wave_row0 = row0 + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave) * kRowsPerWave;
+        const int wave_last = wave_row0 + kRowsPerWave - 1;
+        wave_end = wave_row0 < rows.size ? seen(wave_last < last ? wave_last : last) : 0;
     }
 };
 
@@ -120,9 +123,9 @@ __global__ __launch_bounds__(kBlock, 2) void attention_packed_kernel(Rows q, Row
     RowState<DP> state = {};
     state.top = -INFINITY;
     forward_keys<T, DP>(state, k_even, v_even, k_odd, v_odd,
-                        PackedRows<DP, kKeyTile>{k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim},
-                        PackedRows<DP, kKeyTile>{v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim}, qf, c, 0,
-                        range.end, range.full, [&](int k0) { return first_keys(range.count, k0); });
+                        PackedRows<DP, kKeyTile>(k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim),
+                        PackedRows<DP, kKeyTile>(v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim), qf, c, 0,
+                        range.end, range.wave_end, range.full, [&](int k0) { return first_keys(range.count, k0); });
     const float total = halves_sum(state.total);
     if (!there) return;
     store_row<T, DP>(out, rows.begin + row, head, state.acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
@@ -196,13 +199,14 @@ __global__ __launch_bounds__(kBlock, 2) void attention_dq_kernel(Rows q, Rows k,
     const float delta = there ? stats[static_cast<int64_t>(shape.q_heads) * shape.q_tokens + stat] : 0.f;
     for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile>(tile, shape.dim);
     F32x16 acc[DP / 32] = {};
-    const PackedRows<DP, kKeyTile> key_rows{k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim};
-    const PackedRows<DP, kKeyTile> value_rows{v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim};
+    const PackedRows<DP, kKeyTile> key_rows(k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim);
+    const PackedRows<DP, kKeyTile> value_rows(v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim);
     const auto load = [&](char* k_tile, char* v_tile, int k0) {
         key_rows.load(k_tile, k0);
         value_rows.load(v_tile, k0);
     };
     const auto step = [&](const char* k_tile, const char* v_tile, int k0) {
+        if (k0 >= range.wave_end) return;
 #pragma unroll
         for (int b = 0; b < kKeyTile / 32; ++b) {
             F32x16 s = {}, dp = {};
@@ -264,6 +268,8 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, R
     const int first = shape.causal && key - shift > 0 ? key - shift : 0;
     int start = shape.causal && key0 - shift > 0 ? key0 - shift : 0;
     start -= start % kQueryTile;
+    const int wave_key0 = key0 + __builtin_amdgcn_readfirstlane(wave) * kRowsPerWave;
+    const int wave_start = wave_key0 >= keys.size ? rows.size : shape.causal ? wave_key0 - shift : 0;
     const int full = shape.causal && key0 + kRowTile - 1 - shift > 0 ? key0 + kRowTile - 1 - shift : 0;
     const float c = shape.scale * kLog2e;
 
@@ -272,21 +278,32 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, R
     load_row<DP>(vf, v, keys.begin + key, kv_head, there, shape.dim);
     for (char* tile : {q_even, o_even, q_odd, o_odd}) clear_past<DP, kQueryTile>(tile, shape.dim);
     F32x16 dk_acc[DP / 32] = {}, dv_acc[DP / 32] = {};
-    // The tiles of all heads of the group in one sequence: tile x is rows of head x / per.
+    // The tiles of all heads of the group, one after another.
     const int per = rows.size > start ? (rows.size - start + kQueryTile - 1) / kQueryTile : 0;
-    const auto load = [&](char* q_tile, char* o_tile, float* s_tile, int x) {
-        const int head = kv_head * group + x / per, r0 = start + x % per * kQueryTile;
-        PackedRows<DP, kQueryTile>{q.at(rows.begin, head), q.token_bytes, rows.size, shape.dim}.load(q_tile, r0);
-        PackedRows<DP, kQueryTile>{dout.at(rows.begin, head), dout.token_bytes, rows.size, shape.dim}.load(o_tile, r0);
+    PackedRows<DP, kQueryTile> q_rows(q.at(rows.begin, kv_head * group), q.token_bytes, rows.size, shape.dim);
+    PackedRows<DP, kQueryTile> o_rows(dout.at(rows.begin, kv_head * group), dout.token_bytes, rows.size, shape.dim);
+    const float* s_rows = stats + (static_cast<int64_t>(half) * shape.q_heads + kv_head * group) * shape.q_tokens + rows.begin;
+    int load_row0 = start, step_row0 = start;
+    const auto load = [&](char* q_tile, char* o_tile, float* s_tile) {
+        q_rows.load(q_tile, load_row0);
+        o_rows.load(o_tile, load_row0);
         if (wave == 0) {
-            const int row = r0 + lane % 32 < rows.size ? r0 + lane % 32 : rows.size - 1;
-            const float* from = stats + (static_cast<int64_t>(half) * shape.q_heads + head) * shape.q_tokens + rows.begin + row;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(from),
+            const int row = load_row0 + lane % 32 < rows.size ? load_row0 + lane % 32 : rows.size - 1;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(s_rows + row),
                                              (__attribute__((address_space(3))) uint32_t*)(s_tile), 4, 0, 0);
         }
+        load_row0 += kQueryTile;
+        if (load_row0 >= rows.size) {
+            load_row0 = start;
+            q_rows.base += q.head_bytes;
+            o_rows.base += dout.head_bytes;
+            s_rows += shape.q_tokens;
+        }
     };
-    const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile, int x) {
-        const int r0 = start + x % per * kQueryTile;
+    const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile) {
+        const int r0 = step_row0;
+        step_row0 = step_row0 + kQueryTile < rows.size ? step_row0 + kQueryTile : start;
+        if (r0 + kQueryTile <= wave_start) return;
         F32x16 s = {}, dp = {};
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) {
@@ -323,8 +340,8 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, R
             }
         }
     };
-    pass_tiles<1>(0, per * group, [&](int x) { load(q_even, o_even, s_even, x); }, [&](int x) { load(q_odd, o_odd, s_odd, x); },
-                  [&](int x) { step(q_even, o_even, s_even, x); }, [&](int x) { step(q_odd, o_odd, s_odd, x); });
+    pass_tiles<1>(0, per * group, [&](int) { load(q_even, o_even, s_even); }, [&](int) { load(q_odd, o_odd, s_odd); },
+                  [&](int) { step(q_even, o_even, s_even); }, [&](int) { step(q_odd, o_odd, s_odd); });
     if (!there) return;
     store_row<T, DP>(dk, keys.begin + key, kv_head, dk_acc, shape.scale, shape.dim);
     store_row<T, DP>(dv, keys.begin + key, kv_head, dv_acc, 1.f, shape.dim);
@@ -344,6 +361,10 @@ int check_shape(const char* what, uint32_t sequences, uint64_t q_tokens, uint64_
     if (!(scale > 0.f) || scale == INFINITY) return set_error(kInvalidArgument, "%s: the scale must be positive and finite", what);
     return kOk;
 }
+
+// A tile's bytes fit 31 bits.
+bool too_wide(const lcpp_hip_rows* r) { return r != nullptr && r->token_stride >= 1 << 24; }
+int refuse_wide(const char* what) { return set_error(kUnsupported, "%s: token strides must be below 2^24 items", what); }
 
 // Tiles that a ragged batch may have, and the launch over (tile, head).
 int check_grid(const char* what, uint64_t tokens, uint32_t sequences, uint32_t heads, unsigned& tiles, unsigned& grid) {
@@ -365,6 +386,7 @@ int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* 
     if (!q_offsets || !k_offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
     if (!usable(q) || !usable(out) || (k_tokens && (!usable(k) || !usable(v))))
         return unusable(what);
+    if (k_tokens && (too_wide(k) || too_wide(v))) return refuse_wide(what);
     unsigned tiles, grid;
     if (int st = check_grid(what, q_tokens, sequences, q_heads, tiles, grid); st != kOk) return st;
     const Shape shape{static_cast<int>(sequences), static_cast<int>(q_tokens), static_cast<int>(k_tokens),
@@ -372,7 +394,7 @@ int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* 
     const Rows none{nullptr, 0, 0};
     const Rows kr = k_tokens ? rows_of(k) : none, vr = k_tokens ? rows_of(v) : none;
     LaunchScope scope("attention_packed", stream);
-    auto* kernel = dim <= 64 ? attention_packed_kernel<T, 64> : attention_packed_kernel<T, 128>;
+    auto* kernel = dim <= 64 ? attention_packed_kernel<T, 64> : dim <= 96 ? attention_packed_kernel<T, 96> : attention_packed_kernel<T, 128>;
     kernel<<<grid, kBlock, 0, stream>>>(rows_of(q), kr, vr, rows_of(out), lse, q_offsets, k_offsets, shape, tiles);
     return check_hip(hipGetLastError(), "attention_packed launch");
 }
@@ -396,6 +418,7 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
         return unusable(what);
     if (temp_bytes < backward_bytes(q_tokens, q_heads) || (q_tokens && !temp))
         return set_error(kTempTooSmall, "%s: temp storage too small", what);
+    if ((k_tokens && (too_wide(k) || too_wide(v))) || (q_tokens && (too_wide(q) || too_wide(dout)))) return refuse_wide(what);
     unsigned tiles, grid, key_tiles, key_grid;
     if (int st = check_grid(what, q_tokens, sequences, q_heads, tiles, grid); st != kOk) return st;
     if (int st = check_grid(what, k_tokens, sequences, kv_heads, key_tiles, key_grid); st != kOk) return st;
@@ -415,13 +438,13 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
     }
     if (k_tokens) {
         LaunchScope scope("attention_dkv", stream);
-        auto* kernel = dim <= 64 ? attention_dkv_kernel<T, 64> : attention_dkv_kernel<T, 128>;
+        auto* kernel = dim <= 64 ? attention_dkv_kernel<T, 64> : dim <= 96 ? attention_dkv_kernel<T, 96> : attention_dkv_kernel<T, 128>;
         kernel<<<key_grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dk), rows_of(dv), stats, q_offsets, k_offsets, shape);
         if (int st = check_hip(hipGetLastError(), "attention_dkv launch"); st != kOk) return st;
     }
     if (q_tokens) {
         LaunchScope scope("attention_dq", stream);
-        auto* kernel = dim <= 64 ? attention_dq_kernel<T, 64> : attention_dq_kernel<T, 128>;
+        auto* kernel = dim <= 64 ? attention_dq_kernel<T, 64> : dim <= 96 ? attention_dq_kernel<T, 96> : attention_dq_kernel<T, 128>;
         kernel<<<grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dq), stats, q_offsets, k_offsets, shape, tiles);
         return check_hip(hipGetLastError(), "attention_dq launch");
     }

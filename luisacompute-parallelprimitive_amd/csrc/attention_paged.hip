@@ -335,7 +335,7 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
     float* part_out = parts > 1 ? reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(parts, q_tokens * q_heads)) : nullptr;
     {
         LaunchScope scope("attention_paged", stream);
-        auto* kernel = dim <= 64 ? attention_paged_kernel<T, 64> : attention_paged_kernel<T, 128>;
+        auto* kernel = dim <= 64 ? attention_paged_kernel<T, 64> : dim <= 96 ? attention_paged_kernel<T, 96> : attention_paged_kernel<T, 128>;
         kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), kBlock, 0, stream>>>(
             rows_of(q), pages_of(key_cache), pages_of(value_cache), rows_of(out), lse, part_out, part_stats, block_table,
             q_offsets, kv_lengths, tree, p);
