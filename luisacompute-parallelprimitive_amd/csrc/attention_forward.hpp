@@ -19,18 +19,19 @@ constexpr int kKeyTile = 64;                     // keys in LDS at a time
 // of 2): weights are then at most 2^8, within the 16-bit types, and the products are rescaled a few times a row at most.
 constexpr float kSlack = 8.f;
 
-// Direct loads of a tile, a block of rows each: a lane's chunk is the same in all of them, and its row goes up by kRowStep.
+// Direct loads of a tile by four waves, a block of rows each: a lane's chunk is the same in all of them, and its row goes up
+// by kRowStep.
 template <int DP, int ROWS>
 struct TileLoads {
     static constexpr int kRowStep = kWaves * Tile<DP>::kBlockRows;
     static constexpr int kPerWave = ROWS / kRowStep;
     static_assert(kPerWave > 0 && ROWS % kRowStep == 0);
     __device__ __forceinline__ static int row() {
-        return threadIdx.x / kWave * Tile<DP>::kBlockRows + Tile<DP>::lane_row(threadIdx.x % kWave);
+        return threadIdx.x % kBlock / kWave * Tile<DP>::kBlockRows + Tile<DP>::lane_row(threadIdx.x % kWave);
     }
     __device__ __forceinline__ static int chunk() { return Tile<DP>::lane_chunk(threadIdx.x % kWave); }
     __device__ __forceinline__ static char* place(char* tile, int i) {
-        return tile + (i * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x / kWave)) * Tile<DP>::kBlockBytes;
+        return tile + (i * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x % kBlock / kWave)) * Tile<DP>::kBlockBytes;
     }
 };
 
@@ -63,9 +64,9 @@ struct PackedRows {
         : base(first), token_bytes(bytes), size(rows),
           offset(static_cast<uint32_t>(Loads::row()) * static_cast<uint32_t>(bytes) + Loads::chunk() * 16u),
           has(Loads::chunk() * 8 < dim) {}
-    __device__ __forceinline__ void load(char* tile, int row0) const {
+    __device__ __forceinline__ void load(char* tile, int row0, int64_t more = 0) const {
         if (!has) return;
-        const char* from = base + row0 * token_bytes;
+        const char* from = base + more + row0 * token_bytes;
         if (row0 + ROWS <= size) {
 #pragma unroll
             for (int i = 0; i < Loads::kPerWave; ++i)

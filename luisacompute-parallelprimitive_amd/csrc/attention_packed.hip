@@ -237,21 +237,34 @@ __global__ __launch_bounds__(kBlock, 2) void attention_dq_kernel(Rows q, Rows k,
 }
 
 // dK and dV of a tile of keys of one key head: the rows of every query head of its group pass by, so that the sum
-// over the group is taken in registers and in one order.
+// over the group is taken in registers and in one order.  The tiles of rows, of one head after the other, are dealt to two
+// teams of four waves, which hold the same keys and add their sums at the end: a tile of keys that many rows see is done
+// sooner, and each of a SIMD's two waves has products to run while the other's exponentials do.  Where there are few tiles
+// of keys, the rows are split further over `parts` workgroups, whose sums go to memory in 32 bits.
 constexpr int kQueryTile = 32;
+constexpr int kTeams = 2;
+
+struct RowTiles {  // of one team: which head of the group, which row
+    int head, row0, start, size;
+    __device__ __forceinline__ void skip(int count) {
+        for (row0 += count * kQueryTile; row0 >= size; row0 -= round()) ++head;
+    }
+    __device__ __forceinline__ int round() const { return (size - start + kQueryTile - 1) / kQueryTile * kQueryTile; }
+};
 
 template <typename T, int DP>
-__global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, Rows v, Rows dout, Rows dk, Rows dv,
-                                                                  const float* __restrict__ stats,
-                                                                  const int32_t* __restrict__ q_offsets,
-                                                                  const int32_t* __restrict__ k_offsets, Shape shape) {
+__global__ __launch_bounds__(kTeams* kBlock, 2) void attention_dkv_kernel(Rows q, Rows k, Rows v, Rows dout, Rows dk, Rows dv,
+                                                                          const float* __restrict__ stats, float* __restrict__ part_sums,
+                                                                          const int32_t* __restrict__ q_offsets,
+                                                                          const int32_t* __restrict__ k_offsets, Shape shape) {
     constexpr int kTileBytes = Tile<DP>::bytes(kQueryTile);
-    __shared__ __attribute__((aligned(16))) char q_even[kTileBytes];
-    __shared__ __attribute__((aligned(16))) char o_even[kTileBytes];
-    __shared__ __attribute__((aligned(16))) char q_odd[kTileBytes];
-    __shared__ __attribute__((aligned(16))) char o_odd[kTileBytes];
-    __shared__ __attribute__((aligned(16))) float s_even[2 * kQueryTile];
-    __shared__ __attribute__((aligned(16))) float s_odd[2 * kQueryTile];
+    __shared__ __attribute__((aligned(16))) char q_even[kTeams][kTileBytes];
+    __shared__ __attribute__((aligned(16))) char o_even[kTeams][kTileBytes];
+    __shared__ __attribute__((aligned(16))) char q_odd[kTeams][kTileBytes];
+    __shared__ __attribute__((aligned(16))) char o_odd[kTeams][kTileBytes];
+    __shared__ __attribute__((aligned(16))) float s_even[kTeams][2 * kQueryTile];
+    __shared__ __attribute__((aligned(16))) float s_odd[kTeams][2 * kQueryTile];
+    __shared__ F32x4 join[DP / 8][kBlock];
     const int kv_head = blockIdx.x % shape.kv_heads;
     const TilePlace place = find_tile(k_offsets, shape.sequences, 1, kRowTile, static_cast<int>(blockIdx.x / shape.kv_heads));
     if (place.sequence < 0) return;
@@ -260,7 +273,9 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, R
     if (key0 >= keys.size) return;
     const Span rows = span_of(q_offsets, place.sequence, shape.q_tokens);
     const int group = shape.q_heads / shape.kv_heads;
-    const int lane = threadIdx.x % kWave, half = lane / 32, wave = threadIdx.x / kWave;
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x % kBlock / kWave);
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / kBlock);
     const int key = key0 + wave * kRowsPerWave + lane % 32;
     const bool there = key < keys.size;
     const int shift = keys.size - rows.size;
@@ -268,41 +283,40 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, R
     const int first = shape.causal && key - shift > 0 ? key - shift : 0;
     int start = shape.causal && key0 - shift > 0 ? key0 - shift : 0;
     start -= start % kQueryTile;
-    const int wave_key0 = key0 + __builtin_amdgcn_readfirstlane(wave) * kRowsPerWave;
-    const int wave_start = wave_key0 >= keys.size ? rows.size : shape.causal ? wave_key0 - shift : 0;
     const int full = shape.causal && key0 + kRowTile - 1 - shift > 0 ? key0 + kRowTile - 1 - shift : 0;
+    const int wave_key0 = key0 + wave * kRowsPerWave;
+    const int wave_start = wave_key0 >= keys.size ? rows.size : shape.causal ? wave_key0 - shift : 0;
     const float c = shape.scale * kLog2e;
 
     U32x4 kf[DP / 16], vf[DP / 16];
     load_row<DP>(kf, k, keys.begin + key, kv_head, there, shape.dim);
     load_row<DP>(vf, v, keys.begin + key, kv_head, there, shape.dim);
-    for (char* tile : {q_even, o_even, q_odd, o_odd}) clear_past<DP, kQueryTile>(tile, shape.dim);
+    for (auto* tile : {q_even, o_even, q_odd, o_odd}) clear_past<DP, kQueryTile>(tile[team], shape.dim);
     F32x16 dk_acc[DP / 32] = {}, dv_acc[DP / 32] = {};
-    // The tiles of all heads of the group, one after another.
-    const int per = rows.size > start ? (rows.size - start + kQueryTile - 1) / kQueryTile : 0;
-    PackedRows<DP, kQueryTile> q_rows(q.at(rows.begin, kv_head * group), q.token_bytes, rows.size, shape.dim);
-    PackedRows<DP, kQueryTile> o_rows(dout.at(rows.begin, kv_head * group), dout.token_bytes, rows.size, shape.dim);
-    const float* s_rows = stats + (static_cast<int64_t>(half) * shape.q_heads + kv_head * group) * shape.q_tokens + rows.begin;
-    int load_row0 = start, step_row0 = start;
-    const auto load = [&](char* q_tile, char* o_tile, float* s_tile) {
-        q_rows.load(q_tile, load_row0);
-        o_rows.load(o_tile, load_row0);
+    const int all = rows.size > start ? (rows.size - start + kQueryTile - 1) / kQueryTile * group : 0;
+    const int per = (all + static_cast<int>(gridDim.y) - 1) / static_cast<int>(gridDim.y);
+    const int from = static_cast<int>(blockIdx.y) * per, to = from + per < all ? from + per : all;
+    RowTiles loads{kv_head * group, start, start, rows.size}, steps = loads;
+    if (from < to) loads.skip(from + team), steps.skip(from + team);
+    const PackedRows<DP, kQueryTile> q_rows(q.at(rows.begin, 0), q.token_bytes, rows.size, shape.dim);
+    const PackedRows<DP, kQueryTile> o_rows(dout.at(rows.begin, 0), dout.token_bytes, rows.size, shape.dim);
+    const float* s_rows = stats + static_cast<int64_t>(half) * shape.q_heads * shape.q_tokens + rows.begin;
+    const auto load = [&](char* q_tile, char* o_tile, float* s_tile, int at) {
+        if (at + team >= to) return;
+        q_rows.load(q_tile, loads.row0, loads.head * q.head_bytes);
+        o_rows.load(o_tile, loads.row0, loads.head * dout.head_bytes);
         if (wave == 0) {
-            const int row = load_row0 + lane % 32 < rows.size ? load_row0 + lane % 32 : rows.size - 1;
-            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(s_rows + row),
+            const int row = loads.row0 + lane % 32 < rows.size ? loads.row0 + lane % 32 : rows.size - 1;
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(
+                                                 s_rows + static_cast<int64_t>(loads.head) * shape.q_tokens + row),
                                              (__attribute__((address_space(3))) uint32_t*)(s_tile), 4, 0, 0);
         }
-        load_row0 += kQueryTile;
-        if (load_row0 >= rows.size) {
-            load_row0 = start;
-            q_rows.base += q.head_bytes;
-            o_rows.base += dout.head_bytes;
-            s_rows += shape.q_tokens;
-        }
+        loads.skip(kTeams);
     };
-    const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile) {
-        const int r0 = step_row0;
-        step_row0 = step_row0 + kQueryTile < rows.size ? step_row0 + kQueryTile : start;
+    const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile, int at) {
+        if (at + team >= to) return;
+        const int r0 = steps.row0;
+        steps.skip(kTeams);
         if (r0 + kQueryTile <= wave_start) return;
         F32x16 s = {}, dp = {};
 #pragma unroll
@@ -340,11 +354,72 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_kernel(Rows q, Rows k, R
             }
         }
     };
-    pass_tiles<1>(0, per * group, [&](int) { load(q_even, o_even, s_even); }, [&](int) { load(q_odd, o_odd, s_odd); },
-                  [&](int) { step(q_even, o_even, s_even); }, [&](int) { step(q_odd, o_odd, s_odd); });
-    if (!there) return;
-    store_row<T, DP>(dk, keys.begin + key, kv_head, dk_acc, shape.scale, shape.dim);
-    store_row<T, DP>(dv, keys.begin + key, kv_head, dv_acc, 1.f, shape.dim);
+    pass_tiles<kTeams>(from, to, [&](int x) { load(q_even[team], o_even[team], s_even[team], x); },
+                       [&](int x) { load(q_odd[team], o_odd[team], s_odd[team], x); },
+                       [&](int x) { step(q_even[team], o_even[team], s_even[team], x); },
+                       [&](int x) { step(q_odd[team], o_odd[team], s_odd[team], x); });
+    // The first team ends with dK, the second with dV; each hands the other its share.
+    const int mate = threadIdx.x % kBlock;
+    const auto give = [&](const F32x16(&acc)[DP / 32]) {
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i)
+            join[i][mate] = F32x4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]};
+    };
+    const auto take = [&](F32x16(&acc)[DP / 32]) {
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            const F32x4 other = join[i][mate];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i / 4][4 * (i % 4) + j] += other[j];
+        }
+    };
+    const auto store = [&](const Rows& dst, const F32x16(&acc)[DP / 32], float factor, int which) {
+        if (!there) return;
+        if (gridDim.y == 1) {
+            store_row<T, DP>(dst, keys.begin + key, kv_head, acc, factor, shape.dim);
+            return;
+        }
+        const int64_t row = (static_cast<int64_t>(blockIdx.y) * 2 + which) * shape.k_tokens * shape.kv_heads +
+                            static_cast<int64_t>(keys.begin + key) * shape.kv_heads + kv_head;
+#pragma unroll
+        for (int i = 0; i < DP / 8; ++i) {
+            const int d = 8 * i + 4 * half;
+            if (d < shape.dim)
+                *reinterpret_cast<F32x4*>(part_sums + row * shape.dim + d) =
+                    F32x4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]} * factor;
+        }
+    };
+    if (team == 1) give(dk_acc);
+    __syncthreads();
+    if (team == 0) {
+        take(dk_acc);
+        store(dk, dk_acc, shape.scale, 0);
+    }
+    __syncthreads();
+    if (team == 0) give(dv_acc);
+    __syncthreads();
+    if (team == 1) {
+        take(dv_acc);
+        store(dv, dv_acc, 1.f, 1);
+    }
+}
+
+// Adds the parts of dK and dV, in the parts' order: a thread per four items.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void attention_dkv_join_kernel(Rows dk, Rows dv, const float* __restrict__ part_sums, int parts,
+                                                                    const int32_t* __restrict__ k_offsets, Shape shape) {
+    const int quads = shape.dim / 4;
+    const int64_t rows = static_cast<int64_t>(shape.k_tokens) * shape.kv_heads;
+    const int64_t at = static_cast<int64_t>(blockIdx.x) * kBlock + threadIdx.x;
+    if (at >= rows * quads) return;
+    const int64_t row = at / quads, token = row / shape.kv_heads;
+    if (token < k_offsets[0] || token >= k_offsets[shape.sequences]) return;
+    const int head = static_cast<int>(row % shape.kv_heads), quad = static_cast<int>(at % quads);
+    const float* from = part_sums + (blockIdx.y * rows + row) * shape.dim + quad * 4;
+    F32x4 sum = {};
+    for (int i = 0; i < parts; ++i) sum += *reinterpret_cast<const F32x4*>(from + 2 * i * rows * shape.dim);
+    const Rows& dst = blockIdx.y == 0 ? dk : dv;
+    *reinterpret_cast<U32x2*>(dst.at(token, head) + quad * 8) = U32x2{pack2<T>(sum[0], sum[1]), pack2<T>(sum[2], sum[3])};
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
@@ -369,7 +444,7 @@ int refuse_wide(const char* what) { return set_error(kUnsupported, "%s: token st
 // Tiles that a ragged batch may have, and the launch over (tile, head).
 int check_grid(const char* what, uint64_t tokens, uint32_t sequences, uint32_t heads, unsigned& tiles, unsigned& grid) {
     const uint64_t t = tokens / kRowTile + sequences;
-    if (t * heads > 0x7FFFFFFFull / kBlock) return set_error(kInvalidArgument, "%s: too many tiles", what);
+    if (t * heads > 0x7FFFFFFFull / (kTeams * kBlock)) return set_error(kInvalidArgument, "%s: too many tiles", what);
     tiles = static_cast<unsigned>(t);
     grid = static_cast<unsigned>(t * heads);
     return kOk;
@@ -399,7 +474,28 @@ int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* 
     return check_hip(hipGetLastError(), "attention_packed launch");
 }
 
-size_t backward_bytes(uint64_t q_tokens, uint32_t q_heads) { return align_up(q_tokens * q_heads * 2 * sizeof(float), kViewAlign); }
+// Workgroups that share a tile of keys: as many as fill the device (512 waves' worth of workgroups are resident at two a
+// SIMD), while each still has a few tiles of rows.
+constexpr uint64_t kKeyGrid = 256;
+constexpr uint64_t kLeastSteps = 8;
+
+uint64_t key_parts(uint64_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint64_t q_heads, uint64_t kv_heads) {
+    if (sequences == 0 || kv_heads == 0) return 1;
+    // Tiles of keys that there are about, and steps that each has: its sequence's rows for every head of the group.
+    const uint64_t tiles = (k_tokens / kRowTile > sequences ? k_tokens / kRowTile : sequences) * kv_heads;
+    const uint64_t steps = ceil_div(q_tokens / sequences, kQueryTile) * (q_heads / kv_heads);
+    const uint64_t wanted = kKeyGrid / tiles, most = steps / kLeastSteps;
+    const uint64_t parts = wanted < most ? wanted : most;
+    return parts > 1 ? parts : 1;
+}
+
+size_t stats_bytes(uint64_t q_tokens, uint64_t q_heads) { return align_up(q_tokens * q_heads * 2 * sizeof(float), kViewAlign); }
+
+size_t backward_bytes(uint64_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint64_t q_heads, uint64_t kv_heads, uint64_t dim) {
+    const uint64_t parts = key_parts(sequences, q_tokens, k_tokens, q_heads, kv_heads);
+    return stats_bytes(q_tokens, q_heads) +
+           (parts > 1 ? align_up(parts * 2 * k_tokens * kv_heads * dim * sizeof(float), kViewAlign) : 0);
+}
 
 template <typename T>
 int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* v,
@@ -411,12 +507,14 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     if (int st = check_shape(what, sequences, q_tokens, k_tokens, q_heads, kv_heads, dim, scale); st != kOk) return st;
     if (sequences == 0 || (q_tokens == 0 && k_tokens == 0)) return kOk;
+    if (q_tokens * (q_heads / kv_heads) > 0x7FFFFFFFull) return set_error(kInvalidArgument, "%s: too many tokens or sequences", what);
     if (!q_offsets || !k_offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
     if (q_tokens && (!usable(q) || !usable(out) || !usable(dout) || !usable(dq) || !lse))
         return unusable(what);
     if (k_tokens && (!usable(k) || !usable(v) || !usable(dk) || !usable(dv)))
         return unusable(what);
-    if (temp_bytes < backward_bytes(q_tokens, q_heads) || (q_tokens && !temp))
+    const size_t needed = backward_bytes(sequences, q_tokens, k_tokens, q_heads, kv_heads, dim);
+    if (temp_bytes < needed || (needed && !temp))
         return set_error(kTempTooSmall, "%s: temp storage too small", what);
     if ((k_tokens && (too_wide(k) || too_wide(v))) || (q_tokens && (too_wide(q) || too_wide(dout)))) return refuse_wide(what);
     unsigned tiles, grid, key_tiles, key_grid;
@@ -439,8 +537,19 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
     if (k_tokens) {
         LaunchScope scope("attention_dkv", stream);
         auto* kernel = dim <= 64 ? attention_dkv_kernel<T, 64> : dim <= 96 ? attention_dkv_kernel<T, 96> : attention_dkv_kernel<T, 128>;
-        kernel<<<key_grid, kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dk), rows_of(dv), stats, q_offsets, k_offsets, shape);
+        const unsigned parts = static_cast<unsigned>(key_parts(sequences, q_tokens, k_tokens, q_heads, kv_heads));
+        float* part_sums = reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(q_tokens, q_heads));
+        kernel<<<dim3(key_grid, parts), kTeams * kBlock, 0, stream>>>(qr, kr, vr, dor, rows_of(dk), rows_of(dv), stats, part_sums,
+                                                                      q_offsets, k_offsets, shape);
         if (int st = check_hip(hipGetLastError(), "attention_dkv launch"); st != kOk) return st;
+        if (parts > 1) {
+            const uint64_t blocks = ceil_div(k_tokens * kv_heads * (dim / 4), kBlock);
+            if (blocks > 0x7FFFFFFFull / kBlock) return set_error(kInvalidArgument, "%s: too many rows", what);
+            LaunchScope join_scope("attention_dkv_join", stream);
+            attention_dkv_join_kernel<T><<<dim3(static_cast<unsigned>(blocks), 2), kBlock, 0, stream>>>(
+                rows_of(dk), rows_of(dv), part_sums, static_cast<int>(parts), k_offsets, shape);
+            if (int st = check_hip(hipGetLastError(), "attention_dkv_join launch"); st != kOk) return st;
+        }
     }
     if (q_tokens) {
         LaunchScope scope("attention_dq", stream);
@@ -467,8 +576,7 @@ size_t lcpp_hip_attention_packed_temp_bytes(uint32_t sequences, uint64_t q_token
 
 size_t lcpp_hip_attention_packed_backward_temp_bytes(uint32_t sequences, uint64_t q_tokens, uint64_t k_tokens, uint32_t q_heads,
                                                      uint32_t kv_heads, uint32_t head_dim) {
-    (void)sequences, (void)k_tokens, (void)kv_heads, (void)head_dim;
-    return attention::backward_bytes(q_tokens, q_heads);
+    return attention::backward_bytes(sequences, q_tokens, k_tokens, q_heads, kv_heads, head_dim);
 }
 
 #define LCPP_HIP_DEFINE_ATTENTION(S, T)                                                                                     \
