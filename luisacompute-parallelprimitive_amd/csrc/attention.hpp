@@ -192,23 +192,27 @@ struct TilePlace {
     int tile;
 };
 
-__device__ __forceinline__ TilePlace find_tile(const int32_t* offsets, int count, int scale, int size, int number) {
+// The last of `count` ascending numbers that is not above `number` (-1: none): a wave tests 64 at a time.
+template <typename Key>
+__device__ __forceinline__ int find_last(int count, int64_t number, Key key) {
     const int lane = threadIdx.x % kWave;
     int low = 0, high = count;
     while (high - low > 0) {
         const int step = (high - low + kWave - 1) / kWave;
         const int at = low + lane * step;
-        bool below = false;
-        if (at < high) below = static_cast<int64_t>(offsets[at]) * scale / size + at <= number;
-        const int passed = __popcll(wave_ballot(below));
-        if (passed == 0) return {-1, 0};
+        const int passed = __popcll(wave_ballot(at < high && key(at) <= number));
+        if (passed == 0) return -1;
         low += (passed - 1) * step;
         if (step == 1) break;
         high = low + step < high ? low + step : high;
     }
-    low = __builtin_amdgcn_readfirstlane(low);
-    const int first = static_cast<int>(static_cast<int64_t>(offsets[low]) * scale / size) + low;
-    return {low, number - first};
+    return __builtin_amdgcn_readfirstlane(low);
+}
+
+__device__ __forceinline__ TilePlace find_tile(const int32_t* offsets, int count, int scale, int size, int number) {
+    const auto first = [&](int b) { return static_cast<int64_t>(offsets[b]) * scale / size + b; };
+    const int owner = find_last(count, number, first);
+    return {owner, owner < 0 ? 0 : number - static_cast<int>(first(owner))};
 }
 
 }  // namespace attention

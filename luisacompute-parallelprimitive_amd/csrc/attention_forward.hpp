@@ -98,6 +98,38 @@ __device__ __forceinline__ uint32_t first_keys(int count, int k0) {
     return n >= 32 ? ~0u : n <= 0 ? 0u : (1u << n) - 1u;
 }
 
+// Writes column `lane % 32` of a transposed result (rows are items of the head) times `factor`.
+template <typename T, int DP>
+__device__ __forceinline__ void store_row(const Rows& dst, int64_t token, int head, const F32x16 (&acc)[DP / 32], float factor,
+                                          int dim) {
+    const int half = threadIdx.x % kWave / 32;
+    char* row = dst.at(token, head);
+#pragma unroll
+    for (int b = 0; b < DP / 32; ++b) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int d = b * 32 + 8 * g + 4 * half;
+            if (d >= dim) continue;
+            const U32x2 v = {pack2<T>(acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor),
+                             pack2<T>(acc[b][4 * g + 2] * factor, acc[b][4 * g + 3] * factor)};
+            *reinterpret_cast<U32x2*>(row + d * 2) = v;
+        }
+    }
+}
+
+// Moves the row's scale up to `high`, the largest score of the coming keys, where that has outgrown it.
+template <int DP>
+__device__ __forceinline__ void rescale(RowState<DP>& state, float high, float c) {
+    const bool outgrown = (high - state.top) * c > kSlack;  // (from -inf: yes, unless the row still sees nothing)
+    if (wave_ballot(outgrown) == 0) return;
+    const float top = outgrown ? high : state.top;
+    const float alpha = outgrown ? exp2_fast((state.top - top) * c) : 1.f;
+    state.top = top;
+    state.total *= alpha;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d) state.acc[d] *= alpha;
+}
+
 // One tile of keys.  `seen(k0)`: the 32 keys from k0 on that the lane's row sees, as bits; `masked`: some row of the
 // workgroup does not see all of the tile.
 template <typename T, int DP, typename Seen>
@@ -123,16 +155,7 @@ __device__ __forceinline__ void forward_tile(RowState<DP>& state, const char* k_
     for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
         for (int r = 0; r < 16; ++r) high = fmaxf(high, s[b][r]);
-    high = halves_max(high);
-    const bool outgrown = (high - state.top) * c > kSlack;  // (from -inf: yes, unless the row still sees nothing)
-    if (wave_ballot(outgrown) != 0) {
-        const float top = outgrown ? high : state.top;
-        const float alpha = outgrown ? exp2_fast((state.top - top) * c) : 1.f;
-        state.top = top;
-        state.total *= alpha;
-#pragma unroll
-        for (int d = 0; d < DP / 32; ++d) state.acc[d] *= alpha;
-    }
+    rescale(state, halves_max(high), c);
     const float base = state.top == -INFINITY ? 0.f : state.top * c;
     float sum = 0.f;
 #pragma unroll

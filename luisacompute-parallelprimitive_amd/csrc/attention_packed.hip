@@ -32,45 +32,12 @@ __device__ __forceinline__ Span span_of(const int32_t* offsets, int sequence, in
     return {begin, end - begin};
 }
 
-// Rows [row0, row0 + ROWS) of one head into LDS; zeros for rows from `rows` on.
-template <int DP, int ROWS>
-__device__ __forceinline__ void stage(char* tile, const Rows& src, int64_t token0, int head, int rows, int dim) {
-    constexpr int kChunks = DP / 8;
-#pragma unroll
-    for (int i = 0; i < ROWS * kChunks / kBlock; ++i) {
-        const int at = i * kBlock + threadIdx.x;
-        const int row = at / kChunks, chunk = at % kChunks;
-        const bool there = row < rows;
-        const U32x4 v = load_chunk(src.at(token0 + (there ? row : 0), head), chunk, dim, there);
-        *reinterpret_cast<U32x4*>(tile + Tile<DP>::place(row, chunk)) = v;
-    }
-}
-
 // The calling lane's row as a B operand: column lane % 32, all contraction steps.
 template <int DP>
 __device__ __forceinline__ void load_row(U32x4 (&f)[DP / 16], const Rows& src, int64_t token, int head, bool there, int dim) {
     const char* row = src.at(there ? token : 0, head);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) f[s] = load_chunk(row, 2 * s + threadIdx.x % kWave / 32, dim, there);
-}
-
-// Writes column `lane % 32` of a transposed result (rows are items of the head) times `factor`.
-template <typename T, int DP>
-__device__ __forceinline__ void store_row(const Rows& dst, int64_t token, int head, const F32x16 (&acc)[DP / 32], float factor,
-                                          int dim) {
-    const int half = threadIdx.x % kWave / 32;
-    char* row = dst.at(token, head);
-#pragma unroll
-    for (int b = 0; b < DP / 32; ++b) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-            const int d = b * 32 + 8 * g + 4 * half;
-            if (d >= dim) continue;
-            const U32x2 v = {pack2<T>(acc[b][4 * g] * factor, acc[b][4 * g + 1] * factor),
-                             pack2<T>(acc[b][4 * g + 2] * factor, acc[b][4 * g + 3] * factor)};
-            *reinterpret_cast<U32x2*>(row + d * 2) = v;
-        }
-    }
 }
 
 // Keys that a row sees (the first `count`), that every row of its workgroup sees, and that any does, or any of its wave.

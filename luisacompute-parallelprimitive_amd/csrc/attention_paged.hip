@@ -5,21 +5,20 @@
 // word is set (without a tree: j <= i).  n = 1 is plain decoding.
 //
 // The n * group rows of a request that share a key head are one matrix of rows, so a key is read once for all of them.
-// Reading the cache bounds the call; a workgroup takes 32 rows and a part of the keys, its four waves take 32 keys in
-// turn, each with its own running maximum, sum and products, and join them at the end.
-#include "attention.hpp"
+// Reading the cache bounds the call.  Few rows (attention_paged_kernel): a workgroup takes 32 rows and a part of the
+// keys, its four waves take 32 keys in turn, each with its own running maximum, sum and products, and join them at the end.
+// More (attention_paged_wide_kernel): four waves of 32 rows share tiles of 64 keys, as the packed kernel's do.
+#include "attention_forward.hpp"
 
 namespace lcpp_hip {
 namespace attention {
 namespace {
 
-constexpr int kBlock = 256;
-constexpr int kWaves = kBlock / kWave;
-constexpr int kRowTile = 32;
-constexpr int kKeyTile = 32;                  // keys of a wave at a time
-constexpr int kKeyStep = kWaves * kKeyTile;   // keys of a workgroup at a time
-constexpr int kPartKeys = 256;                // at least so many keys make a part
-constexpr int kGridTarget = 1024;             // workgroups that fill the device
+constexpr int kNarrowRows = 32;
+constexpr int kWaveKeys = 32;                  // keys of a wave at a time
+constexpr int kKeyStep = kWaves * kWaveKeys;   // keys of a workgroup at a time
+constexpr int kPartKeys = 256;                 // at least so many keys make a part
+constexpr int kGridTarget = 1024;              // workgroups that fill the device
 
 struct Paged {
     int requests;
@@ -51,22 +50,27 @@ struct Work {
     int length;   // keys
 };
 
-__device__ __forceinline__ bool find_work(Work& w, const int32_t* q_offsets, const int32_t* kv_lengths, const Paged& p,
-                                          int number) {
-    const int group = p.q_heads / p.kv_heads;
-    const TilePlace place = find_tile(q_offsets, p.requests, group, kRowTile, number);
-    if (place.sequence < 0) return false;
-    int begin = q_offsets[place.sequence], end = q_offsets[place.sequence + 1];
+__device__ __forceinline__ void take_request(Work& w, const int32_t* q_offsets, const int32_t* kv_lengths, const Paged& p,
+                                             int request) {
+    int begin = q_offsets[request], end = q_offsets[request + 1];
     begin = begin < 0 ? 0 : begin > p.q_tokens ? p.q_tokens : begin;
     end = end < begin ? begin : end > p.q_tokens ? p.q_tokens : end;
-    w.request = place.sequence;
+    w.request = request;
     w.token0 = begin;
     w.tokens = end - begin;
-    w.row0 = place.tile * kRowTile;
-    w.rows = w.tokens * group;
+    w.rows = w.tokens * (p.q_heads / p.kv_heads);
     const int64_t most = static_cast<int64_t>(p.table_width) * p.page_size;
-    const int length = kv_lengths[place.sequence];
+    const int length = kv_lengths[request];
     w.length = length < 0 ? 0 : length > most ? static_cast<int>(most) : length;
+}
+
+// Tile `number` of `tile_rows` rows.
+__device__ __forceinline__ bool find_work(Work& w, const int32_t* q_offsets, const int32_t* kv_lengths, const Paged& p,
+                                          int tile_rows, int number) {
+    const TilePlace place = find_tile(q_offsets, p.requests, p.q_heads / p.kv_heads, tile_rows, number);
+    if (place.sequence < 0) return false;
+    take_request(w, q_offsets, kv_lengths, p, place.sequence);
+    w.row0 = place.tile * tile_rows;
     return w.row0 < w.rows;
 }
 
@@ -77,105 +81,153 @@ __device__ __forceinline__ uint32_t seen_word(uint64_t tree, int k0, int ahead) 
     if (shift < 0) return static_cast<uint32_t>(tree << -shift) | ((1u << -shift) - 1u);
     return shift < 64 ? static_cast<uint32_t>(tree >> shift) : 0u;
 }
-__device__ __forceinline__ uint32_t chain_word(int token, int k0, int ahead) {
-    const int count = ahead + token + 1 - k0;  // keys from k0 on that the row sees
-    return count >= 32 ? ~0u : count <= 0 ? 0u : (1u << count) - 1u;
+
+// What the row of a lane is.
+struct PagedRow {
+    bool there;
+    int token, head;  // token of its request
+    uint64_t tree;
+    __device__ __forceinline__ PagedRow(const Work& w, const Paged& p, const uint64_t* words, int kv_head, int row) {
+        const int group = p.q_heads / p.kv_heads;
+        there = row < w.rows;
+        token = there ? row / group : 0;
+        head = kv_head * group + (there ? row % group : 0);
+        tree = words != nullptr && there ? words[w.token0 + token] : 0;
+    }
+    __device__ __forceinline__ uint32_t seen(bool tree_given, int k0, int ahead) const {
+        return tree_given ? seen_word(tree, k0, ahead) : first_keys(ahead + token + 1, k0);
+    }
+};
+
+// 16 bytes of a part's sums, or of the output.
+template <typename T>
+__device__ __forceinline__ void store_items(char* to, const F32x4& a, const F32x4& b, float f) {
+    *reinterpret_cast<U32x4*>(to) = U32x4{pack2<T>(a[0] * f, a[1] * f), pack2<T>(a[2] * f, a[3] * f),
+                                          pack2<T>(b[0] * f, b[1] * f), pack2<T>(b[2] * f, b[3] * f)};
 }
 
+// Where a part's results go, and the row's when one part is all.
+struct Parts {
+    float* out;      // [parts][q_heads][q_tokens][dim], unnormalised
+    F32x2* stats;    // [parts][q_heads][q_tokens]: scale and sum
+    __device__ __forceinline__ int64_t row(const Paged& p, int part, int head, int64_t token) const {
+        return (static_cast<int64_t>(part) * p.q_heads + head) * p.q_tokens + token;
+    }
+};
+
+__device__ __forceinline__ float row_lse(float top, float total, float scale) {
+    return total == 0.f ? -INFINITY : top * scale + __logf(total);
+}
+
+// A lane's key of a tile of 32: both halves of the wave have the same.
+struct KeyPlace {
+    int64_t offset;  // of page and slot in the key cache
+    int64_t value_offset;
+    bool held;
+};
+
 template <typename T, int DP>
-__global__ __launch_bounds__(kBlock) void attention_paged_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
-                                                                 float* __restrict__ lse, float* __restrict__ part_out,
-                                                                 F32x2* __restrict__ part_stats,
-                                                                 const int32_t* __restrict__ block_table,
-                                                                 const int32_t* __restrict__ q_offsets,
-                                                                 const int32_t* __restrict__ kv_lengths,
-                                                                 const uint64_t* __restrict__ tree, Paged p) {
-    constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);
+__global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
+                                                                    float* __restrict__ lse, Parts parts,
+                                                                    const int32_t* __restrict__ block_table,
+                                                                    const int32_t* __restrict__ q_offsets,
+                                                                    const int32_t* __restrict__ kv_lengths,
+                                                                    const uint64_t* __restrict__ tree, Paged p) {
+    constexpr int kTileBytes = Tile<DP>::bytes(kWaveKeys);
     constexpr int kJoinStride = DP + 4;  // floats
-    constexpr int kJoinBytes = kWaves * kRowTile * kJoinStride * 4;
-    __shared__ __attribute__((aligned(16))) char tiles[kWaves * 2 * kTileBytes > kJoinBytes ? kWaves * 2 * kTileBytes : kJoinBytes];
-    __shared__ float stats[2][kWaves][kRowTile];
+    constexpr int kJoinBytes = kWaves * kNarrowRows * kJoinStride * 4;
+    static_assert(kWaves * kTileBytes <= kJoinBytes, "the values' tiles lie where the sums are joined");
+    __shared__ __attribute__((aligned(16))) char tiles[kJoinBytes];
+    __shared__ float stats[2][kWaves][kNarrowRows];
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
-    if (!find_work(w, q_offsets, kv_lengths, p, blockIdx.x / p.kv_heads)) return;
+    if (!find_work(w, q_offsets, kv_lengths, p, kNarrowRows, blockIdx.x / p.kv_heads)) return;
     const int per = part_keys(w.length, p.parts);
-    const int begin = blockIdx.y * per;
-    if (begin >= w.length && blockIdx.y > 0) return;
-    const int end = begin + per < w.length ? begin + per : w.length;
+    const int64_t part_begin = static_cast<int64_t>(blockIdx.y) * per;
+    if (part_begin >= w.length && blockIdx.y > 0) return;
+    const int begin = static_cast<int>(part_begin), end = w.length - begin > per ? begin + per : w.length;
     const bool whole = w.length <= per;
     const int group = p.q_heads / p.kv_heads;
-    const int lane = threadIdx.x % kWave, half = lane / 32, wave = threadIdx.x / kWave;
-    const int row = w.row0 + lane % 32;
-    const bool there = row < w.rows;
-    const int token = there ? row / group : 0;
-    const int head = kv_head * group + (there ? row % group : 0);
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const PagedRow row(w, p, tree, kv_head, w.row0 + lane % 32);
     const int ahead = w.length - w.tokens;
-    const uint64_t word = tree != nullptr && there ? tree[w.token0 + token] : 0;
     const float c = p.scale * kLog2e;
     const int32_t* table = block_table + static_cast<int64_t>(w.request) * p.table_stride;
+    const char* keys = key_cache.at(0, 0, kv_head);
+    const char* values = value_cache.at(0, 0, kv_head);
 
     U32x4 qf[DP / 16];
-    const char* q_row = q.at(w.token0 + token, head);
+    const char* q_row = q.at(w.token0 + row.token, row.head);
 #pragma unroll
-    for (int s = 0; s < DP / 16; ++s) qf[s] = load_chunk(q_row, 2 * s + half, p.dim, there);
-    char* k_tile = tiles + wave * 2 * kTileBytes;
-    char* v_tile = k_tile + kTileBytes;
-    F32x16 acc[DP / 32] = {};
-    float top = -INFINITY, total = 0.f;
-    for (int k0 = begin + wave * kKeyTile; k0 < end; k0 += kKeyStep) {
-        // Lane l < 32 finds the page of key k0 + l.
+    for (int s = 0; s < DP / 16; ++s) qf[s] = load_chunk(q_row, 2 * s + half, p.dim, row.there);
+    char* v_tile = tiles + wave * kTileBytes;
+    // Keys go from the cache into the registers that the products read, values into registers and from there into the
+    // wave's tile: both a tile ahead, the page numbers two.
+    U32x4 kf[DP / 16], vf[DP / 16];
+    const auto page_of = [&](int k0) {
         const int position = k0 + lane % 32;
-        int page = -1;
-        if (position < end) page = table[position / p.page_size];
-        const bool held = page >= 0 && page < p.pages;
-        const int slot = position % p.page_size;
-        const uint32_t held_word = static_cast<uint32_t>(wave_ballot(held));
-        wave_lds_order();
+        return position < end ? table[position / p.page_size] : -1;
+    };
+    const auto place_of = [&](int page, int k0) {
+        KeyPlace at;
+        at.held = page >= 0 && page < p.pages;
+        const int64_t pg = at.held ? page : 0, slot = at.held ? (k0 + lane % 32) % p.page_size : 0;
+        at.offset = pg * key_cache.page_bytes + slot * key_cache.token_bytes;
+        at.value_offset = pg * value_cache.page_bytes + slot * value_cache.token_bytes;
+        return at;
+    };
+    const auto load = [&](U32x4(&f)[DP / 16], const char* row, bool held) {
 #pragma unroll
-        for (int i = 0; i < kKeyTile * DP / 8 / kWave; ++i) {
-            const int at = i * kWave + lane;
-            const int key = at / (DP / 8), chunk = at % (DP / 8);
-            const int from_page = __shfl(page, key), from_slot = __shfl(slot, key);
-            const bool here = held_word >> key & 1;
-            const int64_t pg = here ? from_page : 0, sl = here ? from_slot : 0;
-            const U32x4 kc = load_chunk(key_cache.at(pg, sl, kv_head), chunk, p.dim, here);
-            const U32x4 vc = load_chunk(value_cache.at(pg, sl, kv_head), chunk, p.dim, here);
-            *reinterpret_cast<U32x4*>(k_tile + Tile<DP>::place(key, chunk)) = kc;
-            *reinterpret_cast<U32x4*>(v_tile + Tile<DP>::place(key, chunk)) = vc;
-        }
-        wave_lds_order();
+        for (int s = 0; s < DP / 16; ++s) f[s] = load_chunk(row, 2 * s + half, p.dim, held);
+    };
+    RowState<DP> state = {};
+    state.top = -INFINITY;
+    int k0 = begin + wave * kWaveKeys;
+    int page = page_of(k0);
+    KeyPlace at = place_of(page, k0);
+    load(kf, keys + at.offset, at.held);
+    load(vf, values + at.value_offset, at.held);
+    page = page_of(k0 + kKeyStep);
+    for (; k0 < end; k0 += kKeyStep) {
+        const uint32_t held = static_cast<uint32_t>(wave_ballot(at.held));
         F32x16 s = {};
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) s = T::mfma(read_rows<DP>(k_tile, 0, i), qf[i], s);
-        const uint32_t seen = held_word & (tree != nullptr ? seen_word(word, k0, ahead) : chain_word(token, k0, ahead));
-        float high = top;
+        for (int i = 0; i < DP / 16; ++i) s = T::mfma(kf[i], qf[i], s);
+        at = place_of(page, k0 + kKeyStep);
+        page = page_of(k0 + 2 * kKeyStep);
+        load(kf, keys + at.offset, at.held);
+        wave_lds_order();
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            if (!(seen >> acc_row(r, half) & 1)) s[r] = -INFINITY;
-            high = fmaxf(high, s[r]);
+        for (int i = 0; i < DP / 16; ++i) *reinterpret_cast<U32x4*>(v_tile + Tile<DP>::place(lane % 32, 2 * i + half)) = vf[i];
+        wave_lds_order();
+        load(vf, values + at.value_offset, at.held);
+        if (held != ~0u || k0 + kWaveKeys > ahead) {
+            const uint32_t seen = (held & row.seen(tree != nullptr, k0, ahead)) >> (4 * half);
+#pragma unroll
+            for (int r = 0; r < 16; ++r) s[r] = seen & (1u << acc_row(r, 0)) ? s[r] : -INFINITY;
         }
-        high = halves_max(high);
-        const float base = high == -INFINITY ? 0.f : high * c;
-        const float alpha = exp2_fast(top * c - base);
-        top = high;
-        total *= alpha;
+        float high = s[0];
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) acc[d] *= alpha;
+        for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
+        rescale(state, halves_max(high), c);
+        const float base = state.top == -INFINITY ? 0.f : state.top * c;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s[r] = exp2_fast(s[r] * c - base);
-            total += s[r];
+            state.total += s[r];
         }
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const U32x4 pf = pack_step<T>(s, i);
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) acc[d] = T::mfma(read_columns<DP>(v_tile, i * 16, d * 32), pf, acc[d]);
+            for (int d = 0; d < DP / 32; ++d)
+                state.acc[d] = T::mfma(read_columns<DP>(v_tile, i * 16, d * 32), pf, state.acc[d]);
         }
     }
-    total = halves_sum(total);
+    const float total = halves_sum(state.total);
     if (half == 0) {
-        stats[0][wave][lane] = top;
+        stats[0][wave][lane] = state.top;
         stats[1][wave][lane] = total;
     }
     __syncthreads();
@@ -186,33 +238,30 @@ __global__ __launch_bounds__(kBlock) void attention_paged_kernel(Rows q, Pages k
     const float base = all_top == -INFINITY ? 0.f : all_top * c;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) all_total += stats[1][i][lane % 32] * exp2_fast(stats[0][i][lane % 32] * c - base);
-    const float mine = exp2_fast(top * c - base);
+    const float mine = exp2_fast(state.top * c - base);
     float* join = reinterpret_cast<float*>(tiles);
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-            const F32x4 v = {acc[d][4 * g] * mine, acc[d][4 * g + 1] * mine, acc[d][4 * g + 2] * mine, acc[d][4 * g + 3] * mine};
-            *reinterpret_cast<F32x4*>(join + (wave * kRowTile + lane % 32) * kJoinStride + d * 32 + 8 * g + 4 * half) = v;
+            const F32x4 v = {state.acc[d][4 * g], state.acc[d][4 * g + 1], state.acc[d][4 * g + 2], state.acc[d][4 * g + 3]};
+            *reinterpret_cast<F32x4*>(join + (wave * kNarrowRows + lane % 32) * kJoinStride + d * 32 + 8 * g + 4 * half) = v * mine;
         }
     __syncthreads();
-    if (wave == 0 && half == 0) stats[0][0][lane] = all_total;
-    const int64_t stat = static_cast<int64_t>(head) * p.q_tokens + w.token0 + token;
-    if (wave == 0 && half == 0 && there) {
-        if (whole) {
-            if (lse != nullptr) lse[stat] = all_total == 0.f ? -INFINITY : all_top * p.scale + __logf(all_total);
-        } else {
-            part_stats[static_cast<int64_t>(blockIdx.y) * p.q_tokens * p.q_heads + stat] = F32x2{all_top, all_total};
-        }
+    if (threadIdx.x < kNarrowRows) {
+        stats[0][0][lane] = all_total;
+        if (row.there && whole && lse != nullptr)
+            lse[static_cast<int64_t>(row.head) * p.q_tokens + w.token0 + row.token] = row_lse(all_top, all_total, p.scale);
+        if (row.there && !whole) parts.stats[parts.row(p, blockIdx.y, row.head, w.token0 + row.token)] = F32x2{all_top, all_total};
     }
     __syncthreads();
-    for (int at = threadIdx.x; at < kRowTile * DP / 8; at += kBlock) {
-        const int r = at / (DP / 8), chunk = at % (DP / 8);
+    for (int item = threadIdx.x; item < kNarrowRows * DP / 8; item += kBlock) {
+        const int r = item / (DP / 8), chunk = item % (DP / 8);
         if (w.row0 + r >= w.rows || chunk * 8 >= p.dim) continue;
         F32x4 a = {}, b = {};
 #pragma unroll
         for (int i = 0; i < kWaves; ++i) {
-            const float* from = join + (i * kRowTile + r) * kJoinStride + chunk * 8;
+            const float* from = join + (i * kNarrowRows + r) * kJoinStride + chunk * 8;
             a += *reinterpret_cast<const F32x4*>(from);
             b += *reinterpret_cast<const F32x4*>(from + 4);
         }
@@ -220,69 +269,197 @@ __global__ __launch_bounds__(kBlock) void attention_paged_kernel(Rows q, Pages k
         const int h = kv_head * group + (w.row0 + r) % group;
         if (whole) {
             const float sum = stats[0][0][r];
-            const float f = sum == 0.f ? 0.f : 1.f / sum;
-            *reinterpret_cast<U32x4*>(out.at(t, h) + chunk * 16) =
-                U32x4{pack2<T>(a[0] * f, a[1] * f), pack2<T>(a[2] * f, a[3] * f), pack2<T>(b[0] * f, b[1] * f),
-                      pack2<T>(b[2] * f, b[3] * f)};
+            store_items<T>(out.at(t, h) + chunk * 16, a, b, sum == 0.f ? 0.f : 1.f / sum);
         } else {
-            float* to = part_out + ((static_cast<int64_t>(blockIdx.y) * p.q_heads + h) * p.q_tokens + t) * p.dim + chunk * 8;
+            float* to = parts.out + parts.row(p, blockIdx.y, h, t) * p.dim + chunk * 8;
             *reinterpret_cast<F32x4*>(to) = a;
             *reinterpret_cast<F32x4*>(to + 4) = b;
         }
     }
 }
 
-// Joins the parts of a tile's rows, in the parts' order.
-template <typename T>
-__global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, float* __restrict__ lse,
-                                                                      const float* __restrict__ part_out,
-                                                                      const F32x2* __restrict__ part_stats,
-                                                                      const int32_t* __restrict__ q_offsets,
-                                                                      const int32_t* __restrict__ kv_lengths, Paged p) {
-    const int kv_head = blockIdx.x % p.kv_heads;
-    Work w;
-    if (!find_work(w, q_offsets, kv_lengths, p, blockIdx.x / p.kv_heads)) return;
-    const int per = part_keys(w.length, p.parts);
-    if (w.length <= per) return;
-    const int parts = (w.length + per - 1) / per;
-    const int group = p.q_heads / p.kv_heads;
-    const float c = p.scale * kLog2e;
-    // 16 lanes a row, 8 items each.
-    for (int r = threadIdx.x / 16; r < kRowTile && w.row0 + r < w.rows; r += kBlock / 16) {
-        const int64_t t = w.token0 + (w.row0 + r) / group;
-        const int h = kv_head * group + (w.row0 + r) % group;
-        const int chunk = threadIdx.x % 16;
-        const int64_t rows = static_cast<int64_t>(p.q_tokens) * p.q_heads, stat = static_cast<int64_t>(h) * p.q_tokens + t;
-        float top = -INFINITY, total = 0.f;
-        for (int i = 0; i < parts; ++i) top = fmaxf(top, part_stats[i * rows + stat][0]);
-        const float base = top == -INFINITY ? 0.f : top * c;
-        F32x4 a = {}, b = {};
-        for (int i = 0; i < parts; ++i) {
-            const F32x2 st = part_stats[i * rows + stat];
-            const float f = exp2_fast(st[0] * c - base);
-            total += st[1] * f;
-            if (chunk * 8 < p.dim) {
-                const float* from = part_out + (i * rows + stat) * p.dim + chunk * 8;
-                a += *reinterpret_cast<const F32x4*>(from) * f;
-                b += *reinterpret_cast<const F32x4*>(from + 4) * f;
+// Direct loads of tiles of keys and values from the cache.  Positions past the last are loaded as the last, and masked; the
+// chunks of a page that is not there become zeros.
+template <int DP>
+struct PagedTiles {
+    using Loads = TileLoads<DP, kKeyTile>;
+    const char* keys;
+    const char* values;
+    const Pages& key_cache;
+    const Pages& value_cache;
+    const int32_t* table;
+    const Paged& p;
+    int end;
+    int page[Loads::kPerWave];  // of the tile to load next
+    __device__ __forceinline__ int position(int k0, int i) const {
+        const int at = k0 + Loads::row() + i * Loads::kRowStep;
+        return at < end ? at : end - 1;
+    }
+    __device__ __forceinline__ void look_up(int k0) {
+#pragma unroll
+        for (int i = 0; i < Loads::kPerWave; ++i) page[i] = table[position(k0, i) / p.page_size];
+    }
+    __device__ __forceinline__ void load(char* k_tile, char* v_tile, int k0) {
+        const int chunk = Loads::chunk();
+        if (chunk * 8 < p.dim) {
+#pragma unroll
+            for (int i = 0; i < Loads::kPerWave; ++i) {
+                const int64_t slot = position(k0, i) % p.page_size;
+                if (page[i] >= 0 && page[i] < p.pages) {
+                    load_to_lds(keys + page[i] * key_cache.page_bytes + slot * key_cache.token_bytes + chunk * 16, Loads::place(k_tile, i));
+                    load_to_lds(values + page[i] * value_cache.page_bytes + slot * value_cache.token_bytes + chunk * 16,
+                                Loads::place(v_tile, i));
+                } else {
+                    *reinterpret_cast<U32x4*>(Loads::place(k_tile, i) + threadIdx.x % kWave * 16) = U32x4{0u, 0u, 0u, 0u};
+                    *reinterpret_cast<U32x4*>(Loads::place(v_tile, i) + threadIdx.x % kWave * 16) = U32x4{0u, 0u, 0u, 0u};
+                }
             }
         }
-        const float f = total == 0.f ? 0.f : 1.f / total;
-        if (chunk * 8 < p.dim)
-            *reinterpret_cast<U32x4*>(out.at(t, h) + chunk * 16) =
-                U32x4{pack2<T>(a[0] * f, a[1] * f), pack2<T>(a[2] * f, a[3] * f), pack2<T>(b[0] * f, b[1] * f),
-                      pack2<T>(b[2] * f, b[3] * f)};
-        if (chunk == 0 && lse != nullptr) lse[stat] = total == 0.f ? -INFINITY : top * p.scale + __logf(total);
+        if (k0 + kKeyTile < end) look_up(k0 + kKeyTile);
+    }
+};
+
+template <typename T, int DP>
+__global__ __launch_bounds__(kBlock, 2) void attention_paged_wide_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
+                                                                         float* __restrict__ lse, Parts parts,
+                                                                         const int32_t* __restrict__ block_table,
+                                                                         const int32_t* __restrict__ q_offsets,
+                                                                         const int32_t* __restrict__ kv_lengths,
+                                                                         const uint64_t* __restrict__ tree, Paged p) {
+    constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);
+    __shared__ __attribute__((aligned(16))) char k_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char v_even[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char k_odd[kTileBytes];
+    __shared__ __attribute__((aligned(16))) char v_odd[kTileBytes];
+    const int kv_head = blockIdx.x % p.kv_heads;
+    Work w;
+    if (!find_work(w, q_offsets, kv_lengths, p, kRowTile, blockIdx.x / p.kv_heads)) return;
+    const int per = part_keys(w.length, p.parts);
+    const int64_t part_begin = static_cast<int64_t>(blockIdx.y) * per;
+    if (part_begin >= w.length && blockIdx.y > 0) return;
+    const int begin = static_cast<int>(part_begin), end = w.length - begin > per ? begin + per : w.length;
+    const bool whole = w.length <= per;
+    const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const PagedRow row(w, p, tree, kv_head, w.row0 + wave * kRowsPerWave + lane % 32);
+    const int ahead = w.length - w.tokens;
+    const float c = p.scale * kLog2e;
+    const int32_t* table = block_table + static_cast<int64_t>(w.request) * p.table_stride;
+    // A page that is not there: every tile is masked, by what the table says of its keys.
+    bool lost = false;
+    if (begin < end)
+        for (int i = begin / p.page_size + static_cast<int>(threadIdx.x); i <= (end - 1) / p.page_size; i += kBlock)
+            lost |= table[i] < 0 || table[i] >= p.pages;
+    lost = __syncthreads_or(lost);
+
+    U32x4 qf[DP / 16];
+    const char* q_row = q.at(w.token0 + row.token, row.head);
+#pragma unroll
+    for (int s = 0; s < DP / 16; ++s) qf[s] = load_chunk(q_row, 2 * s + half, p.dim, row.there);
+    for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile>(tile, p.dim);
+    RowState<DP> state = {};
+    state.top = -INFINITY;
+    const auto seen = [&](int k0) {
+        uint32_t word = row.seen(tree != nullptr, k0, ahead) & first_keys(end, k0);
+        if (lost) {
+            const int position = k0 + lane % 32;
+            const int page = position < end ? table[position / p.page_size] : -1;
+            word &= static_cast<uint32_t>(wave_ballot(page >= 0 && page < p.pages));
+        }
+        return word;
+    };
+    PagedTiles<DP> source{key_cache.at(0, 0, kv_head), value_cache.at(0, 0, kv_head), key_cache, value_cache, table, p, end, {}};
+    if (begin < end) source.look_up(begin);
+    const int full = lost ? begin : ahead < end ? ahead : end;
+    const int wave_end = w.row0 + wave * kRowsPerWave < w.rows ? end : begin;
+    const auto step = [&](const char* k_tile, const char* v_tile, int k0) {
+        if (k0 < wave_end) forward_tile<T, DP>(state, k_tile, v_tile, qf, c, k0, k0 + kKeyTile > full, seen);
+    };
+    pass_tiles<kKeyTile>(begin, end, [&](int k0) { source.load(k_even, v_even, k0); }, [&](int k0) { source.load(k_odd, v_odd, k0); },
+                         [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
+    const float total = halves_sum(state.total);
+    if (!row.there) return;
+    const int64_t t = w.token0 + row.token;
+    if (whole) {
+        store_row<T, DP>(out, t, row.head, state.acc, total == 0.f ? 0.f : 1.f / total, p.dim);
+        if (lse != nullptr && half == 0) lse[static_cast<int64_t>(row.head) * p.q_tokens + t] = row_lse(state.top, total, p.scale);
+        return;
+    }
+    const int64_t at = parts.row(p, blockIdx.y, row.head, t);
+    if (half == 0) parts.stats[at] = F32x2{state.top, total};
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+        const int d = 8 * i + 4 * half;
+        const F32x16& acc = state.acc[i / 4];
+        if (d < p.dim)
+            *reinterpret_cast<F32x4*>(parts.out + at * p.dim + d) =
+                F32x4{acc[4 * (i % 4)], acc[4 * (i % 4) + 1], acc[4 * (i % 4) + 2], acc[4 * (i % 4) + 3]};
     }
 }
 
+// Joins the parts of one row, in the parts' order: 16 lanes take the row's items, 16 of those groups every 16th part.
+template <typename T>
+__global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, float* __restrict__ lse, Parts parts,
+                                                                      const int32_t* __restrict__ q_offsets,
+                                                                      const int32_t* __restrict__ kv_lengths, Paged p) {
+    constexpr int kGroups = kBlock / 16;
+    __shared__ F32x4 sums[2][kGroups][16];
+    __shared__ F32x2 group_stats[kGroups];
+    const int head = blockIdx.x % p.q_heads;
+    const int64_t token = blockIdx.x / p.q_heads;
+    const int request = find_last(p.requests, token, [&](int r) { return static_cast<int64_t>(q_offsets[r]); });
+    if (request < 0) return;
+    Work w;
+    take_request(w, q_offsets, kv_lengths, p, request);
+    const int per = part_keys(w.length, p.parts);
+    if (token >= w.token0 + w.tokens || w.length <= per) return;
+    const int count = (w.length + per - 1) / per;
+    const int chunk = threadIdx.x % 16, group = threadIdx.x / 16;
+    const float c = p.scale * kLog2e;
+    float top = -INFINITY, total = 0.f;
+    for (int i = group; i < count; i += kGroups) top = fmaxf(top, parts.stats[parts.row(p, i, head, token)][0]);
+    const float base = top == -INFINITY ? 0.f : top * c;
+    F32x4 a = {}, b = {};
+    for (int i = group; i < count; i += kGroups) {
+        const int64_t row = parts.row(p, i, head, token);
+        const F32x2 st = parts.stats[row];
+        const float f = exp2_fast(st[0] * c - base);
+        total += st[1] * f;
+        if (chunk * 8 < p.dim) {
+            const float* from = parts.out + row * p.dim + chunk * 8;
+            a += *reinterpret_cast<const F32x4*>(from) * f;
+            b += *reinterpret_cast<const F32x4*>(from + 4) * f;
+        }
+    }
+    sums[0][group][chunk] = a;
+    sums[1][group][chunk] = b;
+    if (chunk == 0) group_stats[group] = F32x2{top, total};
+    __syncthreads();
+    if (group != 0) return;
+    for (int i = 0; i < kGroups; ++i) top = fmaxf(top, group_stats[i][0]);
+    const float all_base = top == -INFINITY ? 0.f : top * c;
+    a = F32x4{}, b = F32x4{}, total = 0.f;
+    for (int i = 0; i < kGroups; ++i) {
+        const float f = exp2_fast(group_stats[i][0] * c - all_base);
+        total += group_stats[i][1] * f;
+        a += sums[0][i][chunk] * f;
+        b += sums[1][i][chunk] * f;
+    }
+    if (chunk * 8 < p.dim) store_items<T>(out.at(token, head) + chunk * 16, a, b, total == 0.f ? 0.f : 1.f / total);
+    if (chunk == 0 && lse != nullptr) lse[static_cast<int64_t>(head) * p.q_tokens + token] = row_lse(top, total, p.scale);
+}
+
 // ---- host side ---------------------------------------------------------------------------------------------------
-uint64_t tiles_of(uint64_t requests, uint64_t q_tokens, uint64_t group) { return q_tokens * group / kRowTile + requests; }
+// Rows of a tile: 32 while a request has no more on average, else 128.
+uint64_t tile_rows(uint64_t requests, uint64_t q_tokens, uint64_t group) {
+    return q_tokens * group > requests * kNarrowRows ? kRowTile : kNarrowRows;
+}
 
 uint64_t parts_of(uint64_t requests, uint64_t q_tokens, uint64_t max_kv, uint64_t q_heads, uint64_t kv_heads) {
     if (kv_heads == 0 || q_heads < kv_heads) return 1;
     // Tiles that have rows: as many as the rows make, or one a request.
-    const uint64_t rows = ceil_div(q_tokens * (q_heads / kv_heads), kRowTile);
+    const uint64_t group = q_heads / kv_heads;
+    const uint64_t rows = ceil_div(q_tokens * group, tile_rows(requests, q_tokens, group));
     const uint64_t busy = (rows > requests ? rows : requests) * kv_heads;
     const uint64_t most = ceil_div(max_kv, kPartKeys);
     uint64_t parts = ceil_div(kGridTarget, busy ? busy : 1);
@@ -326,25 +503,27 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
     const uint64_t parts = parts_of(requests, q_tokens, max_kv_length, q_heads, kv_heads);
     const size_t needed = paged_bytes(requests, q_tokens, max_kv_length, q_heads, kv_heads, dim);
     if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
-    const uint64_t blocks = tiles_of(requests, q_tokens, q_heads / kv_heads) * kv_heads;
-    if (blocks * parts > 0x7FFFFFFFull / kBlock || parts > 65535) return set_error(kInvalidArgument, "%s: too many tiles", what);
+    const uint64_t rows = tile_rows(requests, q_tokens, q_heads / kv_heads);
+    const uint64_t blocks = (q_tokens * (q_heads / kv_heads) / rows + requests) * kv_heads;
+    if (blocks * parts > 0x7FFFFFFFull / kBlock || parts > 65535 || (parts > 1 && q_tokens * q_heads > 0x7FFFFFFFull / kBlock)) return set_error(kInvalidArgument, "%s: too many tiles", what);
     const Paged p{static_cast<int>(requests), static_cast<int>(q_tokens), static_cast<int>(q_heads), static_cast<int>(kv_heads),
                   static_cast<int>(dim), static_cast<int>(page_size), static_cast<int>(pages), static_cast<int>(table_stride),
                   static_cast<int>(table_width), static_cast<int>(parts), scale};
-    F32x2* part_stats = static_cast<F32x2*>(temp);
-    float* part_out = parts > 1 ? reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(parts, q_tokens * q_heads)) : nullptr;
+    Parts sums{nullptr, static_cast<F32x2*>(temp)};
+    if (parts > 1) sums.out = reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(parts, q_tokens * q_heads));
     {
         LaunchScope scope("attention_paged", stream);
-        auto* kernel = dim <= 64 ? attention_paged_kernel<T, 64> : dim <= 96 ? attention_paged_kernel<T, 96> : attention_paged_kernel<T, 128>;
+        auto* narrow = dim <= 64 ? attention_paged_kernel<T, 64> : dim <= 96 ? attention_paged_kernel<T, 96> : attention_paged_kernel<T, 128>;
+        auto* wide = dim <= 64 ? attention_paged_wide_kernel<T, 64> : dim <= 96 ? attention_paged_wide_kernel<T, 96> : attention_paged_wide_kernel<T, 128>;
+        auto* kernel = rows == kNarrowRows ? narrow : wide;
         kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), kBlock, 0, stream>>>(
-            rows_of(q), pages_of(key_cache), pages_of(value_cache), rows_of(out), lse, part_out, part_stats, block_table,
-            q_offsets, kv_lengths, tree, p);
+            rows_of(q), pages_of(key_cache), pages_of(value_cache), rows_of(out), lse, sums, block_table, q_offsets, kv_lengths, tree, p);
         if (int st = check_hip(hipGetLastError(), "attention_paged launch"); st != kOk) return st;
     }
     if (parts == 1) return kOk;
     LaunchScope scope("attention_paged_join", stream);
-    attention_paged_join_kernel<T><<<static_cast<unsigned>(blocks), kBlock, 0, stream>>>(rows_of(out), lse, part_out, part_stats,
-                                                                                         q_offsets, kv_lengths, p);
+    attention_paged_join_kernel<T><<<static_cast<unsigned>(q_tokens * q_heads), kBlock, 0, stream>>>(rows_of(out), lse, sums, q_offsets,
+                                                                                                     kv_lengths, p);
     return check_hip(hipGetLastError(), "attention_paged_join launch");
 }
 
