@@ -119,13 +119,6 @@ __device__ __forceinline__ float row_lse(float top, float total, float scale) {
     return total == 0.f ? -INFINITY : top * scale + __logf(total);
 }
 
-// A lane's key of a tile of 32: both halves of the wave have the same.
-struct KeyPlace {
-    int64_t offset;  // of page and slot in the key cache
-    int64_t value_offset;
-    bool held;
-};
-
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
                                                                     float* __restrict__ lse, Parts parts,
@@ -136,8 +129,9 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     constexpr int kTileBytes = Tile<DP>::bytes(kWaveKeys);
     constexpr int kJoinStride = DP + 4;  // floats
     constexpr int kJoinBytes = kWaves * kNarrowRows * kJoinStride * 4;
-    static_assert(kWaves * kTileBytes <= kJoinBytes, "the values' tiles lie where the sums are joined");
-    __shared__ __attribute__((aligned(16))) char tiles[kJoinBytes];
+    constexpr int kTilesBytes = kWaves * 2 * kTileBytes;
+    constexpr int kLoads = kWaveKeys / Tile<DP>::kBlockRows;
+    __shared__ __attribute__((aligned(16))) char tiles[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ float stats[2][kWaves][kNarrowRows];
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
@@ -161,47 +155,56 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     const char* q_row = q.at(w.token0 + row.token, row.head);
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) qf[s] = load_chunk(q_row, 2 * s + half, p.dim, row.there);
-    char* v_tile = tiles + wave * kTileBytes;
-    // Keys go from the cache into the registers that the products read, values into registers and from there into the
-    // wave's tile: both a tile ahead, the page numbers two.
-    U32x4 kf[DP / 16], vf[DP / 16];
+    char* k_tile = tiles + wave * 2 * kTileBytes;
+    char* v_tile = k_tile + kTileBytes;
+    // Lane l and l + 32 look key l of a tile up; the tile's rows are then read four lanes to 64 bytes.  Tiles are in
+    // registers one ahead of the one in LDS, page numbers two ahead.
+    const bool alike = key_cache.page_bytes == value_cache.page_bytes && key_cache.token_bytes == value_cache.token_bytes;
+    const bool has = Tile<DP>::lane_chunk(lane) * 8 < p.dim;
     const auto page_of = [&](int k0) {
         const int position = k0 + lane % 32;
         return position < end ? table[position / p.page_size] : -1;
     };
-    const auto place_of = [&](int page, int k0) {
-        KeyPlace at;
-        at.held = page >= 0 && page < p.pages;
-        const int64_t pg = at.held ? page : 0, slot = at.held ? (k0 + lane % 32) % p.page_size : 0;
-        at.offset = pg * key_cache.page_bytes + slot * key_cache.token_bytes;
-        at.value_offset = pg * value_cache.page_bytes + slot * value_cache.token_bytes;
-        return at;
-    };
-    const auto load = [&](U32x4(&f)[DP / 16], const char* row, bool held) {
+    U32x4 kf[kLoads], vf[kLoads];
+    // Loads tile k0; the keys that are there, as bits.
+    const auto load = [&](int page, int k0) {
+        const bool here = page >= 0 && page < p.pages;
+        const uint32_t held = static_cast<uint32_t>(wave_ballot(here));
+        const int64_t pg = here ? page : 0, slot = here ? (k0 + lane % 32) % p.page_size : 0;
+        const int64_t k_at = pg * key_cache.page_bytes + slot * key_cache.token_bytes;
+        const int64_t v_at = alike ? k_at : pg * value_cache.page_bytes + slot * value_cache.token_bytes;
 #pragma unroll
-        for (int s = 0; s < DP / 16; ++s) f[s] = load_chunk(row, 2 * s + half, p.dim, held);
+        for (int i = 0; i < kLoads; ++i) {
+            const int key = i * Tile<DP>::kBlockRows + Tile<DP>::lane_row(lane);
+            const int64_t k_from = __shfl(k_at, key), v_from = alike ? k_from : __shfl(v_at, key);
+            const bool there = has && (held >> key & 1);
+            kf[i] = vf[i] = U32x4{0u, 0u, 0u, 0u};
+            if (there) {
+                kf[i] = *reinterpret_cast<const U32x4*>(keys + k_from + Tile<DP>::lane_chunk(lane) * 16);
+                vf[i] = *reinterpret_cast<const U32x4*>(values + v_from + Tile<DP>::lane_chunk(lane) * 16);
+            }
+        }
+        return held;
     };
     RowState<DP> state = {};
     state.top = -INFINITY;
     int k0 = begin + wave * kWaveKeys;
-    int page = page_of(k0);
-    KeyPlace at = place_of(page, k0);
-    load(kf, keys + at.offset, at.held);
-    load(vf, values + at.value_offset, at.held);
-    page = page_of(k0 + kKeyStep);
+    uint32_t next_held = load(page_of(k0), k0);
+    int page = page_of(k0 + kKeyStep);
     for (; k0 < end; k0 += kKeyStep) {
-        const uint32_t held = static_cast<uint32_t>(wave_ballot(at.held));
+        const uint32_t held = next_held;
+        wave_lds_order();
+#pragma unroll
+        for (int i = 0; i < kLoads; ++i) {
+            *reinterpret_cast<U32x4*>(k_tile + i * Tile<DP>::kBlockBytes + lane * 16) = kf[i];
+            *reinterpret_cast<U32x4*>(v_tile + i * Tile<DP>::kBlockBytes + lane * 16) = vf[i];
+        }
+        wave_lds_order();
+        next_held = load(page, k0 + kKeyStep);
+        page = page_of(k0 + 2 * kKeyStep);
         F32x16 s = {};
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) s = T::mfma(kf[i], qf[i], s);
-        at = place_of(page, k0 + kKeyStep);
-        page = page_of(k0 + 2 * kKeyStep);
-        load(kf, keys + at.offset, at.held);
-        wave_lds_order();
-#pragma unroll
-        for (int i = 0; i < DP / 16; ++i) *reinterpret_cast<U32x4*>(v_tile + Tile<DP>::place(lane % 32, 2 * i + half)) = vf[i];
-        wave_lds_order();
-        load(vf, values + at.value_offset, at.held);
+        for (int i = 0; i < DP / 16; ++i) s = T::mfma(read_rows<DP>(k_tile, 0, i), qf[i], s);
         if (held != ~0u || k0 + kWaveKeys > ahead) {
             const uint32_t seen = (held & row.seen(tree != nullptr, k0, ahead)) >> (4 * half);
 #pragma unroll
@@ -397,16 +400,17 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_wide_kernel(Rows q,
     }
 }
 
-// Joins the parts of one row, in the parts' order: 16 lanes take the row's items, 16 of those groups every 16th part.
-template <typename T>
+// Joins the parts of a token's rows, in the parts' order.  16 lanes take a row's items; GROUPS such groups every GROUPS-th
+// part of it, and a workgroup's rows are heads of one token.
+template <typename T, int GROUPS>
 __global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, float* __restrict__ lse, Parts parts,
                                                                       const int32_t* __restrict__ q_offsets,
                                                                       const int32_t* __restrict__ kv_lengths, Paged p) {
-    constexpr int kGroups = kBlock / 16;
-    __shared__ F32x4 sums[2][kGroups][16];
-    __shared__ F32x2 group_stats[kGroups];
-    const int head = blockIdx.x % p.q_heads;
-    const int64_t token = blockIdx.x / p.q_heads;
+    constexpr int kHeads = kBlock / 16 / GROUPS;
+    __shared__ F32x4 sums[2][GROUPS][kHeads][16];
+    __shared__ F32x2 group_stats[GROUPS][kHeads];
+    const int blocks = (p.q_heads + kHeads - 1) / kHeads;
+    const int64_t token = blockIdx.x / blocks;
     const int request = find_last(p.requests, token, [&](int r) { return static_cast<int64_t>(q_offsets[r]); });
     if (request < 0) return;
     Work w;
@@ -414,37 +418,44 @@ __global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, 
     const int per = part_keys(w.length, p.parts);
     if (token >= w.token0 + w.tokens || w.length <= per) return;
     const int count = (w.length + per - 1) / per;
-    const int chunk = threadIdx.x % 16, group = threadIdx.x / 16;
+    const int chunk = threadIdx.x % 16, group = threadIdx.x / 16 % GROUPS, local = threadIdx.x / 16 / GROUPS;
+    const int head = blockIdx.x % blocks * kHeads + local;
+    const bool there = head < p.q_heads;
     const float c = p.scale * kLog2e;
     float top = -INFINITY, total = 0.f;
-    for (int i = group; i < count; i += kGroups) top = fmaxf(top, parts.stats[parts.row(p, i, head, token)][0]);
-    const float base = top == -INFINITY ? 0.f : top * c;
     F32x4 a = {}, b = {};
-    for (int i = group; i < count; i += kGroups) {
-        const int64_t row = parts.row(p, i, head, token);
-        const F32x2 st = parts.stats[row];
-        const float f = exp2_fast(st[0] * c - base);
-        total += st[1] * f;
-        if (chunk * 8 < p.dim) {
-            const float* from = parts.out + row * p.dim + chunk * 8;
-            a += *reinterpret_cast<const F32x4*>(from) * f;
-            b += *reinterpret_cast<const F32x4*>(from + 4) * f;
+    if (there) {
+        for (int i = group; i < count; i += GROUPS) top = fmaxf(top, parts.stats[parts.row(p, i, head, token)][0]);
+        const float base = top == -INFINITY ? 0.f : top * c;
+#pragma unroll 2
+        for (int i = group; i < count; i += GROUPS) {
+            const int64_t row = parts.row(p, i, head, token);
+            const F32x2 st = parts.stats[row];
+            const float f = exp2_fast(st[0] * c - base);
+            total += st[1] * f;
+            if (chunk * 8 < p.dim) {
+                const float* from = parts.out + row * p.dim + chunk * 8;
+                a += *reinterpret_cast<const F32x4*>(from) * f;
+                b += *reinterpret_cast<const F32x4*>(from + 4) * f;
+            }
         }
     }
-    sums[0][group][chunk] = a;
-    sums[1][group][chunk] = b;
-    if (chunk == 0) group_stats[group] = F32x2{top, total};
-    __syncthreads();
-    if (group != 0) return;
-    for (int i = 0; i < kGroups; ++i) top = fmaxf(top, group_stats[i][0]);
-    const float all_base = top == -INFINITY ? 0.f : top * c;
-    a = F32x4{}, b = F32x4{}, total = 0.f;
-    for (int i = 0; i < kGroups; ++i) {
-        const float f = exp2_fast(group_stats[i][0] * c - all_base);
-        total += group_stats[i][1] * f;
-        a += sums[0][i][chunk] * f;
-        b += sums[1][i][chunk] * f;
+    if constexpr (GROUPS > 1) {
+        sums[0][group][local][chunk] = a;
+        sums[1][group][local][chunk] = b;
+        if (chunk == 0) group_stats[group][local] = F32x2{top, total};
+        __syncthreads();
+        for (int i = 0; i < GROUPS; ++i) top = fmaxf(top, group_stats[i][local][0]);
+        const float base = top == -INFINITY ? 0.f : top * c;
+        a = F32x4{}, b = F32x4{}, total = 0.f;
+        for (int i = 0; i < GROUPS; ++i) {
+            const float f = exp2_fast(group_stats[i][local][0] * c - base);
+            total += group_stats[i][local][1] * f;
+            a += sums[0][i][local][chunk] * f;
+            b += sums[1][i][local][chunk] * f;
+        }
     }
+    if (!there || group != 0) return;
     if (chunk * 8 < p.dim) store_items<T>(out.at(token, head) + chunk * 16, a, b, total == 0.f ? 0.f : 1.f / total);
     if (chunk == 0 && lse != nullptr) lse[static_cast<int64_t>(head) * p.q_tokens + token] = row_lse(top, total, p.scale);
 }
@@ -462,7 +473,9 @@ uint64_t parts_of(uint64_t requests, uint64_t q_tokens, uint64_t max_kv, uint64_
     const uint64_t rows = ceil_div(q_tokens * group, tile_rows(requests, q_tokens, group));
     const uint64_t busy = (rows > requests ? rows : requests) * kv_heads;
     const uint64_t most = ceil_div(max_kv, kPartKeys);
-    uint64_t parts = ceil_div(kGridTarget, busy ? busy : 1);
+    // Half as many wide workgroups, whose sums are four times as many, as narrow ones.
+    const uint64_t target = tile_rows(requests, q_tokens, group) == kNarrowRows ? kGridTarget : kGridTarget / 2;
+    uint64_t parts = ceil_div(target, busy ? busy : 1);
     parts = parts < most ? parts : most;
     return parts ? parts : 1;
 }
@@ -522,8 +535,10 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
     }
     if (parts == 1) return kOk;
     LaunchScope scope("attention_paged_join", stream);
-    attention_paged_join_kernel<T><<<static_cast<unsigned>(q_tokens * q_heads), kBlock, 0, stream>>>(rows_of(out), lse, sums, q_offsets,
-                                                                                                     kv_lengths, p);
+    const bool many = parts > kBlock / 16;
+    auto* join = many ? attention_paged_join_kernel<T, kBlock / 16> : attention_paged_join_kernel<T, 1>;
+    const uint64_t join_blocks = q_tokens * (many ? q_heads : ceil_div(q_heads, kBlock / 16));
+    join<<<static_cast<unsigned>(join_blocks), kBlock, 0, stream>>>(rows_of(out), lse, sums, q_offsets, kv_lengths, p);
     return check_hip(hipGetLastError(), "attention_paged_join launch");
 }
 
