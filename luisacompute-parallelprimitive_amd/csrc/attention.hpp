@@ -112,6 +112,24 @@ struct Pages {
     }
 };
 
+// Division of 32-bit numbers by one that the host knows, without the compiler's twenty-odd instructions: with l the least
+// power that 2^l >= d and m = floor(2^32 (2^l - d) / d) + 1, x / d = (t + (x - t) / 2) / 2^(l - 1) where t is the high word
+// of m x (Granlund and Montgomery, "Division by invariant integers using multiplication"); d = 1 takes no shift.
+struct Divider {
+    uint32_t by, factor, shift1, shift2;
+    explicit Divider(uint32_t d) : by(d) {
+        uint32_t l = 0;
+        while (l < 32 && (uint64_t{1} << l) < d) ++l;
+        factor = static_cast<uint32_t>((uint64_t{1} << 32) * ((uint64_t{1} << l) - d) / d + 1);
+        shift1 = l < 1 ? 0 : 1;
+        shift2 = l < 1 ? 0 : l - 1;
+    }
+    __device__ __forceinline__ uint32_t operator()(uint32_t x) const {
+        const uint32_t t = __umulhi(factor, x);
+        return (t + ((x - t) >> shift1)) >> shift2;
+    }
+};
+
 // What the 16-byte loads and stores of rows need.
 inline bool usable(const lcpp_hip_rows* r) {
     return r != nullptr && r->data != nullptr && reinterpret_cast<uintptr_t>(r->data) % 16 == 0 && r->token_stride >= 0 &&
@@ -193,8 +211,8 @@ struct TilePlace {
 };
 
 // The last of `count` ascending numbers that is not above `number` (-1: none): a wave tests 64 at a time.
-template <typename Key>
-__device__ __forceinline__ int find_last(int count, int64_t number, Key key) {
+template <typename Number, typename Key>
+__device__ __forceinline__ int find_last(int count, Number number, Key key) {
     const int lane = threadIdx.x % kWave;
     int low = 0, high = count;
     while (high - low > 0) {
@@ -211,7 +229,7 @@ __device__ __forceinline__ int find_last(int count, int64_t number, Key key) {
 
 __device__ __forceinline__ TilePlace find_tile(const int32_t* offsets, int count, int scale, int size, int number) {
     const auto first = [&](int b) { return static_cast<int64_t>(offsets[b]) * scale / size + b; };
-    const int owner = find_last(count, number, first);
+    const int owner = find_last<int64_t>(count, number, first);
     return {owner, owner < 0 ? 0 : number - static_cast<int>(first(owner))};
 }
 

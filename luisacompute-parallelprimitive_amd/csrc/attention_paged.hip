@@ -26,13 +26,17 @@ struct Paged {
     int q_heads;
     int kv_heads;
     int dim;
-    int page_size;
+    Divider page_size;
     int pages;
     int table_stride;
     int table_width;
     int parts;  // of a long request
     float scale;
 };
+
+__device__ __forceinline__ int slot_of(const Paged& p, uint32_t position) {
+    return static_cast<int>(position - p.page_size(position) * p.page_size.by);
+}
 
 // Keys of one part of a request: the same for every part, a multiple of a workgroup's step.
 __device__ __forceinline__ int part_keys(int length, int parts) {
@@ -59,7 +63,7 @@ __device__ __forceinline__ void take_request(Work& w, const int32_t* q_offsets, 
     w.token0 = begin;
     w.tokens = end - begin;
     w.rows = w.tokens * (p.q_heads / p.kv_heads);
-    const int64_t most = static_cast<int64_t>(p.table_width) * p.page_size;
+    const int64_t most = static_cast<int64_t>(p.table_width) * p.page_size.by;
     const int length = kv_lengths[request];
     w.length = length < 0 ? 0 : length > most ? static_cast<int>(most) : length;
 }
@@ -163,14 +167,14 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     const bool has = Tile<DP>::lane_chunk(lane) * 8 < p.dim;
     const auto page_of = [&](int k0) {
         const int position = k0 + lane % 32;
-        return position < end ? table[position / p.page_size] : -1;
+        return position < end ? table[p.page_size(position)] : -1;
     };
     U32x4 kf[kLoads], vf[kLoads];
     // Loads tile k0; the keys that are there, as bits.
     const auto load = [&](int page, int k0) {
         const bool here = page >= 0 && page < p.pages;
         const uint32_t held = static_cast<uint32_t>(wave_ballot(here));
-        const int64_t pg = here ? page : 0, slot = here ? (k0 + lane % 32) % p.page_size : 0;
+        const int64_t pg = here ? page : 0, slot = here ? slot_of(p, k0 + lane % 32) : 0;
         const int64_t k_at = pg * key_cache.page_bytes + slot * key_cache.token_bytes;
         const int64_t v_at = alike ? k_at : pg * value_cache.page_bytes + slot * value_cache.token_bytes;
 #pragma unroll
@@ -300,14 +304,14 @@ struct PagedTiles {
     }
     __device__ __forceinline__ void look_up(int k0) {
 #pragma unroll
-        for (int i = 0; i < Loads::kPerWave; ++i) page[i] = table[position(k0, i) / p.page_size];
+        for (int i = 0; i < Loads::kPerWave; ++i) page[i] = table[p.page_size(position(k0, i))];
     }
     __device__ __forceinline__ void load(char* k_tile, char* v_tile, int k0) {
         const int chunk = Loads::chunk();
         if (chunk * 8 < p.dim) {
 #pragma unroll
             for (int i = 0; i < Loads::kPerWave; ++i) {
-                const int64_t slot = position(k0, i) % p.page_size;
+                const int64_t slot = slot_of(p, position(k0, i));
                 if (page[i] >= 0 && page[i] < p.pages) {
                     load_to_lds(keys + page[i] * key_cache.page_bytes + slot * key_cache.token_bytes + chunk * 16, Loads::place(k_tile, i));
                     load_to_lds(values + page[i] * value_cache.page_bytes + slot * value_cache.token_bytes + chunk * 16,
@@ -351,7 +355,7 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_wide_kernel(Rows q,
     // A page that is not there: every tile is masked, by what the table says of its keys.
     bool lost = false;
     if (begin < end)
-        for (int i = begin / p.page_size + static_cast<int>(threadIdx.x); i <= (end - 1) / p.page_size; i += kBlock)
+        for (int i = static_cast<int>(p.page_size(begin) + threadIdx.x); i <= static_cast<int>(p.page_size(end - 1)); i += kBlock)
             lost |= table[i] < 0 || table[i] >= p.pages;
     lost = __syncthreads_or(lost);
 
@@ -366,7 +370,7 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_wide_kernel(Rows q,
         uint32_t word = row.seen(tree != nullptr, k0, ahead) & first_keys(end, k0);
         if (lost) {
             const int position = k0 + lane % 32;
-            const int page = position < end ? table[position / p.page_size] : -1;
+            const int page = position < end ? table[p.page_size(position)] : -1;
             word &= static_cast<uint32_t>(wave_ballot(page >= 0 && page < p.pages));
         }
         return word;
@@ -520,7 +524,7 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
     const uint64_t blocks = (q_tokens * (q_heads / kv_heads) / rows + requests) * kv_heads;
     if (blocks * parts > 0x7FFFFFFFull / kBlock || parts > 65535 || (parts > 1 && q_tokens * q_heads > 0x7FFFFFFFull / kBlock)) return set_error(kInvalidArgument, "%s: too many tiles", what);
     const Paged p{static_cast<int>(requests), static_cast<int>(q_tokens), static_cast<int>(q_heads), static_cast<int>(kv_heads),
-                  static_cast<int>(dim), static_cast<int>(page_size), static_cast<int>(pages), static_cast<int>(table_stride),
+                  static_cast<int>(dim), Divider(page_size), static_cast<int>(pages), static_cast<int>(table_stride),
                   static_cast<int>(table_width), static_cast<int>(parts), scale};
     Parts sums{nullptr, static_cast<F32x2*>(temp)};
     if (parts > 1) sums.out = reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(parts, q_tokens * q_heads));

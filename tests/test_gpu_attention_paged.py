@@ -55,7 +55,7 @@ def test_plan_small(hip, dev, page):
     check_plan(hip, [0, 0], [0, 0], page, 2)
 
 
-@pytest.mark.parametrize("requests", [63, 64, 65, 255, 256, 257, 1000, 1023, 1025, 2049, 5000, 9000])
+@pytest.mark.parametrize("requests", [63, 64, 65, 255, 256, 257, 1000, 1023, 1025, 2049, 4096, 4097, 5000, 5120, 5121, 9000, 11000])
 def test_plan_request_counts(hip, dev, requests):
     rng = random.Random(requests)
     cached = [rng.choice([0, rng.randrange(40)]) for _ in range(requests)]
@@ -65,6 +65,20 @@ def test_plan_request_counts(hip, dev, requests):
 
 def test_plan_one_long_prompt(hip, dev):
     check_plan(hip, [0, 3000, 1], [20_000, 1, 4001], 16, 1300)
+
+
+@pytest.mark.parametrize("low,high", [(0, 300), (1, 3), (2000, 3000)])
+def test_plan_many_tokens(hip, dev, low, high):
+    """More tokens than one a thread: threads take several, across requests, pages and the end of the buffers."""
+    rng = random.Random(high)
+    requests = 300_000 // (high // 2 + 1) + 1
+    requests = min(requests, 8192)
+    cached = [rng.randrange(60) for _ in range(requests)]
+    new = [rng.randrange(low, high + 1) for _ in range(requests)]
+    for page, extra in ((16, 0), (24, 3), (1, 300_000)):
+        if page == 1 and high > 3:
+            continue
+        check_plan(hip, cached, new, page, -(-(60 + high) // page), extra=max(extra, 263_000 - sum(new)))
 
 
 def test_plan_where_pages_run_out(hip, dev):
