@@ -18,7 +18,11 @@ constexpr int kNarrowRows = 32;
 constexpr int kWaveKeys = 32;                  // keys of a wave at a time
 constexpr int kKeyStep = kWaves * kWaveKeys;   // keys of a workgroup at a time
 constexpr int kPartKeys = 256;                 // at least so many keys make a part
-constexpr int kGridTarget = 1024;              // workgroups that fill the device
+// Workgroups wanted, if all requests were the longest.  Narrow: two for each compute unit, which is what is resident (one
+// request of 131,000 keys: 119 us with 1,024, 116 with 512, 120 with 256).  Wide: three times as many, because a long
+// request's parts are few and end together (24 trees: 116 us with 512, 113 with 1,024, 105 with 1,536).
+constexpr int kNarrowGrid = 512;
+constexpr int kWideGrid = 1536;
 
 struct Paged {
     int requests;
@@ -30,7 +34,8 @@ struct Paged {
     int pages;
     int table_stride;
     int table_width;
-    int parts;  // of a long request
+    int parts;  // of the longest request
+    int part;   // keys of each
     float scale;
 };
 
@@ -38,11 +43,12 @@ __device__ __forceinline__ int slot_of(const Paged& p, uint32_t position) {
     return static_cast<int>(position - p.page_size(position) * p.page_size.by);
 }
 
-// Keys of one part of a request: the same for every part, a multiple of a workgroup's step.
-__device__ __forceinline__ int part_keys(int length, int parts) {
-    int per = (length + parts - 1) / parts;
-    per = per > kPartKeys ? per : kPartKeys;
-    return (per + kKeyStep - 1) / kKeyStep * kKeyStep;
+// Keys of one part: the same for every request, so that parts are alike and a short request is one; more where a request is
+// longer than the caller said.
+__device__ __forceinline__ int part_keys(int length, const Paged& p) {
+    const int64_t held = static_cast<int64_t>(p.part) * p.parts;
+    if (length <= held) return p.part;
+    return ((length - 1) / p.parts + kKeyStep) / kKeyStep * kKeyStep;
 }
 
 struct Work {
@@ -140,7 +146,7 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
     if (!find_work(w, q_offsets, kv_lengths, p, kNarrowRows, blockIdx.x / p.kv_heads)) return;
-    const int per = part_keys(w.length, p.parts);
+    const int per = part_keys(w.length, p);
     const int64_t part_begin = static_cast<int64_t>(blockIdx.y) * per;
     if (part_begin >= w.length && blockIdx.y > 0) return;
     const int begin = static_cast<int>(part_begin), end = w.length - begin > per ? begin + per : w.length;
@@ -341,7 +347,7 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_wide_kernel(Rows q,
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
     if (!find_work(w, q_offsets, kv_lengths, p, kRowTile, blockIdx.x / p.kv_heads)) return;
-    const int per = part_keys(w.length, p.parts);
+    const int per = part_keys(w.length, p);
     const int64_t part_begin = static_cast<int64_t>(blockIdx.y) * per;
     if (part_begin >= w.length && blockIdx.y > 0) return;
     const int begin = static_cast<int>(part_begin), end = w.length - begin > per ? begin + per : w.length;
@@ -419,7 +425,7 @@ __global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, 
     if (request < 0) return;
     Work w;
     take_request(w, q_offsets, kv_lengths, p, request);
-    const int per = part_keys(w.length, p.parts);
+    const int per = part_keys(w.length, p);
     if (token >= w.token0 + w.tokens || w.length <= per) return;
     const int count = (w.length + per - 1) / per;
     const int chunk = threadIdx.x % 16, group = threadIdx.x / 16 % GROUPS, local = threadIdx.x / 16 / GROUPS;
@@ -477,12 +483,13 @@ uint64_t parts_of(uint64_t requests, uint64_t q_tokens, uint64_t max_kv, uint64_
     const uint64_t rows = ceil_div(q_tokens * group, tile_rows(requests, q_tokens, group));
     const uint64_t busy = (rows > requests ? rows : requests) * kv_heads;
     const uint64_t most = ceil_div(max_kv, kPartKeys);
-    // Half as many wide workgroups, whose sums are four times as many, as narrow ones.
-    const uint64_t target = tile_rows(requests, q_tokens, group) == kNarrowRows ? kGridTarget : kGridTarget / 2;
+    const uint64_t target = tile_rows(requests, q_tokens, group) == kNarrowRows ? kNarrowGrid : kWideGrid;
     uint64_t parts = ceil_div(target, busy ? busy : 1);
     parts = parts < most ? parts : most;
     return parts ? parts : 1;
 }
+
+uint64_t keys_of_part(uint64_t max_kv, uint64_t parts) { return align_up(ceil_div(max_kv ? max_kv : 1, parts), kKeyStep); }
 
 size_t stats_bytes(uint64_t parts, uint64_t rows) { return align_up(parts * rows * sizeof(F32x2), kViewAlign); }
 
@@ -510,7 +517,7 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
         return set_error(kInvalidArgument, "%s: a block table's row must hold its width", what);
     if (q_tokens > 0x7FFFFFFFull || q_tokens * (q_heads / kv_heads) > 0x7FFFFFFFull || requests > 0x7FFFFFFu)
         return set_error(kInvalidArgument, "%s: too many tokens or requests", what);
-    if (max_kv_length > 0x7FFFFFFFull) return set_error(kInvalidArgument, "%s: requests too long", what);
+    if (max_kv_length > 0x7FFFFF00ull) return set_error(kInvalidArgument, "%s: requests too long", what);
     if (!(scale > 0.f) || scale == INFINITY) return set_error(kInvalidArgument, "%s: the scale must be positive and finite", what);
     if (requests == 0 || q_tokens == 0) return kOk;
     if (!q_offsets || !kv_lengths || (table_width && !block_table))
@@ -525,7 +532,8 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
     if (blocks * parts > 0x7FFFFFFFull / kBlock || parts > 65535 || (parts > 1 && q_tokens * q_heads > 0x7FFFFFFFull / kBlock)) return set_error(kInvalidArgument, "%s: too many tiles", what);
     const Paged p{static_cast<int>(requests), static_cast<int>(q_tokens), static_cast<int>(q_heads), static_cast<int>(kv_heads),
                   static_cast<int>(dim), Divider(page_size), static_cast<int>(pages), static_cast<int>(table_stride),
-                  static_cast<int>(table_width), static_cast<int>(parts), scale};
+                  static_cast<int>(table_width), static_cast<int>(parts),
+                  static_cast<int>(keys_of_part(max_kv_length, parts)), scale};
     Parts sums{nullptr, static_cast<F32x2*>(temp)};
     if (parts > 1) sums.out = reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(parts, q_tokens * q_heads));
     {
