@@ -67,6 +67,17 @@ __device__ __forceinline__ U32x4 pack_step(const F32x16& p, int s) {
                  pack2<T>(p[8 * s + 4], p[8 * s + 5]), pack2<T>(p[8 * s + 6], p[8 * s + 7])};
 }
 
+// Whether any of a lane's sums is an infinity or NaN.
+template <int N>
+__device__ __forceinline__ bool any_not_finite(const F32x16 (&acc)[N]) {
+    float zero = 0.f;
+#pragma unroll
+    for (int d = 0; d < N; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) zero += acc[d][r] * 0.f;
+    return !(zero == 0.f);
+}
+
 // A value of this lane and of the lane 32 away: the lower lane's first.  (The two words are copied out before they are
 // reinterpreted: a bit cast of a vector's element would take its first.)
 struct Halves {

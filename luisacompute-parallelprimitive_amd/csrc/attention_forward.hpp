@@ -176,6 +176,109 @@ __device__ __forceinline__ void forward_tile(RowState<DP>& state, const char* k_
     state.total += sum;
 }
 
+// Infinities and NaN in masked places.  A masked weight is zero, but zero times an infinity or NaN is NaN: in a tile of keys
+// that only some rows see, the matrix product carries such a value to the others.  The kernels do not look for them (the
+// guards in every tile's products cost a third of the registers): a wave whose sums come out as anything but finite numbers
+// takes its rows again, one at a time and without matrix instructions, and never touches what a row does not see.
+
+// The keys of one row, in memory: a packed sequence, or pages (block_table not null).
+struct KeySource {
+    const char* keys;  // of the head; the first row, or the first page
+    const char* values;
+    int64_t key_bytes, value_bytes;            // from a token to the next, in a page or in the sequence
+    int64_t key_page_bytes, value_page_bytes;
+    const int32_t* block_table;  // the request's row of it
+    Divider page_size;
+    int pages;
+    // Offsets of a position; whether its page is there.
+    __device__ __forceinline__ bool find(int position, int64_t& key, int64_t& value) const {
+        key = position * key_bytes, value = position * value_bytes;
+        if (block_table == nullptr) return true;
+        const int cell = static_cast<int>(page_size(position)), page = block_table[cell];
+        const bool there = page >= 0 && page < pages;
+        const int64_t slot = position - static_cast<int64_t>(cell) * page_size.by, held = there ? page : 0;
+        key = held * key_page_bytes + slot * key_bytes, value = held * value_page_bytes + slot * value_bytes;
+        return there;
+    }
+};
+
+// Which keys a row sees: the first `count`, or with a tree those before `ahead` and then the tree's bits.
+struct RowSight {
+    int count, ahead;
+    bool tree_given;
+    uint64_t tree;
+    __device__ __forceinline__ bool sees(int position) const {
+        if (!tree_given || position < ahead) return position < (tree_given ? ahead : count);
+        return position - ahead < 64 && (tree >> (position - ahead) & 1);
+    }
+};
+
+struct CarefulRow {
+    float top, total, low, high;  // scale and sum; the products with the values' items 2 * lane and 2 * lane + 1
+};
+
+// One row against the keys in [begin, end): a lane a key for the scores, a lane two items for the products.
+template <typename T>
+__device__ __forceinline__ CarefulRow careful_row(const char* q_row, KeySource source, RowSight sight, int begin, int end, int dim, float c) {
+    const int lane = threadIdx.x % kWave;
+    CarefulRow row{-INFINITY, 0.f, 0.f, 0.f};
+    for (int k0 = begin; k0 < end; k0 += kWave) {
+        const int position = k0 + lane;
+        int64_t key = 0, value = 0;
+        bool seen = position < end && sight.sees(position);
+        seen = seen && source.find(position, key, value);
+        float score = -INFINITY;
+        if (seen) {
+            score = 0.f;
+            for (int d = 0; d < dim; d += 2) {
+                const uint32_t a = *reinterpret_cast<const uint32_t*>(q_row + d * 2);
+                const uint32_t b = *reinterpret_cast<const uint32_t*>(source.keys + key + d * 2);
+                score += item_low<T>(a) * item_low<T>(b);
+                score += item_high<T>(a) * item_high<T>(b);
+            }
+        }
+        float high = score;
+#pragma unroll
+        for (int step = 32; step > 0; step /= 2) high = fmaxf(high, __shfl_xor(high, step));
+        high = fmaxf(high, row.top);
+        const float base = high == -INFINITY ? 0.f : high * c;
+        const float alpha = row.top == -INFINITY ? 0.f : exp2_fast(row.top * c - base);
+        const float weight = seen ? exp2_fast(score * c - base) : 0.f;
+        float sum = weight;
+#pragma unroll
+        for (int step = 32; step > 0; step /= 2) sum += __shfl_xor(sum, step);
+        row.top = high;
+        row.total = row.total * alpha + sum;
+        row.low *= alpha;
+        row.high *= alpha;
+        uint64_t left = wave_ballot(seen);
+        while (left != 0) {
+            const int j = __ffsll(static_cast<unsigned long long>(left)) - 1;
+            left &= left - 1;
+            const float w = wave_read_lane(weight, j);
+            const int64_t from = wave_read_lane(value, j);
+            if (2 * lane < dim) {
+                const uint32_t v = *reinterpret_cast<const uint32_t*>(source.values + from + lane * 4);
+                row.low += w * item_low<T>(v);
+                row.high += w * item_high<T>(v);
+            }
+        }
+    }
+    return row;
+}
+
+__device__ __forceinline__ float row_lse(float top, float total, float scale) {
+    return total == 0.f ? -INFINITY : top * scale + __logf(total);
+}
+
+// Writes a careful row's output.
+template <typename T>
+__device__ __forceinline__ void store_careful(char* to, const CarefulRow& row, int dim) {
+    const int lane = threadIdx.x % kWave;
+    const float f = row.total == 0.f ? 0.f : 1.f / row.total;
+    if (2 * lane < dim) *reinterpret_cast<uint32_t*>(to + lane * 4) = pack2<T>(row.low * f, row.high * f);
+}
+
 // Runs the tiles from `begin` to `end`, SIZE apart, with two sets of buffers: while one is computed on, the other is loaded.
 // The sets are distinct arrays, so that reads of one do not wait for loads of the other.
 template <int SIZE, typename LoadEven, typename LoadOdd, typename StepEven, typename StepOdd>

@@ -18,6 +18,7 @@ struct Shape {
     int dim;
     float scale;
     int causal;
+    Divider one{1};  // (the pages of keys that are in none)
 };
 
 struct Span {
@@ -57,7 +58,7 @@ struct RowRange {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(kBlock, 2) void attention_packed_kernel(Rows q, Rows k, Rows v, Rows out, float* __restrict__ lse,
+__global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_kernel(Rows q, Rows k, Rows v, Rows out, float* __restrict__ lse,
                                                                      const int32_t* __restrict__ q_offsets,
                                                                      const int32_t* __restrict__ k_offsets, Shape shape,
                                                                      int tiles) {
@@ -93,12 +94,25 @@ __global__ __launch_bounds__(kBlock, 2) void attention_packed_kernel(Rows q, Row
                         PackedRows<DP, kKeyTile>(k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim),
                         PackedRows<DP, kKeyTile>(v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim), qf, c, 0,
                         range.end, range.wave_end, range.full, [&](int k0) { return first_keys(range.count, k0); });
+    if (wave_ballot(any_not_finite(state.acc)) != 0) {
+        const KeySource source{k.at(keys.begin, kv_head), v.at(keys.begin, kv_head), k.token_bytes, v.token_bytes, 0, 0, nullptr,
+                               shape.one, 0};
+        for (int r = row - lane % 32, i = 0; i < kRowsPerWave && r < rows.size; ++i, ++r) {
+            const int count = RowRange(shape, rows, keys, row0, r).count;
+            const CarefulRow result = careful_row<T>(q.at(rows.begin + r, head), source, RowSight{count, 0, false, 0}, 0, count,
+                                                     shape.dim, c);
+            store_careful<T>(out.at(rows.begin + r, head), result, shape.dim);
+            if (lse != nullptr && lane == 0)
+                lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + r] = row_lse(result.top, result.total, shape.scale);
+        }
+        return;
+    }
     const float total = halves_sum(state.total);
     if (!there) return;
     store_row<T, DP>(out, rows.begin + row, head, state.acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
     if (lse != nullptr && half == 0)
         lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row] =
-            total == 0.f ? -INFINITY : state.top * shape.scale + __logf(total);
+            row_lse(state.top, total, shape.scale);
 }
 
 // ---- gradients ---------------------------------------------------------------------------------------------------

@@ -125,8 +125,29 @@ struct Parts {
     }
 };
 
-__device__ __forceinline__ float row_lse(float top, float total, float scale) {
-    return total == 0.f ? -INFINITY : top * scale + __logf(total);
+// Rows [first, first + rows) of a tile again, one wave, every `step`-th: results or a part's sums.
+template <typename T>
+__device__ __forceinline__ void careful_rows(const Rows& q, const Pages& key_cache, const Pages& value_cache, const Rows& out, float* lse,
+                                             const Parts& parts, const int32_t* table, const uint64_t* tree, const Paged& p,
+                                             const Work& w, int kv_head, int begin, int end, bool whole, int first, int rows, int step) {
+    const int lane = threadIdx.x % kWave;
+    const KeySource source{key_cache.at(0, 0, kv_head), value_cache.at(0, 0, kv_head), key_cache.token_bytes, value_cache.token_bytes,
+                           key_cache.page_bytes, value_cache.page_bytes, table, p.page_size, p.pages};
+    const int ahead = w.length - w.tokens;
+    for (int r = first; r < first + rows && r < w.rows; r += step) {
+        const PagedRow row(w, p, tree, kv_head, r);
+        const int64_t t = w.token0 + row.token;
+        const CarefulRow result = careful_row<T>(q.at(t, row.head), source, RowSight{ahead + row.token + 1, ahead, tree != nullptr, row.tree},
+                                                 begin, end, p.dim, p.scale * kLog2e);
+        if (whole) {
+            store_careful<T>(out.at(t, row.head), result, p.dim);
+            if (lse != nullptr && lane == 0) lse[static_cast<int64_t>(row.head) * p.q_tokens + t] = row_lse(result.top, result.total, p.scale);
+        } else {
+            const int64_t at = parts.row(p, blockIdx.y, row.head, t);
+            if (lane == 0) parts.stats[at] = F32x2{result.top, result.total};
+            if (2 * lane < p.dim) *reinterpret_cast<F32x2*>(parts.out + at * p.dim + 2 * lane) = F32x2{result.low, result.high};
+        }
+    }
 }
 
 template <typename T, int DP>
@@ -238,6 +259,11 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
                 state.acc[d] = T::mfma(read_columns<DP>(v_tile, i * 16, d * 32), pf, state.acc[d]);
         }
     }
+    if (__syncthreads_or(any_not_finite(state.acc))) {
+        careful_rows<T>(q, key_cache, value_cache, out, lse, parts, table, tree, p, w, kv_head, begin, end, whole, w.row0 + wave,
+                        kNarrowRows - wave, kWaves);
+        return;
+    }
     const float total = halves_sum(state.total);
     if (half == 0) {
         stats[0][wave][lane] = state.top;
@@ -333,7 +359,7 @@ struct PagedTiles {
 };
 
 template <typename T, int DP>
-__global__ __launch_bounds__(kBlock, 2) void attention_paged_wide_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
+__global__ __launch_bounds__(kBlock, DP <= 64 ? 4 : 2) void attention_paged_wide_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
                                                                          float* __restrict__ lse, Parts parts,
                                                                          const int32_t* __restrict__ block_table,
                                                                          const int32_t* __restrict__ q_offsets,
@@ -390,6 +416,11 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_wide_kernel(Rows q,
     };
     pass_tiles<kKeyTile>(begin, end, [&](int k0) { source.load(k_even, v_even, k0); }, [&](int k0) { source.load(k_odd, v_odd, k0); },
                          [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
+    if (wave_ballot(any_not_finite(state.acc)) != 0) {
+        careful_rows<T>(q, key_cache, value_cache, out, lse, parts, table, tree, p, w, kv_head, begin, end, whole,
+                        w.row0 + wave * kRowsPerWave, kRowsPerWave, 1);
+        return;
+    }
     const float total = halves_sum(state.total);
     if (!row.there) return;
     const int64_t t = w.token0 + row.token;

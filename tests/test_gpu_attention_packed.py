@@ -252,3 +252,36 @@ def test_no_lse_and_nothing_to_do(hip, dev):
     dk, dv = torch.full_like(q, 7.0), torch.full_like(q, 7.0)
     hip.attention_packed_backward("bf16", empty, q, q, empty, torch.empty(2, 0, device="cuda"), empty, none, o, empty, dk, dv)
     assert bool((dk == 0).all()) and bool((dv == 0).all())  # keys without rows
+
+
+@pytest.mark.parametrize("suffix,dim", [("bf16", 64), ("f16", 128), ("bf16", 80)])
+@pytest.mark.parametrize("where", [0, 37, 64, 127, 199])
+def test_infinities_and_nan_reach_the_rows_that_see_them(hip, dev, suffix, dim, where):
+    """A key or value that is not finite, inside a causal sequence: rows before it are as if it were zero, the others hold
+    what the formula gives."""
+    dtype, n = DTYPE[suffix], 200
+    q, k, v = (rows(dtype, n, h, dim, s) for s, h in ((1, 4), (2, 2), (3, 2)))
+    o = oracle.offsets_of([n])
+    clean = [x.clone() for x in (k, v)]
+    for x in clean:
+        x[where] = 0
+    want = oracle.packed(q, clean[0], clean[1], o, o, True, dim ** -0.5)
+    before = torch.arange(n) < where
+    for bad in (math.nan, math.inf, -math.inf):
+        broken = v.clone()
+        broken[where, 1, 5] = bad
+        got = run(hip, suffix, q, k, broken, o, o, True)
+        for name, axis in (("out", 0), ("lse", 1)):
+            pick = lambda x: x.cpu().index_select(axis, before.nonzero()[:, 0])
+            oracle.check(name, pick(got[name]), (pick(want[name][0]), pick(want[name][1])))
+        after = got["out"].cpu()[~before].float()
+        column = after[:, 2:, 5]
+        assert torch.isnan(column).all() if math.isnan(bad) else (column == bad).all()
+        after[:, 2:, 5] = 0
+        assert torch.isfinite(after).all() and torch.isfinite(got["lse"]).all()
+        broken = k.clone()
+        broken[where, 0, 3] = math.nan
+        got = run(hip, suffix, q, broken, v, o, o, True)
+        oracle.check("out", got["out"].cpu()[before], (want["out"][0][before], want["out"][1][before]))
+        assert torch.isnan(got["out"].cpu()[~before][:, :2].float()).all()
+        assert torch.isfinite(got["out"].cpu()[:, 2:].float()).all()

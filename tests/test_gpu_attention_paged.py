@@ -356,3 +356,23 @@ def test_same_bits_again_on_another_stream_and_in_a_graph(hip, dev):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, want)
+
+
+@pytest.mark.parametrize("heads,max_kv", [(2, 400), (2, 9000), (16, 400)])
+def test_infinities_and_nan_reach_the_rows_that_see_them(hip, dev, heads, max_kv):
+    """A drafted token whose value is not finite: its siblings do not see it.  One row of parts, several, and wide tiles."""
+    words = [1, 3, 5, 9, 0b10011]  # a root, three children, and a child of the first child
+    s = make("bf16", [900, 305], [5, 5], heads, 1, 64, 16, tree=words * 2)
+    want = oracle.paged(s["q"], s["key_cache"], s["value_cache"], s["table"], s["q_offsets"], s["kv"], s["tree"], 0.125)
+    place = 305 - 5 + 2  # the second child of the second request
+    page = int(s["table"][1, place // 16])
+    for bad in (math.nan, math.inf):
+        s["value_cache"][page, place % 16, 0, 7] = bad
+        out, lse = run_paged(hip, "bf16", s, max_kv)
+        sees = torch.zeros(10, dtype=torch.bool)
+        sees[7] = True
+        oracle.check("lse", lse, want["lse"])
+        oracle.check("out", out.cpu()[~sees], (want["out"][0][~sees], want["out"][1][~sees]))
+        mine = out.cpu()[sees].float()
+        assert torch.isnan(mine[:, :, 7]).all() if math.isnan(bad) else (mine[:, :, 7] == bad).all()
+        assert torch.isfinite(mine[:, :, :7]).all() and torch.isfinite(mine[:, :, 8:]).all()
