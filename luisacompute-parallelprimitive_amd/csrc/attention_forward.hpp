@@ -19,19 +19,19 @@ constexpr int kKeyTile = 64;                     // keys in LDS at a time
 // of 2): weights are then at most 2^8, within the 16-bit types, and the products are rescaled a few times a row at most.
 constexpr float kSlack = 8.f;
 
-// Direct loads of a tile by four waves, a block of rows each: a lane's chunk is the same in all of them, and its row goes up
-// by kRowStep.
-template <int DP, int ROWS>
+// Direct loads of a tile by some waves side by side, a block of rows each: a lane's chunk is the same in all of them, and its
+// row goes up by kRowStep.
+template <int DP, int ROWS, int WAVES = kWaves>
 struct TileLoads {
-    static constexpr int kRowStep = kWaves * Tile<DP>::kBlockRows;
+    static constexpr int kRowStep = WAVES * Tile<DP>::kBlockRows;
     static constexpr int kPerWave = ROWS / kRowStep;
     static_assert(kPerWave > 0 && ROWS % kRowStep == 0);
     __device__ __forceinline__ static int row() {
-        return threadIdx.x % kBlock / kWave * Tile<DP>::kBlockRows + Tile<DP>::lane_row(threadIdx.x % kWave);
+        return threadIdx.x % (WAVES * kWave) / kWave * Tile<DP>::kBlockRows + Tile<DP>::lane_row(threadIdx.x % kWave);
     }
     __device__ __forceinline__ static int chunk() { return Tile<DP>::lane_chunk(threadIdx.x % kWave); }
     __device__ __forceinline__ static char* place(char* tile, int i) {
-        return tile + (i * kWaves + __builtin_amdgcn_readfirstlane(threadIdx.x % kBlock / kWave)) * Tile<DP>::kBlockBytes;
+        return tile + (i * WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x % (WAVES * kWave) / kWave)) * Tile<DP>::kBlockBytes;
     }
 };
 
@@ -41,9 +41,9 @@ __device__ __forceinline__ void load_to_lds(const char* from, char* to) {
 }
 
 // Zeros where a row of fewer items than DP has none; loads never touch those chunks.
-template <int DP, int ROWS>
+template <int DP, int ROWS, int WAVES = kWaves>
 __device__ __forceinline__ void clear_past(char* tile, int dim) {
-    using Loads = TileLoads<DP, ROWS>;
+    using Loads = TileLoads<DP, ROWS, WAVES>;
     if (Loads::chunk() * 8 < dim) return;
 #pragma unroll
     for (int i = 0; i < Loads::kPerWave; ++i)
@@ -52,9 +52,9 @@ __device__ __forceinline__ void clear_past(char* tile, int dim) {
 
 // Rows of a packed sequence: those past its last are loaded as its last, and masked.  Addresses are a scalar base and a
 // lane's offset of 32 bits, which stays the same from tile to tile (the host keeps a tile's bytes below 2^31).
-template <int DP, int ROWS>
+template <int DP, int ROWS, int WAVES = kWaves>
 struct PackedRows {
-    using Loads = TileLoads<DP, ROWS>;
+    using Loads = TileLoads<DP, ROWS, WAVES>;
     const char* base;  // the sequence's first row of the head
     int64_t token_bytes;
     int size;

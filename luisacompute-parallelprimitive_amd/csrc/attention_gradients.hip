@@ -40,14 +40,17 @@ __global__ __launch_bounds__(kBlock) void attention_row_stats_kernel(Rows out, R
     }
 }
 
-constexpr int kQueryTile = 32;
+constexpr int kQueryTile = 32;  // rows that pass by at a time: the next ones are loaded while these are worked on
+constexpr int kAllWaves = kTeams * kWaves;
 
-// LDS of a gradient workgroup.  Four distinct arrays: reads of one do not wait for loads of another.
+// LDS of a gradient workgroup.  Distinct arrays: reads of one do not wait for loads of another.
 template <int DP>
 struct GradientMemory {
-    static constexpr int kTilesBytes = kTeams * Tile<DP>::bytes(kKeyTile);
-    static_assert(DP / 16 * kBlock * 16 <= kTilesBytes, "half of a team's sums fit where the tiles were");
+    static constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);  // of keys or values, or two teams' rows that pass by
+    static_assert(kTileBytes >= kTeams * Tile<DP>::bytes(kQueryTile));
+    static_assert(DP / 32 * kBlock * 16 <= kTileBytes, "a quarter of a team's sums fits where a tile was");
     char *a, *b, *c, *d;
+    char* values;  // kRowTile rows
     float *stats_even, *stats_odd;
 };
 
@@ -63,40 +66,37 @@ struct GradientArgs {
     int parts;
 };
 
-// dQ of a tile of query rows, of two heads: a team of four waves each, of one key head where its group is even.
+// dQ: two teams of four waves share the keys' and values' tiles.  They take a tile of rows of two heads of one key head, or
+// where its group is odd two tiles of rows of one head.
 template <typename T, int DP>
 __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMemory<DP>& memory, int block) {
-    constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);
     const Shape& shape = g.shape;
-    const int group = shape.q_heads / shape.kv_heads, pairs = (shape.q_heads + 1) / 2;
-    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / kBlock), pair = block % pairs;
-    int kv_head, head;
-    bool here = true;
-    if (group % 2 == 0) {
-        kv_head = pair % shape.kv_heads;
-        head = kv_head * group + pair / shape.kv_heads * 2 + team;
-    } else {
-        const int number = 2 * pair + team;
-        here = number < shape.q_heads;
-        kv_head = number % shape.kv_heads;
-        head = here ? kv_head * group + number / shape.kv_heads : 0;
-    }
-    const TilePlace place = find_tile(g.q_offsets, shape.sequences, 1, kRowTile, g.row_tiles - 1 - block / pairs);
+    const int group = shape.q_heads / shape.kv_heads;
+    const bool two_heads = group % 2 == 0;
+    const int team = __builtin_amdgcn_readfirstlane(threadIdx.x / kBlock);
+    const int units = two_heads ? shape.q_heads / 2 : shape.q_heads, unit = block % units;
+    const int kv_head = unit % shape.kv_heads;
+    const int head = kv_head * group + (two_heads ? unit / shape.kv_heads * 2 + team : unit / shape.kv_heads);
+    const int tile_rows = two_heads ? kRowTile : kTeams * kRowTile;
+    const TilePlace place = find_tile(g.q_offsets, shape.sequences, 1, tile_rows, g.row_tiles - 1 - block / units);
     if (place.sequence < 0) return;
     const Span rows = span_of(g.q_offsets, place.sequence, shape.q_tokens);
-    const int row0 = place.tile * kRowTile;
-    if (row0 >= rows.size) return;
+    const int first_row = place.tile * tile_rows;
+    if (first_row >= rows.size) return;
     const Span keys = span_of(g.k_offsets, place.sequence, shape.k_tokens);
     const int lane = threadIdx.x % kWave, half = lane / 32;
+    const int row0 = two_heads ? first_row : first_row + team * kRowTile;
     const int row = row0 + threadIdx.x % kBlock / kWave * kRowsPerWave + lane % 32;
-    const bool there = here && row < rows.size;
+    const bool there = row < rows.size;
     const RowRange range(shape, rows, keys, row0, row);
-    const int wave_end = here ? range.wave_end : 0;
+    // Keys that any row of either team sees: the later team's, if it has rows.
+    const int end = two_heads || first_row + kRowTile >= rows.size ? RowRange(shape, rows, keys, first_row, row).end
+                                                                   : RowRange(shape, rows, keys, first_row + kRowTile, row).end;
     const float c = shape.scale * kLog2e;
-    char* k_even = memory.a + team * kTileBytes;
-    char* v_even = memory.b + team * kTileBytes;
-    char* k_odd = memory.c + team * kTileBytes;
-    char* v_odd = memory.d + team * kTileBytes;
+    char* k_even = memory.a;
+    char* v_even = memory.b;
+    char* k_odd = memory.c;
+    char* v_odd = memory.d;
 
     U32x4 qf[DP / 16], of[DP / 16];
     load_row<DP>(qf, g.q, rows.begin + row, head, there, shape.dim);
@@ -104,17 +104,16 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
     const int64_t stat = static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row;
     const float base = there ? g.stats[stat] : INFINITY;
     const float delta = there ? g.stats[static_cast<int64_t>(shape.q_heads) * shape.q_tokens + stat] : 0.f;
-    for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile>(tile, shape.dim);
+    for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile, kAllWaves>(tile, shape.dim);
     F32x16 acc[DP / 32] = {};
-    const PackedRows<DP, kKeyTile> key_rows(g.k.at(keys.begin, kv_head), g.k.token_bytes, keys.size, shape.dim);
-    const PackedRows<DP, kKeyTile> value_rows(g.v.at(keys.begin, kv_head), g.v.token_bytes, keys.size, shape.dim);
+    const PackedRows<DP, kKeyTile, kAllWaves> key_rows(g.k.at(keys.begin, kv_head), g.k.token_bytes, keys.size, shape.dim);
+    const PackedRows<DP, kKeyTile, kAllWaves> value_rows(g.v.at(keys.begin, kv_head), g.v.token_bytes, keys.size, shape.dim);
     const auto load = [&](char* k_tile, char* v_tile, int k0) {
-        if (!here) return;
         key_rows.load(k_tile, k0);
         value_rows.load(v_tile, k0);
     };
     const auto step = [&](const char* k_tile, const char* v_tile, int k0) {
-        if (k0 >= wave_end) return;
+        if (k0 >= range.wave_end) return;
 #pragma unroll
         for (int b = 0; b < kKeyTile / 32; ++b) {
             F32x16 s = {}, dp = {};
@@ -139,7 +138,7 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
             }
         }
     };
-    pass_tiles<kKeyTile>(0, range.end, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
+    pass_tiles<kKeyTile>(0, end, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
                          [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
     if (there) store_row<T, DP>(g.dq, rows.begin + row, head, acc, shape.scale, shape.dim);
 }
@@ -190,9 +189,13 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     const int wave_start = wave_key0 >= keys.size ? rows.size : shape.causal ? wave_key0 - shift : 0;
     const float c = shape.scale * kLog2e;
 
-    U32x4 kf[DP / 16], vf[DP / 16];
+    // Keys in registers; values in LDS, where both teams read them (in registers they left no room for fragments of the rows
+    // to be read ahead).  Rows past the last are its copies; their sums are not stored.
+    U32x4 kf[DP / 16];
     load_row<DP>(kf, k, keys.begin + key, kv_head, there, shape.dim);
-    load_row<DP>(vf, v, keys.begin + key, kv_head, there, shape.dim);
+    clear_past<DP, kRowTile, kAllWaves>(memory.values, shape.dim);
+    PackedRows<DP, kRowTile, kAllWaves>(v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim).load(memory.values, key0);
+    const char* values = memory.values + Tile<DP>::bytes(kRowsPerWave) * wave;
     for (char* tile : {q_even, o_even, q_odd, o_odd}) clear_past<DP, kQueryTile>(tile, shape.dim);
     F32x16 dk_acc[DP / 32] = {}, dv_acc[DP / 32] = {};
     const int all = rows.size > start ? (rows.size - start + kQueryTile - 1) / kQueryTile * group : 0;
@@ -207,7 +210,7 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
         if (at + team >= to) return;
         q_rows.load(q_tile, loads.row0, loads.head * q.head_bytes);
         o_rows.load(o_tile, loads.row0, loads.head * dout.head_bytes);
-        if (wave == 0) {
+        if (wave == 0) {  // lse by the lower half of the wave, delta by the upper
             const int row = loads.row0 + lane % 32 < rows.size ? loads.row0 + lane % 32 : rows.size - 1;
             __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) uint32_t*)(
                                                  s_rows + static_cast<int64_t>(loads.head) * shape.q_tokens + row),
@@ -217,42 +220,46 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     };
     const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile, int at) {
         if (at + team >= to) return;
-        const int r0 = steps.row0;
+        const int tile_row0 = steps.row0;
         steps.skip(kTeams);
-        if (r0 + kQueryTile <= wave_start) return;
-        F32x16 s = {}, dp = {};
 #pragma unroll
-        for (int i = 0; i < DP / 16; ++i) {
-            s = T::mfma(read_rows<DP>(q_tile, 0, i), kf[i], s);
-            dp = T::mfma(read_rows<DP>(o_tile, 0, i), vf[i], dp);
-        }
+        for (int b = 0; b < kQueryTile / 32; ++b) {
+            const int r0 = tile_row0 + 32 * b;
+            if (r0 + 32 <= wave_start || r0 >= rows.size) continue;
+            F32x16 s = {}, dp = {};
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const F32x4 l = *reinterpret_cast<const F32x4*>(&s_tile[acc_row(4 * j, half)]);
-            const F32x4 e = *reinterpret_cast<const F32x4*>(&s_tile[kQueryTile + acc_row(4 * j, half)]);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int r = 4 * j + i;
-                s[r] = exp2_fast(s[r] * c - l[i]);
-                dp[r] = s[r] * (dp[r] - e[i]);
+            for (int i = 0; i < DP / 16; ++i) {
+                s = T::mfma(read_rows<DP>(q_tile, 32 * b, i), kf[i], s);
+                dp = T::mfma(read_rows<DP>(o_tile, 32 * b, i), read_rows<DP>(values, 0, i), dp);
             }
-        }
-        if (r0 < full || r0 + kQueryTile > rows.size) {
-            const uint32_t word = (first_keys(rows.size, r0) & ~first_keys(first, r0)) >> (4 * half);
 #pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const bool seen = word & (1u << acc_row(r, 0));
-                s[r] = seen ? s[r] : 0.f;
-                dp[r] = seen ? dp[r] : 0.f;
+            for (int j = 0; j < 4; ++j) {
+                const F32x4 l = *reinterpret_cast<const F32x4*>(&s_tile[32 * b + acc_row(4 * j, half)]);
+                const F32x4 e = *reinterpret_cast<const F32x4*>(&s_tile[kQueryTile + 32 * b + acc_row(4 * j, half)]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int r = 4 * j + i;
+                    s[r] = exp2_fast(s[r] * c - l[i]);
+                    dp[r] = s[r] * (dp[r] - e[i]);
+                }
             }
-        }
+            if (r0 < full || r0 + 32 > rows.size) {
+                const uint32_t word = (first_keys(rows.size, r0) & ~first_keys(first, r0)) >> (4 * half);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const U32x4 pf = pack_step<T>(s, i), sf = pack_step<T>(dp, i);
+                for (int r = 0; r < 16; ++r) {
+                    const bool seen = word & (1u << acc_row(r, 0));
+                    s[r] = seen ? s[r] : 0.f;
+                    dp[r] = seen ? dp[r] : 0.f;
+                }
+            }
 #pragma unroll
-            for (int d = 0; d < DP / 32; ++d) {
-                dv_acc[d] = T::mfma(read_columns<DP>(o_tile, i * 16, d * 32), pf, dv_acc[d]);
-                dk_acc[d] = T::mfma(read_columns<DP>(q_tile, i * 16, d * 32), sf, dk_acc[d]);
+            for (int i = 0; i < 2; ++i) {
+                const U32x4 pf = pack_step<T>(s, i), sf = pack_step<T>(dp, i);
+#pragma unroll
+                for (int d = 0; d < DP / 32; ++d) {
+                    dv_acc[d] = T::mfma(read_columns<DP>(o_tile, 32 * b + i * 16, d * 32), pf, dv_acc[d]);
+                    dk_acc[d] = T::mfma(read_columns<DP>(q_tile, 32 * b + i * 16, d * 32), sf, dk_acc[d]);
+                }
             }
         }
     };
@@ -261,10 +268,11 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
                        [&](int x) { step(q_even, o_even, s_even, x); },
                        [&](int x) { step(q_odd, o_odd, s_odd, x); });
     // The first team ends with dK, the second with dV; each hands the other its share.
-    // (Over the tiles, which nothing is loaded into any more: half of the sums in each of two arrays.)
+    // (Over the tiles, which nothing is loaded into any more: a quarter of the sums in each of the four arrays.)
     const auto join_at = [&](int i) {
-        char* to = i < DP / 16 ? memory.a : memory.b;
-        return reinterpret_cast<F32x4*>(to + (i % (DP / 16) * kBlock + threadIdx.x % kBlock) * 16);
+        constexpr int kQuarter = DP / 32;
+        char* to = i < kQuarter ? memory.a : i < 2 * kQuarter ? memory.b : i < 3 * kQuarter ? memory.c : memory.d;
+        return reinterpret_cast<F32x4*>(to + (i % kQuarter * kBlock + threadIdx.x % kBlock) * 16);
     };
     const auto give = [&](const F32x16(&acc)[DP / 32]) {
 #pragma unroll
@@ -313,13 +321,14 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
 
 template <typename T, int DP>
 __global__ __launch_bounds__(kTeams* kBlock, 2) void attention_gradients_kernel(GradientArgs args) {
-    __shared__ __attribute__((aligned(16))) char a[GradientMemory<DP>::kTilesBytes];
-    __shared__ __attribute__((aligned(16))) char b[GradientMemory<DP>::kTilesBytes];
-    __shared__ __attribute__((aligned(16))) char c[GradientMemory<DP>::kTilesBytes];
-    __shared__ __attribute__((aligned(16))) char d[GradientMemory<DP>::kTilesBytes];
+    __shared__ __attribute__((aligned(16))) char a[GradientMemory<DP>::kTileBytes];
+    __shared__ __attribute__((aligned(16))) char b[GradientMemory<DP>::kTileBytes];
+    __shared__ __attribute__((aligned(16))) char c[GradientMemory<DP>::kTileBytes];
+    __shared__ __attribute__((aligned(16))) char d[GradientMemory<DP>::kTileBytes];
+    __shared__ __attribute__((aligned(16))) char values[Tile<DP>::bytes(kRowTile)];
     __shared__ __attribute__((aligned(16))) float stats_even[kTeams * 2 * kQueryTile];
     __shared__ __attribute__((aligned(16))) float stats_odd[kTeams * 2 * kQueryTile];
-    const GradientMemory<DP> memory{a, b, c, d, stats_even, stats_odd};
+    const GradientMemory<DP> memory{a, b, c, d, values, stats_even, stats_odd};
     const int of_keys = args.key_blocks * args.parts, block = static_cast<int>(blockIdx.x);
     if (block < of_keys) dkv_block<T, DP>(args, memory, block % args.key_blocks, block / args.key_blocks);
     else dq_block<T, DP>(args, memory, block - of_keys);
@@ -388,8 +397,11 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
         return set_error(kTempTooSmall, "%s: temp storage too small", what);
     if ((k_tokens && (too_wide(k) || too_wide(v))) || (q_tokens && (too_wide(q) || too_wide(dout)))) return refuse_wide(what);
     unsigned tiles, grid, key_tiles, key_grid;
-    if (int st = check_grid(what, q_tokens, sequences, (q_heads + 1) / 2, tiles, grid); st != kOk) return st;
-    if (int st = check_grid(what, k_tokens, sequences, kv_heads, key_tiles, key_grid); st != kOk) return st;
+    const bool two_heads = q_heads / kv_heads % 2 == 0;
+    if (int st = check_grid(what, q_tokens, two_heads ? kRowTile : kTeams * kRowTile, sequences, two_heads ? q_heads / 2 : q_heads, tiles, grid);
+        st != kOk)
+        return st;
+    if (int st = check_grid(what, k_tokens, kRowTile, sequences, kv_heads, key_tiles, key_grid); st != kOk) return st;
     const uint64_t parts = key_parts(sequences, q_tokens, k_tokens, q_heads, kv_heads);
     const uint64_t blocks = (q_tokens ? grid : 0) + (k_tokens ? key_grid * parts : 0);
     if (blocks > 0x7FFFFFFFull / (kTeams * kBlock)) return set_error(kInvalidArgument, "%s: too many tiles", what);

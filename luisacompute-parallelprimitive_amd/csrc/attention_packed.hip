@@ -80,7 +80,7 @@ int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* 
         return unusable(what);
     if (k_tokens && (too_wide(k) || too_wide(v))) return refuse_wide(what);
     unsigned tiles, grid;
-    if (int st = check_grid(what, q_tokens, sequences, q_heads, tiles, grid); st != kOk) return st;
+    if (int st = check_grid(what, q_tokens, kRowTile, sequences, q_heads, tiles, grid); st != kOk) return st;
     const Shape shape{static_cast<int>(sequences), static_cast<int>(q_tokens), static_cast<int>(k_tokens),
                       static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(dim), scale, causal != 0};
     const Rows none{nullptr, 0, 0};

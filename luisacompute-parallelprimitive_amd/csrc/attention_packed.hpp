@@ -74,8 +74,9 @@ inline bool too_wide(const lcpp_hip_rows* r) { return r != nullptr && r->token_s
 inline int refuse_wide(const char* what) { return set_error(kUnsupported, "%s: token strides must be below 2^24 items", what); }
 
 // Tiles that a ragged batch may have, and the launch over (tile, head).
-inline int check_grid(const char* what, uint64_t tokens, uint32_t sequences, uint32_t heads, unsigned& tiles, unsigned& grid) {
-    const uint64_t t = tokens / kRowTile + sequences;
+inline int check_grid(const char* what, uint64_t tokens, int tile_rows, uint32_t sequences, uint32_t heads, unsigned& tiles,
+                      unsigned& grid) {
+    const uint64_t t = tokens / tile_rows + sequences;
     if (t * heads > 0x7FFFFFFFull / (kTeams * kBlock)) return set_error(kInvalidArgument, "%s: too many tiles", what);
     tiles = static_cast<unsigned>(t);
     grid = static_cast<unsigned>(t * heads);
