@@ -384,12 +384,13 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 4 : 2) void attention_paged_wide
     const int ahead = w.length - w.tokens;
     const float c = p.scale * kLog2e;
     const int32_t* table = block_table + static_cast<int64_t>(w.request) * p.table_stride;
-    // A page that is not there: every tile is masked, by what the table says of its keys.
+    // A page that is not there: every tile is masked, by what the table says of its keys.  (Each wave looks for itself, so
+    // that nothing waits for it.)
     bool lost = false;
     if (begin < end)
-        for (int i = static_cast<int>(p.page_size(begin) + threadIdx.x); i <= static_cast<int>(p.page_size(end - 1)); i += kBlock)
+        for (int i = static_cast<int>(p.page_size(begin)) + lane; i <= static_cast<int>(p.page_size(end - 1)); i += kWave)
             lost |= table[i] < 0 || table[i] >= p.pages;
-    lost = __syncthreads_or(lost);
+    lost = wave_ballot(lost) != 0;
 
     U32x4 qf[DP / 16];
     const char* q_row = q.at(w.token0 + row.token, row.head);
