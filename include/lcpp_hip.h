@@ -594,9 +594,10 @@ LCPP_HIP_DECLARE_SEGSORT(f64, double)
  * multiples of 16 bytes, and their strides are multiples of 8 items.  `scale` (the products' factor, often
  * 1 / sqrt(head_dim)) is positive.  lse is [q_heads][q_tokens] f32: the logarithm of the row's sum of exponentials.
  * A row that sees no key has zeros for its output and -infinity for its lse, and passes no gradient.  An infinity
- * or NaN in a key or value reaches the rows that see it and no others (batches that hold one take much longer); the gradients
- * of a sequence that holds one may be NaN throughout, those of the others are not touched.  Every
- * result is a sum in one order: the same call gives the same bits.
+ * or NaN in a key or value reaches the rows that see it and no others, and in the backward pass the gradients that the
+ * formulas take it into (a batch that holds one takes a few times as long).  Every result is a sum in one order:
+ * the same call gives the same bits.  Outputs share no memory with inputs or with each other.  A sequence has
+ * fewer than 2^31 - 4096 keys.
  * ------------------------------------------------------------------------------------------- */
 
 /* [tokens][heads][head_dim]: the last axis contiguous, strides of the others in items. */

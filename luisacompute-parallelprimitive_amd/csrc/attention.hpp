@@ -57,6 +57,18 @@ __device__ __forceinline__ float item_high(uint32_t w) {
     return static_cast<float>(__builtin_bit_cast(typename T::Vec2, w)[1]);
 }
 
+// The sum of eight products of 16-bit items.
+template <typename T>
+__device__ __forceinline__ float dot8(U32x4 a, U32x4 b) {
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        sum += item_low<T>(a[i]) * item_low<T>(b[i]);
+        sum += item_high<T>(a[i]) * item_high<T>(b[i]);
+    }
+    return sum;
+}
+
 // Row of a 32x32 result that register r of a lane in half h holds.
 __device__ __forceinline__ constexpr int acc_row(int r, int h) { return 8 * (r / 4) + 4 * h + r % 4; }
 
@@ -98,6 +110,8 @@ __device__ __forceinline__ float halves_sum(float x) {
 }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+
+constexpr uint64_t kMostKeys = 0x7FFFF000;  // of a sequence: a few tiles below what a position may be
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
@@ -238,10 +252,12 @@ __device__ __forceinline__ int find_last(int count, Number number, Key key) {
     return __builtin_amdgcn_readfirstlane(low);
 }
 
+// (Offsets that do not ascend from 0 give wrong tiles, but none before a sequence's first row.)
 __device__ __forceinline__ TilePlace find_tile(const int32_t* offsets, int count, int scale, int size, int number) {
-    const auto first = [&](int b) { return static_cast<int64_t>(offsets[b]) * scale / size + b; };
+    const auto first = [&](int b) { return static_cast<int64_t>(offsets[b] > 0 ? offsets[b] : 0) * scale / size + b; };
     const int owner = find_last<int64_t>(count, number, first);
-    return {owner, owner < 0 ? 0 : number - static_cast<int>(first(owner))};
+    const int64_t tile = owner < 0 ? -1 : number - first(owner);
+    return {tile < 0 ? -1 : owner, static_cast<int>(tile)};
 }
 
 }  // namespace attention

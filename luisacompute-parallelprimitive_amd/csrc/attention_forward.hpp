@@ -179,104 +179,81 @@ __device__ __forceinline__ void forward_tile(RowState<DP>& state, const char* k_
 // Infinities and NaN in masked places.  A masked weight is zero, but zero times an infinity or NaN is NaN: in a tile of keys
 // that only some rows see, the matrix product carries such a value to the others.  The kernels do not look for them (the
 // guards in every tile's products cost a third of the registers): a wave whose sums come out as anything but finite numbers
-// takes its rows again, one at a time and without matrix instructions, and never touches what a row does not see.
+// takes the tiles that all of its rows see again, and then the other keys without matrix instructions, one at a time, where
+// a row adds only what it sees.  A lane keeps the row and the items of it that it has in the matrix products.
 
-// The keys of one row, in memory: a packed sequence, or pages (block_table not null).
-struct KeySource {
-    const char* keys;  // of the head; the first row, or the first page
-    const char* values;
-    int64_t key_bytes, value_bytes;            // from a token to the next, in a page or in the sequence
-    int64_t key_page_bytes, value_page_bytes;
-    const int32_t* block_table;  // the request's row of it
-    Divider page_size;
-    int pages;
-    // Offsets of a position; whether its page is there.
-    __device__ __forceinline__ bool find(int position, int64_t& key, int64_t& value) const {
-        key = position * key_bytes, value = position * value_bytes;
-        if (block_table == nullptr) return true;
-        const int cell = static_cast<int>(page_size(position)), page = block_table[cell];
-        const bool there = page >= 0 && page < pages;
-        const int64_t slot = position - static_cast<int64_t>(cell) * page_size.by, held = there ? page : 0;
-        key = held * key_page_bytes + slot * key_bytes, value = held * value_page_bytes + slot * value_bytes;
-        return there;
-    }
-};
-
-// Which keys a row sees: the first `count`, or with a tree those before `ahead` and then the tree's bits.
-struct RowSight {
-    int count, ahead;
-    bool tree_given;
-    uint64_t tree;
-    __device__ __forceinline__ bool sees(int position) const {
-        if (!tree_given || position < ahead) return position < (tree_given ? ahead : count);
-        return position - ahead < 64 && (tree >> (position - ahead) & 1);
-    }
-};
-
-struct CarefulRow {
-    float top, total, low, high;  // scale and sum; the products with the values' items 2 * lane and 2 * lane + 1
-};
-
-// One row against the keys in [begin, end): a lane a key for the scores, a lane two items for the products.
-template <typename T>
-__device__ __forceinline__ CarefulRow careful_row(const char* q_row, KeySource source, RowSight sight, int begin, int end, int dim, float c) {
-    const int lane = threadIdx.x % kWave;
-    CarefulRow row{-INFINITY, 0.f, 0.f, 0.f};
-    for (int k0 = begin; k0 < end; k0 += kWave) {
-        const int position = k0 + lane;
-        int64_t key = 0, value = 0;
-        bool seen = position < end && sight.sees(position);
-        seen = seen && source.find(position, key, value);
-        float score = -INFINITY;
-        if (seen) {
-            score = 0.f;
-            for (int d = 0; d < dim; d += 2) {
-                const uint32_t a = *reinterpret_cast<const uint32_t*>(q_row + d * 2);
-                const uint32_t b = *reinterpret_cast<const uint32_t*>(source.keys + key + d * 2);
-                score += item_low<T>(a) * item_low<T>(b);
-                score += item_high<T>(a) * item_high<T>(b);
-            }
-        }
-        float high = score;
+// Dot products of the lane's row (a B operand, half its items in each of two lanes) with one row of memory that the
+// whole wave reads.
+template <typename T, int DP, typename Operand>
+__device__ __forceinline__ float careful_dot(Operand operand, const char* row, int dim) {
+    float sum = 0.f;
 #pragma unroll
-        for (int step = 32; step > 0; step /= 2) high = fmaxf(high, __shfl_xor(high, step));
-        high = fmaxf(high, row.top);
-        const float base = high == -INFINITY ? 0.f : high * c;
-        const float alpha = row.top == -INFINITY ? 0.f : exp2_fast(row.top * c - base);
-        const float weight = seen ? exp2_fast(score * c - base) : 0.f;
-        float sum = weight;
-#pragma unroll
-        for (int step = 32; step > 0; step /= 2) sum += __shfl_xor(sum, step);
-        row.top = high;
-        row.total = row.total * alpha + sum;
-        row.low *= alpha;
-        row.high *= alpha;
-        uint64_t left = wave_ballot(seen);
-        while (left != 0) {
-            const int j = __ffsll(static_cast<unsigned long long>(left)) - 1;
-            left &= left - 1;
-            const float w = wave_read_lane(weight, j);
-            const int64_t from = wave_read_lane(value, j);
-            if (2 * lane < dim) {
-                const uint32_t v = *reinterpret_cast<const uint32_t*>(source.values + from + lane * 4);
-                row.low += w * item_low<T>(v);
-                row.high += w * item_high<T>(v);
-            }
-        }
+    for (int s = 0; s < DP / 16; ++s) {
+        sum += dot8<T>(operand(s), load_chunk(row, 2 * s + threadIdx.x % kWave / 32, dim, true));
+        if (s % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // four loads in flight: more would spill
     }
-    return row;
+    return halves_sum(sum);
+}
+
+// acc += weight * the row, where `seen`.
+template <typename T, int DP>
+__device__ __forceinline__ void careful_add(F32x16 (&acc)[DP / 32], float weight, const char* row, int dim, bool seen) {
+    const int half = threadIdx.x % kWave / 32;
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {
+        const int d = 8 * i + 4 * half;
+        if (8 * i >= dim || !seen) continue;
+        const U32x2 v = *reinterpret_cast<const U32x2*>(row + d * 2);
+        acc[i / 4][4 * (i % 4) + 0] += weight * item_low<T>(v[0]);
+        acc[i / 4][4 * (i % 4) + 1] += weight * item_high<T>(v[0]);
+        acc[i / 4][4 * (i % 4) + 2] += weight * item_low<T>(v[1]);
+        acc[i / 4][4 * (i % 4) + 3] += weight * item_high<T>(v[1]);
+        if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Whether any wave of the workgroup has `found`; `flag` was cleared before an earlier barrier.  Waits for LDS only, not
+// for stores to memory that are on their way (__syncthreads_or in its place: 155 -> 162 us for 16 uneven prompts).
+__device__ __forceinline__ bool block_any(bool found, int* flag) {
+    if (wave_ballot(found) != 0 && threadIdx.x % kWave == 0) *flag = 1;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+    return *flag != 0;
+}
+
+// The kernel's only argument, read again: what a rarely taken path needs of it then takes no registers of the usual one.
+template <typename Args>
+__device__ __forceinline__ Args arguments_again() {
+    static_assert(sizeof(Args) % 4 == 0);
+    struct Words {
+        uint32_t word[sizeof(Args) / 4];
+    } words;
+    const auto* from = (const __attribute__((address_space(4))) uint32_t*)__builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(from));
+#pragma unroll
+    for (unsigned i = 0; i < sizeof(Args) / 4; ++i) words.word[i] = from[i];
+    return __builtin_bit_cast(Args, words);
+}
+
+// The end of the tiles from `begin` on that every row sees, when they see all keys below `full` of those below `end`.
+__device__ __forceinline__ int clean_end(int begin, int full, int end) {
+    return full < end ? begin + (full - begin) / kKeyTile * kKeyTile : end;
+}
+
+// One key for the lane's row; the whole wave has the same.
+template <typename T, int DP>
+__device__ __forceinline__ void careful_key(RowState<DP>& state, const U32x4 (&qf)[DP / 16], const char* key, const char* value,
+                                            int dim, float c, bool seen) {
+    const float dot = careful_dot<T, DP>([&](int i) { return qf[i]; }, key, dim), score = seen ? dot : -INFINITY;
+    rescale(state, score, c);
+    const float weight = exp2_fast(score * c - (state.top == -INFINITY ? 0.f : state.top * c));
+    if (threadIdx.x % kWave < 32) state.total += weight;
+    careful_add<T, DP>(state.acc, weight, value, dim, seen);
 }
 
 __device__ __forceinline__ float row_lse(float top, float total, float scale) {
     return total == 0.f ? -INFINITY : top * scale + __logf(total);
-}
-
-// Writes a careful row's output.
-template <typename T>
-__device__ __forceinline__ void store_careful(char* to, const CarefulRow& row, int dim) {
-    const int lane = threadIdx.x % kWave;
-    const float f = row.total == 0.f ? 0.f : 1.f / row.total;
-    if (2 * lane < dim) *reinterpret_cast<uint32_t*>(to + lane * 4) = pack2<T>(row.low * f, row.high * f);
 }
 
 // Runs the tiles from `begin` to `end`, SIZE apart, with two sets of buffers: while one is computed on, the other is loaded.

@@ -52,6 +52,7 @@ struct GradientMemory {
     char *a, *b, *c, *d;
     char* values;  // kRowTile rows
     float *stats_even, *stats_odd;
+    int* broken;  // whether the sums of some wave are not finite
 };
 
 struct GradientArgs {
@@ -105,7 +106,7 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
     const float base = there ? g.stats[stat] : INFINITY;
     const float delta = there ? g.stats[static_cast<int64_t>(shape.q_heads) * shape.q_tokens + stat] : 0.f;
     for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile, kAllWaves>(tile, shape.dim);
-    F32x16 acc[DP / 32] = {};
+    F32x16 acc[DP / 32];
     const PackedRows<DP, kKeyTile, kAllWaves> key_rows(g.k.at(keys.begin, kv_head), g.k.token_bytes, keys.size, shape.dim);
     const PackedRows<DP, kKeyTile, kAllWaves> value_rows(g.v.at(keys.begin, kv_head), g.v.token_bytes, keys.size, shape.dim);
     const auto load = [&](char* k_tile, char* v_tile, int k0) {
@@ -138,9 +139,29 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
             }
         }
     };
-    pass_tiles<kKeyTile>(0, end, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
-                         [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
-    if (there) store_row<T, DP>(g.dq, rows.begin + row, head, acc, shape.scale, shape.dim);
+    const int clean = clean_end(0, two_heads ? range.full : RowRange(shape, rows, keys, first_row, row).full, end);
+    const auto pass = [&](int stop) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) acc[d] = F32x16{};
+        pass_tiles<kKeyTile>(0, stop, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
+                             [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
+    };
+    const auto store = [&] {
+        if (there) store_row<T, DP>(g.dq, rows.begin + row, head, acc, shape.scale, shape.dim);
+    };
+    pass(end);
+    store();  // (before waves wait for each other)
+    if (clean < end && block_any(any_not_finite(acc), memory.broken)) {
+        pass(clean);
+        for (int j = clean; j < range.wave_end; ++j) {
+            const char* key = g.k.at(keys.begin + static_cast<int64_t>(j), kv_head);
+            const char* value = g.v.at(keys.begin + static_cast<int64_t>(j), kv_head);
+            const float s = careful_dot<T, DP>([&](int i) { return qf[i]; }, key, shape.dim);
+            const float dp = careful_dot<T, DP>([&](int i) { return of[i]; }, value, shape.dim);
+            careful_add<T, DP>(acc, exp2_fast(s * c - base) * (dp - delta), key, shape.dim, j < range.count);
+        }
+        store();
+    }
 }
 
 struct RowTiles {  // of one team: which head of the group, which row
@@ -197,12 +218,11 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     PackedRows<DP, kRowTile, kAllWaves>(v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim).load(memory.values, key0);
     const char* values = memory.values + Tile<DP>::bytes(kRowsPerWave) * wave;
     for (char* tile : {q_even, o_even, q_odd, o_odd}) clear_past<DP, kQueryTile>(tile, shape.dim);
-    F32x16 dk_acc[DP / 32] = {}, dv_acc[DP / 32] = {};
+    F32x16 dk_acc[DP / 32], dv_acc[DP / 32];
     const int all = rows.size > start ? (rows.size - start + kQueryTile - 1) / kQueryTile * group : 0;
     const int per = (all + parts - 1) / parts;
     const int from = part * per, to = from + per < all ? from + per : all;
-    RowTiles loads{kv_head * group, start, start, rows.size}, steps = loads;
-    if (from < to) loads.skip(from + team), steps.skip(from + team);
+    RowTiles loads, steps;
     const PackedRows<DP, kQueryTile> q_rows(q.at(rows.begin, 0), q.token_bytes, rows.size, shape.dim);
     const PackedRows<DP, kQueryTile> o_rows(dout.at(rows.begin, 0), dout.token_bytes, rows.size, shape.dim);
     const float* s_rows = stats + static_cast<int64_t>(half) * shape.q_heads * shape.q_tokens + rows.begin;
@@ -218,14 +238,15 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
         }
         loads.skip(kTeams);
     };
-    const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile, int at) {
+    // `clean` leaves out tiles of rows of which some do not see some key.
+    const auto step = [&](const char* q_tile, const char* o_tile, const float* s_tile, int at, bool clean) {
         if (at + team >= to) return;
         const int tile_row0 = steps.row0;
         steps.skip(kTeams);
 #pragma unroll
         for (int b = 0; b < kQueryTile / 32; ++b) {
             const int r0 = tile_row0 + 32 * b;
-            if (r0 + 32 <= wave_start || r0 >= rows.size) continue;
+            if (r0 + 32 <= wave_start || r0 >= rows.size || (clean && r0 < full)) continue;
             F32x16 s = {}, dp = {};
 #pragma unroll
             for (int i = 0; i < DP / 16; ++i) {
@@ -263,10 +284,20 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
             }
         }
     };
-    pass_tiles<kTeams>(from, to, [&](int x) { load(q_even, o_even, s_even, x); },
-                       [&](int x) { load(q_odd, o_odd, s_odd, x); },
-                       [&](int x) { step(q_even, o_even, s_even, x); },
-                       [&](int x) { step(q_odd, o_odd, s_odd, x); });
+    const auto pass = [&](bool clean) {
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) dk_acc[d] = dv_acc[d] = F32x16{};
+        loads = {kv_head * group, start, start, rows.size};
+        if (from < to) loads.skip(from + team);
+        steps = loads;
+        pass_tiles<kTeams>(from, to, [&](int x) { load(q_even, o_even, s_even, x); },
+                           [&](int x) { load(q_odd, o_odd, s_odd, x); },
+                           [&](int x) { step(q_even, o_even, s_even, x, clean); },
+                           [&](int x) { step(q_odd, o_odd, s_odd, x, clean); });
+    };
+    pass(false);
+    const bool clean = start < full && block_any(any_not_finite(dk_acc) || any_not_finite(dv_acc), memory.broken);
+    if (clean) pass(true);
     // The first team ends with dK, the second with dV; each hands the other its share.
     // (Over the tiles, which nothing is loaded into any more: a quarter of the sums in each of the four arrays.)
     const auto join_at = [&](int i) {
@@ -303,11 +334,35 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
                     F32x4{acc[i / 4][4 * (i % 4)], acc[i / 4][4 * (i % 4) + 1], acc[i / 4][4 * (i % 4) + 2], acc[i / 4][4 * (i % 4) + 3]} * factor;
         }
     };
+    // The rows that a clean pass left out, of both teams.
+    const auto add_left_out = [&](F32x16(&acc)[DP / 32], bool of_keys) {
+        const GradientArgs again = arguments_again<GradientArgs>();
+        RowTiles tile{kv_head * group, start, start, rows.size};
+        if (from < to) tile.skip(from);
+        for (int at = from; at < to; ++at, tile.skip(1)) {
+            if (tile.row0 >= full) continue;
+            const int end = tile.row0 + kQueryTile < rows.size ? tile.row0 + kQueryTile : rows.size;
+            for (int row = tile.row0 > wave_start ? tile.row0 : wave_start; row < end; ++row) {
+                const char* q_row = again.q.at(rows.begin + static_cast<int64_t>(row), tile.head);
+                const char* o_row = again.dout.at(rows.begin + static_cast<int64_t>(row), tile.head);
+                const int64_t stat = static_cast<int64_t>(tile.head) * again.shape.q_tokens + rows.begin + row;
+                const float p = exp2_fast(careful_dot<T, DP>([&](int i) { return kf[i]; }, q_row, again.shape.dim) * c - again.stats[stat]);
+                if (of_keys) {
+                    const float dp = careful_dot<T, DP>([&](int i) { return read_rows<DP>(values, 0, i); }, o_row, again.shape.dim);
+                    const float delta = again.stats[static_cast<int64_t>(again.shape.q_heads) * again.shape.q_tokens + stat];
+                    careful_add<T, DP>(acc, p * (dp - delta), q_row, again.shape.dim, row >= first);
+                } else {
+                    careful_add<T, DP>(acc, p, o_row, again.shape.dim, row >= first);
+                }
+            }
+        }
+    };
     __syncthreads();
     if (team == 1) give(dk_acc);
     __syncthreads();
     if (team == 0) {
         take(dk_acc);
+        if (clean) add_left_out(dk_acc, true);
         store(dk, dk_acc, shape.scale, 0);
     }
     __syncthreads();
@@ -315,6 +370,7 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     __syncthreads();
     if (team == 1) {
         take(dv_acc);
+        if (clean) add_left_out(dv_acc, false);
         store(dv, dv_acc, 1.f, 1);
     }
 }
@@ -328,7 +384,9 @@ __global__ __launch_bounds__(kTeams* kBlock, 2) void attention_gradients_kernel(
     __shared__ __attribute__((aligned(16))) char values[Tile<DP>::bytes(kRowTile)];
     __shared__ __attribute__((aligned(16))) float stats_even[kTeams * 2 * kQueryTile];
     __shared__ __attribute__((aligned(16))) float stats_odd[kTeams * 2 * kQueryTile];
-    const GradientMemory<DP> memory{a, b, c, d, values, stats_even, stats_odd};
+    __shared__ int broken;
+    if (threadIdx.x == 0) broken = 0;
+    const GradientMemory<DP> memory{a, b, c, d, values, stats_even, stats_odd, &broken};
     const int of_keys = args.key_blocks * args.parts, block = static_cast<int>(blockIdx.x);
     if (block < of_keys) dkv_block<T, DP>(args, memory, block % args.key_blocks, block / args.key_blocks);
     else dq_block<T, DP>(args, memory, block - of_keys);
@@ -386,7 +444,7 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
     hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     if (int st = check_shape(what, sequences, q_tokens, k_tokens, q_heads, kv_heads, dim, scale); st != kOk) return st;
     if (sequences == 0 || (q_tokens == 0 && k_tokens == 0)) return kOk;
-    if (q_tokens * (q_heads / kv_heads) > 0x7FFFFFFFull) return set_error(kInvalidArgument, "%s: too many tokens or sequences", what);
+    if (q_tokens * (q_heads / kv_heads) > kMostKeys) return set_error(kInvalidArgument, "%s: too many tokens or sequences", what);
     if (!q_offsets || !k_offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
     if (q_tokens && (!usable(q) || !usable(out) || !usable(dout) || !usable(dq) || !lse))
         return unusable(what);

@@ -18,6 +18,8 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_ker
     __shared__ __attribute__((aligned(16))) char v_even[kTileBytes];
     __shared__ __attribute__((aligned(16))) char k_odd[kTileBytes];
     __shared__ __attribute__((aligned(16))) char v_odd[kTileBytes];
+    __shared__ int broken;  // whether the sums of some wave are not finite
+    if (threadIdx.x == 0) broken = 0;
     // Workgroups go to the 8 XCDs in turn: with the key head as the fastest number, those of a key head share an L2.
     // Later tiles, which see more keys, come first.
     const int group = shape.q_heads / shape.kv_heads;
@@ -39,31 +41,32 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_ker
     U32x4 qf[DP / 16];
     load_row<DP>(qf, q, rows.begin + row, head, there, shape.dim);
     for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile>(tile, shape.dim);
-    RowState<DP> state = {};
-    state.top = -INFINITY;
-    forward_keys<T, DP>(state, k_even, v_even, k_odd, v_odd,
-                        PackedRows<DP, kKeyTile>(k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim),
-                        PackedRows<DP, kKeyTile>(v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim), qf, c, 0,
-                        range.end, range.wave_end, range.full, [&](int k0) { return first_keys(range.count, k0); });
-    if (wave_ballot(any_not_finite(state.acc)) != 0) {
-        const KeySource source{k.at(keys.begin, kv_head), v.at(keys.begin, kv_head), k.token_bytes, v.token_bytes, 0, 0, nullptr,
-                               shape.one, 0};
-        for (int r = row - lane % 32, i = 0; i < kRowsPerWave && r < rows.size; ++i, ++r) {
-            const int count = RowRange(shape, rows, keys, row0, r).count;
-            const CarefulRow result = careful_row<T>(q.at(rows.begin + r, head), source, RowSight{count, 0, false, 0}, 0, count,
-                                                     shape.dim, c);
-            store_careful<T>(out.at(rows.begin + r, head), result, shape.dim);
-            if (lse != nullptr && lane == 0)
-                lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + r] = row_lse(result.top, result.total, shape.scale);
-        }
-        return;
+    const PackedRows<DP, kKeyTile> key_rows(k.at(keys.begin, kv_head), k.token_bytes, keys.size, shape.dim);
+    const PackedRows<DP, kKeyTile> value_rows(v.at(keys.begin, kv_head), v.token_bytes, keys.size, shape.dim);
+    const auto pass = [&](RowState<DP>& state, int stop) {
+        state = {};
+        state.top = -INFINITY;
+        forward_keys<T, DP>(state, k_even, v_even, k_odd, v_odd, key_rows, value_rows, qf, c, 0, stop, range.wave_end, range.full,
+                            [&](int k0) { return first_keys(range.count, k0); });
+    };
+    const auto store = [&](const RowState<DP>& state) {
+        const float total = halves_sum(state.total);
+        if (!there) return;
+        store_row<T, DP>(out, rows.begin + row, head, state.acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
+        if (lse != nullptr && half == 0)
+            lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row] = row_lse(state.top, total, shape.scale);
+    };
+    RowState<DP> state;
+    pass(state, range.end);
+    store(state);  // (before waves wait for each other)
+    const int clean = clean_end(0, range.full, range.end);
+    if (clean < range.end && block_any(any_not_finite(state.acc), &broken)) {
+        pass(state, clean);
+        for (int j = clean; j < range.wave_end; ++j)
+            careful_key<T, DP>(state, qf, k.at(keys.begin + static_cast<int64_t>(j), kv_head), v.at(keys.begin + static_cast<int64_t>(j), kv_head),
+                               shape.dim, c, j < range.count);
+        store(state);
     }
-    const float total = halves_sum(state.total);
-    if (!there) return;
-    store_row<T, DP>(out, rows.begin + row, head, state.acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
-    if (lse != nullptr && half == 0)
-        lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row] =
-            row_lse(state.top, total, shape.scale);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------

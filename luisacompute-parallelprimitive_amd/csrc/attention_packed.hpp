@@ -18,7 +18,6 @@ struct Shape {
     int dim;
     float scale;
     int causal;
-    Divider one{1};  // (the pages of keys that are in none)
 };
 
 struct Span {
@@ -63,7 +62,7 @@ inline int check_shape(const char* what, uint32_t sequences, uint64_t q_tokens, 
         return set_error(kInvalidArgument, "%s: query heads must be a multiple of the key heads, and at most 65535", what);
     if (dim == 0 || dim % 8 != 0 || dim > 128)
         return set_error(kUnsupported, "%s: the head size must be a multiple of 8 up to 128", what);
-    if (q_tokens > 0x7FFFFFFFull || k_tokens > 0x7FFFFFFFull || sequences > 0x7FFFFFFu)
+    if (q_tokens > 0x7FFFFFFFull || k_tokens > kMostKeys || sequences > 0x7FFFFFFu)
         return set_error(kInvalidArgument, "%s: too many tokens or sequences", what);
     if (!(scale > 0.f) || scale == INFINITY) return set_error(kInvalidArgument, "%s: the scale must be positive and finite", what);
     return kOk;

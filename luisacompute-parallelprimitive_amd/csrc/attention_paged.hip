@@ -57,7 +57,8 @@ struct Work {
     int tokens;   // new tokens
     int row0;     // first row of the tile
     int rows;     // rows of the request
-    int length;   // keys
+    int length;   // keys that the table holds
+    int ahead;    // keys before the new tokens' own; negative where there are fewer than new tokens
 };
 
 __device__ __forceinline__ void take_request(Work& w, const int32_t* q_offsets, const int32_t* kv_lengths, const Paged& p,
@@ -69,9 +70,11 @@ __device__ __forceinline__ void take_request(Work& w, const int32_t* q_offsets, 
     w.token0 = begin;
     w.tokens = end - begin;
     w.rows = w.tokens * (p.q_heads / p.kv_heads);
-    const int64_t most = static_cast<int64_t>(p.table_width) * p.page_size.by;
-    const int length = kv_lengths[request];
-    w.length = length < 0 ? 0 : length > most ? static_cast<int>(most) : length;
+    int64_t most = static_cast<int64_t>(p.table_width) * p.page_size.by;
+    most = most < static_cast<int64_t>(kMostKeys) ? most : static_cast<int64_t>(kMostKeys);
+    const int length = kv_lengths[request] < 0 ? 0 : kv_lengths[request];
+    w.length = length > most ? static_cast<int>(most) : length;
+    w.ahead = length - w.tokens;
 }
 
 // Tile `number` of `tile_rows` rows.
@@ -83,6 +86,33 @@ __device__ __forceinline__ bool find_work(Work& w, const int32_t* q_offsets, con
     w.row0 = place.tile * tile_rows;
     return w.row0 < w.rows;
 }
+
+// A part's keys as a tile of rows sees them.
+struct Sight {
+    int begin;     // of the part
+    int end;       // keys in [begin, end) that some row of the tile sees
+    int full;      // and those before are seen by all, if their pages are there
+    int wave_end;  // keys that some row of the wave sees
+    bool whole;    // the request has no other part
+    // False where the part holds nothing of the request (and another one writes its rows).
+    __device__ __forceinline__ bool find(const Work& w, const Paged& p, int part, int tile_rows, bool tree_given, int wave_row0, int wave_rows) {
+        const int per = part_keys(w.length, p), group = p.q_heads / p.kv_heads;
+        const int64_t first = static_cast<int64_t>(part) * per;
+        if (first >= w.length && part > 0) return false;
+        begin = static_cast<int>(first);
+        whole = w.length <= per;
+        const int part_end = w.length - begin > per ? begin + per : w.length;
+        // Keys that a row sees, at most and (without a tree) exactly.
+        const auto seen = [&](int row) {
+            const int64_t last = w.ahead + (tree_given ? int64_t{64} : int64_t{row < w.rows ? row : w.rows - 1} / group + 1);
+            return static_cast<int>(last < begin ? begin : last < part_end ? last : part_end);
+        };
+        end = seen(w.row0 + tile_rows - 1);
+        full = tree_given ? (w.ahead < begin ? begin : w.ahead < end ? w.ahead : end) : seen(w.row0);
+        wave_end = wave_row0 < w.rows ? seen(wave_row0 + wave_rows - 1) : begin;
+        return true;
+    }
+};
 
 // Bit b: whether the row sees key k0 + b, of 32, as far as new tokens go.  `ahead` keys lie before the new ones.
 __device__ __forceinline__ uint32_t seen_word(uint64_t tree, int k0, int ahead) {
@@ -125,27 +155,19 @@ struct Parts {
     }
 };
 
-// Rows [first, first + rows) of a tile again, one wave, every `step`-th: results or a part's sums.
-template <typename T>
-__device__ __forceinline__ void careful_rows(const Rows& q, const Pages& key_cache, const Pages& value_cache, const Rows& out, float* lse,
-                                             const Parts& parts, const int32_t* table, const uint64_t* tree, const Paged& p,
-                                             const Work& w, int kv_head, int begin, int end, bool whole, int first, int rows, int step) {
-    const int lane = threadIdx.x % kWave;
-    const KeySource source{key_cache.at(0, 0, kv_head), value_cache.at(0, 0, kv_head), key_cache.token_bytes, value_cache.token_bytes,
-                           key_cache.page_bytes, value_cache.page_bytes, table, p.page_size, p.pages};
-    const int ahead = w.length - w.tokens;
-    for (int r = first; r < first + rows && r < w.rows; r += step) {
-        const PagedRow row(w, p, tree, kv_head, r);
-        const int64_t t = w.token0 + row.token;
-        const CarefulRow result = careful_row<T>(q.at(t, row.head), source, RowSight{ahead + row.token + 1, ahead, tree != nullptr, row.tree},
-                                                 begin, end, p.dim, p.scale * kLog2e);
-        if (whole) {
-            store_careful<T>(out.at(t, row.head), result, p.dim);
-            if (lse != nullptr && lane == 0) lse[static_cast<int64_t>(row.head) * p.q_tokens + t] = row_lse(result.top, result.total, p.scale);
-        } else {
-            const int64_t at = parts.row(p, blockIdx.y, row.head, t);
-            if (lane == 0) parts.stats[at] = F32x2{result.top, result.total};
-            if (2 * lane < p.dim) *reinterpret_cast<F32x2*>(parts.out + at * p.dim + 2 * lane) = F32x2{result.low, result.high};
+// The wave's keys [k0, end), 32 every `step`: those that a row sees and whose page is there.
+template <typename T, int DP>
+__device__ __forceinline__ void careful_keys(RowState<DP>& state, const U32x4 (&qf)[DP / 16], const Pages& key_cache, const Pages& value_cache,
+                                             const int32_t* table, const PagedRow& row, const uint64_t* tree, const Paged& p,
+                                             const Work& w, int kv_head, int k0, int end, int step) {
+    for (; k0 < end; k0 += step) {
+        const uint32_t seen = row.seen(tree != nullptr, k0, w.ahead);
+        for (int j = 0; j < kWaveKeys && k0 + j < end; ++j) {
+            const int cell = static_cast<int>(p.page_size(k0 + j)), page = table[cell];
+            if (page < 0 || page >= p.pages) continue;
+            const int64_t slot = slot_of(p, k0 + j);
+            careful_key<T, DP>(state, qf, key_cache.at(page, slot, kv_head), value_cache.at(page, slot, kv_head), p.dim, p.scale * kLog2e,
+                               seen >> j & 1);
         }
     }
 }
@@ -167,16 +189,14 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
     if (!find_work(w, q_offsets, kv_lengths, p, kNarrowRows, blockIdx.x / p.kv_heads)) return;
-    const int per = part_keys(w.length, p);
-    const int64_t part_begin = static_cast<int64_t>(blockIdx.y) * per;
-    if (part_begin >= w.length && blockIdx.y > 0) return;
-    const int begin = static_cast<int>(part_begin), end = w.length - begin > per ? begin + per : w.length;
-    const bool whole = w.length <= per;
+    Sight sight;
+    if (!sight.find(w, p, blockIdx.y, kNarrowRows, tree != nullptr, w.row0, kNarrowRows)) return;
+    const int begin = sight.begin, end = sight.end;
+    const bool whole = sight.whole;
     const int group = p.q_heads / p.kv_heads;
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const PagedRow row(w, p, tree, kv_head, w.row0 + lane % 32);
-    const int ahead = w.length - w.tokens;
     const float c = p.scale * kLog2e;
     const int32_t* table = block_table + static_cast<int64_t>(w.request) * p.table_stride;
     const char* keys = key_cache.at(0, 0, kv_head);
@@ -217,12 +237,18 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
         }
         return held;
     };
-    RowState<DP> state = {};
-    state.top = -INFINITY;
+    RowState<DP> state;
     int k0 = begin + wave * kWaveKeys;
-    uint32_t next_held = load(page_of(k0), k0);
-    int page = page_of(k0 + kKeyStep);
-    for (; k0 < end; k0 += kKeyStep) {
+    uint32_t next_held;
+    int page;
+    const auto start = [&] {
+        state = {};
+        state.top = -INFINITY;
+        k0 = begin + wave * kWaveKeys;
+        next_held = load(page_of(k0), k0);
+        page = page_of(k0 + kKeyStep);
+    };
+    const auto step = [&] {
         const uint32_t held = next_held;
         wave_lds_order();
 #pragma unroll
@@ -236,8 +262,8 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
         F32x16 s = {};
 #pragma unroll
         for (int i = 0; i < DP / 16; ++i) s = T::mfma(read_rows<DP>(k_tile, 0, i), qf[i], s);
-        if (held != ~0u || k0 + kWaveKeys > ahead) {
-            const uint32_t seen = (held & row.seen(tree != nullptr, k0, ahead)) >> (4 * half);
+        if (held != ~0u || k0 + kWaveKeys > sight.full) {
+            const uint32_t seen = (held & row.seen(tree != nullptr, k0, w.ahead)) >> (4 * half);
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = seen & (1u << acc_row(r, 0)) ? s[r] : -INFINITY;
         }
@@ -258,11 +284,13 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
             for (int d = 0; d < DP / 32; ++d)
                 state.acc[d] = T::mfma(read_columns<DP>(v_tile, i * 16, d * 32), pf, state.acc[d]);
         }
-    }
-    if (__syncthreads_or(any_not_finite(state.acc))) {
-        careful_rows<T>(q, key_cache, value_cache, out, lse, parts, table, tree, p, w, kv_head, begin, end, whole, w.row0 + wave,
-                        kNarrowRows - wave, kWaves);
-        return;
+    };
+    start();
+    for (; k0 < end; k0 += kKeyStep) step();
+    if (sight.full < end && wave_ballot(any_not_finite(state.acc)) != 0) {
+        start();
+        for (; k0 + kWaveKeys <= sight.full; k0 += kKeyStep) step();
+        careful_keys<T, DP>(state, qf, key_cache, value_cache, table, row, tree, p, w, kv_head, k0, end, kKeyStep);
     }
     const float total = halves_sum(state.total);
     if (half == 0) {
@@ -370,18 +398,18 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 4 : 2) void attention_paged_wide
     __shared__ __attribute__((aligned(16))) char v_even[kTileBytes];
     __shared__ __attribute__((aligned(16))) char k_odd[kTileBytes];
     __shared__ __attribute__((aligned(16))) char v_odd[kTileBytes];
+    __shared__ int broken;  // whether the sums of some wave are not finite
+    if (threadIdx.x == 0) broken = 0;
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
     if (!find_work(w, q_offsets, kv_lengths, p, kRowTile, blockIdx.x / p.kv_heads)) return;
-    const int per = part_keys(w.length, p);
-    const int64_t part_begin = static_cast<int64_t>(blockIdx.y) * per;
-    if (part_begin >= w.length && blockIdx.y > 0) return;
-    const int begin = static_cast<int>(part_begin), end = w.length - begin > per ? begin + per : w.length;
-    const bool whole = w.length <= per;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave_row0 = w.row0 + wave * kRowsPerWave;
+    Sight sight;
+    if (!sight.find(w, p, blockIdx.y, kRowTile, tree != nullptr, wave_row0, kRowsPerWave)) return;
+    const int begin = sight.begin, end = sight.end, wave_end = sight.wave_end;
+    const bool whole = sight.whole;
     const int lane = threadIdx.x % kWave, half = lane / 32;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    const PagedRow row(w, p, tree, kv_head, w.row0 + wave * kRowsPerWave + lane % 32);
-    const int ahead = w.length - w.tokens;
+    const PagedRow row(w, p, tree, kv_head, wave_row0 + lane % 32);
     const float c = p.scale * kLog2e;
     const int32_t* table = block_table + static_cast<int64_t>(w.request) * p.table_stride;
     // A page that is not there: every tile is masked, by what the table says of its keys.  (Each wave looks for itself, so
@@ -397,10 +425,9 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 4 : 2) void attention_paged_wide
 #pragma unroll
     for (int s = 0; s < DP / 16; ++s) qf[s] = load_chunk(q_row, 2 * s + half, p.dim, row.there);
     for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile>(tile, p.dim);
-    RowState<DP> state = {};
-    state.top = -INFINITY;
+    RowState<DP> state;
     const auto seen = [&](int k0) {
-        uint32_t word = row.seen(tree != nullptr, k0, ahead) & first_keys(end, k0);
+        uint32_t word = row.seen(tree != nullptr, k0, w.ahead) & first_keys(end, k0);
         if (lost) {
             const int position = k0 + lane % 32;
             const int page = position < end ? table[p.page_size(position)] : -1;
@@ -409,36 +436,44 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 4 : 2) void attention_paged_wide
         return word;
     };
     PagedTiles<DP> source{key_cache.at(0, 0, kv_head), value_cache.at(0, 0, kv_head), key_cache, value_cache, table, p, end, {}};
-    if (begin < end) source.look_up(begin);
-    const int full = lost ? begin : ahead < end ? ahead : end;
-    const int wave_end = w.row0 + wave * kRowsPerWave < w.rows ? end : begin;
+    const int full = lost ? begin : sight.full;
     const auto step = [&](const char* k_tile, const char* v_tile, int k0) {
         if (k0 < wave_end) forward_tile<T, DP>(state, k_tile, v_tile, qf, c, k0, k0 + kKeyTile > full, seen);
     };
-    pass_tiles<kKeyTile>(begin, end, [&](int k0) { source.load(k_even, v_even, k0); }, [&](int k0) { source.load(k_odd, v_odd, k0); },
-                         [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
-    if (wave_ballot(any_not_finite(state.acc)) != 0) {
-        careful_rows<T>(q, key_cache, value_cache, out, lse, parts, table, tree, p, w, kv_head, begin, end, whole,
-                        w.row0 + wave * kRowsPerWave, kRowsPerWave, 1);
-        return;
-    }
-    const float total = halves_sum(state.total);
-    if (!row.there) return;
-    const int64_t t = w.token0 + row.token;
-    if (whole) {
-        store_row<T, DP>(out, t, row.head, state.acc, total == 0.f ? 0.f : 1.f / total, p.dim);
-        if (lse != nullptr && half == 0) lse[static_cast<int64_t>(row.head) * p.q_tokens + t] = row_lse(state.top, total, p.scale);
-        return;
-    }
-    const int64_t at = parts.row(p, blockIdx.y, row.head, t);
-    if (half == 0) parts.stats[at] = F32x2{state.top, total};
+    const int clean = clean_end(begin, sight.full, end);
+    const auto pass = [&](RowState<DP>& state, int stop) {
+        state = {};
+        state.top = -INFINITY;
+        if (begin < stop) source.look_up(begin);
+        pass_tiles<kKeyTile>(begin, stop, [&](int k0) { source.load(k_even, v_even, k0); }, [&](int k0) { source.load(k_odd, v_odd, k0); },
+                             [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
+    };
+    const auto store = [&](const RowState<DP>& state) {
+        const float total = halves_sum(state.total);
+        if (!row.there) return;
+        const int64_t t = w.token0 + row.token;
+        if (whole) {
+            store_row<T, DP>(out, t, row.head, state.acc, total == 0.f ? 0.f : 1.f / total, p.dim);
+            if (lse != nullptr && half == 0) lse[static_cast<int64_t>(row.head) * p.q_tokens + t] = row_lse(state.top, total, p.scale);
+            return;
+        }
+        const int64_t at = parts.row(p, blockIdx.y, row.head, t);
+        if (half == 0) parts.stats[at] = F32x2{state.top, total};
 #pragma unroll
-    for (int i = 0; i < DP / 8; ++i) {
-        const int d = 8 * i + 4 * half;
-        const F32x16& acc = state.acc[i / 4];
-        if (d < p.dim)
-            *reinterpret_cast<F32x4*>(parts.out + at * p.dim + d) =
-                F32x4{acc[4 * (i % 4)], acc[4 * (i % 4) + 1], acc[4 * (i % 4) + 2], acc[4 * (i % 4) + 3]};
+        for (int i = 0; i < DP / 8; ++i) {
+            const int d = 8 * i + 4 * half;
+            const F32x16& acc = state.acc[i / 4];
+            if (d < p.dim)
+                *reinterpret_cast<F32x4*>(parts.out + at * p.dim + d) =
+                    F32x4{acc[4 * (i % 4)], acc[4 * (i % 4) + 1], acc[4 * (i % 4) + 2], acc[4 * (i % 4) + 3]};
+        }
+    };
+    pass(state, end);
+    store(state);  // (before waves wait for each other)
+    if (clean < end && block_any(any_not_finite(state.acc), &broken)) {
+        pass(state, clean);
+        careful_keys<T, DP>(state, qf, key_cache, value_cache, table, row, tree, p, w, kv_head, clean, wave_end, kWaveKeys);
+        store(state);
     }
 }
 
@@ -547,9 +582,9 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
         return set_error(kInvalidArgument, "%s: page size or page count out of range", what);
     if (table_width > table_stride || table_stride > 0x7FFFFFFFu)
         return set_error(kInvalidArgument, "%s: a block table's row must hold its width", what);
-    if (q_tokens > 0x7FFFFFFFull || q_tokens * (q_heads / kv_heads) > 0x7FFFFFFFull || requests > 0x7FFFFFFu)
+    if (q_tokens > 0x7FFFFFFFull || q_tokens * (q_heads / kv_heads) > kMostKeys || requests > 0x7FFFFFFu)
         return set_error(kInvalidArgument, "%s: too many tokens or requests", what);
-    if (max_kv_length > 0x7FFFFF00ull) return set_error(kInvalidArgument, "%s: requests too long", what);
+    if (max_kv_length > kMostKeys) return set_error(kInvalidArgument, "%s: requests too long", what);
     if (!(scale > 0.f) || scale == INFINITY) return set_error(kInvalidArgument, "%s: the scale must be positive and finite", what);
     if (requests == 0 || q_tokens == 0) return kOk;
     if (!q_offsets || !kv_lengths || (table_width && !block_table))

@@ -285,3 +285,49 @@ def test_infinities_and_nan_reach_the_rows_that_see_them(hip, dev, suffix, dim, 
         oracle.check("out", got["out"].cpu()[before], (want["out"][0][before], want["out"][1][before]))
         assert torch.isnan(got["out"].cpu()[~before][:, :2].float()).all()
         assert torch.isfinite(got["out"].cpu()[:, 2:].float()).all()
+
+
+@pytest.mark.parametrize("suffix,n,heads,kv_heads,dim", [("bf16", 200, 4, 2, 128), ("f16", 200, 4, 2, 64), ("bf16", 700, 8, 1, 80),
+                                                         ("f16", 300, 3, 1, 128)])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_gradients_pass_infinities_and_nan_along_what_is_seen(hip, dev, suffix, n, heads, kv_heads, dim, bad):
+    """A row or key that is not finite inside a causal sequence: the gradients of what does not meet it are as if it were
+    zero."""
+    dtype, group = DTYPE[suffix], heads // kv_heads
+    tensors = [rows(dtype, n, h, dim, s) for s, h in enumerate((heads, kv_heads, kv_heads, heads))]  # q, k, v, dout
+    o, place = oracle.offsets_of([n]), torch.arange(n)
+    for which, name in enumerate(("q", "k", "v", "dout")):
+        log(name)
+        of_keys = name in "kv"
+        h = (kv_heads if of_keys else heads) - 1
+        own = slice(h * group, heads) if of_keys else slice(h, heads)  # the query heads that meet it, and their key head
+        for where in (0, 45, 64, n - 1):
+            clean, broken = [x.clone() for x in tensors], [x.clone() for x in tensors]
+            clean[which][where, h] = 0
+            broken[which][where, h, 5] = bad
+            want = oracle.packed(*clean[:3], o, o, True, dim ** -0.5, clean[3])
+            got = run(hip, suffix, *broken[:3], o, o, True, None, broken[3])
+            row_hit = place >= where if of_keys else place == where
+            key_hit = torch.ones(n, dtype=torch.bool) if of_keys else place <= where
+            for gradient in ("dq", "dk", "dv"):
+                hit = torch.zeros(got[gradient].shape[:2], dtype=torch.bool)
+                if gradient == "dq":
+                    hit[:, own] = row_hit[:, None]
+                elif not (gradient == "dv" and name == "v"):  # (dV does not depend on V)
+                    hit[:, kv_heads - 1] = key_hit
+                value = got[gradient].cpu()
+                oracle.check(f"{gradient} of {name} at {where}", value[~hit], (want[gradient][0][~hit], want[gradient][1][~hit]))
+                if hit.any() and math.isnan(bad):
+                    assert not torch.isfinite(value[hit].float()).all(1).any()
+
+
+def test_rows_that_see_nothing_pass_nothing(hip, dev):
+    """Fewer keys than rows: what the first rows hold, NaN too, reaches no gradient."""
+    n, m, dim = 100, 70, 128
+    q, k, v, dout = (rows(torch.bfloat16, t, 2, dim, s) for s, t in enumerate((n, m, m, n)))
+    qo, ko = oracle.offsets_of([n]), oracle.offsets_of([m])
+    want = oracle.packed(q, k, v, qo, ko, True, dim ** -0.5, dout)
+    q[:n - m], dout[:n - m] = math.nan, math.nan
+    got = run(hip, "bf16", q, k, v, qo, ko, True, None, dout)
+    for name in ("lse", "out", "dv", "dq", "dk"):
+        oracle.check(name, got[name], want[name])

@@ -376,3 +376,24 @@ def test_infinities_and_nan_reach_the_rows_that_see_them(hip, dev, heads, max_kv
         mine = out.cpu()[sees].float()
         assert torch.isnan(mine[:, :, 7]).all() if math.isnan(bad) else (mine[:, :, 7] == bad).all()
         assert torch.isfinite(mine[:, :, :7]).all() and torch.isfinite(mine[:, :, 8:]).all()
+
+
+@pytest.mark.parametrize("heads,tree", [(2, None), (16, None), (2, "random")])
+def test_lengths_past_the_table(hip, dev, heads, tree):
+    """New tokens keep their places where the table ends before their request does: the keys past it are not seen, those
+    before are."""
+    s = make("bf16", [100, 60, 90], [5, 20, 60], heads, 1, 64, 16, tree=tree)
+    ends = s["table"].clone()
+    ends[:, 4:] = -1
+    want = oracle.paged(s["q"], s["key_cache"], s["value_cache"], ends, s["q_offsets"], s["kv"], s["tree"], 0.125)
+    s["table"] = s["table"][:, :4].contiguous()
+    out, lse = run_paged(hip, "bf16", s)
+    oracle.check("lse", lse, want["lse"])
+    oracle.check("out", out, want["out"])
+
+
+@pytest.mark.parametrize("max_kv", [None, 9000])
+def test_long_chunks(hip, dev, max_kv):
+    """A part of a prompt over what came before it: tiles of rows that see some of the new keys, all or none."""
+    compare(hip, "bf16", [700, 1300], [400, 150], 4, 1, 64, 16, max_kv=max_kv)
+    compare(hip, "f16", [600], [290], 2, 2, 128, 24, max_kv=max_kv)
