@@ -289,12 +289,10 @@ __global__ __launch_bounds__(kTokenBlock) void page_plan_tokens_kernel(
 }
 
 // ---- rows into pages ---------------------------------------------------------------------------------------------
-// A thread keeps its place in the row (`per` 16-byte chunks) and moves it for EACH tokens, `group` tokens apart; rows of
-// more chunks than a workgroup has threads are split over blockIdx.y.  Bound by memory, and for few tokens by latency.
-constexpr int kWriteTokens = 4;
-constexpr uint64_t kWriteGrid = 2048;  // fewer workgroups than this: one token a thread (256 rows of 1,024 items: 3.7 -> 2.2 us)
-
-template <int EACH>
+// A copy: a thread a 16-byte chunk of a token's key and value, neighbours next to each other.  A row has `per` chunks; a
+// workgroup takes `group` short rows, or one of blockIdx.y parts of a long one.  Bound by memory (65,521 tokens of 8 x 128
+// items, 537 MB, from a cold cache: 95 us, 5.6 TB/s; four tokens a thread: 102 us), and
+// by latency for a step's few tokens (256 of them: 2.2 us; four a thread: 3.5 us).
 __global__ __launch_bounds__(kTokenBlock) void paged_write_kernel(attention::Rows key, attention::Rows value,
                                                                   attention::Pages key_cache, attention::Pages value_cache,
                                                                   const int64_t* __restrict__ slots, int64_t tokens, int per,
@@ -303,33 +301,19 @@ __global__ __launch_bounds__(kTokenBlock) void paged_write_kernel(attention::Row
     const int rest = static_cast<int>(blockIdx.y) * kTokenBlock + static_cast<int>(threadIdx.x) % (group > 1 ? per : kTokenBlock);
     const int mine = group > 1 ? static_cast<int>(threadIdx.x) / per : 0;
     if (rest >= per || mine >= group) return;
+    const int64_t token = static_cast<int64_t>(blockIdx.x) * group + mine;
+    if (token >= tokens) return;
+    const int64_t slot = slots[token];
+    if (slot < 0) return;
     const int head = rest / chunks, chunk = rest % chunks;
-    const int64_t first = static_cast<int64_t>(blockIdx.x) * group * EACH + mine;
-    U32x4 k[EACH], v[EACH];
-    int64_t slot[EACH];
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int64_t token = first + i * group;
-        slot[i] = token < tokens ? slots[token] : -1;
-    }
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        const int64_t token = first + i * group;
-        if (slot[i] < 0) continue;
-        k[i] = __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(key.at(token, head) + chunk * 16));
-        v[i] = __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(value.at(token, head) + chunk * 16));
-    }
-#pragma unroll
-    for (int i = 0; i < EACH; ++i) {
-        if (slot[i] < 0) continue;
-        // Division in 32 bits where the slot allows.
-        const bool narrow = slot[i] <= 0xFFFFFFFFll;
-        const int64_t page = narrow ? page_size(static_cast<uint32_t>(slot[i])) : slot[i] / page_size.by;
-        if (page >= pages) continue;
-        const int64_t within = slot[i] - page * page_size.by;
-        *reinterpret_cast<U32x4*>(key_cache.at(page, within, head) + chunk * 16) = k[i];
-        *reinterpret_cast<U32x4*>(value_cache.at(page, within, head) + chunk * 16) = v[i];
-    }
+    const U32x4 k = __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(key.at(token, head) + chunk * 16));
+    const U32x4 v = __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(value.at(token, head) + chunk * 16));
+    // Division in 32 bits where the slot allows.
+    const int64_t page = slot <= 0xFFFFFFFFll ? page_size(static_cast<uint32_t>(slot)) : slot / page_size.by;
+    if (page >= pages) return;
+    const int64_t within = slot - page * page_size.by;
+    *reinterpret_cast<U32x4*>(key_cache.at(page, within, head) + chunk * 16) = k;
+    *reinterpret_cast<U32x4*>(value_cache.at(page, within, head) + chunk * 16) = v;
 }
 
 int page_plan(void* temp, size_t temp_bytes, const int32_t* cached, const int32_t* fresh, uint32_t requests, uint32_t page_size,
@@ -395,15 +379,19 @@ int paged_write(const lcpp_hip_rows* key, const lcpp_hip_rows* value, const int6
     const int chunks = static_cast<int>(dim / 8), per = static_cast<int>(kv_heads) * chunks;
     const int group = per <= kTokenBlock / 2 ? kTokenBlock / per : 1;
     const uint64_t splits = ceil_div(per, kTokenBlock);
-    const int each = ceil_div(tokens, static_cast<uint64_t>(group) * kWriteTokens) * splits < kWriteGrid ? 1 : kWriteTokens;
-    const uint64_t blocks = ceil_div(tokens, static_cast<uint64_t>(group) * each);
-    if (blocks * splits > 0xFFFFFFFFull / kTokenBlock || splits > 65535) return set_error(kInvalidArgument, "%s: too many tokens", what);
+    if (splits > 65535) return set_error(kInvalidArgument, "%s: rows too long", what);
+    const uint64_t most = 0x7FFFFFFFull / kTokenBlock / splits * group;  // tokens of a launch
     LaunchScope scope("paged_write", stream);
-    auto* kernel = each == 1 ? paged_write_kernel<1> : paged_write_kernel<kWriteTokens>;
-    kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(splits)), kTokenBlock, 0, stream>>>(
-        attention::rows_of(key), attention::rows_of(value), attention::pages_of(key_cache), attention::pages_of(value_cache), slots,
-        static_cast<int64_t>(tokens), per, chunks, group, attention::Divider(page_size),
-        static_cast<int64_t>(pages));
+    attention::Rows k = attention::rows_of(key), v = attention::rows_of(value);
+    for (uint64_t first = 0; first < tokens; first += most) {
+        const uint64_t count = tokens - first < most ? tokens - first : most;
+        const unsigned blocks = static_cast<unsigned>(ceil_div(count, static_cast<uint64_t>(group)));
+        paged_write_kernel<<<dim3(blocks, static_cast<unsigned>(splits)), kTokenBlock, 0, stream>>>(
+            k, v, attention::pages_of(key_cache), attention::pages_of(value_cache), slots + first, static_cast<int64_t>(count), per,
+            chunks, group, attention::Divider(page_size), static_cast<int64_t>(pages));
+        k.data += static_cast<int64_t>(count) * k.token_bytes;
+        v.data += static_cast<int64_t>(count) * v.token_bytes;
+    }
     return check_hip(hipGetLastError(), "paged_write launch");
 }
 
