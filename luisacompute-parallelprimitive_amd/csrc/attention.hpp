@@ -109,6 +109,7 @@ __device__ __forceinline__ float halves_sum(float x) {
     return h.low + h.high;
 }
 
+// (An ulp or so; results below the least normal number are 0, which is 2^-126 of a row's largest weight.)
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
 constexpr uint64_t kMostKeys = 0x7FFFF000;  // of a sequence: a few tiles below what a position may be
@@ -174,11 +175,11 @@ inline Pages pages_of(const lcpp_hip_pages* c) {
 }
 
 // A tile of rows in LDS: DP items a row (the head size rounded up; zeros past it), in chunks of 16 bytes, with room for 64
-// or 128 items.  A wave's direct load writes 64 chunks in lane order: 4 rows of 128 items, or 8 of 64.  Within these four chunks of a row lie side by side
-// (64 bytes that a load reads together), then the same four of the next row; and from one 4 rows to the next a chunk moves
-// by 16 bytes, by padding or by exchanging neighbours.  So the same chunk of 16 rows (a read along rows), and four chunks
-// of four rows (a transposed read), fill the 64 banks of 4 bytes once; and a lane's addresses in one tile differ by
-// constants.
+// or 128 items.  A wave's direct load writes 64 chunks in lane order: 4 rows of 128 items, or 8 of 64.  Within these four
+// chunks of a row lie side by side (64 bytes that a load reads together), then the same four of the next row; and from one
+// 4 rows to the next a chunk moves by 16 bytes, by padding or by exchanging neighbours.  So the same chunk of 16 rows (a
+// read along rows), and four chunks of four rows (a transposed read), fill the 64 banks of 4 bytes once; and a lane's
+// addresses in one tile differ by constants.
 template <int DP>
 struct Tile {
     static_assert(DP % 32 == 0 && DP <= 128);

@@ -8,11 +8,13 @@ namespace {
 constexpr int kScanBlock = 1024;
 constexpr int kTokenBlock = 256;
 // Requests that every workgroup scans for itself, so that a plan is one launch; more are scanned by one workgroup first.
-// (64 requests: 4.7 us for two launches, 3.7 us for one.)  Twelve bytes of LDS a request leave room for two workgroups on a
-// compute unit.
+// (64 requests: 5.3 us for two launches, 3.3 us for one; 4,096 requests and tokens: 9.0 and 6.1.)  Twelve bytes of LDS a
+// request leave room for two workgroups on a compute unit.
 constexpr int kRequestsPerThread = 5;
 constexpr int kFusedRequests = kRequestsPerThread * kScanBlock;
-constexpr int kTokensPerThread = 4;  // where there are tokens for every compute unit at that (kFusedTokens)
+// Where there are tokens for every compute unit at that (kFusedTokens): 250,000 tokens take 7.0 us with one a thread, 9.2
+// with four, 600,000 13.5 and 10.1, 1.2 million 20 and 12.6.
+constexpr int kTokensPerThread = 4;
 constexpr uint64_t kFusedTokens = 256 * kScanBlock;
 
 struct Plan {
@@ -135,7 +137,7 @@ __device__ __forceinline__ int owner_of(Token t, int low, int high, Offset offse
 // A plan of at most kFusedRequests requests.  Every workgroup scans all of them into LDS, a few consecutive requests a
 // thread; the first writes the requests' outputs, and each places its tokens, EACH consecutive ones a thread: the tokens of
 // a wave lie between the owners of its first and its last, which it finds together.  Bound by latency up to some hundred
-// thousand tokens, then by the instructions a token takes (with one token a thread 1.2 million took 24 us).
+// thousand tokens, then by the instructions a token takes: 1.2 million tokens, 19.8 MB, take 12.6 us, 1.6 TB/s.
 template <int EACH>
 __global__ __launch_bounds__(kScanBlock) void page_plan_kernel(const int32_t* __restrict__ cached, const int32_t* __restrict__ fresh,
                                                                const int32_t* __restrict__ free_pages, int32_t* __restrict__ block_table,
