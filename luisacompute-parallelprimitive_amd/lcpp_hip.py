@@ -525,7 +525,7 @@ def _temp_for(nbytes: int, like, temp):
 
 
 def _tb(temp) -> int:
-    return temp.numel() * temp.element_size()
+    return 0 if temp is None else temp.numel() * temp.element_size()
 
 
 def select_flagged(suffix: str, flag_suffix: str, d_in, flags, d_out, num_out, n: int, temp=None, stream=None):
@@ -750,6 +750,18 @@ def _axes(name: str, t, axes: int) -> tuple:
     return tuple(t.shape)
 
 
+def _scratch(nbytes: int, device, stream):
+    """Temporary storage of one call: none where none is needed, otherwise memory of the stream that the call runs on (what
+    another stream has freed may still be in use there)."""
+    if nbytes == 0:
+        return None
+    if stream is None:
+        return _temp(nbytes, device)
+    import torch
+    with torch.cuda.stream(stream):
+        return _temp(nbytes, device)
+
+
 def page_plan_temp_bytes(requests: int) -> int:
     return lib().lcpp_hip_page_plan_temp_bytes(requests)
 
@@ -762,7 +774,7 @@ def page_plan(cached_lengths, new_lengths, page_size: int, free_pages, block_tab
     _, _, i32, i64 = _row_types("bf16")
     table, table_stride, width = _table(i32, block_table, requests)
     if temp is None:
-        temp = _temp(page_plan_temp_bytes(requests), cached_lengths.device)
+        temp = _scratch(page_plan_temp_bytes(requests), cached_lengths.device, stream)
     call("lcpp_hip_page_plan", ptr(temp), _tb(temp), _array(i32, "cached_lengths", cached_lengths, requests),
          _array(i32, "new_lengths", new_lengths, requests), requests, page_size,
          _array(i32, "free_pages", free_pages, 0), free_pages.numel(), table, table_stride, width,
@@ -803,7 +815,7 @@ def attention_packed(suffix: str, q, k, v, q_offsets, k_offsets, out, lse=None, 
     keys, kv_heads, _ = _axes("k", k, 3)
     sequences = q_offsets.numel() - 1
     if temp is None:
-        temp = _temp(attention_packed_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device)
+        temp = _scratch(attention_packed_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device, stream)
     shape = (keys, kv_heads, dim)
     call(f"lcpp_hip_attention_packed_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows), _rows(dt, "k", k, shape),
          _rows(dt, "v", v, shape), _array(i32, "q_offsets", q_offsets, 1),
@@ -820,7 +832,7 @@ def attention_packed_backward(suffix: str, q, k, v, out, lse, dout, q_offsets, k
     keys, kv_heads, _ = _axes("k", k, 3)
     sequences = q_offsets.numel() - 1
     if temp is None:
-        temp = _temp(attention_packed_backward_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device)
+        temp = _scratch(attention_packed_backward_temp_bytes(sequences, tokens, keys, heads, kv_heads, dim), q.device, stream)
     shape = (keys, kv_heads, dim)
     call(f"lcpp_hip_attention_packed_backward_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows),
          _rows(dt, "k", k, shape), _rows(dt, "v", v, shape), _rows(dt, "out", out, rows),
@@ -850,7 +862,7 @@ def attention_paged(suffix: str, q, key_cache, value_cache, block_table, q_offse
     if max_kv_length is None:
         max_kv_length = width * page_size
     if temp is None:
-        temp = _temp(attention_paged_temp_bytes(requests, tokens, max_kv_length, heads, kv_heads, dim), q.device)
+        temp = _scratch(attention_paged_temp_bytes(requests, tokens, max_kv_length, heads, kv_heads, dim), q.device, stream)
     call(f"lcpp_hip_attention_paged_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows),
          _pages(dt, "key_cache", key_cache, cache),
          _pages(dt, "value_cache", value_cache, cache), table, table_stride, width,

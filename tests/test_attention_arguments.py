@@ -157,3 +157,16 @@ def test_temp_bytes_hold_their_parts(hip):
     one = hip.attention_paged_temp_bytes(1, 1, 131_000, 32, 8, 128)
     assert 0 < one < 64 << 20
     assert isinstance(C.sizeof(hip.Rows), int) and C.sizeof(hip.Rows) == 24 and C.sizeof(hip.Pages) == 32
+
+
+def test_calls_that_need_no_scratch_take_none(hip, monkeypatch):
+    """No allocation where none is needed; the caller's storage is passed on as it is."""
+    calls = []
+    monkeypatch.setattr(hip, "call", lambda name, *args: calls.append(args))
+    monkeypatch.setattr(hip, "stream_handle", lambda stream=None: None)
+    q, o = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
+    hip.attention_packed("bf16", q, q, q, o, o, q.clone())
+    assert calls[0][:2] == (None, 0)
+    mine = torch.zeros(10, dtype=torch.uint8)
+    hip.attention_packed("bf16", q, q, q, o, o, q.clone(), temp=mine)
+    assert calls[1][:2] == (mine.data_ptr(), 10)

@@ -397,3 +397,23 @@ def test_long_chunks(hip, dev, max_kv):
     """A part of a prompt over what came before it: tiles of rows that see some of the new keys, all or none."""
     compare(hip, "bf16", [700, 1300], [400, 150], 4, 1, 64, 16, max_kv=max_kv)
     compare(hip, "f16", [600], [290], 2, 2, 128, 24, max_kv=max_kv)
+
+
+def test_scratch_belongs_to_the_stream_of_the_call(hip, dev):
+    """Calls on a given stream, without temporary storage of the caller's, beside the current stream's own allocations."""
+    s = make("bf16", [2777, 900], [1, 1], 4, 1, 64, 16)
+    d = {k: None if v is None else v.cuda() for k, v in s.items()}
+    want, want_lse = run_paged(hip, "bf16", s, 200_000)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    need = hip.attention_paged_temp_bytes(2, 2, 200_000, 4, 1, 64)
+    assert need > 0
+    for _ in range(5):
+        out, lse = torch.full_like(want, 7.0), torch.full_like(want_lse, 7.0)
+        side.wait_stream(torch.cuda.current_stream())
+        hip.attention_paged("bf16", d["q"], d["key_cache"], d["value_cache"], d["table"], d["q_offsets"], d["kv"], out, lse,
+                            max_kv_length=200_000, stream=side)
+        busy = torch.full((need,), 255, dtype=torch.uint8, device="cuda")  # would be the call's storage, if it were this stream's
+        del busy
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
