@@ -14,3 +14,4 @@
 #include "lcpp/device/device_segmented_scan.h"
 #include "lcpp/device/device_segmented_sort.h"
 #include "lcpp/device/device_segmented_radix_sort.h"
+#include "lcpp/device/device_attention.h"

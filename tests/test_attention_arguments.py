@@ -1,6 +1,8 @@
 """Attention's refusals through the C-ABI and the binding, on a machine without a GPU: arguments are checked before any HIP
 call."""
 import ctypes as C
+import pathlib
+import subprocess
 import types
 
 import pytest
@@ -170,3 +172,11 @@ def test_calls_that_need_no_scratch_take_none(hip, monkeypatch):
     mine = torch.zeros(10, dtype=torch.uint8)
     hip.attention_packed("bf16", q, q, q, o, o, q.clone(), temp=mine)
     assert calls[1][:2] == (mine.data_ptr(), 10)
+
+
+def test_cpp_module_builds_and_lists_its_cases():
+    repo = pathlib.Path(__file__).resolve().parents[1]
+    subprocess.run(["make", "-s", "-C", str(repo / "tests" / "cpp")], check=True)
+    out = subprocess.run([str(repo / "tests" / "cpp" / "bin" / "attention_test"), "--list"], check=True, capture_output=True,
+                         text=True).stdout.split()
+    assert out == ["packed_forward", "plan_write_and_paged", "packed_gradients", "refusals"]
