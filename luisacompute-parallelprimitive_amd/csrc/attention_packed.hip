@@ -10,7 +10,7 @@
 // 4 * dim operations a pair of row and key, and little to read (each row of K and V once for 128 query rows): long
 // sequences are bound by the matrix cores.  One of 16,384 rows, 16 heads of 128: 1,070 to 1,100 us, 1,000 to 1,030 TFLOP/s,
 // where a large library product reaches 1,168; the clock falls as low as 1.7 GHz under it, so what is left is power.
-// Uneven prompts of 60 to 2,500 rows (32 heads of 128) take 155 us, 660 TFLOP/s: their last tiles are part empty, and a
+// Uneven prompts of 60 to 2,500 rows (32 heads of 128) take 148 us, 700 TFLOP/s: their last tiles are part empty, and a
 // workgroup of few keys is latency.  Seven prompts of up to 200 rows: 7.2 us, all of it latency.
 //
 // A workgroup: four waves of 32 rows and 64 keys at a time, keys and values shared in LDS (33 KB a set of buffers at 128
@@ -22,13 +22,56 @@ namespace lcpp_hip {
 namespace attention {
 namespace {
 
+struct GreaterOp {
+    template <typename T>
+    __device__ static T identity() { return std::numeric_limits<T>::lowest(); }
+    template <typename T>
+    __device__ T operator()(T a, T b) const { return a < b ? b : a; }
+};
+
+// Tiles of a batch of at most 64 sequences in the order of the keys that they see, the most first: a workgroup of a long
+// sequence's last rows takes half of an uneven batch's time, and has to start early (16 uneven prompts: 154 us in the
+// tiles' order, 148 so; finding the place takes half a microsecond more).  A lane holds a sequence; its tiles are at
+// consecutive levels (128 keys each; all at one without a causal mask), and the level of number `number` is found by
+// halving.
+struct OrderedTile {
+    int tile;  // -1: none
+    Span rows, keys;
+    __device__ __forceinline__ OrderedTile(const int32_t* q_offsets, const int32_t* k_offsets, const Shape& shape, int number) {
+        const int lane = threadIdx.x % kWave, sequence = lane < shape.sequences ? lane : shape.sequences - 1;
+        const Span r = span_of(q_offsets, sequence, shape.q_tokens), k = span_of(k_offsets, sequence, shape.k_tokens);
+        const int tiles = lane < shape.sequences ? (r.size + kRowTile - 1) / kRowTile : 0;
+        const int first = (shape.causal ? k.size - r.size : k.size) >> 7;  // the level of the first tile
+        static_assert(kRowTile == 1 << 7);
+        const auto from = [&](int level) {  // tiles at this level or above
+            if (!shape.causal) return level <= first ? tiles : 0;
+            const int n = first + tiles - level;
+            return n < 0 ? 0 : n < tiles ? n : tiles;
+        };
+        int low = -wave_reduce(tiles ? -first : -INT32_MAX, GreaterOp{}), high = wave_reduce(tiles ? first + tiles : -INT32_MAX, GreaterOp{});
+        tile = -1;
+        if (wave_reduce(tiles, SumOp{}) <= number) return;
+        int above = 0;  // tiles above `high`, or at it: not more than number; at `low` there are more
+        while (high - low > 1) {
+            const int level = low + (high - low) / 2, n = wave_reduce(from(level), SumOp{});
+            if (n > number) low = level;
+            else high = level, above = n;
+        }
+        const int mine = from(low) - from(high), before = wave_inclusive_scan(mine, SumOp{}) - mine, rest = number - above - before;
+        const int owner = __ffsll(static_cast<unsigned long long>(wave_ballot(rest >= 0 && rest < mine))) - 1;
+        tile = wave_read_lane(shape.causal ? low - first : rest, owner);
+        rows = {wave_read_lane(r.begin, owner), wave_read_lane(r.size, owner)};
+        keys = {wave_read_lane(k.begin, owner), wave_read_lane(k.size, owner)};
+    }
+};
+
 // DP, the head size that registers and LDS are laid out for: 64, 96 or 128 (heads of 80 in 96 items 16.8 us, in 128 18.9;
 // of 64 in 64 items 9.8 us, in 128 11.8).  At 64, three waves a SIMD need no scratch; four took the same time.
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_kernel(Rows q, Rows k, Rows v, Rows out, float* __restrict__ lse,
                                                                      const int32_t* __restrict__ q_offsets,
                                                                      const int32_t* __restrict__ k_offsets, Shape shape,
-                                                                     int tiles) {
+                                                                     int tiles, bool ordered_tiles) {
     constexpr int kTileBytes = Tile<DP>::bytes(kKeyTile);
     __shared__ __attribute__((aligned(16))) char k_even[kTileBytes];
     __shared__ __attribute__((aligned(16))) char v_even[kTileBytes];
@@ -37,17 +80,25 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_ker
     __shared__ int broken;  // whether the sums of some wave are not finite
     if (threadIdx.x == 0) broken = 0;
     // Workgroups go to the 8 XCDs in turn: with the key head as the fastest number, those of a key head share an L2.
-    // Later tiles, which see more keys, come first.
+    // Tiles that see more keys come first.
     const int group = shape.q_heads / shape.kv_heads;
     const int kv_head = blockIdx.x % shape.kv_heads;
     const int head = kv_head * group + blockIdx.x / shape.kv_heads % group;
-    const int number = tiles - 1 - static_cast<int>(blockIdx.x / shape.q_heads);
-    const TilePlace place = find_tile(q_offsets, shape.sequences, 1, kRowTile, number);
-    if (place.sequence < 0) return;
-    const Span rows = span_of(q_offsets, place.sequence, shape.q_tokens);
-    const int row0 = place.tile * kRowTile;
+    const int number = static_cast<int>(blockIdx.x / shape.q_heads);
+    Span rows, keys;
+    int row0;
+    if (ordered_tiles) {
+        const OrderedTile ordered(q_offsets, k_offsets, shape, number);
+        if (ordered.tile < 0) return;
+        rows = ordered.rows, keys = ordered.keys, row0 = ordered.tile * kRowTile;
+    } else {
+        const TilePlace place = find_tile(q_offsets, shape.sequences, 1, kRowTile, tiles - 1 - number);
+        if (place.sequence < 0) return;
+        rows = span_of(q_offsets, place.sequence, shape.q_tokens);
+        keys = span_of(k_offsets, place.sequence, shape.k_tokens);
+        row0 = place.tile * kRowTile;
+    }
     if (row0 >= rows.size) return;
-    const Span keys = span_of(k_offsets, place.sequence, shape.k_tokens);
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int row = row0 + threadIdx.x / kWave * kRowsPerWave + lane % 32;
     const bool there = row < rows.size;
@@ -86,6 +137,8 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_ker
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
+constexpr unsigned kResident = 512;  // workgroups that run at once, two a compute unit
+
 template <typename T>
 int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* v, const int32_t* q_offsets,
            const int32_t* k_offsets, const lcpp_hip_rows* out, float* lse, uint32_t sequences, uint64_t q_tokens,
@@ -102,13 +155,15 @@ int packed(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const lcpp_hip_rows* 
     if (int st = check_grid(what, q_tokens, kRowTile, sequences, q_heads, tiles, grid); st != kOk) return st;
     const Shape shape{static_cast<int>(sequences), static_cast<int>(q_tokens), static_cast<int>(k_tokens),
                       static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(dim), scale, causal != 0};
+    // Several sequences, one for each lane of a wave at most, and more workgroups than run at once: see OrderedTile.
+    const bool ordered_tiles = sequences > 1 && sequences <= kWave && grid > kResident;
     const Rows none{nullptr, 0, 0};
     const Rows kr = k_tokens ? rows_of(k) : none, vr = k_tokens ? rows_of(v) : none;
     LaunchScope scope("attention_packed", stream);
     auto* kernel = dim <= 64   ? attention_packed_kernel<T, 64>
                    : dim <= 96 ? attention_packed_kernel<T, 96>
                                : attention_packed_kernel<T, 128>;
-    kernel<<<grid, kBlock, 0, stream>>>(rows_of(q), kr, vr, rows_of(out), lse, q_offsets, k_offsets, shape, tiles);
+    kernel<<<grid, kBlock, 0, stream>>>(rows_of(q), kr, vr, rows_of(out), lse, q_offsets, k_offsets, shape, tiles, ordered_tiles);
     return check_hip(hipGetLastError(), "attention_packed launch");
 }
 

@@ -331,3 +331,16 @@ def test_rows_that_see_nothing_pass_nothing(hip, dev):
     got = run(hip, "bf16", q, k, v, qo, ko, True, None, dout)
     for name in ("lse", "out", "dv", "dq", "dk"):
         oracle.check(name, got[name], want[name])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("sequences", [2, 63, 64, 65])
+def test_batches_of_more_workgroups_than_run_at_once(hip, dev, causal, sequences):
+    """Tiles are then taken in the order of their keys, up to 64 sequences: short and long ones, empty ones, keys with a head
+    start, and fewer keys than rows."""
+    lengths = [(37 * i * i) % 140 + (i % 5 == 0) * 150 for i in range(sequences)]
+    lengths[1], lengths[-1] = 0, 300
+    keys = [max(0, n + (-40, 0, 170)[i % 3]) for i, n in enumerate(lengths)]
+    heads = 32 if sequences > 2 else 260
+    assert sum(-(-n // 128) for n in lengths) * heads > 512
+    compare(hip, "bf16", lengths, keys, heads, heads // 4, 32, causal)
