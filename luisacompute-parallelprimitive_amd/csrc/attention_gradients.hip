@@ -77,6 +77,7 @@ struct GradientArgs {
     int row_tiles;    // tiles of rows, and workgroups of keys and parts of each
     int key_blocks;
     int parts;
+    bool ordered_tiles;
 };
 
 // dQ: two teams of four waves share the keys' and values' tiles.  They take a tile of rows of two heads of one key head, or
@@ -92,12 +93,20 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
     const int kv_head = unit % shape.kv_heads;
     const int head = kv_head * group + (two_heads ? unit / shape.kv_heads * 2 + team : unit / shape.kv_heads);
     const int tile_rows = two_heads ? kRowTile : kTeams * kRowTile;
-    const TilePlace place = find_tile(g.q_offsets, shape.sequences, 1, tile_rows, g.row_tiles - 1 - block / units);
-    if (place.sequence < 0) return;
-    const Span rows = span_of(g.q_offsets, place.sequence, shape.q_tokens);
-    const int first_row = place.tile * tile_rows;
+    Span rows, keys;
+    int first_row;
+    if (g.ordered_tiles) {
+        if (!(two_heads ? take_ordered_tile<kRowTile>(g.q_offsets, g.k_offsets, shape, block / units, rows, keys, first_row)
+                        : take_ordered_tile<kTeams * kRowTile>(g.q_offsets, g.k_offsets, shape, block / units, rows, keys, first_row)))
+            return;
+    } else {
+        const TilePlace place = find_tile(g.q_offsets, shape.sequences, 1, tile_rows, g.row_tiles - 1 - block / units);
+        if (place.sequence < 0) return;
+        rows = span_of(g.q_offsets, place.sequence, shape.q_tokens);
+        keys = span_of(g.k_offsets, place.sequence, shape.k_tokens);
+        first_row = place.tile * tile_rows;
+    }
     if (first_row >= rows.size) return;
-    const Span keys = span_of(g.k_offsets, place.sequence, shape.k_tokens);
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int row0 = two_heads ? first_row : first_row + team * kRowTile;
     const int row = row0 + threadIdx.x % kBlock / kWave * kRowsPerWave + lane % 32;
@@ -193,14 +202,20 @@ struct RowTiles {  // of one team: which head of the group, which row
 template <typename T, int DP>
 __device__ __forceinline__ void dkv_block(const GradientArgs& args, const GradientMemory<DP>& memory, int block, int part) {
     constexpr int kTileBytes = Tile<DP>::bytes(kQueryTile);
-    const auto& [q, k, v, dout, dq, dk, dv, stats, part_sums, q_offsets, k_offsets, shape, row_tiles, key_blocks, parts] = args;
+    const auto& [q, k, v, dout, dq, dk, dv, stats, part_sums, q_offsets, k_offsets, shape, row_tiles, key_blocks, parts, ordered_tiles] = args;
     const int kv_head = block % shape.kv_heads;
-    const TilePlace place = find_tile(k_offsets, shape.sequences, 1, kRowTile, block / shape.kv_heads);
-    if (place.sequence < 0) return;
-    const Span keys = span_of(k_offsets, place.sequence, shape.k_tokens);
-    const int key0 = place.tile * kRowTile;
+    Span rows, keys;
+    int key0;
+    if (ordered_tiles) {
+        if (!take_ordered_keys<kRowTile>(q_offsets, k_offsets, shape, block / shape.kv_heads, rows, keys, key0)) return;
+    } else {
+        const TilePlace place = find_tile(k_offsets, shape.sequences, 1, kRowTile, block / shape.kv_heads);
+        if (place.sequence < 0) return;
+        keys = span_of(k_offsets, place.sequence, shape.k_tokens);
+        rows = span_of(q_offsets, place.sequence, shape.q_tokens);
+        key0 = place.tile * kRowTile;
+    }
     if (key0 >= keys.size) return;
-    const Span rows = span_of(q_offsets, place.sequence, shape.q_tokens);
     const int group = shape.q_heads / shape.kv_heads;
     const int lane = threadIdx.x % kWave, half = lane / 32;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x % kBlock / kWave);
@@ -424,6 +439,8 @@ __global__ __launch_bounds__(kBlock) void attention_dkv_join_kernel(Rows dk, Row
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
+constexpr uint64_t kResident = 256;  // workgroups that run at once, one a compute unit
+
 // Workgroups that share a tile of keys: as many as there are compute units, while each still has a few tiles of rows (one
 // sequence of 1,024 rows, 32 heads on 8 keys' heads: 130 us unsplit, 86 so, 104 with twice as many; on one: 835, 90, 111).
 constexpr uint64_t kKeyGrid = 256;
@@ -484,7 +501,8 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
                             reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(q_tokens, q_heads)), q_offsets, k_offsets,
                             Shape{static_cast<int>(sequences), static_cast<int>(q_tokens), static_cast<int>(k_tokens),
                                   static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(dim), scale, causal != 0},
-                            static_cast<int>(tiles), k_tokens ? static_cast<int>(key_grid) : 0, static_cast<int>(parts)};
+                            static_cast<int>(tiles), k_tokens ? static_cast<int>(key_grid) : 0, static_cast<int>(parts),
+                            sequences > 1 && sequences <= kWave && blocks > kResident};
     if (q_tokens) {
         LaunchScope scope("attention_row_stats", stream);
         const uint64_t stat_blocks = ceil_div(q_tokens * q_heads, kBlock / 16);

@@ -22,49 +22,6 @@ namespace lcpp_hip {
 namespace attention {
 namespace {
 
-struct GreaterOp {
-    template <typename T>
-    __device__ static T identity() { return std::numeric_limits<T>::lowest(); }
-    template <typename T>
-    __device__ T operator()(T a, T b) const { return a < b ? b : a; }
-};
-
-// Tiles of a batch of at most 64 sequences in the order of the keys that they see, the most first: a workgroup of a long
-// sequence's last rows takes half of an uneven batch's time, and has to start early (16 uneven prompts: 154 us in the
-// tiles' order, 148 so; finding the place takes half a microsecond more).  A lane holds a sequence; its tiles are at
-// consecutive levels (128 keys each; all at one without a causal mask), and the level of number `number` is found by
-// halving.
-struct OrderedTile {
-    int tile;  // -1: none
-    Span rows, keys;
-    __device__ __forceinline__ OrderedTile(const int32_t* q_offsets, const int32_t* k_offsets, const Shape& shape, int number) {
-        const int lane = threadIdx.x % kWave, sequence = lane < shape.sequences ? lane : shape.sequences - 1;
-        const Span r = span_of(q_offsets, sequence, shape.q_tokens), k = span_of(k_offsets, sequence, shape.k_tokens);
-        const int tiles = lane < shape.sequences ? (r.size + kRowTile - 1) / kRowTile : 0;
-        const int first = (shape.causal ? k.size - r.size : k.size) >> 7;  // the level of the first tile
-        static_assert(kRowTile == 1 << 7);
-        const auto from = [&](int level) {  // tiles at this level or above
-            if (!shape.causal) return level <= first ? tiles : 0;
-            const int n = first + tiles - level;
-            return n < 0 ? 0 : n < tiles ? n : tiles;
-        };
-        int low = -wave_reduce(tiles ? -first : -INT32_MAX, GreaterOp{}), high = wave_reduce(tiles ? first + tiles : -INT32_MAX, GreaterOp{});
-        tile = -1;
-        if (wave_reduce(tiles, SumOp{}) <= number) return;
-        int above = 0;  // tiles above `high`, or at it: not more than number; at `low` there are more
-        while (high - low > 1) {
-            const int level = low + (high - low) / 2, n = wave_reduce(from(level), SumOp{});
-            if (n > number) low = level;
-            else high = level, above = n;
-        }
-        const int mine = from(low) - from(high), before = wave_inclusive_scan(mine, SumOp{}) - mine, rest = number - above - before;
-        const int owner = __ffsll(static_cast<unsigned long long>(wave_ballot(rest >= 0 && rest < mine))) - 1;
-        tile = wave_read_lane(shape.causal ? low - first : rest, owner);
-        rows = {wave_read_lane(r.begin, owner), wave_read_lane(r.size, owner)};
-        keys = {wave_read_lane(k.begin, owner), wave_read_lane(k.size, owner)};
-    }
-};
-
 // DP, the head size that registers and LDS are laid out for: 64, 96 or 128 (heads of 80 in 96 items 16.8 us, in 128 18.9;
 // of 64 in 64 items 9.8 us, in 128 11.8).  At 64, three waves a SIMD need no scratch; four took the same time.
 template <typename T, int DP>
@@ -88,9 +45,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_ker
     Span rows, keys;
     int row0;
     if (ordered_tiles) {
-        const OrderedTile ordered(q_offsets, k_offsets, shape, number);
-        if (ordered.tile < 0) return;
-        rows = ordered.rows, keys = ordered.keys, row0 = ordered.tile * kRowTile;
+        if (!take_ordered_tile<kRowTile>(q_offsets, k_offsets, shape, number, rows, keys, row0)) return;
     } else {
         const TilePlace place = find_tile(q_offsets, shape.sequences, 1, kRowTile, tiles - 1 - number);
         if (place.sequence < 0) return;
