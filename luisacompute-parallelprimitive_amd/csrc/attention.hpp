@@ -212,8 +212,11 @@ template <int DP>
 __device__ __forceinline__ U32x4 read_columns(const char* tile, int row0, int col0) {
     using LdsPtr = __attribute__((address_space(3))) S16x4*;
     const int lane = threadIdx.x % kWave;
-    const char* p = tile + Tile<DP>::place(4 * (lane / 32) + lane % 16 / 4, 2 * (lane / 16 % 2) + lane % 4 / 2) + lane % 2 * 8;
-    p += Tile<DP>::bytes(row0) + col0 / 32 * 256;
+    // One offset, which the compiler does not take apart: behind more than a few steps of address arithmetic it no longer knows
+    // which array is read, and waits for the loads into all of them.
+    int at = Tile<DP>::place(4 * (lane / 32) + lane % 16 / 4, 2 * (lane / 16 % 2) + lane % 4 / 2) + lane % 2 * 8;
+    asm("" : "+v"(at));
+    const char* p = tile + at + (Tile<DP>::bytes(row0) + col0 / 32 * 256);
     const S16x4 a = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p));
     const S16x4 b = __builtin_amdgcn_ds_read_tr16_b64_v4i16((LdsPtr)(p + Tile<DP>::bytes(8)));
     const U32x2 x = __builtin_bit_cast(U32x2, a), y = __builtin_bit_cast(U32x2, b);

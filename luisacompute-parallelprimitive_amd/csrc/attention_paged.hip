@@ -23,9 +23,11 @@ constexpr int kNarrowRows = 32;
 constexpr int kWaveKeys = 32;                  // keys of a wave at a time
 constexpr int kKeyStep = kWaves * kWaveKeys;   // keys of a workgroup at a time
 constexpr int kPartKeys = 256;  // at least so many keys make a part: two turns of a workgroup (1,024 took the same time)
-// Workgroups wanted, if all requests were the longest.  Narrow: two for each compute unit, which is what is resident (one
-// request of 131,000 keys: 119 us with 1,024, 116 with 512, 120 with 256).  Wide: three times as many, because a long
-// request's parts are few and end together (24 trees: 116 us with 512, 113 with 1,024, 105 with 1,536).
+// Workgroups wanted at most, if all requests were the longest.  Narrow: two for each compute unit, which is what is resident
+// (one request of 131,000 keys: 119 us with 1,024, 116 with 512, 120 with 256).  Wide: three times as many, because a long
+// request's parts are few and end together (24 trees: 116 us with 512, 113 with 1,024, 105 with 1,536).  The parts are
+// rounded down: one more would pass that number (a chunk of 4,096 rows, which then has no parts, 213 us where two parts
+// take 265, 11 requests of 30,000 keys 265 and 300, 24 of 4,000 94 and 102; 40 of 4,000 150 and 145).
 constexpr int kNarrowGrid = 512;
 constexpr int kWideGrid = 1536;
 
@@ -353,8 +355,11 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     }
 }
 
-// Direct loads of tiles of keys and values from the cache.  Positions past the last are loaded as the last, and masked; the
-// chunks of a page that is not there become zeros.
+// A row of zeros, for a page that is not there.
+__device__ __attribute__((aligned(16))) const uint32_t zero_row[64] = {};
+
+// Direct loads of tiles of keys and values from the cache.  Positions past the last are loaded as the last, and masked; rows
+// of a page that is not there are loaded from a row of zeros.
 template <int DP>
 struct PagedTiles {
     using Loads = TileLoads<DP, kKeyTile>;
@@ -380,14 +385,11 @@ struct PagedTiles {
 #pragma unroll
             for (int i = 0; i < Loads::kPerWave; ++i) {
                 const int64_t slot = slot_of(p, position(k0, i));
-                if (page[i] >= 0 && page[i] < p.pages) {
-                    load_to_lds(keys + page[i] * key_cache.page_bytes + slot * key_cache.token_bytes + chunk * 16, Loads::place(k_tile, i));
-                    load_to_lds(values + page[i] * value_cache.page_bytes + slot * value_cache.token_bytes + chunk * 16,
-                                Loads::place(v_tile, i));
-                } else {
-                    *reinterpret_cast<U32x4*>(Loads::place(k_tile, i) + threadIdx.x % kWave * 16) = U32x4{0u, 0u, 0u, 0u};
-                    *reinterpret_cast<U32x4*>(Loads::place(v_tile, i) + threadIdx.x % kWave * 16) = U32x4{0u, 0u, 0u, 0u};
-                }
+                const bool there = page[i] >= 0 && page[i] < p.pages;
+                const char* key = keys + page[i] * key_cache.page_bytes + slot * key_cache.token_bytes;
+                const char* value = values + page[i] * value_cache.page_bytes + slot * value_cache.token_bytes;
+                load_to_lds((there ? key : reinterpret_cast<const char*>(zero_row)) + chunk * 16, Loads::place(k_tile, i));
+                load_to_lds((there ? value : reinterpret_cast<const char*>(zero_row)) + chunk * 16, Loads::place(v_tile, i));
             }
         }
         if (k0 + kKeyTile < end) look_up(k0 + kKeyTile);
@@ -397,7 +399,7 @@ struct PagedTiles {
 // Many rows of a request: 24 trees of 5 to 48 tokens over 500 to 8,000 keys, 4 heads a key head: 302 MB in 94 to 98 us,
 // 3.1 TB/s, and 13 us to join.  Bound by the latency of a tile: a workgroup has one in flight while it works on another.
 template <typename T, int DP>
-__global__ __launch_bounds__(kBlock, DP <= 64 ? 4 : 2) void attention_paged_wide_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
+__global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_paged_wide_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
                                                                          float* __restrict__ lse, Parts parts,
                                                                          const int32_t* __restrict__ block_table,
                                                                          const int32_t* __restrict__ q_offsets,
@@ -412,7 +414,8 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 4 : 2) void attention_paged_wide
     if (threadIdx.x == 0) broken = 0;
     const int kv_head = blockIdx.x % p.kv_heads;
     Work w;
-    if (!find_work(w, q_offsets, kv_lengths, p, kRowTile, blockIdx.x / p.kv_heads)) return;
+    // Without a tree later tiles see more keys: they come first.
+    if (!find_work(w, q_offsets, kv_lengths, p, kRowTile, static_cast<int>((gridDim.x - 1 - blockIdx.x) / p.kv_heads))) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave_row0 = w.row0 + wave * kRowsPerWave;
     Sight sight;
     if (!sight.find(w, p, blockIdx.y, kRowTile, tree != nullptr, wave_row0, kRowsPerWave)) return;
@@ -563,7 +566,7 @@ uint64_t parts_of(uint64_t requests, uint64_t q_tokens, uint64_t max_kv, uint64_
     const uint64_t busy = (rows > requests ? rows : requests) * kv_heads;
     const uint64_t most = ceil_div(max_kv, kPartKeys);
     const uint64_t target = tile_rows(requests, q_tokens, group) == kNarrowRows ? kNarrowGrid : kWideGrid;
-    uint64_t parts = ceil_div(target, busy ? busy : 1);
+    uint64_t parts = target / (busy ? busy : 1);
     parts = parts < most ? parts : most;
     return parts ? parts : 1;
 }
