@@ -728,11 +728,15 @@ def _pages(dtype, name: str, t, shape: tuple, written: bool = False) -> Pages:
 
 
 def _table(i32, t, requests: int) -> tuple:
-    """Address, row stride and width of a block table."""
+    """Address, row stride and width of a block table, whose rows may lie apart but share no entries."""
     if t.dtype is not i32 or t.dim() != 2 or t.shape[0] < requests or (t.shape[1] > 1 and t.stride(1) != 1):
         raise ValueError(f"block_table: [{requests}, width] of int32, its rows contiguous")
     width = t.shape[1]
-    return t.data_ptr(), max(width, t.stride(0)), width
+    if requests < 2:
+        return t.data_ptr(), width, width
+    if t.stride(0) < width:
+        raise ValueError(f"block_table: rows of {width} entries, {t.stride(0)} apart, share memory (copy an expanded table)")
+    return t.data_ptr(), t.stride(0), width
 
 
 def _array(dtype, name: str, t, count: int):
