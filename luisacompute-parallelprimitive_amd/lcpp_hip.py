@@ -696,8 +696,8 @@ def _row_types(suffix: str) -> tuple:
 def _strides(name: str, t, written: bool) -> list:
     """The strides of a tensor whose last axis has to be contiguous; 0 along axes of one item."""
     strides = [s if n > 1 else 0 for s, n in zip(t.stride(), t.shape)]
-    if strides[-1] > 1:
-        raise ValueError(f"{name}: the last axis has to be contiguous")
+    if strides[-1] != 1 and t.shape[-1] > 1 and t.numel() > 0:
+        raise ValueError(f"{name}: the last axis has to be contiguous (copy what is expanded along it)")
     if written and any(s == 0 and n > 1 for s, n in zip(strides, t.shape)):
         raise ValueError(f"{name}: rows that are written share no memory")
     return strides

@@ -57,3 +57,60 @@ def test_block_tables_are_passed_as_they_are(hip, calls, run, first, table, requ
     run(hip, table(), requests)
     (_, args), = calls
     assert args[first + 1] == width and (stride is None or args[first] == stride) and args[first] >= width
+
+
+# ---- the last axis ---------------------------------------------------------------------------------
+def repeated(*shape, step=0):
+    """One item for all of the last axis; `step` items apart otherwise (0: one item for everything)."""
+    strides = [step * n for n in (shape[1] if len(shape) == 3 else 1, 1)] if step else [0, 0]
+    if len(shape) == 4:
+        strides = [0, *strides]
+    return torch.zeros(4096, dtype=torch.bfloat16).as_strided(shape, (*strides, 0))
+
+
+@pytest.mark.parametrize("step", [0, 8])
+@pytest.mark.parametrize("name", ["q", "k", "v", "dout", "out"])
+def test_rows_that_repeat_one_item_are_refused(hip, calls, name, step):
+    """What `out.sum()` hands back as the gradient of `out` is one item expanded over every axis."""
+    n, heads, dim = 4, 2, 64
+    rows = {k: torch.zeros(n, heads, dim, dtype=torch.bfloat16) for k in ("q", "k", "v", "out", "dout")}
+    rows[name] = repeated(n, heads, dim, step=step)
+    offsets, lse, grads = torch.tensor([0, n], dtype=torch.int32), torch.zeros(heads, n), [torch.zeros(n, heads, dim, dtype=torch.bfloat16)
+                                                                                          for _ in range(3)]
+    temp = torch.zeros(1 << 16, dtype=torch.uint8)
+    with pytest.raises(ValueError, match=name):
+        hip.attention_packed_backward("bf16", rows["q"], rows["k"], rows["v"], rows["out"], lse, rows["dout"], offsets, offsets, *grads,
+                                      temp=temp, stream=STREAM)
+    if name != "dout":
+        with pytest.raises(ValueError, match=name):
+            hip.attention_packed("bf16", rows["q"], rows["k"], rows["v"], offsets, offsets, rows["out"], lse, temp=temp, stream=STREAM)
+    assert not calls
+
+
+def test_caches_and_new_rows_that_repeat_one_item_are_refused(hip, calls):
+    x, cache = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.zeros(9, 16, 2, 64, dtype=torch.bfloat16)
+    bad = repeated(9, 16, 2, 64)
+    for keys, values in ((bad, cache), (cache, bad)):
+        with pytest.raises(ValueError, match="cache"):
+            hip.attention_paged("bf16", x, keys, values, ints(4, 8), ints(5), ints(4), torch.zeros_like(x),
+                                temp=torch.zeros(1 << 20, dtype=torch.uint8), stream=STREAM)
+    for key, value in ((repeated(4, 2, 64), x), (x, repeated(4, 2, 64))):
+        with pytest.raises(ValueError, match="key|value"):
+            hip.paged_write("bf16", key, value, torch.zeros(4, dtype=torch.int64), cache, cache.clone(), stream=STREAM)
+    assert not calls
+
+
+def test_rows_broadcast_over_tokens_and_heads_are_passed(hip, calls):
+    """Strides of zero before the last axis are what they say, where nothing is written."""
+    q, offsets = torch.zeros(4, 2, 64, dtype=torch.bfloat16), torch.tensor([0, 4], dtype=torch.int32)
+    one = torch.zeros(64, dtype=torch.bfloat16).expand(4, 2, 64)
+    hip.attention_packed("bf16", one, one, one, offsets, offsets, q, stream=STREAM)
+    (_, args), = calls
+    assert all((r.token_stride, r.head_stride) == (0, 0) for r in args[2:5]) and args[7].token_stride == 128
+
+
+def test_rows_that_are_not_there_may_have_any_strides(hip, calls):
+    q, offsets = torch.zeros(0, 2, 64, dtype=torch.bfloat16), torch.tensor([0, 0], dtype=torch.int32)
+    none = torch.zeros((), dtype=torch.bfloat16).expand(0, 2, 64)
+    hip.attention_packed("bf16", none, none, none, offsets, offsets, q, stream=STREAM)
+    assert len(calls) == 1
