@@ -863,6 +863,8 @@ def attention_paged(suffix: str, q, key_cache, value_cache, block_table, q_offse
     cache = (pages, page_size, kv_heads, dim)
     requests = kv_lengths.numel()
     table, table_stride, width = _table(i32, block_table, requests)
+    if table_stride > 0x7FFFFFFF:
+        raise ValueError(f"block_table: rows {table_stride} entries apart, at most 2^31 - 1 are possible")
     if max_kv_length is None:
         max_kv_length = width * page_size
     if temp is None:

@@ -114,3 +114,13 @@ def test_rows_that_are_not_there_may_have_any_strides(hip, calls):
     none = torch.zeros((), dtype=torch.bfloat16).expand(0, 2, 64)
     hip.attention_packed("bf16", none, none, none, offsets, offsets, q, stream=STREAM)
     assert len(calls) == 1
+
+
+def test_table_rows_too_far_apart_for_the_library(hip, calls):
+    """A row stride that the paged call's 32 bits do not hold is refused, not cut off; a plan takes it."""
+    far = torch.empty_strided((4, 8), ((1 << 32) + 8, 1), dtype=torch.int32, device="meta")
+    with pytest.raises(ValueError, match="block_table"):
+        paged(hip, far)
+    assert not calls
+    plan(hip, far)
+    assert calls[0][1][9] == (1 << 32) + 8
