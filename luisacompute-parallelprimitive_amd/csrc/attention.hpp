@@ -23,7 +23,9 @@ using U32x4 = uint32_t __attribute__((ext_vector_type(4)));
 using U32x2 = uint32_t __attribute__((ext_vector_type(2)));
 using S16x4 = short __attribute__((ext_vector_type(4)));
 
+// kNarrow: exponents are too few for what products make as it comes, and operands are taken times powers of two.
 struct Bf16 {
+    static constexpr bool kNarrow = false;
     using Item = __bf16;
     using Vec2 = Item __attribute__((ext_vector_type(2)));
     using Vec8 = Item __attribute__((ext_vector_type(8)));
@@ -33,6 +35,7 @@ struct Bf16 {
 };
 
 struct F16 {
+    static constexpr bool kNarrow = true;
     using Item = _Float16;
     using Vec2 = Item __attribute__((ext_vector_type(2)));
     using Vec8 = Item __attribute__((ext_vector_type(8)));

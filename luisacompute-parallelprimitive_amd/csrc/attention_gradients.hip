@@ -23,8 +23,29 @@ namespace lcpp_hip {
 namespace attention {
 namespace {
 
-// What the gradients need of a row: stats[h][t] = lse in powers of 2 (infinity for a row that saw nothing: its weights
-// are then 2^-inf = 0), and behind all of those delta[h][t] = sum over the head's items of dO * O.  16 lanes a row.  Bound
+// f16 holds normal numbers from 2^-14 to 2^16 only: weights of long rows are below, and dS goes with the sizes of dO and V, which
+// training scales at will.  (With P and dS as they come, 3,000 rows and dO of width 1e-4: dQ 0.9% from the formula, where
+// rounding the result makes 0.25%; and a dS past 65,504 was an infinity.)  So P is taken times 2^kWeightRaise, which leaves room
+// for weights of 16, where the lse of very large scores is off; and dS times a power of two that a lane has for its row (dQ)
+// or key (dK).  That one starts at 2^kFirstRaise and comes down with the running sums, as a softmax's scale does, whenever a
+// |dS| would pass 2^15.  Both are undone in f32.  (The maxima and products cost 3% of a training step: 11,059 tokens in six
+// sequences 1,206 -> 1,244 us, five short examples 46.3 -> 47.9.)
+template <typename T>
+constexpr int kWeightRaise = T::kNarrow ? 12 : 0;
+constexpr int kFirstRaise = 32;
+
+// By how many powers of two a lane's values, of a row or key that it shares with the lane 32 away, have to come down: none up to
+// 2^15, else to 2^8, so that sums are seldom rescaled.  (Infinities stay: the sums of their row or key are not finite either.)
+__device__ __forceinline__ int too_large_by(const F32x16& x) {
+    float most = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) most = fmaxf(most, fabsf(x[r]));
+    most = halves_max(most);
+    return most > 32768.f && most < INFINITY ? __builtin_amdgcn_frexp_expf(most) - 8 : 0;
+}
+
+// What the gradients need of a row: stats[h][t] = lse in powers of 2, less kWeightRaise (infinity for a row that saw nothing: its
+// weights are then 2^-inf = 0), and behind all of those delta[h][t] = sum over the head's items of dO * O.  16 lanes a row.  Bound
 // by memory (the rows of O and dO, 181 MB for 11,059 tokens of 32 heads: 36 us, 5.0 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void attention_row_stats_kernel(Rows out, Rows dout, const float* __restrict__ lse,
@@ -47,7 +68,7 @@ __global__ __launch_bounds__(kBlock) void attention_row_stats_kernel(Rows out, R
     if (chunk == 0) {
         const int64_t at = static_cast<int64_t>(head) * q_tokens + token;
         const float l = lse[at];
-        stats[at] = l == -INFINITY ? INFINITY : l * kLog2e;
+        stats[at] = l == -INFINITY ? INFINITY : l * kLog2e - kWeightRaise<T>;
         stats[rows + at] = sum;
     }
 }
@@ -125,7 +146,9 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
     load_row<DP>(qf, g.q, rows.begin + row, head, there, shape.dim);
     load_row<DP>(of, g.dout, rows.begin + row, head, there, shape.dim);
     const int64_t stat = static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row;
-    const float base = there ? g.stats[stat] : INFINITY;
+    const float row_base = there ? g.stats[stat] : INFINITY;
+    float base = row_base;  // of dS, `raise` powers of two lower
+    int raise = kWeightRaise<T>;
     const float delta = there ? g.stats[static_cast<int64_t>(shape.q_heads) * shape.q_tokens + stat] : 0.f;
     for (char* tile : {k_even, v_even, k_odd, v_odd}) clear_past<DP, kKeyTile, kAllWaves>(tile, shape.dim);
     F32x16 acc[DP / 32];
@@ -152,6 +175,16 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = word & (1u << acc_row(r, 0)) ? s[r] : 0.f;
             }
+            if constexpr (T::kNarrow) {
+                const int down = too_large_by(s);
+                if (wave_ballot(down != 0) != 0) {
+                    const float f = ldexpf(1.f, -down);
+                    base += down, raise -= down;
+                    s *= f;
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) acc[d] *= f;
+                }
+            }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const U32x4 ds = pack_step<T>(s, i);
@@ -165,11 +198,12 @@ __device__ __forceinline__ void dq_block(const GradientArgs& g, const GradientMe
     const auto pass = [&](int stop) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) acc[d] = F32x16{};
+        if constexpr (T::kNarrow) base = row_base - kFirstRaise, raise = kWeightRaise<T> + kFirstRaise;
         pass_tiles<kKeyTile>(0, stop, [&](int k0) { load(k_even, v_even, k0); }, [&](int k0) { load(k_odd, v_odd, k0); },
                              [&](int k0) { step(k_even, v_even, k0); }, [&](int k0) { step(k_odd, v_odd, k0); });
     };
     const auto store = [&] {
-        if (there) store_row<T, DP>(g.dq, rows.begin + row, head, acc, shape.scale, shape.dim);
+        if (there) store_row<T, DP>(g.dq, rows.begin + row, head, acc, ldexpf(shape.scale, -raise), shape.dim);
     };
     pass(end);
     store();  // (before waves wait for each other)
@@ -247,6 +281,7 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     const char* values = memory.values + Tile<DP>::bytes(kRowsPerWave) * wave;
     for (char* tile : {q_even, o_even, q_odd, o_odd}) clear_past<DP, kQueryTile>(tile, shape.dim);
     F32x16 dk_acc[DP / 32], dv_acc[DP / 32];
+    float lift = 1.f;  // of dS
     const int all = rows.size > start ? (rows.size - start + kQueryTile - 1) / kQueryTile * group : 0;
     const int per = (all + parts - 1) / parts;
     const int from = part * per, to = from + per < all ? from + per : all;
@@ -289,7 +324,7 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
                 for (int i = 0; i < 4; ++i) {
                     const int r = 4 * j + i;
                     s[r] = exp2_fast(s[r] * c - l[i]);
-                    dp[r] = s[r] * (dp[r] - e[i]);
+                    dp[r] = s[r] * (T::kNarrow ? (dp[r] - e[i]) * lift : dp[r] - e[i]);
                 }
             }
             if (r0 < full || r0 + 32 > rows.size) {
@@ -299,6 +334,16 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
                     const bool seen = word & (1u << acc_row(r, 0));
                     s[r] = seen ? s[r] : 0.f;
                     dp[r] = seen ? dp[r] : 0.f;
+                }
+            }
+            if constexpr (T::kNarrow) {
+                const int down = too_large_by(dp);
+                if (wave_ballot(down != 0) != 0) {
+                    const float f = ldexpf(1.f, -down);
+                    lift *= f;
+                    dp *= f;
+#pragma unroll
+                    for (int d = 0; d < DP / 32; ++d) dk_acc[d] *= f;
                 }
             }
 #pragma unroll
@@ -315,6 +360,7 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     const auto pass = [&](bool clean) {
 #pragma unroll
         for (int d = 0; d < DP / 32; ++d) dk_acc[d] = dv_acc[d] = F32x16{};
+        if constexpr (T::kNarrow) lift = ldexpf(1.f, kFirstRaise);
         loads = {kv_head * group, start, start, rows.size};
         if (from < to) loads.skip(from + team);
         steps = loads;
@@ -326,6 +372,11 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     pass(false);
     const bool clean = start < full && block_any(any_not_finite(dk_acc) || any_not_finite(dv_acc), memory.broken);
     if (clean) pass(true);
+    if constexpr (T::kNarrow) {
+        const float f = 1.f / lift;  // (a power of two)
+#pragma unroll
+        for (int d = 0; d < DP / 32; ++d) dk_acc[d] *= f;
+    }
     // The first team ends with dK, the second with dV; each hands the other its share.
     // (Over the tiles, which nothing is loaded into any more: a quarter of the sums in each of the four arrays.)
     const auto join_at = [&](int i) {
@@ -391,7 +442,7 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     if (team == 0) {
         take(dk_acc);
         if (clean) add_left_out(dk_acc, true);
-        store(dk, dk_acc, shape.scale, 0);
+        store(dk, dk_acc, ldexpf(shape.scale, -kWeightRaise<T>), 0);
     }
     __syncthreads();
     if (team == 0) give(dv_acc);
@@ -399,7 +450,7 @@ __device__ __forceinline__ void dkv_block(const GradientArgs& args, const Gradie
     if (team == 1) {
         take(dv_acc);
         if (clean) add_left_out(dv_acc, false);
-        store(dv, dv_acc, 1.f, 1);
+        store(dv, dv_acc, ldexpf(1.f, -kWeightRaise<T>), 1);
     }
 }
 
