@@ -282,11 +282,13 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
         for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
         rescale(state, halves_max(high), c);
         const float base = state.top == -INFINITY ? 0.f : state.top * c;
+        float sum = 0.f;  // (a weight alone may be below the last bit of a long row's total)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             s[r] = exp2_fast(s[r] * c - base);
-            state.total += s[r];
+            sum += s[r];
         }
+        state.total += sum;
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const U32x4 pf = pack_step<T>(s, i);
