@@ -19,6 +19,11 @@ constexpr int kKeyTile = 64;                     // keys in LDS at a time
 // of 2): weights are then at most 2^8, within the 16-bit types, and the products are rescaled a few times a row at most
 // (16,384 rows: 1,138 us, with a slack of 0 1,180; uneven prompts 157 and 165).
 constexpr float kSlack = 8.f;
+// Weights are taken times 2^kRaise, in f16 as far as the slack leaves room below 2^16: its normal numbers end at 2^-14, and a long
+// row's many small weights would be rounded away or up together (100,000 keys e^-17 below one: the output was 9% off).  The
+// factor is in the products and in their sum alike, and out of the latter for the lse.
+template <typename T>
+constexpr int kRaise = T::kNarrow ? 7 : 0;
 
 // Direct loads of a tile by some waves side by side, a block of rows each: a lane's chunk is the same in all of them, and its
 // row goes up by kRowStep.
@@ -131,6 +136,12 @@ __device__ __forceinline__ void rescale(RowState<DP>& state, float high, float c
     for (int d = 0; d < DP / 32; ++d) state.acc[d] *= alpha;
 }
 
+// What a score's exponent is taken from (a row that sees nothing has no scale: its scores are -inf).
+template <typename T>
+__device__ __forceinline__ float weight_base(float top, float c) {
+    return top == -INFINITY ? 0.f : top * c - kRaise<T>;
+}
+
 // One tile of keys.  `seen(k0)`: the 32 keys from k0 on that the lane's row sees, as bits; `masked`: some row of the
 // workgroup does not see all of the tile.
 template <typename T, int DP, typename Seen>
@@ -157,7 +168,7 @@ __device__ __forceinline__ void forward_tile(RowState<DP>& state, const char* k_
 #pragma unroll
         for (int r = 0; r < 16; ++r) high = fmaxf(high, s[b][r]);
     rescale(state, halves_max(high), c);
-    const float base = state.top == -INFINITY ? 0.f : state.top * c;
+    const float base = weight_base<T>(state.top, c);
     float sum = 0.f;
 #pragma unroll
     for (int b = 0; b < kBlocks; ++b) {
@@ -248,14 +259,15 @@ __device__ __forceinline__ void careful_key(RowState<DP>& state, const U32x4 (&q
                                             int dim, float c, bool seen) {
     const float dot = careful_dot<T, DP>([&](int i) { return qf[i]; }, key, dim), score = seen ? dot : -INFINITY;
     rescale(state, score, c);
-    const float weight = exp2_fast(score * c - (state.top == -INFINITY ? 0.f : state.top * c));
+    const float weight = exp2_fast(score * c - weight_base<T>(state.top, c));
     if (threadIdx.x % kWave < 32) state.total += weight;
     careful_add<T, DP>(state.acc, weight, value, dim, seen);
 }
 
 // (The hardware's logarithm, right to an ulp or so, as the sum it is taken of.)
+template <typename T>
 __device__ __forceinline__ float row_lse(float top, float total, float scale) {
-    return total == 0.f ? -INFINITY : top * scale + __logf(total);
+    return total == 0.f ? -INFINITY : top * scale + __logf(ldexpf(total, -kRaise<T>));
 }
 
 // Runs the tiles from `begin` to `end`, SIZE apart, with two sets of buffers: while one is computed on, the other is loaded.

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_packed_ker
         if (!there) return;
         store_row<T, DP>(out, rows.begin + row, head, state.acc, total == 0.f ? 0.f : 1.f / total, shape.dim);
         if (lse != nullptr && half == 0)
-            lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row] = row_lse(state.top, total, shape.scale);
+            lse[static_cast<int64_t>(head) * shape.q_tokens + rows.begin + row] = row_lse<T>(state.top, total, shape.scale);
     };
     RowState<DP> state;
     pass(state, range.end);

@@ -281,7 +281,7 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
 #pragma unroll
         for (int r = 1; r < 16; ++r) high = fmaxf(high, s[r]);
         rescale(state, halves_max(high), c);
-        const float base = state.top == -INFINITY ? 0.f : state.top * c;
+        const float base = weight_base<T>(state.top, c);
         float sum = 0.f;  // (a weight alone may be below the last bit of a long row's total)
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -330,7 +330,7 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     if (threadIdx.x < kNarrowRows) {
         stats[0][0][lane] = all_total;
         if (row.there && whole && lse != nullptr)
-            lse[static_cast<int64_t>(row.head) * p.q_tokens + w.token0 + row.token] = row_lse(all_top, all_total, p.scale);
+            lse[static_cast<int64_t>(row.head) * p.q_tokens + w.token0 + row.token] = row_lse<T>(all_top, all_total, p.scale);
         if (row.there && !whole) parts.stats[parts.row(p, blockIdx.y, row.head, w.token0 + row.token)] = F32x2{all_top, all_total};
     }
     __syncthreads();
@@ -469,7 +469,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_paged_wide
         const int64_t t = w.token0 + row.token;
         if (whole) {
             store_row<T, DP>(out, t, row.head, state.acc, total == 0.f ? 0.f : 1.f / total, p.dim);
-            if (lse != nullptr && half == 0) lse[static_cast<int64_t>(row.head) * p.q_tokens + t] = row_lse(state.top, total, p.scale);
+            if (lse != nullptr && half == 0) lse[static_cast<int64_t>(row.head) * p.q_tokens + t] = row_lse<T>(state.top, total, p.scale);
             return;
         }
         const int64_t at = parts.row(p, blockIdx.y, row.head, t);
@@ -550,7 +550,7 @@ __global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, 
     }
     if (!there || group != 0) return;
     if (chunk * 8 < p.dim) store_items<T>(out.at(token, head) + chunk * 16, a, b, total == 0.f ? 0.f : 1.f / total);
-    if (chunk == 0 && lse != nullptr) lse[static_cast<int64_t>(head) * p.q_tokens + token] = row_lse(top, total, p.scale);
+    if (chunk == 0 && lse != nullptr) lse[static_cast<int64_t>(head) * p.q_tokens + token] = row_lse<T>(top, total, p.scale);
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------

@@ -113,3 +113,59 @@ def test_gradients_of_rows_of_all_sizes(hip, dev, lengths, heads, kv_heads, risi
         near(f"dq {at}", got["dq"][at:at + 250], want["dq"][at:at + 250])
     for name in ("dk", "dv"):
         near(name, got[name], want[name])
+
+
+# ---- weights far below a row's largest -------------------------------------------------------------
+def one_key_above(m, dim, n, seed=5):
+    """n rows whose score with key 0 is 17 above those with the other m - 1, whose weights together are m e^-17."""
+    q, k = torch.zeros(n, 1, dim), torch.zeros(m, 1, dim)
+    q[:, 0, 0], k[0, 0, 0] = 4.0, 4.25
+    k[1:, 0, 0] = torch.randn(m - 1, generator=torch.Generator().manual_seed(seed)) * 0.1
+    v = 1.0 + rows(m, 1, dim, seed + 1, 0.1).float()
+    v[0] = 0.0
+    return q.half(), k.half(), v.half()
+
+
+def check_one_key_above(q, k, v, new, out, lse):
+    """Weights are off by a part of u, or by what the range leaves: 2^-25 of a weight that is at least 2^7 where the row's largest
+    is 1, 2^-32 of the row's sum each.  (32-bit exponentials and sums as in the other tests: 2^-17.)"""
+    m = k.shape[0]
+    scores = q.double()[:, 0] @ k.double()[:, 0].t()
+    scores = scores.masked_fill(~torch.ones(new, m, dtype=torch.bool).tril(m - new), -math.inf)
+    weights, values = torch.softmax(scores, 1), v.double()[:, 0]
+    want = weights @ values
+    bound = (2 * U + 2.0 ** -17) * want + 2.0 ** -32 * values.abs().sum(0) + 2.0 ** -25
+    off = (out.cpu().double()[:, 0] - want).abs()
+    log(f"off by {float((off / want).max()):.2e} of the output, allowed {float((bound / want).min()):.2e}")
+    assert (off <= bound).all()
+    assert (lse.cpu().double()[0] - torch.logsumexp(scores, 1)).abs().max() <= 2.0 ** -15
+
+
+@pytest.mark.parametrize("n", [1, 130])
+def test_packed_weights_far_below_the_largest(hip, dev, n):
+    m, dim = 100_000, 64
+    q, k, v = one_key_above(m, dim, n)
+    out, lse = torch.full((n, 1, dim), 7.0, dtype=torch.float16, device="cuda"), torch.full((1, n), 7.0, device="cuda")
+    hip.attention_packed("f16", q.cuda(), k.cuda(), v.cuda(), oracle.offsets_of([n]).cuda(), oracle.offsets_of([m]).cuda(), out, lse,
+                         scale=1.0)
+    torch.cuda.synchronize()
+    check_one_key_above(q, k, v, n, out, lse)
+
+
+@pytest.mark.parametrize("n", [1, 60])
+@pytest.mark.parametrize("parts", [False, True])
+def test_paged_weights_far_below_the_largest(hip, dev, n, parts):
+    """Rows of a narrow and a wide tile, in one part and in many."""
+    m, dim, page = 100_000, 128, 32
+    q, k, v = one_key_above(m, dim, n)
+    pages = -(-m // page)
+    caches = [torch.zeros(pages * page, 1, dim, dtype=torch.float16, device="cuda") for _ in range(2)]
+    for cache, x in zip(caches, (k, v)):
+        cache[:m] = x.cuda()
+    caches = [c.view(pages, page, 1, dim) for c in caches]
+    table = torch.arange(pages, dtype=torch.int32, device="cuda")[None]
+    out, lse = torch.full((n, 1, dim), 7.0, dtype=torch.float16, device="cuda"), torch.full((1, n), 7.0, device="cuda")
+    hip.attention_paged("f16", q.cuda(), *caches, table, oracle.offsets_of([n]).cuda(), torch.tensor([m], dtype=torch.int32).cuda(), out,
+                        lse, max_kv_length=m if parts else 1, scale=1.0)
+    torch.cuda.synchronize()
+    check_one_key_above(q, k, v, n, out, lse)
