@@ -104,7 +104,7 @@ class DeviceAttention : public LuisaModule {
     template <AttentionItemT T>
     void PagedWrite(CommandList& cmdlist, AttentionRows<T> key, AttentionRows<T> value, BufferView<int64_t> slots,
                     AttentionCache<T> key_cache, AttentionCache<T> value_cache, const AttentionShape& shape, PageShape page) {
-        const size_t tokens = slots.size();
+        const size_t tokens = count_of(slots.size(), "tokens");
         auto k = rows(key, tokens, shape.kv_heads, shape.head_dim), v = rows(value, tokens, shape.kv_heads, shape.head_dim);
         auto kc = cache(key_cache, shape, page), vc = cache(value_cache, shape, page);
         cmdlist << [=](hipStream_t s) {
