@@ -748,6 +748,15 @@ def _array(dtype, name: str, t, count: int):
     return t.data_ptr()
 
 
+def _lse(f32, t, heads: int, tokens: int):
+    """Device address of an lse [heads, tokens]: flat, or of that order (axes of one item, and rows past the last, are free)."""
+    if t is not None and t.dim() > 1 and t.shape[-1] != tokens > 1:
+        axes = [n for n in t.shape if n != 1]
+        if len(axes) > 1 and axes[-1] != tokens:
+            raise ValueError(f"lse: {tuple(t.shape)} where [query heads, query tokens], {(heads, tokens)}, is needed")
+    return _array(f32, "lse", t, heads * tokens)
+
+
 def _axes(name: str, t, axes: int) -> tuple:
     if t.dim() != axes:
         raise ValueError(f"{name}: {axes} axes are needed, not {t.dim()}")
@@ -824,7 +833,7 @@ def attention_packed(suffix: str, q, k, v, q_offsets, k_offsets, out, lse=None, 
     call(f"lcpp_hip_attention_packed_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows), _rows(dt, "k", k, shape),
          _rows(dt, "v", v, shape), _array(i32, "q_offsets", q_offsets, 1),
          _array(i32, "k_offsets", k_offsets, sequences + 1), _rows(dt, "out", out, rows, True),
-         _array(f32, "lse", lse, heads * tokens), sequences, tokens, keys, heads, kv_heads, dim,
+         _lse(f32, lse, heads, tokens), sequences, tokens, keys, heads, kv_heads, dim,
          dim ** -0.5 if scale is None else scale, int(causal), stream_handle(stream))
 
 
@@ -840,7 +849,7 @@ def attention_packed_backward(suffix: str, q, k, v, out, lse, dout, q_offsets, k
     shape = (keys, kv_heads, dim)
     call(f"lcpp_hip_attention_packed_backward_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows),
          _rows(dt, "k", k, shape), _rows(dt, "v", v, shape), _rows(dt, "out", out, rows),
-         _array(f32, "lse", lse, heads * tokens), _rows(dt, "dout", dout, rows),
+         _lse(f32, lse, heads, tokens), _rows(dt, "dout", dout, rows),
          _array(i32, "q_offsets", q_offsets, 1), _array(i32, "k_offsets", k_offsets, sequences + 1),
          _rows(dt, "dq", dq, rows, True), _rows(dt, "dk", dk, shape, True), _rows(dt, "dv", dv, shape, True), sequences,
          tokens, keys, heads, kv_heads, dim, dim ** -0.5 if scale is None else scale, int(causal), stream_handle(stream))
@@ -874,6 +883,6 @@ def attention_paged(suffix: str, q, key_cache, value_cache, block_table, q_offse
          _pages(dt, "value_cache", value_cache, cache), table, table_stride, width,
          _array(i32, "q_offsets", q_offsets, requests + 1),
          _array(i32, "kv_lengths", kv_lengths, requests), _array(i64, "tree", tree, tokens),
-         _rows(dt, "out", out, rows, True), _array(f32, "lse", lse, heads * tokens), requests, tokens,
+         _rows(dt, "out", out, rows, True), _lse(f32, lse, heads, tokens), requests, tokens,
          max_kv_length, heads, kv_heads, dim, page_size, pages, dim ** -0.5 if scale is None else scale,
          stream_handle(stream))

@@ -124,3 +124,34 @@ def test_table_rows_too_far_apart_for_the_library(hip, calls):
     assert not calls
     plan(hip, far)
     assert calls[0][1][9] == (1 << 32) + 8
+
+
+# ---- lse -------------------------------------------------------------------------------------------
+def with_lse(hip, which, lse, n, heads):
+    x, offsets = torch.zeros(n, heads, 64, dtype=torch.bfloat16), torch.tensor([0, n], dtype=torch.int32)
+    temp = torch.zeros(1 << 20, dtype=torch.uint8)
+    if which == "packed":
+        hip.attention_packed("bf16", x, x, x, offsets, offsets, x.clone(), lse, temp=temp, stream=STREAM)
+    elif which == "backward":
+        hip.attention_packed_backward("bf16", x, x, x, x, lse, x, offsets, offsets, x.clone(), x.clone(), x.clone(), temp=temp, stream=STREAM)
+    else:
+        cache = torch.zeros(9, 16, heads, 64, dtype=torch.bfloat16)
+        hip.attention_paged("bf16", x, cache, cache, ints(1, 8), ints(2), ints(1), x.clone(), lse, temp=temp, stream=STREAM)
+
+
+@pytest.mark.parametrize("which", ["packed", "backward", "paged"])
+@pytest.mark.parametrize("n,heads,shape", [(6, 4, (6, 4)), (6, 4, (4, 7)), (6, 4, (2, 12)), (6, 1, (2, 3)), (6, 4, (1, 6, 4)),
+                                           (6, 4, (6, 4, 1))])
+def test_lse_with_its_axes_the_wrong_way_is_refused(hip, calls, which, n, heads, shape):
+    """[heads, tokens] is what is filled: another shape of as many items would be read as something else."""
+    with pytest.raises(ValueError, match="lse"):
+        with_lse(hip, which, torch.zeros(shape), n, heads)
+    assert not calls
+
+
+@pytest.mark.parametrize("which", ["packed", "backward", "paged"])
+@pytest.mark.parametrize("n,heads,shape", [(6, 4, (4, 6)), (6, 4, (24,)), (6, 4, (30,)), (6, 4, (24, 1)), (6, 4, (5, 6)), (6, 1, (6, 1)), (1, 4, (1, 4)), (1, 4, (4, 1)),
+                                           (6, 4, (1, 4, 6)), (6, 4, (4, 6, 1)), (6, 4, (2, 2, 6)), (4, 4, (4, 4))])
+def test_lse_of_any_shape_in_the_same_order_is_taken(hip, calls, which, n, heads, shape):
+    with_lse(hip, which, torch.zeros(shape), n, heads)
+    assert len(calls) == 1
