@@ -527,7 +527,8 @@ int packed_backward(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const
     if (sequences == 0 || (q_tokens == 0 && k_tokens == 0)) return kOk;
     if (q_tokens * (q_heads / kv_heads) > kMostKeys) return set_error(kInvalidArgument, "%s: too many tokens or sequences", what);
     if (!q_offsets || !k_offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
-    if (q_tokens && (!usable(q) || !usable(out) || !usable(dout) || !usable(dq) || !lse))
+    if (q_tokens && !lse) return set_error(kInvalidArgument, "%s: null lse, which the forward pass gives", what);
+    if (q_tokens && (!usable(q) || !usable(out) || !usable(dout) || !usable(dq)))
         return unusable(what);
     if (k_tokens && (!usable(k) || !usable(v) || !usable(dk) || !usable(dv)))
         return unusable(what);

@@ -155,3 +155,13 @@ def test_lse_with_its_axes_the_wrong_way_is_refused(hip, calls, which, n, heads,
 def test_lse_of_any_shape_in_the_same_order_is_taken(hip, calls, which, n, heads, shape):
     with_lse(hip, which, torch.zeros(shape), n, heads)
     assert len(calls) == 1
+
+
+def test_a_backward_call_without_lse_says_so(hip):
+    """(The library's own refusal, before any HIP call.)"""
+    r = hip.Rows(1 << 20, 64, 64)
+    need = hip.attention_packed_backward_temp_bytes(1, 4, 4, 2, 1, 64)
+    status = hip.lib().lcpp_hip_attention_packed_backward_f16(1 << 20, need, r, r, r, r, None, r, 1 << 20, 1 << 20, r, r, r, 1, 4, 4, 2, 1, 64,
+                                                              0.125, 1, None)
+    assert status == hip.ERR_INVALID_ARGUMENT
+    assert "lse" in hip.lib().lcpp_hip_last_error().decode() and "aligned" not in hip.lib().lcpp_hip_last_error().decode()
