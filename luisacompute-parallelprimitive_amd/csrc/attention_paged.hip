@@ -41,8 +41,8 @@ struct Paged {
     int pages;
     int table_stride;
     int table_width;
-    int parts;  // of the longest request
-    int part;   // keys of each
+    int parts;   // at most, of a request as long as stated
+    int stated;  // the longest request's keys, as the caller said
     float scale;
 };
 
@@ -50,12 +50,28 @@ __device__ __forceinline__ int slot_of(const Paged& p, uint32_t position) {
     return static_cast<int>(position - p.page_size(position) * p.page_size.by);
 }
 
-// Keys of one part: the same for every request, so that parts are alike and a short request is one; more where a request is
-// longer than the caller said.
-__device__ __forceinline__ int part_keys(int length, const Paged& p) {
-    const int64_t held = static_cast<int64_t>(p.part) * p.parts;
-    if (length <= held) return p.part;
-    return ((length - 1) / p.parts + kKeyStep) / kKeyStep * kKeyStep;
+__device__ __forceinline__ int whole_steps(int keys) { return (keys + kKeyStep - 1) / kKeyStep * kKeyStep; }
+
+// Keys of one part: the same for every request, so that parts are alike and a short request is one.  The longest request decides
+// it, not what the caller stated: a table's width, or a maximum that a recorded graph was given, may be far more (one request
+// of 8,000 keys, 131,072 stated: 39 us by the statement, 17 so; four of 2,000 to 8,000: 116 and 35), and the same
+// parts make the same bits.  Where there are parts, requests are some hundred at most, a few loads a lane.
+__device__ __forceinline__ int part_of(const int32_t* kv_lengths, const Paged& p) {
+    int longest = p.stated;
+    if (p.parts > 1) {
+        int length = 1;
+        for (int r = threadIdx.x % kWave; r < p.requests; r += kWave) length = kv_lengths[r] > length ? kv_lengths[r] : length;
+        length = wave_reduce(length, MaxValueOp{});
+        longest = length < longest ? length : longest;
+    }
+    const int part = whole_steps((longest - 1) / p.parts + 1);
+    return part > kPartKeys ? part : kPartKeys;
+}
+
+// More where a request is longer than the caller said.
+__device__ __forceinline__ int part_keys(int length, const Paged& p, int part) {
+    const int64_t held = static_cast<int64_t>(part) * p.parts;
+    return length <= held ? part : whole_steps((length - 1) / p.parts + 1);
 }
 
 struct Work {
@@ -102,8 +118,9 @@ struct Sight {
     int wave_end;  // keys that some row of the wave sees
     bool whole;    // the request has no other part
     // False where the part holds nothing of the request (and another one writes its rows).
-    __device__ __forceinline__ bool find(const Work& w, const Paged& p, int part, int tile_rows, bool tree_given, int wave_row0, int wave_rows) {
-        const int per = part_keys(w.length, p), group = p.q_heads / p.kv_heads;
+    __device__ __forceinline__ bool find(const Work& w, const Paged& p, int keys, int part, int tile_rows, bool tree_given, int wave_row0,
+                                         int wave_rows) {
+        const int per = part_keys(w.length, p, keys), group = p.q_heads / p.kv_heads;
         const int64_t first = static_cast<int64_t>(part) * per;
         if (first >= w.length && part > 0) return false;
         begin = static_cast<int>(first);
@@ -197,10 +214,11 @@ __global__ __launch_bounds__(kBlock, 2) void attention_paged_kernel(Rows q, Page
     __shared__ __attribute__((aligned(16))) char tiles[kTilesBytes > kJoinBytes ? kTilesBytes : kJoinBytes];
     __shared__ float stats[2][kWaves][kNarrowRows];
     const int kv_head = blockIdx.x % p.kv_heads;
+    const int part = part_of(kv_lengths, p);
     Work w;
     if (!find_work(w, q_offsets, kv_lengths, p, kNarrowRows, blockIdx.x / p.kv_heads)) return;
     Sight sight;
-    if (!sight.find(w, p, blockIdx.y, kNarrowRows, tree != nullptr, w.row0, kNarrowRows)) return;
+    if (!sight.find(w, p, part, blockIdx.y, kNarrowRows, tree != nullptr, w.row0, kNarrowRows)) return;
     const int begin = sight.begin, end = sight.end;
     const bool whole = sight.whole;
     const int group = p.q_heads / p.kv_heads;
@@ -415,12 +433,13 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_paged_wide
     __shared__ int broken;  // whether the sums of some wave are not finite
     if (threadIdx.x == 0) broken = 0;
     const int kv_head = blockIdx.x % p.kv_heads;
+    const int part = part_of(kv_lengths, p);
     Work w;
     // Without a tree later tiles see more keys: they come first.
     if (!find_work(w, q_offsets, kv_lengths, p, kRowTile, static_cast<int>((gridDim.x - 1 - blockIdx.x) / p.kv_heads))) return;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave_row0 = w.row0 + wave * kRowsPerWave;
     Sight sight;
-    if (!sight.find(w, p, blockIdx.y, kRowTile, tree != nullptr, wave_row0, kRowsPerWave)) return;
+    if (!sight.find(w, p, part, blockIdx.y, kRowTile, tree != nullptr, wave_row0, kRowsPerWave)) return;
     const int begin = sight.begin, end = sight.end, wave_end = sight.wave_end;
     const bool whole = sight.whole;
     const int lane = threadIdx.x % kWave, half = lane / 32;
@@ -502,13 +521,13 @@ __global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, 
     constexpr int kHeads = kBlock / 16 / GROUPS;
     __shared__ F32x4 sums[2][GROUPS][kHeads][16];
     __shared__ F32x2 group_stats[GROUPS][kHeads];
-    const int blocks = (p.q_heads + kHeads - 1) / kHeads;
+    const int blocks = (p.q_heads + kHeads - 1) / kHeads, part = part_of(kv_lengths, p);
     const int64_t token = blockIdx.x / blocks;
     const int request = find_last(p.requests, token, [&](int r) { return static_cast<int64_t>(q_offsets[r]); });
     if (request < 0) return;
     Work w;
     take_request(w, q_offsets, kv_lengths, p, request);
-    const int per = part_keys(w.length, p);
+    const int per = part_keys(w.length, p, part);
     if (token >= w.token0 + w.tokens || w.length <= per) return;
     const int count = (w.length + per - 1) / per;
     const int chunk = threadIdx.x % 16, group = threadIdx.x / 16 % GROUPS, local = threadIdx.x / 16 / GROUPS;
@@ -573,8 +592,6 @@ uint64_t parts_of(uint64_t requests, uint64_t q_tokens, uint64_t max_kv, uint64_
     return parts ? parts : 1;
 }
 
-uint64_t keys_of_part(uint64_t max_kv, uint64_t parts) { return align_up(ceil_div(max_kv ? max_kv : 1, parts), kKeyStep); }
-
 size_t stats_bytes(uint64_t parts, uint64_t rows) { return align_up(parts * rows * sizeof(F32x2), kViewAlign); }
 
 size_t paged_bytes(uint64_t requests, uint64_t q_tokens, uint64_t max_kv, uint64_t q_heads, uint64_t kv_heads, uint64_t dim) {
@@ -617,8 +634,7 @@ int paged(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_
         return set_error(kInvalidArgument, "%s: too many tiles", what);
     const Paged p{static_cast<int>(requests), static_cast<int>(q_tokens), static_cast<int>(q_heads), static_cast<int>(kv_heads),
                   static_cast<int>(dim), Divider(page_size), static_cast<int>(pages), static_cast<int>(table_stride),
-                  static_cast<int>(table_width), static_cast<int>(parts),
-                  static_cast<int>(keys_of_part(max_kv_length, parts)), scale};
+                  static_cast<int>(table_width), static_cast<int>(parts), static_cast<int>(max_kv_length ? max_kv_length : 1), scale};
     Parts sums{nullptr, static_cast<F32x2*>(temp)};
     if (parts > 1) sums.out = reinterpret_cast<float*>(static_cast<char*>(temp) + stats_bytes(parts, q_tokens * q_heads));
     {
