@@ -57,9 +57,11 @@ __device__ __forceinline__ void clear_past(char* tile, int dim) {
 }
 
 // Rows of a packed sequence: those past its last are loaded as its last, and masked.  Addresses are a scalar base and a
-// lane's offset of 32 bits, which stays the same from tile to tile (the host keeps a tile's bytes below 2^31).
+// lane's offset of 32 bits without a sign, which stays the same from tile to tile: rows are less than 2^25 bytes apart (the host
+// sees to it), and a tile has 128 of them at most, so that the last one's chunks begin below 127 * 2^25 + 256 < 2^32.
 template <int DP, int ROWS, int WAVES = kWaves>
 struct PackedRows {
+    static_assert(ROWS <= 128, "a lane's offset within a tile has 32 bits");
     using Loads = TileLoads<DP, ROWS, WAVES>;
     const char* base;  // the sequence's first row of the head
     int64_t token_bytes;

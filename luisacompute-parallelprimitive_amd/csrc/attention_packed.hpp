@@ -141,7 +141,7 @@ inline int check_shape(const char* what, uint32_t sequences, uint64_t q_tokens, 
     return kOk;
 }
 
-// A tile's bytes fit 31 bits.
+// Rows so far apart that a lane's offset within a tile would not fit its 32 bits (PackedRows).
 inline bool too_wide(const lcpp_hip_rows* r) { return r != nullptr && r->token_stride >= 1 << 24; }
 inline int refuse_wide(const char* what) { return set_error(kUnsupported, "%s: token strides must be below 2^24 items", what); }
 
