@@ -56,13 +56,6 @@ struct RowRange {
     }
 };
 
-struct GreaterOp {
-    template <typename T>
-    __device__ static T identity() { return std::numeric_limits<T>::lowest(); }
-    template <typename T>
-    __device__ T operator()(T a, T b) const { return a < b ? b : a; }
-};
-
 // Tiles of a batch of at most 64 sequences in the order of the work that they are, the most first: a workgroup of a long
 // sequence's last rows takes half of an uneven batch's time, and has to start early.  16 uneven prompts: 154 us in the
 // tiles' order, 148 so.  Gradients of 8 sequences of 500 rows (32 heads of 128 on 8): 121 and 111 us; of six from 700 to 4,096
@@ -79,7 +72,7 @@ struct OrderedTile {
             return n < 0 ? 0 : n < tiles ? n : tiles;
         };
         if (wave_reduce(tiles, SumOp{}) <= number) return;
-        int low = -wave_reduce(tiles ? -first : -INT32_MAX, GreaterOp{}), high = wave_reduce(tiles ? first + tiles : -INT32_MAX, GreaterOp{});
+        int low = -wave_reduce(tiles ? -first : -INT32_MAX, MaxValueOp{}), high = wave_reduce(tiles ? first + tiles : -INT32_MAX, MaxValueOp{});
         int above = 0;  // tiles at `high` or above: not more than number; at `low` there are more
         while (high - low > 1) {
             const int level = low + (high - low) / 2, n = wave_reduce(from(level), SumOp{});
