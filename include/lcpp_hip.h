@@ -588,8 +588,10 @@ LCPP_HIP_DECLARE_SEGSORT(f64, double)
  *
  * A batch holds the rows of all its sequences one after another; offsets[b] .. offsets[b + 1] are those of
  * sequence b (offsets in device memory, ascending, one more than there are sequences).  Rows that no sequence
- * has are neither read nor written.  Types: bf16 and f16, in both directions; sums, maxima and the
- * softmax are f32.  Head sizes: multiples of 8 up to 128 (others: LCPP_HIP_ERR_UNSUPPORTED).  `q_heads` is a
+ * has may hold anything and are not written.  Types: bf16 and f16, in both directions; sums, maxima and the
+ * softmax are f32.  Softmax weights, and in the backward pass dS, are rounded to 16 bits as operands of the matrix
+ * instructions (in f16 times powers of two that keep small and large ones within its exponents), and
+ * rowsum(dout * out) takes `out` as it was stored.  Head sizes: multiples of 8 up to 128 (others: LCPP_HIP_ERR_UNSUPPORTED).  `q_heads` is a
  * multiple of `kv_heads`; query head h reads key head h / (q_heads / kv_heads).  Rows and pages start at
  * multiples of 16 bytes, and their strides are multiples of 8 items.  `scale` (the products' factor, often
  * 1 / sqrt(head_dim)) is positive.  lse is [q_heads][q_tokens] f32: the logarithm of the row's sum of exponentials.
@@ -675,8 +677,9 @@ LCPP_HIP_DECLARE_ATTENTION(f16)
  * token i sees every key before them, and new key j where bit j of tree[i] is set: a tree of drafted tokens (at most
  * 64 a request; keys from the 65th on are not seen).  Without a tree (null): j <= i.  A single new token a request
  * is plain decoding.  Keys in pages outside [0, pages), or past table_width pages, are not seen.  max_kv_length is
- * the longest request's length, or more: it decides how long requests are split and sizes temp; longer
- * requests are right too, only slower. */
+ * the longest request's length, or more: it sizes temp, and with it the number of parts that a long request may
+ * be split into.  How requests are split goes by their own lengths, so stating more costs storage and next to no time; requests
+ * longer than stated are right too, only slower. */
 size_t lcpp_hip_attention_paged_temp_bytes(uint32_t requests, uint64_t q_tokens, uint64_t max_kv_length, uint32_t q_heads,
                                            uint32_t kv_heads, uint32_t head_dim);
 #define LCPP_HIP_DECLARE_ATTENTION_PAGED(S)                                                                      \

@@ -14,9 +14,10 @@
 // and the results alone makes 0.2%.  Sums, dP and dP - rowsum are f32.
 //
 // 10 * dim operations a pair of row and key if S and dP were made once, 14 with both roles; bound by the matrix cores and by
-// what feeds them: 11,059 tokens in six sequences (32 heads of 128 on 8) take 895 us, 890 TFLOP/s of what runs, 640 of
+// what feeds them: 11,059 tokens in six sequences (32 heads of 128 on 8) take 926 us, 865 TFLOP/s of what runs, 620 of
 // what has to.  LDS holds the tiles that pass by, twice, and 128 keys' values (101 KB at 128 items: one workgroup of eight
-// waves a compute unit, two waves a SIMD).
+// waves a compute unit, two waves a SIMD).  At 128 items a wave has all of its 256 registers and keeps two values in scratch memory
+// over the loops.
 #include "attention_packed.hpp"
 
 namespace lcpp_hip {
@@ -46,7 +47,7 @@ __device__ __forceinline__ int too_large_by(const F32x16& x) {
 
 // What the gradients need of a row: stats[h][t] = lse in powers of 2, less kWeightRaise (infinity for a row that saw nothing: its
 // weights are then 2^-inf = 0), and behind all of those delta[h][t] = sum over the head's items of dO * O.  16 lanes a row.  Bound
-// by memory (the rows of O and dO, 181 MB for 11,059 tokens of 32 heads: 36 us, 5.0 TB/s).
+// by memory (the rows of O and dO, 181 MB for 11,059 tokens of 32 heads: 34 us, 5.3 TB/s).
 template <typename T>
 __global__ __launch_bounds__(kBlock) void attention_row_stats_kernel(Rows out, Rows dout, const float* __restrict__ lse,
                                                                      float* __restrict__ stats, int q_tokens, int q_heads, int dim) {

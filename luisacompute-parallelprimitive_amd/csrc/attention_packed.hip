@@ -8,10 +8,10 @@
 // are rounded to 16 bits for the product with V, whose operands are 16 bits wide (l adds them up unrounded).
 //
 // 4 * dim operations a pair of row and key, and little to read (each row of K and V once for 128 query rows): long
-// sequences are bound by the matrix cores.  One of 16,384 rows, 16 heads of 128: 1,070 to 1,100 us, 1,000 to 1,030 TFLOP/s,
-// where a large library product reaches 1,168; the clock falls as low as 1.7 GHz under it, so what is left is power.
-// Uneven prompts of 60 to 2,500 rows (32 heads of 128) take 148 us, 700 TFLOP/s: their last tiles are part empty, and a
-// workgroup of few keys is latency.  Seven prompts of up to 200 rows: 7.2 us, all of it latency.
+// sequences are bound by the matrix cores.  One of 16,384 rows, 16 heads of 128: 1,080 to 1,120 us, 980 to 1,020 TFLOP/s,
+// where a large library product reaches 1,186; the clock falls as low as 1.7 GHz under it, so what is left is power.
+// Uneven prompts of 60 to 2,500 rows (32 heads of 128) take 145 to 165 us, 630 to 710 TFLOP/s: their last tiles are part empty, and a
+// workgroup of few keys is latency.  Seven prompts of up to 200 rows: 8.2 us, all of it latency.
 //
 // A workgroup: four waves of 32 rows and 64 keys at a time, keys and values shared in LDS (33 KB a set of buffers at 128
 // items, two sets, so two workgroups a compute unit).  Eight waves a workgroup, and a wave's products and exponentials

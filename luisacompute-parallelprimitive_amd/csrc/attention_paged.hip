@@ -6,8 +6,8 @@
 //
 // The n * group rows of a request that share a key head are one matrix of rows, so a key is read once for all of them.
 // Reading the cache bounds the call: 4 * dim bytes a key and key head.  256 requests of 200 to 4,000 keys, 8 key heads of
-// 128: 1.38 GB in 283 us, 4.9 TB/s, what a large copy reaches.  One request of 131,000: 537 MB in 100 us, 5.3 TB/s, and
-// 9 us to join.
+// 128: 1.38 GB in 281 us, 4.9 TB/s, where reads alone reach 7.0 on this card.  One request of 131,000: 537 MB in 98 us,
+// 5.5 TB/s, and 7 us to join.
 //
 // Few rows (attention_paged_kernel): a workgroup takes 32 rows and a part of the keys, its four waves take 32 keys in turn,
 // each with its own running maximum, sum and products, and join them at the end.  More (attention_paged_wide_kernel): four
@@ -416,8 +416,8 @@ struct PagedTiles {
     }
 };
 
-// Many rows of a request: 24 trees of 5 to 48 tokens over 500 to 8,000 keys, 4 heads a key head: 302 MB in 94 to 98 us,
-// 3.1 TB/s, and 13 us to join.  Bound by the latency of a tile: a workgroup has one in flight while it works on another.
+// Many rows of a request: 24 trees of 5 to 48 tokens over 500 to 8,000 keys, 4 heads a key head: 302 MB in 91 us,
+// 3.3 TB/s, and 11 us to join.  Bound by the latency of a tile: a workgroup has one in flight while it works on another.
 template <typename T, int DP>
 __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_paged_wide_kernel(Rows q, Pages key_cache, Pages value_cache, Rows out,
                                                                          float* __restrict__ lse, Parts parts,
@@ -513,7 +513,7 @@ __global__ __launch_bounds__(kBlock, DP <= 64 ? 3 : 2) void attention_paged_wide
 
 // Joins the parts of a token's rows, in the parts' order: with t the largest of the parts' scales, O = sum exp(t_i - t) A_i /
 // sum exp(t_i - t) l_i.  16 lanes take a row's items; GROUPS such groups every GROUPS-th part of it, and a workgroup's rows
-// are heads of one token.  Bound by latency (64 parts of 32 rows, 16 groups: 9 us; one group: 51).
+// are heads of one token.  Bound by latency (64 parts of 32 rows, 16 groups: 7 us; one group: 51).
 template <typename T, int GROUPS>
 __global__ __launch_bounds__(kBlock) void attention_paged_join_kernel(Rows out, float* __restrict__ lse, Parts parts,
                                                                       const int32_t* __restrict__ q_offsets,
