@@ -695,6 +695,161 @@ LCPP_HIP_DECLARE_ATTENTION_PAGED(f16)
 #undef LCPP_HIP_DECLARE_ATTENTION_PAGED
 
 /* ---------------------------------------------------------------------------------------------
+ * Rotary positions (no reference counterpart).
+ *
+ * Pair i of the first rotary_dim items of each head is turned by the angle (position + shift) * frequencies[i] and made
+ * `factor` times as long; items from rotary_dim on are copied.  A pair is items i and i + rotary_dim / 2, or, interleaved,
+ * 2 i and 2 i + 1.  rotary_dim is even, at most the head size, which is a multiple of 8 up to 1,024 (others:
+ * LCPP_HIP_ERR_UNSUPPORTED).  Rows as for attention: bf16 or f16, starts at multiples of 16 bytes, strides in multiples of 8
+ * items.  Angles are taken in 64 bits, turns in f32, and results are rounded once.
+ *
+ * positions [tokens]; requests [tokens] or null: rows whose request is negative (page_plan's, past the last token) are
+ * left as they are; shifts [num_shifts] or null: what is added to the positions of each request's rows, for requests that had
+ * keys evicted (requests outside [0, num_shifts): nothing).  Output rows are the input rows (same address and strides) or
+ * share no memory with them.  q or k may be left out by zero heads.
+ * ------------------------------------------------------------------------------------------- */
+#define LCPP_HIP_ROTARY_PLAIN 0  /* base^(-2 i / rotary_dim)                                                            */
+#define LCPP_HIP_ROTARY_LINEAR 1 /* that divided by scale                                                               */
+#define LCPP_HIP_ROTARY_BASE 2   /* with the base times scale^(rotary_dim / (rotary_dim - 2)): the last is divided by scale */
+#define LCPP_HIP_ROTARY_BANDS 3  /* divided by scale where a pair makes at most `low` turns in the `trained` length, as it */
+                                 /* is from `high` turns on, and in between in proportion                              */
+/* Fills rotary_dim / 2 frequencies, in radians a position, in host memory. */
+int lcpp_hip_rotary_frequencies(double* out, uint32_t rotary_dim, double base, int scaling, double scale, double trained,
+                                double low, double high);
+/* `inverse`: the turn by the negative angles, times the same factor, which takes the gradients of the outputs to those of
+ * the inputs. */
+#define LCPP_HIP_DECLARE_ROTARY(S)                                                                                     \
+    int lcpp_hip_rotary_##S(const lcpp_hip_rows* q, const lcpp_hip_rows* k, const int32_t* positions,                  \
+                            const int32_t* requests, const int32_t* shifts, uint32_t num_shifts,                       \
+                            const double* frequencies, const lcpp_hip_rows* q_out, const lcpp_hip_rows* k_out,         \
+                            uint64_t tokens, uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim,                   \
+                            uint32_t rotary_dim, int interleaved, int inverse, float factor, void* stream);
+LCPP_HIP_DECLARE_ROTARY(bf16)
+LCPP_HIP_DECLARE_ROTARY(f16)
+#undef LCPP_HIP_DECLARE_ROTARY
+/* rotary and paged_write in one: turned queries to q_out, turned keys and the values as they are to slots[t] of the caches
+ * (slots that are negative or past the last page: only the queries).  slot_positions [pages][page_size] or null: the slots'
+ * positions, shifts included, as evict_plan reads them.  No two rows share a slot. */
+#define LCPP_HIP_DECLARE_PAGED_WRITE_ROTARY(S)                                                                         \
+    int lcpp_hip_paged_write_rotary_##S(                                                                               \
+        const lcpp_hip_rows* q, const lcpp_hip_rows* key, const lcpp_hip_rows* value, const int32_t* positions,        \
+        const int32_t* requests, const int32_t* shifts, uint32_t num_shifts, const double* frequencies,                \
+        const int64_t* slots, const lcpp_hip_rows* q_out, const lcpp_hip_pages* key_cache,                             \
+        const lcpp_hip_pages* value_cache, int32_t* slot_positions, uint64_t tokens, uint32_t q_heads,                 \
+        uint32_t kv_heads, uint32_t head_dim, uint32_t rotary_dim, int interleaved, float factor, uint32_t page_size,  \
+        uint32_t pages, void* stream);
+LCPP_HIP_DECLARE_PAGED_WRITE_ROTARY(bf16)
+LCPP_HIP_DECLARE_PAGED_WRITE_ROTARY(f16)
+#undef LCPP_HIP_DECLARE_PAGED_WRITE_ROTARY
+
+/* ---------------------------------------------------------------------------------------------
+ * Eviction from the paged cache by accumulated attention weight (no reference counterpart).
+ *
+ * weights [pages][page_size] f32 holds a sum for each slot: the softmax weights of all rows and heads that saw its key.  A step
+ * of one layer: attention_paged with its lse, attention_paged_weights, and where requests have grown too long page_release
+ * (once for all layers, whose lengths are the same), evict_plan and paged_move (each layer).  Keys keep the positions that they
+ * were turned by, and attention does not ask for their order, so a kept key past the new end moves into the place of an
+ * evicted one, and no other row moves.
+ * ------------------------------------------------------------------------------------------- */
+
+/* weights_out of a request's keys: the softmax weights exp(scale q k - lse) that this step's rows gave them, all heads
+ * together, plus `decay` times weights_in for the first known_lengths[r] keys (null: all before the new ones; weights_in null:
+ * nothing is added).  Rows, pages, tree and the keys that a row sees are those of attention_paged, and lse [q_heads][q_tokens]
+ * is what it gave; rows with an lse of -infinity give no weight.  weights_out may be weights_in.  Slots that hold no key of a
+ * request are left as they are.  Requests share no slots.  max_kv_length, the longest request's length or more, only
+ * says how a request is dealt out. */
+size_t lcpp_hip_attention_paged_weights_temp_bytes(uint32_t requests, uint64_t q_tokens, uint64_t max_kv_length,
+                                                   uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim);
+#define LCPP_HIP_DECLARE_ATTENTION_WEIGHTS(S)                                                                          \
+    int lcpp_hip_attention_paged_weights_##S(                                                                          \
+        void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_pages* key_cache,                        \
+        const int32_t* block_table, uint64_t table_stride, uint32_t table_width, const int32_t* q_offsets,             \
+        const int32_t* kv_lengths, const int32_t* known_lengths, const uint64_t* tree, const float* lse,               \
+        const float* weights_in, float* weights_out, uint32_t requests, uint64_t q_tokens, uint64_t max_kv_length,     \
+        uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size, uint32_t pages, float scale,       \
+        float decay, void* stream);
+LCPP_HIP_DECLARE_ATTENTION_WEIGHTS(bf16)
+LCPP_HIP_DECLARE_ATTENTION_WEIGHTS(f16)
+#undef LCPP_HIP_DECLARE_ATTENTION_WEIGHTS
+
+/* Lengths after an eviction: kept_lengths[r] = min(kv_lengths[r], keep_lengths[r]) (negative ones count as 0), and the pages
+ * that no kept key is in, in the requests' order, to `released` (pages that were not there, negative entries, are left out).  A
+ * request of n keys that would keep K of them and may need more than most_moves moves, min(K, n - K), keeps all n.  shifts_out [requests]
+ * or null: shifts (null: 0) plus the number of keys evicted, what rotary adds to the positions of later tokens; it may be
+ * `shifts`.  counts[0] pages released (those from max_released on are left out of the list), counts[1] keys kept.  The block
+ * table is read alone: entries past a request's pages are not looked at by the other calls. */
+int lcpp_hip_page_release(const int32_t* kv_lengths, const int32_t* keep_lengths, uint32_t requests, uint32_t page_size,
+                          const int32_t* block_table, uint64_t table_stride, uint32_t table_width, uint64_t most_moves,
+                          const int32_t* shifts, int32_t* kept_lengths, int32_t* shifts_out, int32_t* released,
+                          uint64_t max_released, int32_t* counts, void* stream);
+
+/* The moves that cut each request to kept_lengths[r] keys.  Kept are, before all others, keys whose position is below `first` or among
+ * the latest `recent` ones (at least shifts[r] + kv_lengths[r] - recent), then those of the largest sums; equal ones by
+ * the lower index.  NaN counts as less than any number, and a key whose page is not there as less than that.  The i-th kept
+ * key past the new end, move_from[r][i], goes to the i-th place of an evicted key before it, move_to[r][i], as slots (-1: the
+ * page is not there); entries past the last move are -1.  A request makes at most min(K, n - K) moves; those past `width` are
+ * left out (see page_release's most_moves).  positions (slots' positions) may be null where first and recent are 0, shifts where nothing
+ * was evicted before.  kv_lengths are those before the eviction.  max_kv_length is the longest of them, or more. */
+size_t lcpp_hip_evict_plan_temp_bytes(uint32_t requests, uint64_t max_kv_length);
+int lcpp_hip_evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_t* positions,
+                        const int32_t* block_table, uint64_t table_stride, uint32_t table_width, const int32_t* kv_lengths,
+                        const int32_t* kept_lengths, const int32_t* shifts, uint32_t requests, uint64_t max_kv_length,
+                        uint32_t page_size, uint32_t pages, uint32_t first, uint32_t recent, int64_t* move_from,
+                        int64_t* move_to, uint64_t width, void* stream);
+
+/* Copies the rows of slot move_from[i] of both caches to slot move_to[i], and their sums and positions where given (moves
+ * of which either slot is negative or past the last page are left out).  No slot is moved to twice, or both from and to. */
+#define LCPP_HIP_DECLARE_PAGED_MOVE(S)                                                                                 \
+    int lcpp_hip_paged_move_##S(const int64_t* move_from, const int64_t* move_to, uint64_t moves,                      \
+                                const lcpp_hip_pages* key_cache, const lcpp_hip_pages* value_cache, float* weights,    \
+                                int32_t* positions, uint32_t kv_heads, uint32_t head_dim, uint32_t page_size,          \
+                                uint32_t pages, void* stream);
+LCPP_HIP_DECLARE_PAGED_MOVE(bf16)
+LCPP_HIP_DECLARE_PAGED_MOVE(f16)
+#undef LCPP_HIP_DECLARE_PAGED_MOVE
+
+/* ---------------------------------------------------------------------------------------------
+ * A gated linear recurrence over the sequences of a ragged batch (no reference counterpart), channel by channel:
+ *
+ *     h_t = exp(log_decay_t) h_{t-1} + x_t,   out_t = h_t rounded,
+ *
+ * from the sequence's initial state (null: 0) to its final one.  Rows and offsets as for attention over packed sequences;
+ * x, log_decay, out and their gradients are [tokens][channels] of one type, bf16, f16 or f32, any number of channels, rows any
+ * whole number of items apart.  States are [num_states][channels] f32: sequence b has row state_rows[b] (null: b; a row
+ * outside [0, num_states): starts from 0 and is not kept).  final_states (or null) may be the same memory as `initial`, and then no two
+ * sequences share a row.  A sequence of no tokens hands its initial state on; one of a single token is a step of serving.
+ * log_decay is at most 0 in use (-infinity forgets the state); growth is right as long as products over 512 steps stay finite.
+ * What is not finite stays in its channel and sequence.  Sums have one order: the same call gives the same bits.
+ *
+ * The backward pass takes dout, and dfinal [sequences][channels] f32 (null: 0), to dx, dlog_decay and dinitial [sequences][channels]
+ * f32 (or null); `initial` is [sequences][channels].  dlog_decay = dh_t exp(log_decay_t) h_{t-1} takes h as `out` has it.
+ * ------------------------------------------------------------------------------------------- */
+
+/* [tokens][channels]: the channels contiguous, the tokens' stride in items. */
+typedef struct lcpp_hip_steps {
+    void* data;
+    int64_t token_stride;
+} lcpp_hip_steps;
+
+/* Of both directions. */
+size_t lcpp_hip_recurrence_temp_bytes(uint32_t sequences, uint64_t tokens, uint32_t channels);
+#define LCPP_HIP_DECLARE_RECURRENCE(S)                                                                                 \
+    int lcpp_hip_recurrence_##S(void* temp, size_t temp_bytes, const lcpp_hip_steps* x,                                \
+                                const lcpp_hip_steps* log_decay, const int32_t* offsets, const float* initial,         \
+                                const int32_t* state_rows, uint32_t num_states, const lcpp_hip_steps* out,             \
+                                float* final_states, uint32_t sequences, uint64_t tokens, uint32_t channels,           \
+                                void* stream);                                                                         \
+    int lcpp_hip_recurrence_backward_##S(                                                                              \
+        void* temp, size_t temp_bytes, const lcpp_hip_steps* log_decay, const lcpp_hip_steps* out,                     \
+        const lcpp_hip_steps* dout, const int32_t* offsets, const float* initial, const float* dfinal,                 \
+        const lcpp_hip_steps* dx, const lcpp_hip_steps* dlog_decay, float* dinitial, uint32_t sequences,               \
+        uint64_t tokens, uint32_t channels, void* stream);
+LCPP_HIP_DECLARE_RECURRENCE(bf16)
+LCPP_HIP_DECLARE_RECURRENCE(f16)
+LCPP_HIP_DECLARE_RECURRENCE(f32)
+#undef LCPP_HIP_DECLARE_RECURRENCE
+
+/* ---------------------------------------------------------------------------------------------
  * Seeded synthetic workloads for tests and benchmarks (no reference counterpart; the reference
  * generates on the host, e.g. tests/lcpp_cub_bench.cpp:516-521,666-672,814).
  * Stream: splitmix64, r_i = mix(seed + (start + i + 1) * 0x9E3779B97F4A7C15).

@@ -9,7 +9,9 @@ The operation names follow the reference API (``DeviceReduce::Sum``, ``DeviceSca
 ``DeviceReduce::ReduceByKey``, ``DeviceSelect``, ``DevicePartition``, ``DeviceRunLengthEncode``;
 src/lcpp/device/*.h) and the
 temp-storage queries return the reference's ``Get*TempStorageBytes`` values.  Attention over ragged batches and its
-paged cache (:func:`page_plan`, :func:`paged_write`, :func:`attention_packed`, :func:`attention_paged`) have no
+paged cache (:func:`page_plan`, :func:`paged_write`, :func:`attention_packed`, :func:`attention_paged`), rotary positions
+(:func:`rotary`, :func:`paged_write_rotary`), eviction from the cache (:func:`attention_paged_weights`, :func:`page_release`,
+:func:`evict_plan`, :func:`paged_move`) and the gated recurrence (:func:`recurrence`, :func:`recurrence_backward`) have no
 counterpart there.
 """
 from __future__ import annotations
@@ -37,6 +39,8 @@ SPMV_SUFFIXES = [(v, i) for v in ("f32", "f64", "i32", "u32") for i in ("i32", "
 BY_KEY_KEY_SUFFIXES = ("i32", "u32", "i64", "u64")
 BY_KEY_VALUE_SUFFIXES = SCALAR_SUFFIXES
 ATTENTION_SUFFIXES = ("bf16", "f16")
+RECURRENCE_SUFFIXES = ("bf16", "f16", "f32")
+ROTARY_SCALINGS = ("plain", "linear", "base", "bands")
 FLAG_SUFFIXES = ("b8", "i32", "u32", "i64", "u64")
 
 # Predicate clause ops (include/lcpp_hip.h LCPP_HIP_PRED_*).
@@ -56,6 +60,11 @@ class Rows(C.Structure):
 class Pages(C.Structure):
     """lcpp_hip_pages: [pages, page size, kv heads, head_dim], strides of the first three axes in items."""
     _fields_ = [("data", C.c_void_p), ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class Steps(C.Structure):
+    """lcpp_hip_steps: [tokens, channels], the stride of the tokens in items."""
+    _fields_ = [("data", C.c_void_p), ("token_stride", C.c_int64)]
 
 
 _CTYPE = {
@@ -202,6 +211,23 @@ def _declare(lib: C.CDLL) -> None:
             u64, u32, u32, u32, f32, i32, vp)
         sig(f"lcpp_hip_attention_paged_{t}", i32, vp, sz, rp, gp, gp, vp, u32, u32, vp, vp, vp, rp, vp, u32, u64, u64, u32,
             u32, u32, u32, u32, f32, vp)
+    f64, sp = C.c_double, C.POINTER(Steps)
+    sig("lcpp_hip_rotary_frequencies", i32, vp, u32, f64, i32, f64, f64, f64, f64)
+    sig("lcpp_hip_attention_paged_weights_temp_bytes", sz, u32, u64, u64, u32, u32, u32)
+    sig("lcpp_hip_page_release", i32, vp, vp, u32, u32, vp, u64, u32, u64, vp, vp, vp, vp, u64, vp, vp)
+    sig("lcpp_hip_evict_plan_temp_bytes", sz, u32, u64)
+    sig("lcpp_hip_evict_plan", i32, vp, sz, vp, vp, vp, u64, u32, vp, vp, vp, u32, u64, u32, u32, u32, u32, vp, vp, u64, vp)
+    for t in ATTENTION_SUFFIXES:
+        sig(f"lcpp_hip_rotary_{t}", i32, rp, rp, vp, vp, vp, u32, vp, rp, rp, u64, u32, u32, u32, u32, i32, i32, f32, vp)
+        sig(f"lcpp_hip_paged_write_rotary_{t}", i32, rp, rp, rp, vp, vp, vp, u32, vp, vp, rp, gp, gp, vp, u64, u32, u32, u32, u32,
+            i32, f32, u32, u32, vp)
+        sig(f"lcpp_hip_attention_paged_weights_{t}", i32, vp, sz, rp, gp, vp, u64, u32, vp, vp, vp, vp, vp, vp, vp, u32, u64,
+            u64, u32, u32, u32, u32, u32, f32, f32, vp)
+        sig(f"lcpp_hip_paged_move_{t}", i32, vp, vp, u64, gp, gp, vp, vp, u32, u32, u32, u32, vp)
+    sig("lcpp_hip_recurrence_temp_bytes", sz, u32, u64, u32)
+    for t in RECURRENCE_SUFFIXES:
+        sig(f"lcpp_hip_recurrence_{t}", i32, vp, sz, sp, sp, vp, vp, vp, u32, sp, vp, u32, u64, u32, vp)
+        sig(f"lcpp_hip_recurrence_backward_{t}", i32, vp, sz, sp, sp, sp, vp, vp, vp, sp, sp, vp, u32, u64, u32, vp)
 
 
 def lib() -> C.CDLL:
@@ -886,3 +912,214 @@ def attention_paged(suffix: str, q, key_cache, value_cache, block_table, q_offse
          _rows(dt, "out", out, rows, True), _lse(f32, lse, heads, tokens), requests, tokens,
          max_kv_length, heads, kv_heads, dim, page_size, pages, dim ** -0.5 if scale is None else scale,
          stream_handle(stream))
+
+
+# ---- rotary positions -----------------------------------------------------------------------------
+def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "plain", scale: float = 1.0, trained: float = 0.0,
+                       low: float = 1.0, high: float = 4.0, device="cuda"):
+    """Frequencies of rotary_dim / 2 pairs in radians a position, float64.  `scaling`: "plain", or stretched for contexts
+    `scale` times as long, by "linear" division, by the "base", or in "bands" (pairs that turn less than `low` times in the
+    `trained` length are divided by `scale`, from `high` times on they are not)."""
+    import torch
+    if scaling not in ROTARY_SCALINGS:
+        raise ValueError(f"rotary scaling {scaling!r}: one of {', '.join(ROTARY_SCALINGS)}")
+    out = torch.empty(max(0, rotary_dim // 2), dtype=torch.float64)
+    check(lib().lcpp_hip_rotary_frequencies(out.data_ptr(), max(0, rotary_dim), base, ROTARY_SCALINGS.index(scaling), scale, trained,
+                                            low, high))
+    return out.to(device)
+
+
+def _turns(frequencies) -> tuple:
+    """Address of the frequencies and the items that they turn."""
+    import torch
+    return _array(torch.float64, "frequencies", frequencies, 1), 2 * frequencies.numel()
+
+
+def _shifts(i32, shifts, requests):
+    if shifts is not None and requests is None:
+        raise ValueError("shifts: the rows' requests are needed with them")
+    return _array(i32, "shifts", shifts, 0), 0 if shifts is None else shifts.numel()
+
+
+def rotary(suffix: str, q, k, positions, frequencies, q_out, k_out, interleaved: bool = False, inverse: bool = False,
+           factor: float = 1.0, requests=None, shifts=None, stream=None) -> None:
+    """Rows q [tokens, q heads, head_dim] and k [tokens, kv heads, head_dim] (or None) turned by positions [tokens] int32 times
+    frequencies float64 into q_out and k_out, which may be q and k.  `inverse` takes the outputs' gradients to the inputs'.
+    Rows whose entry of `requests` is negative are left as they are; `shifts` (one a request) are added to the positions."""
+    dt, _, i32, _ = _row_types(suffix)
+    tokens, heads, dim = rows = _axes("q", q, 3)
+    keys = None if k is None else (tokens, _axes("k", k, 3)[1], dim)
+    turns, rotary_dim = _turns(frequencies)
+    shift, num_shifts = _shifts(i32, shifts, requests)
+    call(f"lcpp_hip_rotary_{suffix}", _rows(dt, "q", q, rows), None if k is None else _rows(dt, "k", k, keys),
+         _array(i32, "positions", positions, tokens), _array(i32, "requests", requests, tokens), shift, num_shifts, turns,
+         _rows(dt, "q_out", q_out, rows, True), None if k is None else _rows(dt, "k_out", k_out, keys, True), tokens, heads,
+         0 if k is None else keys[1], dim, rotary_dim, int(interleaved), int(inverse), factor, stream_handle(stream))
+
+
+def paged_write_rotary(suffix: str, q, key, value, positions, frequencies, slots, q_out, key_cache, value_cache,
+                       slot_positions=None, interleaved: bool = False, factor: float = 1.0, requests=None, shifts=None,
+                       stream=None) -> None:
+    """rotary and paged_write in one: turned queries to q_out, turned keys and the values to their slots, and the slots'
+    positions to slot_positions [pages, page size] int32."""
+    dt, _, i32, i64 = _row_types(suffix)
+    tokens, heads, dim = rows = _axes("q", q, 3)
+    pages, page_size, kv_heads, _ = _axes("key_cache", key_cache, 4)
+    cache, keys = (pages, page_size, kv_heads, dim), (tokens, kv_heads, dim)
+    turns, rotary_dim = _turns(frequencies)
+    shift, num_shifts = _shifts(i32, shifts, requests)
+    call(f"lcpp_hip_paged_write_rotary_{suffix}", _rows(dt, "q", q, rows), _rows(dt, "key", key, keys), _rows(dt, "value", value, keys),
+         _array(i32, "positions", positions, tokens), _array(i32, "requests", requests, tokens), shift, num_shifts, turns,
+         _array(i64, "slots", slots, tokens), _rows(dt, "q_out", q_out, rows, True), _pages(dt, "key_cache", key_cache, cache, True),
+         _pages(dt, "value_cache", value_cache, cache, True), _array(i32, "slot_positions", slot_positions, pages * page_size),
+         tokens, heads, kv_heads, dim, rotary_dim, int(interleaved), factor, page_size, pages, stream_handle(stream))
+
+
+# ---- eviction from the paged cache ----------------------------------------------------------------
+def attention_paged_weights_temp_bytes(requests: int, q_tokens: int, max_kv_length: int, q_heads: int, kv_heads: int,
+                                       head_dim: int) -> int:
+    return lib().lcpp_hip_attention_paged_weights_temp_bytes(requests, q_tokens, max_kv_length, q_heads, kv_heads, head_dim)
+
+
+def attention_paged_weights(suffix: str, q, key_cache, block_table, q_offsets, kv_lengths, lse, weights_out, weights_in=None,
+                            known_lengths=None, decay: float = 1.0, tree=None, max_kv_length=None, scale=None, temp=None,
+                            stream=None) -> None:
+    """weights_out [pages, page size] f32, for each request's keys: the softmax weights that this step's rows q gave them
+    (lse: attention_paged's), plus `decay` times weights_in for its first known_lengths keys (all before the new ones by
+    default).  weights_out may be weights_in."""
+    dt, f32, i32, i64 = _row_types(suffix)
+    tokens, heads, dim = rows = _axes("q", q, 3)
+    pages, page_size, kv_heads, _ = _axes("key_cache", key_cache, 4)
+    requests = kv_lengths.numel()
+    table, table_stride, width = _table(i32, block_table, requests)
+    if max_kv_length is None:
+        max_kv_length = width * page_size
+    if temp is None:
+        temp = _scratch(attention_paged_weights_temp_bytes(requests, tokens, max_kv_length, heads, kv_heads, dim), q.device, stream)
+    call(f"lcpp_hip_attention_paged_weights_{suffix}", ptr(temp), _tb(temp), _rows(dt, "q", q, rows),
+         _pages(dt, "key_cache", key_cache, (pages, page_size, kv_heads, dim)), table, table_stride, width,
+         _array(i32, "q_offsets", q_offsets, requests + 1), _array(i32, "kv_lengths", kv_lengths, requests),
+         _array(i32, "known_lengths", known_lengths, requests), _array(i64, "tree", tree, tokens), _lse(f32, lse, heads, tokens),
+         _array(f32, "weights_in", weights_in, pages * page_size), _array(f32, "weights_out", weights_out, pages * page_size),
+         requests, tokens, max_kv_length, heads, kv_heads, dim, page_size, pages, dim ** -0.5 if scale is None else scale, decay,
+         stream_handle(stream))
+
+
+def page_release(kv_lengths, keep_lengths, page_size: int, block_table, kept_lengths, released, counts, shifts=None,
+                 shifts_out=None, most_moves=None, stream=None) -> None:
+    """kept_lengths of requests cut to keep_lengths, the pages that come free (released, counts[0] of them; counts[1] keys are
+    kept), and shifts_out: `shifts` plus the keys evicted.  Requests that may need more than most_moves moves (evict_plan's
+    width) are not cut.  All int32."""
+    _, _, i32, _ = _row_types("bf16")
+    requests = kv_lengths.numel()
+    table, table_stride, width = _table(i32, block_table, requests)
+    call("lcpp_hip_page_release", _array(i32, "kv_lengths", kv_lengths, requests), _array(i32, "keep_lengths", keep_lengths, requests),
+         requests, page_size, table, table_stride, width, 0x7FFFFFFF if most_moves is None else most_moves,
+         _array(i32, "shifts", shifts, requests), _array(i32, "kept_lengths", kept_lengths, requests),
+         _array(i32, "shifts_out", shifts_out, requests), _array(i32, "released", released, 0), released.numel(),
+         _array(i32, "counts", counts, 2), stream_handle(stream))
+
+
+def evict_plan_temp_bytes(requests: int, max_kv_length: int) -> int:
+    return lib().lcpp_hip_evict_plan_temp_bytes(requests, max_kv_length)
+
+
+def evict_plan(weights, positions, block_table, kv_lengths, kept_lengths, move_from, move_to, first: int = 0, recent: int = 0,
+               shifts=None, max_kv_length=None, temp=None, stream=None) -> None:
+    """The moves, slots move_from[r] to move_to[r] (int64 [requests, width], -1 past the last), that cut each request from
+    kv_lengths to kept_lengths keys: the `first` positions and the latest `recent` ones stay, then the largest of
+    weights [pages, page size].  positions [pages, page size] int32, or None where first and recent are 0."""
+    _, f32, i32, i64 = _row_types("bf16")
+    requests = kv_lengths.numel()
+    pages, page_size = _axes("weights", weights, 2)
+    table, table_stride, width = _table(i32, block_table, requests)
+    if move_from.shape != move_to.shape or move_from.dim() != 2 or move_from.shape[0] != requests:
+        raise ValueError(f"move_from and move_to: [{requests}, width] of one shape")
+    if max_kv_length is None:
+        max_kv_length = width * page_size
+    if temp is None:
+        temp = _scratch(evict_plan_temp_bytes(requests, max_kv_length), weights.device, stream)
+    call("lcpp_hip_evict_plan", ptr(temp), _tb(temp), _array(f32, "weights", weights, pages * page_size),
+         _array(i32, "positions", positions, pages * page_size), table, table_stride, width,
+         _array(i32, "kv_lengths", kv_lengths, requests), _array(i32, "kept_lengths", kept_lengths, requests),
+         _array(i32, "shifts", shifts, requests), requests, max_kv_length, page_size, pages, first, recent,
+         _array(i64, "move_from", move_from, 0), _array(i64, "move_to", move_to, 0), move_from.shape[1], stream_handle(stream))
+
+
+def paged_move(suffix: str, move_from, move_to, key_cache, value_cache, weights=None, positions=None, stream=None) -> None:
+    """Rows of slots move_from (int64, any shape) of both caches [pages, page size, kv heads, head_dim] to slots move_to, with
+    their weights and positions [pages, page size] where given.  Moves with a negative slot are left out."""
+    dt, f32, i32, i64 = _row_types(suffix)
+    pages, page_size, heads, dim = cache = _axes("key_cache", key_cache, 4)
+    moves = move_from.numel()
+    if move_to.numel() != moves:
+        raise ValueError(f"move_to: {move_to.numel()} slots for {moves} moves")
+    call(f"lcpp_hip_paged_move_{suffix}", _array(i64, "move_from", move_from, moves), _array(i64, "move_to", move_to, moves), moves,
+         _pages(dt, "key_cache", key_cache, cache, True), _pages(dt, "value_cache", value_cache, cache, True),
+         _array(f32, "weights", weights, pages * page_size), _array(i32, "positions", positions, pages * page_size), heads, dim,
+         page_size, pages, stream_handle(stream))
+
+
+# ---- a gated linear recurrence --------------------------------------------------------------------
+def _step_types(suffix: str) -> tuple:
+    """The torch dtypes of steps of the suffix, and of f32 and i32 arrays."""
+    if suffix == "f32":
+        _, f32, i32, _ = _row_types("bf16")
+        return f32, f32, i32
+    return _row_types(suffix)[:3]
+
+
+def _steps(dtype, name: str, t, shape: tuple) -> Steps:
+    if t.dtype is not dtype or t.shape != shape:
+        _refuse(name, t, dtype, shape)
+    token, item = t.stride()
+    if item != 1 and shape[1] > 1 or token < shape[1] and shape[0] > 1:
+        raise ValueError(f"{name}: rows of contiguous channels that share no memory are needed (copy what is expanded)")
+    return Steps(t.data_ptr(), token if shape[0] > 1 else shape[1])
+
+
+def _states(f32, name: str, t, channels: int, least: int) -> tuple:
+    """Device address and number of contiguous rows of states (None: none)."""
+    if t is None:
+        return None, 0
+    if t.dtype is not f32 or t.dim() != 2 or t.shape[0] < least or t.shape[1] != channels or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous rows of {channels} items of {f32} are needed, {least} or more")
+    return t.data_ptr(), t.shape[0]
+
+
+def recurrence_temp_bytes(sequences: int, tokens: int, channels: int) -> int:
+    return lib().lcpp_hip_recurrence_temp_bytes(sequences, tokens, channels)
+
+
+def recurrence(suffix: str, x, log_decay, offsets, out, initial=None, final=None, rows=None, temp=None, stream=None) -> None:
+    """out[t] = exp(log_decay[t]) out[t - 1] + x[t] along each sequence of a ragged batch, [tokens, channels], from the rows of
+    `initial` [states, channels] f32 to those of `final`, which may be the same tensor: sequence b's is rows[b] (int32), or b."""
+    dt, f32, i32 = _step_types(suffix)
+    tokens, channels = shape = _axes("x", x, 2)
+    sequences = offsets.numel() - 1
+    least = sequences if rows is None else 0
+    start, starts = _states(f32, "initial", initial, channels, least)
+    end, ends = _states(f32, "final", final, channels, least)
+    if initial is not None and final is not None and starts != ends:
+        raise ValueError(f"initial and final: {starts} and {ends} rows where both need the same number")
+    if temp is None:
+        temp = _scratch(recurrence_temp_bytes(sequences, tokens, channels), x.device, stream)
+    call(f"lcpp_hip_recurrence_{suffix}", ptr(temp), _tb(temp), _steps(dt, "x", x, shape), _steps(dt, "log_decay", log_decay, shape),
+         _array(i32, "offsets", offsets, 1), start, _array(i32, "rows", rows, sequences), max(starts, ends),
+         _steps(dt, "out", out, shape), end, sequences, tokens, channels, stream_handle(stream))
+
+
+def recurrence_backward(suffix: str, log_decay, out, dout, offsets, dx, dlog_decay, initial=None, dfinal=None, dinitial=None,
+                        temp=None, stream=None) -> None:
+    """Gradients of recurrence: dx and dlog_decay, and dinitial [sequences, channels] f32 if given, from dout and dfinal, and
+    from the out that the forward call gave; states are in the sequences' order."""
+    dt, f32, i32 = _step_types(suffix)
+    tokens, channels = shape = _axes("out", out, 2)
+    sequences = offsets.numel() - 1
+    if temp is None:
+        temp = _scratch(recurrence_temp_bytes(sequences, tokens, channels), out.device, stream)
+    call(f"lcpp_hip_recurrence_backward_{suffix}", ptr(temp), _tb(temp), _steps(dt, "log_decay", log_decay, shape),
+         _steps(dt, "out", out, shape), _steps(dt, "dout", dout, shape), _array(i32, "offsets", offsets, 1),
+         _states(f32, "initial", initial, channels, sequences)[0], _states(f32, "dfinal", dfinal, channels, sequences)[0],
+         _steps(dt, "dx", dx, shape), _steps(dt, "dlog_decay", dlog_decay, shape),
+         _states(f32, "dinitial", dinitial, channels, sequences)[0], sequences, tokens, channels, stream_handle(stream))

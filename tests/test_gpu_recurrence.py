@@ -1,0 +1,270 @@
+"""The gated recurrence and its gradients, against a plain 64-bit form that goes token by token."""
+import math
+
+import pytest
+import torch
+
+import long_request_oracle as oracle
+from attention_oracle import offsets_of
+from gpu_util import log
+
+pytestmark = pytest.mark.gpu
+
+DTYPE = {"bf16": torch.bfloat16, "f16": torch.float16, "f32": torch.float32}
+
+
+def made(seed, suffix, lengths, channels, span=200.0, gap=0):
+    """x, log_decay, dout [tokens, channels] and states; `gap`: rows of a wider array."""
+    g = torch.Generator().manual_seed(seed)
+    tokens, dtype = sum(lengths), DTYPE[suffix]
+    randn = lambda *s: torch.randn(*s, generator=g)
+    remember = torch.exp(-math.log(span) * torch.rand(channels, generator=g))
+    wide = lambda x: torch.nn.functional.pad(x.to(dtype), (0, gap)).cuda()[:, :channels]
+    x, dout = wide(randn(tokens, channels)), wide(randn(tokens, channels))
+    l = wide(-0.7 * remember * torch.exp(0.5 * randn(tokens, channels)))
+    return x, l, dout, randn(len(lengths), channels).cuda(), randn(len(lengths), channels).cuda()
+
+
+def run(hip, suffix, lengths, x, l, dout, initial=None, dfinal=None, temp=None):
+    offsets = offsets_of(lengths).cuda()
+    out, dx, dl = (torch.full(x.shape, 7.0, dtype=x.dtype, device="cuda") for _ in range(3))
+    final, dinitial = (torch.full((len(lengths), x.shape[1]), 7.0, device="cuda") for _ in range(2))
+    hip.recurrence(suffix, x, l, offsets, out, initial=initial, final=final, temp=temp)
+    hip.recurrence_backward(suffix, l, out, dout, offsets, dx, dl, initial=initial, dfinal=dfinal, dinitial=dinitial, temp=temp)
+    torch.cuda.synchronize()
+    return {"out": out, "final": final, "dx": dx, "dlog_decay": dl, "dinitial": dinitial}
+
+
+def check(hip, suffix, lengths, channels, seed=1, states=True, **kind):
+    log(f"{suffix} lengths {lengths[:12]} channels {channels}")
+    x, l, dout, initial, dfinal = made(seed, suffix, lengths, channels, **kind)
+    initial, dfinal = (initial, dfinal) if states else (None, None)
+    got = run(hip, suffix, lengths, x, l, dout, initial, dfinal)
+    want = oracle.recurrence(x, l, lengths, initial, dout, dfinal)
+    for name, value in want.items():
+        oracle.check(name, got[name], value)
+    return got
+
+
+@pytest.mark.parametrize("suffix", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("channels", [1, 2, 3, 7, 64, 65, 127, 130, 256, 258, 513, 1000])
+def test_widths(hip, dev, suffix, channels):
+    check(hip, suffix, [5, 0, 130, 1, 33], channels)
+
+
+@pytest.mark.parametrize("suffix", ["bf16", "f32"])
+@pytest.mark.parametrize("length", [1, 2, 15, 16, 17, 31, 32, 63, 64, 65, 127, 128, 129, 255, 256, 257, 511, 512, 513, 1025, 2500])
+def test_lengths(hip, dev, suffix, length):
+    check(hip, suffix, [length], 72)
+    check(hip, suffix, [length, 3, length], 36, states=False)
+
+
+@pytest.mark.parametrize("suffix", ["bf16", "f16", "f32"])
+def test_strides(hip, dev, suffix):
+    for gap in (1, 2, 3, 4, 8, 100):
+        check(hip, suffix, [40, 300], 68, gap=gap)
+        check(hip, suffix, [40, 300], 33, gap=gap)
+
+
+@pytest.mark.parametrize("suffix", ["bf16", "f32"])
+def test_ragged(hip, dev, suffix):
+    check(hip, suffix, [0, 0, 700, 0, 1, 1, 260, 128, 0, 256, 2, 0], 260, seed=4)
+    check(hip, suffix, [1] * 300, 40, seed=5)
+    check(hip, suffix, [3, 1, 4, 1, 5, 9, 2, 6] * 40, 24, seed=6)
+    check(hip, suffix, [6000, 50, 50], 16, seed=7, span=3000.0)
+
+
+def test_no_tokens_and_no_sequences(hip, dev):
+    none = torch.empty(0, 12, dtype=torch.bfloat16, device=dev)
+    states = torch.randn(3, 12, device=dev)
+    final, dinitial = torch.zeros_like(states), torch.zeros_like(states)
+    offsets = torch.zeros(4, dtype=torch.int32, device=dev)
+    hip.recurrence("bf16", none, none, offsets, none, initial=states, final=final)
+    hip.recurrence_backward("bf16", none, none, none, offsets, none, none, initial=states, dfinal=states, dinitial=dinitial)
+    assert torch.equal(final, states) and torch.equal(dinitial, states)
+    hip.recurrence("bf16", none, none, offsets, none, final=final)
+    assert not bool(final.any())
+    hip.recurrence("bf16", none, none, offsets[:1], none)
+
+
+def test_rows_of_no_sequence_are_left(hip, dev):
+    """Offsets that begin past the first row and end before the last."""
+    x, l, dout, _, _ = made(3, "f32", [100], 20)
+    offsets = torch.tensor([7, 40, 90], dtype=torch.int32).cuda()
+    out, dx, dl = (torch.full_like(x, 5.0) for _ in range(3))
+    hip.recurrence("f32", x, l, offsets, out)
+    hip.recurrence_backward("f32", l, out, dout, offsets, dx, dl)
+    want = oracle.recurrence(x[7:90], l[7:90], [33, 50], None, dout[7:90])
+    for name, got in (("out", out), ("dx", dx), ("dlog_decay", dl)):
+        oracle.check(name, got[7:90], want[name])
+        assert bool((got[:7] == 5.0).all()) and bool((got[90:] == 5.0).all())
+
+
+def test_state_rows(hip, dev):
+    """Serving: a pool of states, kept in place; a request without a row starts from zero and is not kept."""
+    lengths, channels = [1, 1, 40, 1, 0], 96
+    x, l, _, _, _ = made(9, "bf16", lengths, channels)
+    pool = torch.randn(8, channels, device=dev)
+    before = pool.clone()
+    rows = torch.tensor([5, 0, 7, -1, 2], dtype=torch.int32).cuda()
+    out = torch.empty_like(x)
+    hip.recurrence("bf16", x, l, offsets_of(lengths).cuda(), out, initial=pool, final=pool, rows=rows)
+    first = before[rows.clamp_min(0).long()] * (rows >= 0)[:, None]
+    want = oracle.recurrence(x, l, lengths, first)
+    oracle.check("out", out, want["out"])
+    for b, row in enumerate(rows.tolist()):
+        if row >= 0:
+            oracle.check("state", pool[row], (want["final"][0][b], want["final"][1][b]))
+    for row in (1, 3, 4, 6):
+        assert torch.equal(pool[row], before[row])
+    rows[1] = 8  # past the pool: as -1
+    again = torch.empty_like(x)
+    hip.recurrence("bf16", x, l, offsets_of(lengths).cuda(), again, initial=before, rows=rows)
+    first[1] = 0
+    oracle.check("out", again, oracle.recurrence(x, l, lengths, first)["out"])
+
+
+def test_token_by_token_is_the_scan(hip, dev):
+    """A sequence fed one token a call, or in pieces, comes out as the whole one within both bounds."""
+    length, channels = 300, 64
+    x, l, _, _, _ = made(2, "f32", [length], channels)
+    want = oracle.recurrence(x, l, [length])
+    for pieces in ([1] * length, [128, 1, 2, 169], [299, 1]):
+        state, at = torch.zeros(1, channels, device=dev), 0
+        out = torch.empty_like(x)
+        for n in pieces:
+            hip.recurrence("f32", x[at:at + n], l[at:at + n], offsets_of([n]).cuda(), out[at:at + n], initial=state, final=state)
+            at += n
+        oracle.check("out", out, want["out"])
+        oracle.check("final", state, want["final"])
+
+
+def test_forgetting_and_growing(hip, dev):
+    """-infinity forgets the state exactly; 0 keeps it; growth by a little is the formula's."""
+    x, _, dout, initial, dfinal = made(5, "f32", [400, 70], 40)
+    l = torch.full_like(x, -0.01)
+    l[50], l[300], l[430] = -math.inf, -math.inf, -math.inf
+    l[60:200] = 0.0
+    l[200:260] = 0.02
+    l[:, ::5] = -90.0
+    l[:, 1::5] = -0.0625
+    l[:, 2::5] = -0.0624
+    got = run(hip, "f32", [400, 70], x, l, dout, initial, dfinal)
+    want = oracle.recurrence(x, l, [400, 70], initial, dout, dfinal)
+    for name, value in want.items():
+        oracle.check(name, got[name], value)
+    for t in (50, 300):
+        forgot = l[t] == -math.inf  # channels 3 and 4 of five
+        assert torch.equal(got["out"][t, forgot], x[t, forgot])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_not_finite_stays_in_its_channel_and_sequence(hip, dev, bad):
+    lengths, channels = [300, 300, 40], 130
+    x, l, dout, initial, dfinal = made(6, "bf16", lengths, channels)
+    clean = run(hip, "bf16", lengths, x, l, dout, initial, dfinal)
+    x[310, 17] = bad
+    dout[450, 90] = bad
+    got = run(hip, "bf16", lengths, x, l, dout, initial, dfinal)
+    for name in got:
+        broken = ~got[name].isfinite()
+        if name in ("out", "dx", "dlog_decay"):
+            channel, first, last = {"out": (17, 310, 600), "dx": (90, 300, 451), "dlog_decay": (17, 311, 600)}[name]
+            assert bool(broken[first:last, channel].all()), name
+        allowed = torch.zeros_like(broken)
+        if broken.shape[0] == 3:
+            allowed[1, [17, 90]] = True
+        else:
+            allowed[300:600, [17, 90]] = True
+        assert not bool((broken & ~allowed).any()), name
+        assert torch.equal(got[name][~allowed], clean[name][~allowed]), name
+
+
+@pytest.mark.parametrize("limit", [0, 1])
+def test_chunks_that_are_not_waited_for(hip, dev, limit):
+    """With no patience a workgroup makes what it needs of the chunks before its own itself: the same bits."""
+    lengths = [3000, 10, 900]
+    x, l, dout, initial, dfinal = made(7, "bf16", lengths, 300, span=2000.0)
+    want = run(hip, "bf16", lengths, x, l, dout, initial, dfinal)
+    before = hip.lib().lcpp_hip_get_lookback_spin_limit()
+    try:
+        hip.check(hip.lib().lcpp_hip_set_lookback_spin_limit(limit))
+        got = run(hip, "bf16", lengths, x, l, dout, initial, dfinal)
+    finally:
+        hip.check(hip.lib().lcpp_hip_set_lookback_spin_limit(before))
+    for name in want:
+        assert torch.equal(got[name], want[name]), name
+
+
+def test_the_same_bits_again(hip, dev):
+    lengths = [5000, 1, 2000, 4000]
+    x, l, dout, initial, dfinal = made(8, "bf16", lengths, 600, span=2000.0)
+    want = run(hip, "bf16", lengths, x, l, dout, initial, dfinal)
+    for _ in range(4):
+        got = run(hip, "bf16", lengths, x, l, dout, initial, dfinal)
+        assert all(torch.equal(got[name], want[name]) for name in want)
+
+
+def test_differences(hip, dev):
+    """dx: the loss is linear in x, so a difference along a direction is the derivative.  dlog_decay: the central difference is
+    off by a sixth of the step squared times the third derivative, for which the oracle's difference of the same step stands."""
+    lengths, channels, step = [90, 200], 24, 2.0 ** -7
+    x, l, dout, initial, dfinal = made(11, "f32", lengths, channels, span=30.0)
+    got = run(hip, "f32", lengths, x, l, dout, initial, dfinal)
+    v = torch.randn(x.shape, generator=torch.Generator().manual_seed(3)).cuda()
+
+    def loss(x, l, initial):
+        r = run(hip, "f32", lengths, x, l, dout, initial, dfinal)
+        return float((r["out"].double() * dout).sum() + (r["final"].double() * dfinal).sum())
+
+    def plain(x, l, initial):
+        w = oracle.recurrence(x, l, lengths, initial)
+        value = float((w["out"][0] * dout.cpu().double()).sum() + (w["final"][0] * dfinal.cpu().double()).sum())
+        return value, float((w["out"][1] * dout.cpu().double().abs()).sum() + (w["final"][1] * dfinal.cpu().double().abs()).sum())
+
+    for name, up, down, direction in (
+            ("dx", (x + step * v, l, initial), (x - step * v, l, initial), (v, x + step * v, x - step * v)),
+            ("dlog_decay", (x, l + step * v, initial), (x, l - step * v, initial), (v, l + step * v, l - step * v)),
+            ("dinitial", (x, l, initial + 1.0), (x, l, initial - 1.0), (None, initial + 1.0, initial - 1.0))):
+        moved = (direction[1].double() - direction[2].double()) / 2
+        along = float((got[name].double() * moved).sum())
+        a, b = plain(*up), plain(*down)
+        measured, exact = (loss(*up) - loss(*down)) / 2, (a[0] - b[0]) / 2
+        assert abs(measured - exact) <= (a[1] + b[1]) / 2, name
+        want = oracle.recurrence(x, l, lengths, initial, dout, dfinal)[name]
+        remainder = abs(exact - float((want[0] * moved.cpu()).sum()))
+        size = float((want[0].abs() * moved.cpu().abs()).sum())
+        assert remainder <= (1e-12 if name != "dlog_decay" else 0.02) * size, name
+        assert abs(along - measured) <= float((want[1] * moved.cpu().abs()).sum()) + (a[1] + b[1]) / 2 + remainder, name
+
+
+def test_graphs_and_streams(hip, dev):
+    """Two graphs that share a workspace, replayed with other inputs between eager calls; and another stream."""
+    lengths, channels = [600, 1, 300], 200
+    offsets = offsets_of(lengths).cuda()
+    x, l, dout, initial, dfinal = made(12, "bf16", lengths, channels)
+    temp = torch.empty(max(16, hip.recurrence_temp_bytes(3, x.shape[0], channels)), dtype=torch.uint8, device=dev)
+    run(hip, "bf16", lengths, x, l, dout, initial, dfinal, temp)
+    out, dx, dl = (torch.empty_like(x) for _ in range(3))
+    final, dinitial = torch.empty_like(initial), torch.empty_like(initial)
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    with torch.cuda.graph(graphs[0]):
+        hip.recurrence("bf16", x, l, offsets, out, initial=initial, final=final, temp=temp)
+    with torch.cuda.graph(graphs[1]):
+        hip.recurrence_backward("bf16", l, out, dout, offsets, dx, dl, initial=initial, dfinal=dfinal, dinitial=dinitial, temp=temp)
+    for turn in range(3):
+        fresh = made(30 + turn, "bf16", lengths, channels)
+        x.copy_(fresh[0])
+        l.copy_(fresh[1])
+        graphs[0].replay()
+        graphs[1].replay()
+        torch.cuda.synchronize()
+        want = run(hip, "bf16", lengths, x, l, dout, initial, dfinal, temp)
+        for name, got in (("out", out), ("final", final), ("dx", dx), ("dlog_decay", dl), ("dinitial", dinitial)):
+            assert torch.equal(got, want[name]), (turn, name)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    other = torch.empty_like(x)
+    hip.recurrence("bf16", x, l, offsets, other, initial=initial, stream=stream)
+    stream.synchronize()
+    assert torch.equal(other, want["out"])
