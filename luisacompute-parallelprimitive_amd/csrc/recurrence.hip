@@ -9,6 +9,8 @@
 #include "../../include/lcpp_hip.h"
 #include "attention.hpp"
 
+#include <initializer_list>
+
 namespace lcpp_hip {
 namespace recurrence {
 namespace {
@@ -72,70 +74,520 @@ __device__ __forceinline__ int64_t state_of(const int32_t* rows, int sequence, i
     return row >= 0 && row < num_states ? row : -1;
 }
 
-constexpr int kWalkBlock = 256;
+// ---- chunks ------------------------------------------------------------------------------------------------------
+// A chunk of a sequence is waves of kRows tokens; a lane has V neighbouring channels of a token, 8 bytes of them where the
+// rows allow.  A chunk's effect on the state is h -> A h + B.  A workgroup reads its chunk into registers once, makes each wave's
+// (A, B) and the chunk's, hands that on, gets the state that enters the chunk, and goes through its rows again with it.  The
+// backward pass does the same towards the sequence's start, with c in the place of h.
+//
+// The state that enters a chunk is made from one that is known, the nearest, by the (A, B) of the chunks in between, in their order:
+// it is the same sum whichever that was, so results do not depend on timing.  A workgroup that has polled for a chunk's (A, B) long
+// enough makes it itself, from the rows: nothing has to run for another to end.
+constexpr int kRows = 16;
+constexpr uint32_t kNotYet = ~0u;  // a NaN that is never handed on
 
-// A thread walks a channel of a sequence.
-template <typename T>
-__global__ __launch_bounds__(kWalkBlock) void recurrence_walk_kernel(Steps x, Steps log_decay, const int32_t* __restrict__ offsets,
-                                                                     const float* initial, const int32_t* __restrict__ rows, Steps out,
-                                                                     float* final, Shape p) {
-    using Item = typename T::Item;
-    const int blocks = (p.channels + kWalkBlock - 1) / kWalkBlock, sequence = static_cast<int>(blockIdx.x / blocks);
-    const int channel = static_cast<int>(blockIdx.x % blocks) * kWalkBlock + static_cast<int>(threadIdx.x);
-    if (channel >= p.channels) return;
-    const Span span = span_of(offsets, sequence, p.tokens);
-    const int64_t row = state_of(rows, sequence, p.num_states);
-    float h = initial != nullptr && row >= 0 ? initial[row * p.channels + channel] : 0.f;
-    for (int64_t t = span.begin; t < span.begin + span.size; ++t) {
-        h = Decay(to_float<T>(log_decay.at<Item>(t)[channel])).step(h, to_float<T>(x.at<Item>(t)[channel]));
-        out.at<Item>(t)[channel] = static_cast<Item>(h);
-    }
-    if (final != nullptr && row >= 0) final[row * p.channels + channel] = h;
+__device__ __forceinline__ uint32_t handed(float x) {
+    const uint32_t bits = __builtin_bit_cast(uint32_t, x);
+    return bits == kNotYet ? 0x7FC00000u : bits;
 }
 
-template <typename T>
-__global__ __launch_bounds__(kWalkBlock) void recurrence_walk_back_kernel(Steps log_decay, Steps out, Steps dout,
-                                                                          const int32_t* __restrict__ offsets,
-                                                                          const float* __restrict__ initial,
-                                                                          const float* __restrict__ dfinal, Steps dx, Steps dlog_decay,
-                                                                          float* __restrict__ dinitial, Shape p) {
-    using Item = typename T::Item;
-    const int blocks = (p.channels + kWalkBlock - 1) / kWalkBlock, sequence = static_cast<int>(blockIdx.x / blocks);
-    const int channel = static_cast<int>(blockIdx.x % blocks) * kWalkBlock + static_cast<int>(threadIdx.x);
-    if (channel >= p.channels) return;
-    const Span span = span_of(offsets, sequence, p.tokens);
-    const int64_t state = static_cast<int64_t>(sequence) * p.channels + channel;
-    float c = dfinal != nullptr ? dfinal[state] : 0.f;
-    for (int64_t t = span.begin + span.size - 1; t >= span.begin; --t) {
-        const float g = to_float<T>(dout.at<Item>(t)[channel]) + c;
-        c = Decay(to_float<T>(log_decay.at<Item>(t)[channel])).times(g);
-        const float before = t > span.begin ? to_float<T>(out.at<Item>(t - 1)[channel]) : initial != nullptr ? initial[state] : 0.f;
-        dx.at<Item>(t)[channel] = static_cast<Item>(g);
-        dlog_decay.at<Item>(t)[channel] = static_cast<Item>(c * before);
+// h -> a h + b.
+struct Effect {
+    float a, b;
+    // This one, then another.
+    __device__ __forceinline__ void then(Effect next) {
+        b = __builtin_fmaf(next.a, b, next.b);
+        a = next.a * a;
     }
-    if (dinitial != nullptr) dinitial[state] = c;
+    // This one, then a row.
+    template <bool BACK>
+    __device__ __forceinline__ void row(float l, float x) {
+        const Decay d(l);
+        b = BACK ? d.times(x + b) : d.step(b, x);
+        a = d.times(a);
+    }
+    __device__ __forceinline__ float of(float h) const { return __builtin_fmaf(a, h, b); }
+};
+
+__device__ __forceinline__ uint64_t handed(Effect e) { return static_cast<uint64_t>(handed(e.b)) << 32 | handed(e.a); }
+
+// What workgroups hand on, a word a channel of a chunk: (A, B), and the state that enters the chunk.
+struct Handed {
+    uint64_t* effects;
+    uint32_t* states;
+    int64_t stride;  // channels, rounded up
+};
+
+template <typename Item, int V>
+struct alignas(sizeof(Item) * V) Items {
+    Item at[V];
+};
+
+struct Inputs {
+    Steps first;  // x, or dout
+    Steps log_decay;
+    Steps out;    // written forwards, read backwards
+    Steps dx, dlog_decay;
+    const int32_t* offsets;
+    const float* initial;
+    const float* dfinal;
+    const int32_t* state_rows;
+    float* last;  // final, or dinitial
+};
+
+// Rows [token, token + count) of an array as a wave reads and writes them: what lies past them, or is asked for at kNowhere, reads
+// as zeros and is not written.  (Offsets are below 2^31, as strides are below 2^26 bytes.)
+constexpr uint32_t kNowhere = 0x7FFFFFFF;
+
+template <typename Vec>
+struct Window {
+    __amdgpu_buffer_rsrc_t rows;
+    uint32_t token_bytes;
+    __device__ __forceinline__ Window(const Steps& s, int64_t token, int count, int row_bytes)
+        : rows(__builtin_amdgcn_make_buffer_rsrc(s.data + token * s.token_bytes, 0,
+                                                 count > 0 ? (count - 1) * static_cast<int>(s.token_bytes) + row_bytes : 0, 0x00020000)),
+          token_bytes(static_cast<uint32_t>(s.token_bytes)) {}
+    __device__ __forceinline__ Vec load(int row, uint32_t at) const {
+        const int offset = static_cast<int>(at + row * token_bytes);
+        if constexpr (sizeof(Vec) == 8) return __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b64(rows, offset, 0, 0));
+        else if constexpr (sizeof(Vec) == 4) return __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b32(rows, offset, 0, 0));
+        else return __builtin_bit_cast(Vec, __builtin_amdgcn_raw_buffer_load_b16(rows, offset, 0, 0));
+    }
+    __device__ __forceinline__ void store(int row, uint32_t at, Vec x) const {
+        const int offset = static_cast<int>(at + row * token_bytes);
+        if constexpr (sizeof(Vec) == 8) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(attention::U32x2, x), rows, offset, 0, 0);
+        else if constexpr (sizeof(Vec) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), rows, offset, 0, 0);
+        else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, x), rows, offset, 0, 0);
+    }
+};
+
+// A wave's rows of its channels; zeros, which are what is not there, leave a state as it is.
+template <typename T, int V, bool BACK>
+struct WaveRows {
+    using Vec = Items<typename T::Item, V>;
+    Vec x[kRows], l[kRows];
+    __device__ __forceinline__ void load(const Window<Vec>& first, const Window<Vec>& log_decay, uint32_t at) {
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            x[r] = first.load(r, at);
+            l[r] = log_decay.load(r, at);
+        }
+    }
+    // Forgets what is known of the rows, so that nothing made of them for their effect is kept for the second time through them.
+    __device__ __forceinline__ void forget() {
+        using Word = std::conditional_t<sizeof(Vec) == 8, attention::U32x2, std::conditional_t<sizeof(Vec) == 4, uint32_t, uint16_t>>;
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            Word a = __builtin_bit_cast(Word, x[r]), b = __builtin_bit_cast(Word, l[r]);
+            asm volatile("" : "+v"(a), "+v"(b));
+            x[r] = __builtin_bit_cast(Vec, a);
+            l[r] = __builtin_bit_cast(Vec, b);
+        }
+    }
+    __device__ __forceinline__ void effect(Effect (&e)[V], int count) const {
+#pragma unroll
+        for (int v = 0; v < V; ++v) e[v] = {1.f, 0.f};
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int r = BACK ? kRows - 1 - i : i;
+            if (r < count)
+#pragma unroll
+                for (int v = 0; v < V; ++v) e[v].template row<BACK>(to_float<T>(l[r].at[v]), to_float<T>(x[r].at[v]));
+            __builtin_amdgcn_sched_barrier(0);  // (a row at a time: all decays at once would take the registers)
+        }
+    }
+};
+
+// A chunk's place: chunk `index` of its sequence's, tokens [token, token + count).
+struct Chunk {
+    int sequence, index, chunks;
+    int64_t begin;  // of the sequence
+    int64_t size;
+    template <int WAVES>
+    __device__ __forceinline__ bool find(const int32_t* offsets, const Shape& p, int number) {
+        constexpr int kChunk = WAVES * kRows;
+        const attention::TilePlace place = attention::find_tile(offsets, p.sequences, 1, kChunk, number);
+        if (place.sequence < 0) return false;
+        const Span span = span_of(offsets, place.sequence, p.tokens);
+        sequence = place.sequence;
+        index = place.tile;
+        begin = span.begin;
+        size = span.size;
+        chunks = static_cast<int>((span.size + kChunk - 1) / kChunk);
+        return index < chunks || (index == 0 && size == 0);
+    }
+};
+
+// What the owner of a chunk makes of it, the same way, for a channel.
+template <typename T, bool BACK, int WAVES>
+__device__ __forceinline__ Effect effect_of_chunk(const Inputs& in, int64_t token, int count, int channel) {
+    using Item = typename T::Item;
+    Effect all = {1.f, 0.f};
+#pragma unroll 1
+    for (int i = 0; i < WAVES; ++i) {
+        const int w = BACK ? WAVES - 1 - i : i, rows = count - w * kRows < kRows ? count - w * kRows : kRows;
+        Effect part = {1.f, 0.f};
+#pragma unroll 1
+        for (int k = 0; k < rows; ++k) {
+            const int64_t t = token + w * kRows + (BACK ? rows - 1 - k : k);
+            part.row<BACK>(to_float<T>(in.log_decay.template at<Item>(t)[channel]), to_float<T>(in.first.template at<Item>(t)[channel]));
+        }
+        all.then(part);
+    }
+    return all;
+}
+
+// The state that enters chunk `number`, `before` chunks after the sequence's first one (the last one, backwards); a channel a lane.
+template <typename T, bool BACK, int WAVES>
+__device__ __forceinline__ float look_back(const Inputs& in, const Handed& h, const Chunk& chunk, int64_t number, int before, int channel,
+                                           bool active, uint32_t patience) {
+    constexpr int kChunk = WAVES * kRows, kAtOnce = 4;
+    const int64_t step = BACK ? h.stride : -h.stride;  // to the chunk before
+    const uint32_t* states = h.states + number * h.stride;
+    const uint64_t* effects = h.effects + number * h.stride;
+    const uint32_t lane_at = active ? channel : 0;
+    // The nearest known state: of the chunk itself (0), or `back` before it.  (The first chunk's is there from the start.)
+    int back = 0;
+    uint32_t state = kNotYet;
+    for (bool found = false; !found;) {
+        uint32_t words[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) words[i] = atomic_load_agent(states + (back + i < before ? back + i : before) * step + lane_at);
+        int nearest = before;
+#pragma unroll
+        for (int i = kAtOnce - 1; i >= 0; --i) {
+            if (wave_ballot(active && words[i] == kNotYet) == 0) {
+                found = true;
+                nearest = back + i < before ? back + i : before;
+                state = words[i];
+            }
+        }
+        back = found ? nearest : back + kAtOnce < before ? back + kAtOnce : before;
+    }
+    float value = __builtin_bit_cast(float, state);
+    // Then the chunks in between, as they come.
+    for (; back > 0; back -= kAtOnce) {
+        uint64_t words[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) words[i] = atomic_load_agent(effects + (back - i > 1 ? back - i : 1) * step + lane_at);
+#pragma unroll
+        for (int i = 0; i < kAtOnce; ++i) {
+            const int at = back - i;
+            if (at < 1) continue;
+            for (uint32_t polls = 0; wave_ballot(active && words[i] == ~uint64_t{0}) != 0; ++polls) {
+                if (polls < patience) {
+                    __builtin_amdgcn_s_sleep(1);
+                    words[i] = atomic_load_agent(effects + at * step + lane_at);
+                    continue;
+                }
+                const int64_t row0 = static_cast<int64_t>(BACK ? chunk.index + at : chunk.index - at) * kChunk;
+                const int count = chunk.size - row0 < kChunk ? static_cast<int>(chunk.size - row0) : kChunk;
+                words[i] = handed(effect_of_chunk<T, BACK, WAVES>(in, chunk.begin + row0, count, active ? channel : 0));
+                break;
+            }
+            const Effect e = {__builtin_bit_cast(float, static_cast<uint32_t>(words[i])),
+                              __builtin_bit_cast(float, static_cast<uint32_t>(words[i] >> 32))};
+            value = e.of(value);
+        }
+    }
+    return value;
+}
+
+// Steps of serving: a lane walks its channels through a sequence of a token or two, kWalkRows at a time.
+constexpr int kWalkRows = 4;
+
+template <typename T, int V, bool BACK>
+__global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape p, int blocks) {
+    using Item = typename T::Item;
+    using Vec = Items<Item, V>;
+    const int sequence = static_cast<int>(blockIdx.x / blocks);
+    const int channel = (static_cast<int>(blockIdx.x % blocks) * kWave + static_cast<int>(threadIdx.x)) * V;
+    if (channel >= p.channels) return;
+    const Span span = span_of(in.offsets, sequence, p.tokens);
+    const int64_t held = BACK ? sequence : state_of(in.state_rows, sequence, p.num_states);
+    const float* from = BACK ? in.dfinal : in.initial;
+    float state[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) state[v] = from != nullptr && held >= 0 ? from[held * p.channels + channel + v] : 0.f;
+    const auto row = [&](const Steps& s, int64_t t) { return reinterpret_cast<Vec*>(s.template at<Item>(t) + channel); };
+    for (int64_t done = 0; done < span.size; done += kWalkRows) {
+        Vec x[kWalkRows], l[kWalkRows], h[kWalkRows];
+#pragma unroll
+        for (int i = 0; i < kWalkRows; ++i) {
+            if (done + i >= span.size) continue;
+            const int64_t t = BACK ? span.begin + span.size - 1 - done - i : span.begin + done + i;
+            x[i] = *row(in.first, t);
+            l[i] = *row(in.log_decay, t);
+            if (BACK && t > span.begin) h[i] = *row(in.out, t - 1);
+        }
+#pragma unroll
+        for (int i = 0; i < kWalkRows; ++i) {
+            if (done + i >= span.size) continue;
+            const int64_t t = BACK ? span.begin + span.size - 1 - done - i : span.begin + done + i;
+            Vec a, b;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const Decay d(to_float<T>(l[i].at[v]));
+                const float input = to_float<T>(x[i].at[v]);
+                if constexpr (BACK) {
+                    const float g = input + state[v];
+                    state[v] = d.times(g);
+                    const float before = t > span.begin ? to_float<T>(h[i].at[v])
+                                         : in.initial != nullptr ? in.initial[held * p.channels + channel + v] : 0.f;
+                    a.at[v] = static_cast<Item>(g);
+                    b.at[v] = static_cast<Item>(state[v] * before);
+                } else {
+                    state[v] = d.step(state[v], input);
+                    a.at[v] = static_cast<Item>(state[v]);
+                }
+            }
+            *row(BACK ? in.dx : in.out, t) = a;
+            if constexpr (BACK) *row(in.dlog_decay, t) = b;
+        }
+    }
+    if (in.last == nullptr || held < 0) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) in.last[held * p.channels + channel + v] = state[v];
+}
+
+// Before the chunks: no effect is there, and of the states that of each sequence's first chunk (the last one, backwards).
+constexpr int kClearBlock = 256;
+
+template <bool BACK, int WAVES>
+__global__ __launch_bounds__(kClearBlock) void recurrence_clear_kernel(Inputs in, Handed h, Shape p, int blocks) {
+    const int number = static_cast<int>(blockIdx.x / blocks);
+    const int channel = static_cast<int>(blockIdx.x % blocks) * kClearBlock + static_cast<int>(threadIdx.x);
+    Chunk chunk;
+    const bool there = chunk.find<WAVES>(in.offsets, p, number);
+    if (!there || channel >= p.channels) return;
+    uint32_t state = kNotYet;
+    if (chunk.index == (BACK ? chunk.chunks - 1 : 0)) {
+        if constexpr (BACK) {
+            state = in.dfinal != nullptr ? handed(in.dfinal[static_cast<int64_t>(chunk.sequence) * p.channels + channel]) : 0u;
+        } else {
+            const int64_t row = state_of(in.state_rows, chunk.sequence, p.num_states);
+            state = in.initial != nullptr && row >= 0 ? handed(in.initial[row * p.channels + channel]) : 0u;
+        }
+    }
+    h.states[number * h.stride + channel] = state;
+    h.effects[number * h.stride + channel] = ~uint64_t{0};
+}
+
+template <typename T, int V, bool BACK, int WAVES>
+__global__ __launch_bounds__(WAVES * kWave, 4) void recurrence_kernel(Inputs in, Handed h, Shape p, int numbers, int blocks, uint32_t patience) {
+    using Item = typename T::Item;
+    using Vec = Items<Item, V>;
+    constexpr int kChunk = WAVES * kRows, kTile = kWave * V;
+    __shared__ __attribute__((aligned(16))) Effect parts[WAVES][kTile];
+    __shared__ __attribute__((aligned(16))) float entering[kTile];
+    // Chunks in the order that states go through them, all channels of one together.
+    const int ordinal = static_cast<int>(blockIdx.x / blocks), number = BACK ? numbers - 1 - ordinal : ordinal;
+    Chunk chunk;
+    if (!chunk.find<WAVES>(in.offsets, p, number)) return;
+    const int lane = threadIdx.x % kWave, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int own = (static_cast<int>(blockIdx.x % blocks) * kWave + lane) * V;
+    const bool active = own < p.channels;
+    const int64_t row0 = static_cast<int64_t>(chunk.index) * kChunk;
+    const int count = chunk.size - row0 < kChunk ? static_cast<int>(chunk.size - row0) : kChunk;
+    const int mine = count - wave * kRows;  // rows of this wave, if it has some
+    const int64_t token = chunk.begin + row0 + wave * kRows;
+    const int before = BACK ? chunk.chunks - 1 - chunk.index : chunk.index, after = chunk.chunks - 1 - before;
+    const bool alone = chunk.chunks <= 1;
+
+    WaveRows<T, V, BACK> rows;
+    const int row_bytes = p.channels * static_cast<int>(sizeof(Item)), some = mine < kRows ? mine : kRows;
+    const uint32_t at = active ? static_cast<uint32_t>(own) * sizeof(Item) : kNowhere;
+    rows.load(Window<Vec>(in.first, token, some, row_bytes), Window<Vec>(in.log_decay, token, some, row_bytes), at);
+    if (!alone || WAVES > 1) {
+        Effect effect[V];
+        rows.effect(effect, mine);
+#pragma unroll
+        for (int v = 0; v < V; ++v) parts[wave][lane * V + v] = effect[v];
+    }
+    // Backwards: the states before each token, as they were stored.
+    Vec stored[BACK ? kRows : 1];
+    if constexpr (BACK) {
+        // (The window begins a row before the wave's, or where the sequence does: then it is read a row late.)
+        const int late = token == chunk.begin;
+        const Window<Vec> out(in.out, token - 1 + late, some - late, row_bytes);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r)
+            if (r >= late) stored[r] = out.load(r - late, at);
+    }
+    // The states that enter the chunk, 64 channels a wave.
+    const int64_t held = BACK ? chunk.sequence : state_of(in.state_rows, chunk.sequence, p.num_states);
+    if constexpr (WAVES > 1) __syncthreads();
+    else wave_lds_order();
+    for (int group = wave; group < V; group += WAVES) {
+        const int at = group * kWave + lane, target = own - lane * V + at;
+        const bool there = target < p.channels;
+        float state = 0.f;
+        if (alone) {
+            const float* from = BACK ? in.dfinal : in.initial;
+            if (from != nullptr && held >= 0 && there) state = from[held * p.channels + target];
+        } else {
+            Effect all = {1.f, 0.f};
+#pragma unroll
+            for (int w = 0; w < WAVES; ++w) all.then(parts[BACK ? WAVES - 1 - w : w][at]);
+            if (after > 0 && there) atomic_store_agent(h.effects + number * h.stride + target, handed(all));
+            state = look_back<T, BACK, WAVES>(in, h, chunk, number, before, target, there, patience);
+            if (after > 0 && there) atomic_store_agent(h.states + (BACK ? number - 1 : number + 1) * h.stride + target, handed(all.of(state)));
+        }
+        entering[at] = state;
+    }
+    if constexpr (WAVES > 1) __syncthreads();
+    else wave_lds_order();
+    float state[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        state[v] = entering[lane * V + v];
+        if constexpr (BACK) {
+            for (int w = WAVES - 1; w > wave; --w) state[v] = parts[w][lane * V + v].of(state[v]);
+        } else {
+            for (int w = 0; w < wave; ++w) state[v] = parts[w][lane * V + v].of(state[v]);
+        }
+    }
+    rows.forget();
+    if constexpr (BACK) {
+        const Window<Vec> dx(in.dx, token, some, row_bytes), dlog_decay(in.dlog_decay, token, some, row_bytes);
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+            const int r = kRows - 1 - i;
+            __builtin_amdgcn_sched_barrier(0);
+            if (r >= mine) continue;
+            Vec g_row, l_row;
+            const bool first = r == 0 && token == chunk.begin;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                const float g = to_float<T>(rows.x[r].at[v]) + state[v];
+                state[v] = Decay(to_float<T>(rows.l[r].at[v])).times(g);
+                float h = to_float<T>(stored[r].at[v]);
+                if (first) h = in.initial != nullptr && active ? in.initial[static_cast<int64_t>(chunk.sequence) * p.channels + own + v] : 0.f;
+                g_row.at[v] = static_cast<Item>(g);
+                l_row.at[v] = static_cast<Item>(state[v] * h);
+            }
+            dx.store(r, at, g_row);
+            dlog_decay.store(r, at, l_row);
+        }
+    } else {
+        const Window<Vec> out(in.out, token, some, row_bytes);
+#pragma unroll
+        for (int r = 0; r < kRows; ++r) {
+            __builtin_amdgcn_sched_barrier(0);
+            if (r >= mine) continue;
+            Vec row;
+#pragma unroll
+            for (int v = 0; v < V; ++v) {
+                state[v] = Decay(to_float<T>(rows.l[r].at[v])).step(state[v], to_float<T>(rows.x[r].at[v]));
+                row.at[v] = static_cast<Item>(state[v]);
+            }
+            out.store(r, at, row);
+        }
+    }
+    // The last state: forwards of the wave that has the sequence's last token, backwards of the first.
+    const bool ends = BACK ? chunk.index == 0 && wave == 0 : after <= 0 && (count == 0 ? wave == 0 : (count - 1) / kRows == wave);
+    if (!ends || !active || in.last == nullptr) return;
+    if (held < 0) return;
+#pragma unroll
+    for (int v = 0; v < V; ++v) in.last[held * p.channels + own + v] = state[v];
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
+// (A wave's rows lie within 2^30 bytes.)
+constexpr int64_t kMostStride = int64_t{1} << 24;
+
+// Waves of a chunk: one while sequences have no more than a wave's rows on average, else eight.
+constexpr int kLongWaves = 8;
+bool short_sequences(uint64_t sequences, uint64_t tokens) { return tokens <= sequences * kRows; }
+
+// Steps of serving, a token or two a sequence, are walked: no chunk hands anything on, and there is one launch.
+bool walked(uint64_t sequences, uint64_t tokens) { return tokens <= sequences * 2; }
+
+uint64_t numbers_of(uint64_t sequences, uint64_t tokens) {
+    return tokens / (short_sequences(sequences, tokens) ? kRows : kRows * kLongWaves) + sequences;
+}
+// No sequence has two chunks where all tokens fit one.
+bool handing(uint64_t sequences, uint64_t tokens) {
+    return !walked(sequences, tokens) && tokens > static_cast<uint64_t>(short_sequences(sequences, tokens) ? kRows : kRows * kLongWaves);
+}
+uint64_t stride_of(uint64_t channels) { return align_up(channels, 64); }
+size_t effects_bytes(uint64_t sequences, uint64_t tokens, uint64_t channels) {
+    return align_up(numbers_of(sequences, tokens) * stride_of(channels) * sizeof(uint64_t), kViewAlign);
+}
+size_t needed_bytes(uint64_t sequences, uint64_t tokens, uint64_t channels) {
+    if (sequences == 0 || !handing(sequences, tokens)) return 0;
+    return effects_bytes(sequences, tokens, channels) +
+           align_up(numbers_of(sequences, tokens) * stride_of(channels) * sizeof(uint32_t), kViewAlign);
+}
+
 template <typename T>
 bool usable(const lcpp_hip_steps* s, uint32_t channels) {
     return s != nullptr && s->data != nullptr && reinterpret_cast<uintptr_t>(s->data) % sizeof(typename T::Item) == 0 &&
-           s->token_stride >= static_cast<int64_t>(channels) && s->token_stride <= (int64_t{1} << 40);
+           s->token_stride >= static_cast<int64_t>(channels) && s->token_stride < kMostStride;
 }
 template <typename T>
 Steps steps_of(const lcpp_hip_steps* s) {
     return {static_cast<char*>(s->data), s->token_stride * static_cast<int64_t>(sizeof(typename T::Item))};
 }
 int unusable(const char* what) {
-    return set_error(kInvalidArgument, "%s: rows must be there and aligned to their items, at least their channels apart", what);
+    return set_error(kInvalidArgument, "%s: rows must be there and aligned to their items, at least their channels apart and less than 2^24 items", what);
 }
 
 int check_sizes(const char* what, uint32_t sequences, uint64_t tokens, uint32_t channels) {
-    if (channels == 0 || channels > 0x7FFFFFFu) return set_error(kInvalidArgument, "%s: no channels, or too many", what);
-    if (ceil_div(channels, kWalkBlock) * sequences > 0x7FFFFFFFull / kWalkBlock)
-        return set_error(kInvalidArgument, "%s: too many sequences of so many channels", what);
+    if (channels == 0 || channels >= kMostStride) return set_error(kInvalidArgument, "%s: no channels, or too many", what);
     if (tokens > 0x7FFFFFFFull) return set_error(kInvalidArgument, "%s: too many tokens", what);
+    if (sequences > 0x7FFFFFFu || numbers_of(sequences, tokens) * ceil_div(channels, kWave) > 0x7FFFFFFFull / (kLongWaves * kWave))
+        return set_error(kInvalidArgument, "%s: too many sequences, tokens and channels", what);
     return kOk;
+}
+
+// Channels a lane: the most, up to 8 bytes of them, that divide the channels and that all rows are aligned to.
+template <typename T>
+int width_of(uint32_t channels, std::initializer_list<const lcpp_hip_steps*> rows) {
+    uint64_t bits = channels;
+    for (const lcpp_hip_steps* r : rows)
+        bits |= static_cast<uint64_t>(r->token_stride) | reinterpret_cast<uintptr_t>(r->data) / sizeof(typename T::Item);
+    constexpr int kMost = 8 / static_cast<int>(sizeof(typename T::Item));
+    return bits % kMost == 0 ? kMost : bits % 2 == 0 ? 2 : 1;
+}
+
+template <typename T, int V, bool BACK, int WAVES>
+int run(const char* what, const Inputs& in, const Handed& h, const Shape& p, bool hands, hipStream_t stream) {
+    const int numbers = static_cast<int>(numbers_of(p.sequences, p.tokens));
+    if (walked(p.sequences, p.tokens)) {
+        LaunchScope scope(what, stream);
+        const int blocks = static_cast<int>(ceil_div(p.channels, kWave * V));
+        recurrence_walk_kernel<T, V, BACK><<<static_cast<unsigned>(p.sequences * blocks), kWave, 0, stream>>>(in, p, blocks);
+        return check_hip(hipGetLastError(), what);
+    }
+    if (hands) {
+        LaunchScope scope(BACK ? "recurrence_backward_clear" : "recurrence_clear", stream);
+        const int blocks = static_cast<int>(ceil_div(p.channels, kClearBlock));
+        recurrence_clear_kernel<BACK, WAVES><<<static_cast<unsigned>(numbers * blocks), kClearBlock, 0, stream>>>(in, h, p, blocks);
+        if (int st = check_hip(hipGetLastError(), what); st != kOk) return st;
+    }
+    LaunchScope scope(what, stream);
+    const int blocks = static_cast<int>(ceil_div(p.channels, kWave * V));
+    recurrence_kernel<T, V, BACK, WAVES><<<static_cast<unsigned>(numbers * blocks), WAVES * kWave, 0, stream>>>(in, h, p, numbers, blocks,
+                                                                                                                lookback_spin_limit());
+    return check_hip(hipGetLastError(), what);
+}
+
+template <typename T, bool BACK>
+int launch(const char* what, void* temp, size_t temp_bytes, const Inputs& in, const Shape& p, int width, hipStream_t stream) {
+    const size_t needed = needed_bytes(p.sequences, p.tokens, p.channels);
+    if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
+    Handed h{static_cast<uint64_t*>(temp), nullptr, static_cast<int64_t>(stride_of(p.channels))};
+    if (needed) h.states = reinterpret_cast<uint32_t*>(static_cast<char*>(temp) + effects_bytes(p.sequences, p.tokens, p.channels));
+    const bool few = short_sequences(p.sequences, p.tokens);
+    const auto choose = [&](auto v) {
+        constexpr int kWide = decltype(v)::value;
+        return few ? run<T, kWide, BACK, 1>(what, in, h, p, needed != 0, stream)
+                   : run<T, kWide, BACK, kLongWaves>(what, in, h, p, needed != 0, stream);
+    };
+    if constexpr (sizeof(typename T::Item) == 2)
+        if (width == 4) return choose(std::integral_constant<int, 4>{});
+    return width == 2 ? choose(std::integral_constant<int, 2>{}) : choose(std::integral_constant<int, 1>{});
 }
 
 template <typename T>
@@ -143,19 +595,20 @@ int forward(void* temp, size_t temp_bytes, const lcpp_hip_steps* x, const lcpp_h
             const float* initial, const int32_t* state_rows, uint32_t num_states, const lcpp_hip_steps* out, float* final_states,
             uint32_t sequences, uint64_t tokens, uint32_t channels, void* stream_ptr) {
     const char* what = "recurrence";
-    hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     if (int st = check_sizes(what, sequences, tokens, channels); st != kOk) return st;
     if (num_states > 0x7FFFFFFFu) return set_error(kInvalidArgument, "%s: too many states", what);
     if (sequences == 0) return kOk;
     if (!offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
     if (tokens && (!usable<T>(x, channels) || !usable<T>(log_decay, channels) || !usable<T>(out, channels))) return unusable(what);
-    const size_t needed = lcpp_hip_recurrence_temp_bytes(sequences, tokens, channels);
-    if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
     const Shape p{static_cast<int>(sequences), static_cast<int64_t>(tokens), static_cast<int>(channels), static_cast<int>(num_states)};
-    LaunchScope scope(what, stream);
-    recurrence_walk_kernel<T><<<static_cast<unsigned>(ceil_div(channels, kWalkBlock) * sequences), kWalkBlock, 0, stream>>>(
-        steps_of<T>(x), steps_of<T>(log_decay), offsets, initial, state_rows, steps_of<T>(out), final_states, p);
-    return check_hip(hipGetLastError(), "recurrence launch");
+    Inputs in{};
+    if (tokens) in = {steps_of<T>(x), steps_of<T>(log_decay), steps_of<T>(out)};
+    in.offsets = offsets;
+    in.initial = initial;
+    in.state_rows = state_rows;
+    in.last = final_states;
+    const int width = tokens ? width_of<T>(channels, {x, log_decay, out}) : 1;
+    return launch<T, false>(what, temp, temp_bytes, in, p, width, static_cast<hipStream_t>(stream_ptr));
 }
 
 template <typename T>
@@ -163,21 +616,21 @@ int backward(void* temp, size_t temp_bytes, const lcpp_hip_steps* log_decay, con
              const int32_t* offsets, const float* initial, const float* dfinal, const lcpp_hip_steps* dx,
              const lcpp_hip_steps* dlog_decay, float* dinitial, uint32_t sequences, uint64_t tokens, uint32_t channels, void* stream_ptr) {
     const char* what = "recurrence_backward";
-    hipStream_t stream = static_cast<hipStream_t>(stream_ptr);
     if (int st = check_sizes(what, sequences, tokens, channels); st != kOk) return st;
     if (sequences == 0) return kOk;
     if (!offsets) return set_error(kInvalidArgument, "%s: null offsets", what);
     if (tokens && (!usable<T>(log_decay, channels) || !usable<T>(out, channels) || !usable<T>(dout, channels) ||
                    !usable<T>(dx, channels) || !usable<T>(dlog_decay, channels)))
         return unusable(what);
-    const size_t needed = lcpp_hip_recurrence_temp_bytes(sequences, tokens, channels);
-    if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
     const Shape p{static_cast<int>(sequences), static_cast<int64_t>(tokens), static_cast<int>(channels), static_cast<int>(sequences)};
-    LaunchScope scope(what, stream);
-    recurrence_walk_back_kernel<T><<<static_cast<unsigned>(ceil_div(channels, kWalkBlock) * sequences), kWalkBlock, 0, stream>>>(
-        steps_of<T>(log_decay), steps_of<T>(out), steps_of<T>(dout), offsets, initial, dfinal, steps_of<T>(dx), steps_of<T>(dlog_decay),
-        dinitial, p);
-    return check_hip(hipGetLastError(), "recurrence_backward launch");
+    Inputs in{};
+    if (tokens) in = {steps_of<T>(dout), steps_of<T>(log_decay), steps_of<T>(out), steps_of<T>(dx), steps_of<T>(dlog_decay)};
+    in.offsets = offsets;
+    in.initial = initial;
+    in.dfinal = dfinal;
+    in.last = dinitial;
+    const int width = tokens ? width_of<T>(channels, {log_decay, out, dout, dx, dlog_decay}) : 1;
+    return launch<T, true>(what, temp, temp_bytes, in, p, width, static_cast<hipStream_t>(stream_ptr));
 }
 
 }  // namespace
@@ -188,7 +641,9 @@ using namespace lcpp_hip;
 
 extern "C" {
 
-size_t lcpp_hip_recurrence_temp_bytes(uint32_t, uint64_t, uint32_t) { return 0; }
+size_t lcpp_hip_recurrence_temp_bytes(uint32_t sequences, uint64_t tokens, uint32_t channels) {
+    return recurrence::needed_bytes(sequences, tokens, channels);
+}
 
 #define LCPP_HIP_DEFINE_RECURRENCE(S, T)                                                                                      \
     int lcpp_hip_recurrence_##S(void* temp, size_t temp_bytes, const lcpp_hip_steps* x, const lcpp_hip_steps* log_decay,      \
