@@ -40,18 +40,19 @@ __device__ __forceinline__ int64_t cells_of(int64_t length, const Release& p) {
 }
 
 // Exclusive sums over a workgroup's threads, and the sum of all.
+template <typename T, int WAVES>
 struct BlockScan {
-    int64_t sums[kEvictWaves];
-    __device__ __forceinline__ int64_t run(int64_t x, int64_t& all) {
+    T sums[WAVES];
+    __device__ __forceinline__ T run(T x, T& all) {
         const int wave = threadIdx.x / kWave;
-        const int64_t inclusive = wave_inclusive_scan(x, SumOp{});
+        const T inclusive = wave_inclusive_scan(x, SumOp{});
         __syncthreads();
         if (threadIdx.x % kWave == kWave - 1) sums[wave] = inclusive;
         __syncthreads();
-        int64_t before = 0;
+        T before = 0;
         all = 0;
 #pragma unroll
-        for (int w = 0; w < kEvictWaves; ++w) {
+        for (int w = 0; w < WAVES; ++w) {
             before += w < wave ? sums[w] : 0;
             all += sums[w];
         }
@@ -67,7 +68,7 @@ __global__ __launch_bounds__(kEvictBlock) void page_release_kernel(const int32_t
                                                                    int32_t* __restrict__ released, int32_t* __restrict__ counts,
                                                                    Release p) {
     constexpr int kCells = 4;
-    __shared__ BlockScan scan;
+    __shared__ BlockScan<int64_t, kEvictWaves> scan;
     __shared__ int64_t begins[kEvictBlock];
     __shared__ int32_t first_cells[kEvictBlock];
     int64_t given = 0, all_kept = 0;
@@ -171,81 +172,163 @@ struct Keys {
     }
 };
 
-// A workgroup a request.  Wave w has the keys [w per, (w + 1) per), so that counts of the waves before give a key its rank.
+// A request's lengths.
+struct Lengths {
+    int n, keep;
+    int64_t late;  // positions from here on are protected
+    __device__ __forceinline__ Lengths(const int32_t* kv_lengths, const int32_t* kept_lengths, const int32_t* shifts, int request,
+                                       const Evict& p) {
+        const int64_t length = at_least_0(kv_lengths[request]), asked = at_least_0(kept_lengths[request]);
+        const int64_t room = static_cast<int64_t>(p.table_width) * p.page_size.by;
+        n = static_cast<int>(length < room ? length : room);
+        keep = static_cast<int>(asked < n ? asked : n);
+        late = p.recent ? (shifts != nullptr ? shifts[request] : 0) + length - p.recent : INT64_MAX;
+    }
+    __device__ __forceinline__ bool as_it_is() const { return keep == 0 || keep == n; }
+};
+
+// Radix selection: 11, 11 and 10 bits of the orders, the highest first.  (11 bits of a float reach into its fraction, so that
+// sums of like size spread over the bins.)
+constexpr int kDigits = 3;
+constexpr int kBins = 2048;
+constexpr int kShifts[kDigits] = {21, 10, 0};
+
+// What a digit's counts say: the bin that holds the need-th largest, and which of the bin's it is.
+template <int WAVES>
+struct Chooser {
+    BlockScan<uint32_t, WAVES> scan;
+    uint32_t bin, need;
+    __device__ __forceinline__ void run(const uint32_t* bins, uint32_t wanted) {
+        constexpr int kEach = kBins / (WAVES * kWave);
+        uint32_t own[kEach], sum = 0, all;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) sum += own[i] = bins[kBins - 1 - (threadIdx.x * kEach + i)];
+        uint32_t before = scan.run(sum, all);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            if (before < wanted && wanted <= before + own[i]) {
+                bin = kBins - 1 - (threadIdx.x * kEach + i);
+                need = wanted - before;
+            }
+            before += own[i];
+        }
+        __syncthreads();
+    }
+};
+
+// Of a wave's keys in order: which stay, with `tie` of the threshold's equals before them, and what moves.
+struct Sorted {
+    uint32_t threshold, need;
+    int keep, tie;
+    __device__ __forceinline__ void next(int j, bool there, uint32_t order, bool& mover, bool& hole) {
+        const uint64_t equal = wave_ballot(there && order == threshold);
+        const bool stays = order > threshold || (order == threshold && tie + static_cast<int>(popc_lanes_below(equal)) < static_cast<int>(need));
+        tie += __popcll(equal);
+        mover = there && stays && j >= keep;
+        hole = there && !stays && j < keep;
+    }
+};
+
+// A wave's keys [begin, end): ITEMS of a lane's orders stay in registers, a longer run is read again each time.
+template <int ITEMS>
+struct Run {
+    int begin, end;
+    bool held;
+    uint32_t orders[ITEMS];
+    __device__ __forceinline__ Run(const Keys& keys, int first, int last) : begin(first), end(last), held(last - first <= ITEMS * kWave) {
+        if (!held) return;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int j = begin + i * kWave + static_cast<int>(threadIdx.x % kWave);
+            orders[i] = j < end ? keys.order(j) : 0u;
+        }
+    }
+    // 64 keys at a time: f(index, whether there is one, order).
+    template <typename F>
+    __device__ __forceinline__ void each(const Keys& keys, F f) const {
+        const int lane = threadIdx.x % kWave;
+        if (held) {
+#pragma unroll
+            for (int i = 0; i < ITEMS; ++i)
+                if (begin + i * kWave < end) f(begin + i * kWave + lane, begin + i * kWave + lane < end, orders[i]);
+        } else {
+            for (int j = begin + lane; j - lane < end; j += kWave) f(j, j < end, j < end ? keys.order(j) : 0u);
+        }
+    }
+};
+
+// Slots of movers and holes, each from its own number on.
+struct Emitter {
+    int64_t* from;
+    int64_t* to;
+    int64_t mover_at, hole_at;
+    __device__ __forceinline__ void put(const Keys& keys, int64_t width, int j, bool mover, bool hole) {
+        const uint64_t moving = wave_ballot(mover), open = wave_ballot(hole);
+        if (mover) {
+            const int64_t at = mover_at + popc_lanes_below(moving);
+            if (at < width) from[at] = keys.slot(j);
+        }
+        if (hole) {
+            const int64_t at = hole_at + popc_lanes_below(open);
+            if (at < width) to[at] = keys.slot(j);
+        }
+        mover_at += __popcll(moving);
+        hole_at += __popcll(open);
+    }
+};
+
+// A workgroup a request.  Wave w has the keys [w per, (w + 1) per), so that counts of the waves before give a key its rank.  ITEMS
+// of a lane's orders stay in registers; a request that has more is read again each time.
+template <int ITEMS>
 __global__ __launch_bounds__(kEvictBlock) void evict_plan_kernel(const float* __restrict__ weights, const int32_t* __restrict__ positions,
                                                                  const int32_t* __restrict__ block_table,
                                                                  const int32_t* __restrict__ kv_lengths,
                                                                  const int32_t* __restrict__ kept_lengths,
                                                                  const int32_t* __restrict__ shifts, int64_t* __restrict__ move_from,
                                                                  int64_t* __restrict__ move_to, Evict p) {
-    __shared__ uint32_t bins[256];
-    __shared__ uint32_t chosen, wanted;
+    __shared__ uint32_t bins[kBins];
+    __shared__ Chooser<kEvictWaves> chooser;
     __shared__ int32_t tie_sums[kEvictWaves], mover_sums[kEvictWaves], hole_sums[kEvictWaves];
     const int request = blockIdx.x, lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
-    const int64_t length = at_least_0(kv_lengths[request]);
-    const int64_t room = static_cast<int64_t>(p.table_width) * p.page_size.by;
-    const int n = static_cast<int>(length < room ? length : room);
-    const int64_t asked = at_least_0(kept_lengths[request]);
-    const int keep = static_cast<int>(asked < n ? asked : n);
+    const Lengths lengths(kv_lengths, kept_lengths, shifts, request, p);
+    const int n = lengths.n;
     int64_t* from = move_from + request * p.width;
     int64_t* to = move_to + request * p.width;
-    if (keep == 0 || keep == n) {
+    if (lengths.as_it_is()) {
         for (int64_t i = threadIdx.x; i < p.width; i += kEvictBlock) from[i] = to[i] = -1;
         return;
     }
-    const Keys keys{weights, positions, block_table + request * p.table_stride,
-                    p.recent ? (shifts != nullptr ? shifts[request] : 0) + length - p.recent : INT64_MAX, p};
-    // The keep-th largest: the bytes of its order, highest first.
-    uint32_t prefix = 0, need = static_cast<uint32_t>(keep);
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (threadIdx.x < 256) bins[threadIdx.x] = 0;
-        __syncthreads();
-        for (int j = threadIdx.x; j < n; j += kEvictBlock) {
-            const uint32_t order = keys.order(j);
-            if (shift == 24 || order >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&bins[order >> shift & 255], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {  // bins from the largest down, four a lane
-            uint32_t own[4], sum = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) sum += own[i] = bins[255 - (4 * lane + i)];
-            uint32_t before = wave_inclusive_scan(sum, SumOp{}) - sum;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (before < need && need <= before + own[i]) {
-                    chosen = 255 - (4 * lane + i);
-                    wanted = need - before;
-                }
-                before += own[i];
-            }
-        }
-        __syncthreads();
-        prefix |= chosen << shift;
-        need = wanted;
-    }
+    const Keys keys{weights, positions, block_table + request * p.table_stride, lengths.late, p};
     const int per = ((n + kEvictWaves - 1) / kEvictWaves + kWave - 1) / kWave * kWave;
-    const int begin = wave * per, end = begin + per < n ? begin + per : n;
+    const int begin = wave * per < n ? wave * per : n, end = begin + per < n ? begin + per : n;
+    const Run<ITEMS> run(keys, begin, end);
+    const auto each = [&](auto f) { run.each(keys, f); };
+    Sorted sorted{0, static_cast<uint32_t>(lengths.keep), lengths.keep, 0};
+#pragma unroll 1
+    for (int digit = 0; digit < kDigits; ++digit) {
+        const int shift = digit == 0 ? kShifts[0] : digit == 1 ? kShifts[1] : kShifts[2];
+        const uint32_t above = digit == 0 ? 0u : digit == 1 ? ~0u << kShifts[0] : ~0u << kShifts[1];
+        for (int i = threadIdx.x; i < kBins; i += kEvictBlock) bins[i] = 0;
+        __syncthreads();
+        each([&](int, bool there, uint32_t order) {
+            if (there && (order & above) == sorted.threshold) atomicAdd(&bins[(order & ~above) >> shift], 1u);
+        });
+        __syncthreads();
+        chooser.run(bins, sorted.need);
+        sorted.threshold |= chooser.bin << shift;
+        sorted.need = chooser.need;
+    }
     // Of the keys equal to it, the first `need` stay.
     int ties = 0;
-    for (int j0 = begin; j0 < end; j0 += kWave) ties += __popcll(wave_ballot(j0 + lane < end && keys.order(j0 + lane) == prefix));
+    each([&](int, bool there, uint32_t order) { ties += __popcll(wave_ballot(there && order == sorted.threshold)); });
     if (lane == 0) tie_sums[wave] = ties;
     __syncthreads();
-    int tie_base = 0;
-    for (int w = 0; w < wave; ++w) tie_base += tie_sums[w];
-    const auto sweep = [&](auto emit) {
-        int tie = tie_base;
-        for (int j0 = begin; j0 < end; j0 += kWave) {
-            const int j = j0 + lane;
-            const uint32_t order = j < end ? keys.order(j) : 0u;
-            const uint64_t equal = wave_ballot(j < end && order == prefix);
-            const bool stays = order > prefix || (order == prefix && tie + static_cast<int>(popc_lanes_below(equal)) < static_cast<int>(need));
-            tie += __popcll(equal);
-            const bool mover = j < end && stays && j >= keep, hole = j < end && !stays && j < keep;
-            emit(j, mover, hole);
-        }
-    };
+    for (int w = 0; w < wave; ++w) sorted.tie += tie_sums[w];
+    const int first_tie = sorted.tie;
     int movers = 0, holes = 0;
-    sweep([&](int, bool mover, bool hole) {
+    each([&](int j, bool there, uint32_t order) {
+        bool mover, hole;
+        sorted.next(j, there, order, mover, hole);
         movers += __popcll(wave_ballot(mover));
         holes += __popcll(wave_ballot(hole));
     });
@@ -254,28 +337,213 @@ __global__ __launch_bounds__(kEvictBlock) void evict_plan_kernel(const float* __
         hole_sums[wave] = holes;
     }
     __syncthreads();
-    int64_t mover_at = 0, hole_at = 0, moves = 0;
+    Emitter emitter{from, to, 0, 0};
+    int64_t moves = 0;
     for (int w = 0; w < kEvictWaves; ++w) {
         if (w < wave) {
-            mover_at += mover_sums[w];
-            hole_at += hole_sums[w];
+            emitter.mover_at += mover_sums[w];
+            emitter.hole_at += hole_sums[w];
         }
         moves += mover_sums[w];
     }
-    sweep([&](int j, bool mover, bool hole) {
-        const uint64_t moving = wave_ballot(mover), open = wave_ballot(hole);
-        if (mover) {
-            const int64_t at = mover_at + popc_lanes_below(moving);
-            if (at < p.width) from[at] = keys.slot(j);
-        }
-        if (hole) {
-            const int64_t at = hole_at + popc_lanes_below(open);
-            if (at < p.width) to[at] = keys.slot(j);
-        }
-        mover_at += __popcll(moving);
-        hole_at += __popcll(open);
+    sorted.tie = first_tie;
+    each([&](int j, bool there, uint32_t order) {
+        bool mover, hole;
+        sorted.next(j, there, order, mover, hole);
+        if (wave_ballot(mover || hole) != 0) emitter.put(keys, p.width, j, mover, hole);
     });
     for (int64_t i = moves + threadIdx.x; i < p.width; i += kEvictBlock) from[i] = to[i] = -1;
+}
+
+// Long requests: `parts` workgroups a request, each a run of its keys, in launches that each end a step: the counts of a digit
+// (three times), the counts of what stays, and the moves.
+constexpr int kPartBlock = 256;
+constexpr int kPartWaves = kPartBlock / kWave;
+constexpr int kPartItems = 8;
+constexpr int kPartKeys = kPartItems * kPartBlock;  // keys of a part, of a request as long as stated
+constexpr int kPartLeast = 1024;                    // and at least, of a shorter one
+
+struct PartCounts {
+    int32_t low, low_equal, high, high_equal;  // above the threshold, or equal to it; before the new end, or past it
+};
+
+struct Parts {
+    uint32_t* bins;      // [requests][kDigits][kBins]
+    PartCounts* counts;  // [requests][parts]
+    int parts;
+};
+
+// A part's keys [begin, end), a run of each wave's.
+struct PartRange {
+    int begin, end, wave_begin, wave_end;
+    __device__ __forceinline__ PartRange(int n, int parts, int part) {
+        int64_t per = (static_cast<int64_t>(n) + parts - 1) / parts;
+        per = per < kPartLeast ? kPartLeast : (per + kPartBlock - 1) / kPartBlock * kPartBlock;
+        const auto bound = [](int64_t x, int64_t most) { return static_cast<int>(x < most ? x : most); };
+        begin = bound(part * per, n);
+        end = bound(part * per + per, n);
+        const int64_t run = per / kPartWaves, wave = threadIdx.x / kWave;
+        wave_begin = bound(begin + wave * run, end);
+        wave_end = bound(begin + wave * run + run, end);
+    }
+};
+
+// The threshold as far as the digits before `digit` say.
+template <int DIGIT>
+__device__ __forceinline__ void threshold_of(Chooser<kPartWaves>& chooser, const Parts& parts, int request, Sorted& sorted) {
+    const uint32_t* bins = parts.bins + static_cast<int64_t>(request) * kDigits * kBins;
+#pragma unroll
+    for (int d = 0; d < DIGIT; ++d) {
+        chooser.run(bins + d * kBins, sorted.need);
+        sorted.threshold |= chooser.bin << kShifts[d];
+        sorted.need = chooser.need;
+        __syncthreads();
+    }
+}
+
+struct EvictArrays {
+    const float* weights;
+    const int32_t* positions;
+    const int32_t* block_table;
+    const int32_t* kv_lengths;
+    const int32_t* kept_lengths;
+    const int32_t* shifts;
+};
+
+template <int DIGIT>
+__global__ __launch_bounds__(kPartBlock) void evict_digit_kernel(EvictArrays a, Parts parts, Evict p) {
+    __shared__ uint32_t bins[kBins];
+    __shared__ Chooser<kPartWaves> chooser;
+    const int request = static_cast<int>(blockIdx.x / parts.parts), part = static_cast<int>(blockIdx.x % parts.parts);
+    const Lengths lengths(a.kv_lengths, a.kept_lengths, a.shifts, request, p);
+    const PartRange range(lengths.n, parts.parts, part);
+    if (lengths.as_it_is() || range.begin >= range.end) return;
+    const Keys keys{a.weights, a.positions, a.block_table + request * p.table_stride, lengths.late, p};
+    const Run<kPartItems> run(keys, range.wave_begin, range.wave_end);
+    for (int i = threadIdx.x; i < kBins; i += kPartBlock) bins[i] = 0;
+    __syncthreads();
+    Sorted sorted{0, static_cast<uint32_t>(lengths.keep), lengths.keep, 0};
+    threshold_of<DIGIT>(chooser, parts, request, sorted);
+    constexpr uint32_t kAbove = DIGIT == 0 ? 0u : ~0u << kShifts[DIGIT > 0 ? DIGIT - 1 : 0];
+    run.each(keys, [&](int, bool there, uint32_t order) {
+        if (there && (order & kAbove) == sorted.threshold) atomicAdd(&bins[(order & ~kAbove) >> kShifts[DIGIT]], 1u);
+    });
+    __syncthreads();
+    uint32_t* all = parts.bins + (static_cast<int64_t>(request) * kDigits + DIGIT) * kBins;
+    for (int i = threadIdx.x; i < kBins; i += kPartBlock)
+        if (bins[i] != 0) atomic_add_agent(&all[i], bins[i]);
+}
+
+__global__ __launch_bounds__(kPartBlock) void evict_count_kernel(EvictArrays a, Parts parts, Evict p) {
+    __shared__ Chooser<kPartWaves> chooser;
+    __shared__ PartCounts sums[kPartWaves];
+    const int request = static_cast<int>(blockIdx.x / parts.parts), part = static_cast<int>(blockIdx.x % parts.parts);
+    const Lengths lengths(a.kv_lengths, a.kept_lengths, a.shifts, request, p);
+    const PartRange range(lengths.n, parts.parts, part);
+    if (lengths.as_it_is()) return;
+    PartCounts mine{0, 0, 0, 0};
+    if (range.begin < range.end) {
+        const Keys keys{a.weights, a.positions, a.block_table + request * p.table_stride, lengths.late, p};
+        const Run<kPartItems> run(keys, range.wave_begin, range.wave_end);
+        Sorted sorted{0, static_cast<uint32_t>(lengths.keep), lengths.keep, 0};
+        threshold_of<kDigits>(chooser, parts, request, sorted);
+        run.each(keys, [&](int j, bool there, uint32_t order) {
+            const bool low = j < lengths.keep, above = there && order > sorted.threshold, equal = there && order == sorted.threshold;
+            mine.low += __popcll(wave_ballot(above && low));
+            mine.high += __popcll(wave_ballot(above && !low));
+            mine.low_equal += __popcll(wave_ballot(equal && low));
+            mine.high_equal += __popcll(wave_ballot(equal && !low));
+        });
+    }
+    if (threadIdx.x % kWave == 0) sums[threadIdx.x / kWave] = mine;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+#pragma unroll
+    for (int w = 1; w < kPartWaves; ++w) {
+        mine.low += sums[w].low;
+        mine.low_equal += sums[w].low_equal;
+        mine.high += sums[w].high;
+        mine.high_equal += sums[w].high_equal;
+    }
+    parts.counts[static_cast<int64_t>(request) * parts.parts + part] = mine;
+}
+
+__global__ __launch_bounds__(kPartBlock) void evict_moves_kernel(EvictArrays a, Parts parts, int64_t* __restrict__ move_from,
+                                                                 int64_t* __restrict__ move_to, Evict p) {
+    __shared__ Chooser<kPartWaves> chooser;
+    __shared__ int32_t tie_sums[kPartWaves], mover_sums[kPartWaves], hole_sums[kPartWaves];
+    const int request = static_cast<int>(blockIdx.x / parts.parts), part = static_cast<int>(blockIdx.x % parts.parts);
+    const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
+    const Lengths lengths(a.kv_lengths, a.kept_lengths, a.shifts, request, p);
+    int64_t* from = move_from + request * p.width;
+    int64_t* to = move_to + request * p.width;
+    const int64_t stride = static_cast<int64_t>(parts.parts) * kPartBlock, own = static_cast<int64_t>(part) * kPartBlock + threadIdx.x;
+    if (lengths.as_it_is()) {
+        for (int64_t i = own; i < p.width; i += stride) from[i] = to[i] = -1;
+        return;
+    }
+    const PartRange range(lengths.n, parts.parts, part);
+    const Keys keys{a.weights, a.positions, a.block_table + request * p.table_stride, lengths.late, p};
+    const Run<kPartItems> run(keys, range.wave_begin, range.wave_end);
+    Sorted sorted{0, static_cast<uint32_t>(lengths.keep), lengths.keep, 0};
+    threshold_of<kDigits>(chooser, parts, request, sorted);
+    // What the parts before this one hold, and all of them: ties stay from the first on until enough do.
+    Emitter emitter{from, to, 0, 0};
+    int64_t moves = 0;
+    int ties = 0;
+    for (int first = 0; first < parts.parts; first += kWave) {
+        const int other = first + lane;
+        PartCounts c{0, 0, 0, 0};
+        int low = 0;
+        if (other < parts.parts) {
+            c = parts.counts[static_cast<int64_t>(request) * parts.parts + other];
+            const PartRange at(lengths.n, parts.parts, other);
+            low = (at.end < lengths.keep ? at.end : lengths.keep) - at.begin;
+            low = low > 0 ? low : 0;
+        }
+        const int equal = c.low_equal + c.high_equal, through = wave_inclusive_scan(equal, SumOp{});
+        const int ahead = ties + through - equal, left = static_cast<int>(sorted.need) - ahead;
+        const int staying = left <= 0 ? 0 : left < equal ? left : equal, staying_low = staying < c.low_equal ? staying : c.low_equal;
+        const int movers = c.high + staying - staying_low, holes = low - c.low - staying_low;
+        const bool before = other < part;
+        emitter.mover_at += wave_reduce(before ? movers : 0, SumOp{});
+        emitter.hole_at += wave_reduce(before ? holes : 0, SumOp{});
+        sorted.tie += wave_reduce(before ? equal : 0, SumOp{});
+        moves += wave_reduce(movers, SumOp{});
+        ties += wave_read_lane(through, kWave - 1);
+    }
+    for (int64_t i = moves + own; i < p.width; i += stride) from[i] = to[i] = -1;
+    if (range.begin >= range.end) return;
+    // Then the waves before this one.
+    const auto each = [&](auto f) { run.each(keys, f); };
+    int equal = 0;
+    each([&](int, bool there, uint32_t order) { equal += __popcll(wave_ballot(there && order == sorted.threshold)); });
+    if (lane == 0) tie_sums[wave] = equal;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) sorted.tie += tie_sums[w];
+    const int first_tie = sorted.tie;
+    int movers = 0, holes = 0;
+    each([&](int j, bool there, uint32_t order) {
+        bool mover, hole;
+        sorted.next(j, there, order, mover, hole);
+        movers += __popcll(wave_ballot(mover));
+        holes += __popcll(wave_ballot(hole));
+    });
+    if (lane == 0) {
+        mover_sums[wave] = movers;
+        hole_sums[wave] = holes;
+    }
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) {
+        emitter.mover_at += mover_sums[w];
+        emitter.hole_at += hole_sums[w];
+    }
+    sorted.tie = first_tie;
+    each([&](int j, bool there, uint32_t order) {
+        bool mover, hole;
+        sorted.next(j, there, order, mover, hole);
+        if (wave_ballot(mover || hole) != 0) emitter.put(keys, p.width, j, mover, hole);
+    });
 }
 
 // ---- rows from slot to slot --------------------------------------------------------------------------------------
@@ -311,6 +579,15 @@ __global__ __launch_bounds__(kMoveBlock) void paged_move_kernel(Pages key_cache,
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
+// Workgroups of a request: one up to kLongRequest keys, then one for every kPartKeys.
+constexpr uint64_t kLongRequest = 16384;
+uint64_t parts_of(uint64_t max_kv_length) { return max_kv_length <= kLongRequest ? 1 : ceil_div(max_kv_length, kPartKeys); }
+size_t bins_bytes(uint64_t requests) { return align_up(requests * kDigits * kBins * sizeof(uint32_t), kViewAlign); }
+size_t plan_bytes(uint64_t requests, uint64_t max_kv_length) {
+    const uint64_t parts = parts_of(max_kv_length);
+    return requests == 0 || parts == 1 ? 0 : bins_bytes(requests) + align_up(requests * parts * sizeof(PartCounts), kViewAlign);
+}
+
 int check_pages(const char* what, uint32_t requests, uint32_t page_size, uint64_t table_stride, uint32_t table_width) {
     if (page_size == 0 || page_size > 0x7FFFFFFFu) return set_error(kInvalidArgument, "%s: page size out of range", what);
     if (requests > 0x7FFFFFFu) return set_error(kInvalidArgument, "%s: too many requests", what);
@@ -358,9 +635,26 @@ int evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_
     if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
     const Evict p{Divider(page_size), static_cast<int64_t>(table_stride), static_cast<int>(table_width), static_cast<int>(pages),
                   static_cast<int64_t>(width), static_cast<int>(first), static_cast<int>(recent)};
+    const uint64_t count = parts_of(max_kv_length);
+    if (count == 1) {
+        LaunchScope scope(what, stream);
+        auto* kernel = max_kv_length <= 2 * kEvictBlock ? evict_plan_kernel<2> : max_kv_length <= 8 * kEvictBlock ? evict_plan_kernel<8>
+                                                                                                                 : evict_plan_kernel<32>;
+        kernel<<<requests, kEvictBlock, 0, stream>>>(weights, positions, block_table, kv_lengths, kept_lengths, shifts, move_from, move_to, p);
+        return check_hip(hipGetLastError(), "evict_plan launch");
+    }
+    if (requests * count > 0x7FFFFFFFull / kPartBlock) return set_error(kInvalidArgument, "%s: too many requests of such length", what);
+    const EvictArrays a{weights, positions, block_table, kv_lengths, kept_lengths, shifts};
+    const Parts parts{static_cast<uint32_t*>(temp), reinterpret_cast<PartCounts*>(static_cast<char*>(temp) + bins_bytes(requests)),
+                      static_cast<int>(count)};
+    if (int st = launch_fill_u32(parts.bins, static_cast<uint64_t>(requests) * kDigits * kBins, 0, stream); st != kOk) return st;
+    const unsigned blocks = static_cast<unsigned>(requests * count);
     LaunchScope scope(what, stream);
-    evict_plan_kernel<<<requests, kEvictBlock, 0, stream>>>(weights, positions, block_table, kv_lengths, kept_lengths, shifts, move_from,
-                                                            move_to, p);
+    evict_digit_kernel<0><<<blocks, kPartBlock, 0, stream>>>(a, parts, p);
+    evict_digit_kernel<1><<<blocks, kPartBlock, 0, stream>>>(a, parts, p);
+    evict_digit_kernel<2><<<blocks, kPartBlock, 0, stream>>>(a, parts, p);
+    evict_count_kernel<<<blocks, kPartBlock, 0, stream>>>(a, parts, p);
+    evict_moves_kernel<<<blocks, kPartBlock, 0, stream>>>(a, parts, move_from, move_to, p);
     return check_hip(hipGetLastError(), "evict_plan launch");
 }
 
@@ -408,7 +702,9 @@ int lcpp_hip_page_release(const int32_t* kv_lengths, const int32_t* keep_lengths
                                    shifts, kept_lengths, shifts_out, released, max_released, counts, stream);
 }
 
-size_t lcpp_hip_evict_plan_temp_bytes(uint32_t, uint64_t) { return 0; }
+size_t lcpp_hip_evict_plan_temp_bytes(uint32_t requests, uint64_t max_kv_length) {
+    return attention::plan_bytes(requests, max_kv_length);
+}
 
 int lcpp_hip_evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_t* positions, const int32_t* block_table,
                         uint64_t table_stride, uint32_t table_width, const int32_t* kv_lengths, const int32_t* kept_lengths,
