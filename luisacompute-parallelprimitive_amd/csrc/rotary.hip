@@ -70,64 +70,49 @@ __device__ __forceinline__ void turn2(uint32_t& x, uint32_t& y, F32x2 cs0, F32x2
     y = pack2<T>(a0 * cs0[1] + b0 * cs0[0], a1 * cs1[1] + b1 * cs1[0]);
 }
 
-// EACH units a thread of `group` tokens, or of a part of a token's (blockIdx.y): loads first, then the workgroup's table of
-// cosines and sines, then the turns.
+// What a token's rows need to know: where its slot is (in the paged form), and whether they are written at all.
+struct TokenPlace {
+    int64_t key_bytes, value_bytes;
+    bool rows, slot;
+};
+
+// EACH units a thread of `group` tokens, or of a part of a token's (blockIdx.y).  Rows are loaded first; while they come, some
+// threads make the workgroup's table of cosines and sines and others look up the tokens' slots.
 template <typename T, Layout LAYOUT, bool PAGED, int EACH>
 __global__ __launch_bounds__(kTurnBlock) void rotary_kernel(TurnRows rows, const int32_t* __restrict__ positions,
                                                             const int32_t* __restrict__ requests, const int32_t* __restrict__ shifts,
                                                             const double* __restrict__ frequencies, Turn p) {
     using Item = typename T::Item;
     extern __shared__ __attribute__((aligned(16))) char shared[];
-    F32x2* table = reinterpret_cast<F32x2*>(shared);
     const int64_t token0 = static_cast<int64_t>(blockIdx.x) * p.group;
     const int count = static_cast<int>(p.tokens - token0 < p.group ? p.tokens - token0 : p.group);
-    const int heads = p.q_heads + p.kv_heads + (PAGED ? p.kv_heads : 0);
+    TokenPlace* places = reinterpret_cast<TokenPlace*>(shared);
+    F32x2* table = reinterpret_cast<F32x2*>(places + p.group);
     const uint32_t all = static_cast<uint32_t>(count) * p.units.by;
     const uint32_t first = blockIdx.y * (kTurnBlock * EACH) + threadIdx.x;
+    const int pair_units = LAYOUT == Layout::kOdd ? (p.half + 7) / 8 : p.half / 8;
 
     U32x4 x[EACH], y[EACH];
     const char* from[EACH];
-    char* to[EACH];
-    int unit[EACH], local[EACH];
-    bool turned[EACH];
+    int unit[EACH], local[EACH], head[EACH];
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-        const uint32_t at = first + e * kTurnBlock;
-        to[e] = nullptr;
-        if (at >= all) continue;
+        // (Past the last unit, the last one again, which is not written.)
+        const uint32_t at = first + e * kTurnBlock < all ? first + e * kTurnBlock : all - 1;
         local[e] = static_cast<int>(p.units(at));
         const int rest = static_cast<int>(at - local[e] * p.units.by);
-        const int head = static_cast<int>(p.per_head(rest));
-        unit[e] = rest - head * static_cast<int>(p.per_head.by);
+        head[e] = static_cast<int>(p.per_head(rest));
+        unit[e] = rest - head[e] * static_cast<int>(p.per_head.by);
         const int64_t token = token0 + local[e];
-        turned[e] = head < p.q_heads + p.kv_heads;
-        if (requests != nullptr && requests[token] < 0) continue;
-        if (head < p.q_heads) {
-            from[e] = rows.q.at(token, head);
-            to[e] = rows.q_out.at(token, head);
-        } else {
-            const int kv_head = (head - p.q_heads) % p.kv_heads;
-            from[e] = turned[e] ? rows.k.at(token, kv_head) : rows.v.at(token, kv_head);
-            if constexpr (PAGED) {
-                const int64_t slot = rows.slots[token];
-                const int64_t page = slot < 0 ? rows.pages
-                                     : slot <= 0xFFFFFFFFll ? rows.page_size(static_cast<uint32_t>(slot)) : slot / rows.page_size.by;
-                if (page >= rows.pages) continue;
-                const int64_t within = slot - page * rows.page_size.by;
-                to[e] = (turned[e] ? rows.key_cache : rows.value_cache).at(page, within, kv_head);
-            } else {
-                to[e] = rows.k_out.at(token, kv_head);
-            }
-        }
-        if constexpr (LAYOUT == Layout::kOdd) continue;
-        const int pair_units = p.half / 8;
-        if (LAYOUT == Layout::kInterleaved) {
+        const int kv_head = head[e] - p.q_heads;
+        from[e] = kv_head < 0 ? rows.q.at(token, head[e]) : !PAGED || kv_head < p.kv_heads ? rows.k.at(token, kv_head)
+                                                                                           : rows.v.at(token, kv_head - p.kv_heads);
+        if constexpr (LAYOUT == Layout::kInterleaved) {
             x[e] = *reinterpret_cast<const U32x4*>(from[e] + unit[e] * 16);
-        } else if (unit[e] < pair_units) {
-            x[e] = *reinterpret_cast<const U32x4*>(from[e] + unit[e] * 16);
-            y[e] = *reinterpret_cast<const U32x4*>(from[e] + p.half * 2 + unit[e] * 16);
-        } else {
-            x[e] = *reinterpret_cast<const U32x4*>(from[e] + p.half * 2 + unit[e] * 16);
+        } else if constexpr (LAYOUT == Layout::kHalves) {
+            const int more = unit[e] < pair_units ? 0 : p.half * 2;
+            x[e] = *reinterpret_cast<const U32x4*>(from[e] + more + unit[e] * 16);
+            if (more == 0) y[e] = *reinterpret_cast<const U32x4*>(from[e] + p.half * 2 + unit[e] * 16);
         }
     }
     for (int i = threadIdx.x; i < count * p.half; i += kTurnBlock) {
@@ -139,35 +124,64 @@ __global__ __launch_bounds__(kTurnBlock) void rotary_kernel(TurnRows rows, const
         sincospif(2.f * static_cast<float>(turns), &s, &c);
         table[i] = F32x2{c * p.factor, (p.inverse ? -s : s) * p.factor};
     }
-    if constexpr (PAGED) {
-        if (rows.slot_positions != nullptr && blockIdx.y == 0)
-            for (int t = threadIdx.x; t < count; t += kTurnBlock) {
-                const int64_t token = token0 + t, slot = rows.slots[token];
-                if ((requests != nullptr && requests[token] < 0) || slot < 0 || slot / rows.page_size.by >= rows.pages) continue;
-                rows.slot_positions[slot] = static_cast<int32_t>(position_of(positions, requests, shifts, p.num_shifts, token));
+    for (int t = kTurnBlock - 1 - static_cast<int>(threadIdx.x); t < count; t += kTurnBlock) {
+        const int64_t token = token0 + t;
+        TokenPlace place{0, 0, requests == nullptr || requests[token] >= 0, false};
+        if constexpr (PAGED) {
+            const int64_t slot = rows.slots[token];
+            if (place.rows && slot >= 0) {
+                const int64_t page = slot <= 0xFFFFFFFFll ? rows.page_size(static_cast<uint32_t>(slot)) : slot / rows.page_size.by;
+                if (page < rows.pages) {
+                    const int64_t within = slot - page * rows.page_size.by;
+                    place.slot = true;
+                    place.key_bytes = page * rows.key_cache.page_bytes + within * rows.key_cache.token_bytes;
+                    place.value_bytes = page * rows.value_cache.page_bytes + within * rows.value_cache.token_bytes;
+                    if (rows.slot_positions != nullptr && blockIdx.y == 0)
+                        rows.slot_positions[slot] = static_cast<int32_t>(position_of(positions, requests, shifts, p.num_shifts, token));
+                }
             }
+        }
+        places[t] = place;
     }
     __syncthreads();
 #pragma unroll
     for (int e = 0; e < EACH; ++e) {
-        if (to[e] == nullptr) continue;
+        if (first + e * kTurnBlock >= all) continue;
+        const TokenPlace place = places[local[e]];
+        const int64_t token = token0 + local[e];
+        const int kv_head = head[e] - p.q_heads;
+        const bool turned = !PAGED || kv_head < p.kv_heads;
+        char* to;
+        if (kv_head < 0) {
+            if (!place.rows) continue;
+            to = rows.q_out.at(token, head[e]);
+        } else if constexpr (PAGED) {
+            if (!place.slot) continue;
+            to = turned ? rows.key_cache.data + place.key_bytes + kv_head * rows.key_cache.head_bytes
+                        : rows.value_cache.data + place.value_bytes + (kv_head - p.kv_heads) * rows.value_cache.head_bytes;
+        } else {
+            if (!place.rows) continue;
+            to = rows.k_out.at(token, kv_head);
+        }
         const F32x2* cs = table + local[e] * p.half;
         if constexpr (LAYOUT == Layout::kInterleaved) {
+            if (turned && 4 * unit[e] < p.half) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int pair = 4 * unit[e] + i;
-                if (!turned[e] || pair >= p.half) continue;
-                const float a = item_low<T>(x[e][i]), b = item_high<T>(x[e][i]);
-                const F32x2 t = cs[pair];
-                x[e][i] = pack2<T>(a * t[0] - b * t[1], a * t[1] + b * t[0]);
+                for (int i = 0; i < 4; ++i) {
+                    const int pair = 4 * unit[e] + i;
+                    const float a = item_low<T>(x[e][i]), b = item_high<T>(x[e][i]);
+                    const F32x2 t = cs[pair < p.half ? pair : 0];
+                    const uint32_t turn = pack2<T>(a * t[0] - b * t[1], a * t[1] + b * t[0]);
+                    x[e][i] = pair < p.half ? turn : x[e][i];
+                }
             }
-            *reinterpret_cast<U32x4*>(to[e] + unit[e] * 16) = x[e];
+            *reinterpret_cast<U32x4*>(to + unit[e] * 16) = x[e];
         } else if constexpr (LAYOUT == Layout::kHalves) {
-            if (unit[e] >= p.half / 8) {
-                *reinterpret_cast<U32x4*>(to[e] + p.half * 2 + unit[e] * 16) = x[e];
+            if (unit[e] >= pair_units) {
+                *reinterpret_cast<U32x4*>(to + p.half * 2 + unit[e] * 16) = x[e];
                 continue;
             }
-            if (turned[e]) {
+            if (turned) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     uint32_t a = x[e][i], b = y[e][i];
@@ -176,12 +190,11 @@ __global__ __launch_bounds__(kTurnBlock) void rotary_kernel(TurnRows rows, const
                     y[e][i] = b;
                 }
             }
-            *reinterpret_cast<U32x4*>(to[e] + unit[e] * 16) = x[e];
-            *reinterpret_cast<U32x4*>(to[e] + p.half * 2 + unit[e] * 16) = y[e];
+            *reinterpret_cast<U32x4*>(to + unit[e] * 16) = x[e];
+            *reinterpret_cast<U32x4*>(to + p.half * 2 + unit[e] * 16) = y[e];
         } else {
             const Item* in = reinterpret_cast<const Item*>(from[e]);
-            Item* out = reinterpret_cast<Item*>(to[e]);
-            const int pair_units = (p.half + 7) / 8;
+            Item* out = reinterpret_cast<Item*>(to);
             for (int i = 0; i < 8; ++i) {
                 if (unit[e] < pair_units) {
                     const int pair = 8 * unit[e] + i;
@@ -189,8 +202,8 @@ __global__ __launch_bounds__(kTurnBlock) void rotary_kernel(TurnRows rows, const
                     const Item first_item = in[pair], second_item = in[pair + p.half];
                     const float a = static_cast<float>(first_item), b = static_cast<float>(second_item);
                     const F32x2 t = cs[pair];
-                    out[pair] = turned[e] ? static_cast<Item>(a * t[0] - b * t[1]) : first_item;
-                    out[pair + p.half] = turned[e] ? static_cast<Item>(a * t[1] + b * t[0]) : second_item;
+                    out[pair] = turned ? static_cast<Item>(a * t[0] - b * t[1]) : first_item;
+                    out[pair + p.half] = turned ? static_cast<Item>(a * t[1] + b * t[0]) : second_item;
                 } else {
                     const int at = 2 * p.half + 8 * (unit[e] - pair_units) + i;
                     if (at >= p.dim) break;
@@ -218,13 +231,14 @@ int launch(const char* what, const TurnRows& rows, const int32_t* positions, con
     const uint64_t block_units = kTurnBlock * (many ? kEach : 1);
     uint64_t group = units >= block_units ? 1 : block_units / units;
     if (group * half > kMostPairs) group = half < kMostPairs ? kMostPairs / half : 1;
+    if (group > kTurnBlock) group = kTurnBlock;
     const uint64_t blocks = ceil_div(tokens, group), parts = ceil_div(group * units, block_units);
     if (blocks > 0x7FFFFFFFull / kTurnBlock || parts > 65535)
         return set_error(kInvalidArgument, "%s: too many tokens or heads", what);
     const Turn p{static_cast<int64_t>(tokens), static_cast<int>(q_heads), static_cast<int>(kv_heads), static_cast<int>(dim), half,
                  inverse, factor, static_cast<int>(num_shifts), Divider(static_cast<uint32_t>(units)),
                  Divider(static_cast<uint32_t>(per_head)), Divider(static_cast<uint32_t>(half)), static_cast<int>(group)};
-    const size_t lds = group * half * sizeof(F32x2);
+    const size_t lds = group * (half * sizeof(F32x2) + sizeof(TokenPlace));
     const auto run = [&](auto kernel) {
         kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(parts)), kTurnBlock, lds, stream>>>(
             rows, positions, requests, shifts, frequencies, p);
