@@ -16,8 +16,6 @@ namespace {
 
 constexpr int kWeightWaves = 4;
 constexpr int kWeightBlock = kWeightWaves * kWave;
-constexpr int kUnitKeys = 64;           // of a workgroup at a time
-constexpr int kGroups = kUnitKeys / 16;  // matrix products side by side
 constexpr int kRowsAtOnce = 16;
 
 using Acc = F32x4;
@@ -44,130 +42,369 @@ struct Weigh {
     int64_t table_stride;
     int table_width;
     uint32_t parts;  // workgroups of a request
-    int splits;  // waves that share a key head's rows
+    int few;         // rows of a key head that make a request one of few
     float scale;
     float decay;
 };
 
-template <typename T, int DP>
-__global__ __launch_bounds__(kWeightBlock) void attention_weights_kernel(Rows q, Pages key_cache, const int32_t* __restrict__ block_table,
-                                                                         const int32_t* __restrict__ q_offsets,
-                                                                         const int32_t* __restrict__ kv_lengths,
-                                                                         const int32_t* __restrict__ known_lengths,
-                                                                         const uint64_t* __restrict__ tree, const float* __restrict__ lse,
-                                                                         const float* weights_in, float* weights_out, Weigh p) {
-    constexpr int kSteps = DP / 32;
-    __shared__ float sums[kWeightWaves][kUnitKeys];
-    const int request = static_cast<int>(blockIdx.x / p.parts), part = static_cast<int>(blockIdx.x % p.parts), lane = threadIdx.x % kWave;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-    int begin = q_offsets[request], end = q_offsets[request + 1];
-    begin = begin < 0 ? 0 : begin > p.q_tokens ? p.q_tokens : begin;
-    end = end < begin ? begin : end > p.q_tokens ? p.q_tokens : end;
-    const int group = p.q_heads / p.kv_heads, rows = (end - begin) * group;
-    const int length = kv_lengths[request] < 0 ? 0 : kv_lengths[request];
-    const int64_t room = static_cast<int64_t>(p.table_width) * p.page_size.by;
-    const int held = length < room ? length : static_cast<int>(room);
-    const int ahead = length - (end - begin);  // keys before the new tokens' own
-    const int known = known_lengths != nullptr ? known_lengths[request] : ahead;
-    const int32_t* table = block_table + request * p.table_stride;
-    const float c = p.scale * kLog2e;
-    const int column = lane % 16, quarter = lane / 16;
+struct WeighArrays {
+    const int32_t* block_table;
+    const int32_t* q_offsets;
+    const int32_t* kv_lengths;
+    const int32_t* known_lengths;
+    const uint64_t* tree;
+    const float* lse;
+    const float* weights_in;
+    float* weights_out;
+};
 
-    for (int64_t unit = part; unit * kUnitKeys < held; unit += p.parts) {
-        const int key0 = static_cast<int>(unit) * kUnitKeys;
-        const char* key[kGroups];
-        bool there[kGroups];
+// A request's rows and keys.
+struct Request {
+    int begin, group, rows;
+    int held;    // keys that the table has room for
+    int ahead;   // keys before the new tokens' own
+    int known;   // keys that have a sum to add to
+    const int32_t* table;
+    __device__ __forceinline__ Request(const WeighArrays& a, const Weigh& p, int request) {
+        begin = a.q_offsets[request];
+        int end = a.q_offsets[request + 1];
+        begin = begin < 0 ? 0 : begin > p.q_tokens ? p.q_tokens : begin;
+        end = end < begin ? begin : end > p.q_tokens ? p.q_tokens : end;
+        group = p.q_heads / p.kv_heads;
+        rows = (end - begin) * group;
+        const int length = a.kv_lengths[request] < 0 ? 0 : a.kv_lengths[request];
+        const int64_t room = static_cast<int64_t>(p.table_width) * p.page_size.by;
+        held = length < room ? length : static_cast<int>(room);
+        ahead = length - (end - begin);
+        known = a.known_lengths != nullptr ? a.known_lengths[request] : ahead;
+        table = a.block_table + request * p.table_stride;
+    }
+    // The address of row `row` of a key head, and its log-sum as a power of two (infinity where it gives no weight).
+    __device__ __forceinline__ const char* row_at(const Rows& q, const Weigh& p, int kv_head, int row) const {
+        const int token = static_cast<int>(p.group(row));
+        return q.at(begin + token, kv_head * group + row - token * group);
+    }
+    __device__ __forceinline__ float base_of(const WeighArrays& a, const Weigh& p, int kv_head, int row) const {
+        const int token = static_cast<int>(p.group(row));
+        const float l = a.lse[static_cast<int64_t>(kv_head * group + row - token * group) * p.q_tokens + begin + token];
+        return l == -INFINITY ? INFINITY : l * kLog2e;
+    }
+    __device__ __forceinline__ int64_t slot(const Weigh& p, int j) const {
+        const uint32_t cell = p.page_size(j);
+        const int page = table[cell];
+        return page < 0 || page >= p.pages ? -1 : static_cast<int64_t>(page) * p.page_size.by + (j - cell * p.page_size.by);
+    }
+    __device__ __forceinline__ void put(const WeighArrays& a, const Weigh& p, int j, float total, bool first) const {
+        if (j >= held) return;
+        const int64_t at = slot(p, j);
+        if (at < 0) return;
+        if (!first) a.weights_out[at] += total;
+        else a.weights_out[at] = j < known && a.weights_in != nullptr ? a.weights_in[at] * p.decay + total : total;
+    }
+};
+
+// 16 rows on their way from memory to a matrix instruction's operand.  Lanes side by side load a row's 16-byte chunks side by side (a
+// load of 16 rows at a time takes the cache four times as long), write them to LDS, and read back row lane % 16, chunk lane / 16 of
+// every four.  Rows in LDS are 16 bytes further apart than they are long: 16 lanes read 64 banks.  Loads have no branch, so that
+// those in flight are not waited for where paths meet: past a row's items its first ones are loaded, and taken as zeros.
+template <int DP, bool EXACT>
+struct Stage {
+    static constexpr int kSteps = DP / 32;
+    static constexpr int kPerRow = DP > 64 ? 16 : 8;
+    static constexpr int kAtOnce = kWave / kPerRow;
+    static constexpr int kLoads = 16 / kAtOnce;
+    static constexpr int kRowBytes = DP * 2 + 16;
+    static constexpr int kBytes = 16 * kRowBytes;
+    using Chunks = U32x4[kLoads];
+    using Operand = U32x4[kSteps];
+    // The row of load i that a lane reads.
+    __device__ __forceinline__ static int row(int i) { return i * kAtOnce + static_cast<int>(threadIdx.x % kWave) / kPerRow; }
+    __device__ __forceinline__ static int chunk() { return static_cast<int>(threadIdx.x) % kPerRow; }
+    __device__ __forceinline__ static U32x4 load(const char* row, int dim) {
+        return *reinterpret_cast<const U32x4*>(row + (EXACT && DP != 96 ? chunk() : chunk() * 8 < dim ? chunk() : 0) * 16);
+    }
+    __device__ __forceinline__ static void write(char* tile, const Chunks& x, int dim) {
+        if (DP == 96 && chunk() >= DP / 8) return;
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            const int j = key0 + 16 * g + column, at = j < held ? j : held - 1;
-            const uint32_t cell = p.page_size(at);
-            const int page = table[cell];
-            there[g] = page >= 0 && page < p.pages;
-            key[g] = key_cache.at(there[g] ? page : 0, there[g] ? at - static_cast<int>(cell * p.page_size.by) : 0, 0);
+        for (int i = 0; i < kLoads; ++i) {
+            U32x4 v = x[i];
+            if constexpr (!EXACT) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) v[w] = chunk() * 8 < dim ? v[w] : 0u;
+            }
+            *reinterpret_cast<U32x4*>(tile + row(i) * kRowBytes + chunk() * 16) = v;
         }
-        // Rows that see every key of the unit need no masks.
-        const bool masked = key0 + kUnitKeys - 1 > (tree != nullptr ? ahead - 1 : ahead);
-        float sum[kGroups] = {};
-        for (int job = wave; job < p.kv_heads * p.splits; job += kWeightWaves) {
-            const int kv_head = job % p.kv_heads, split = job / p.kv_heads;
-            U32x4 k[kGroups][kSteps];
+    }
+    __device__ __forceinline__ static void read(const char* tile, Operand& x) {
+        const int lane = threadIdx.x % kWave;
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g)
+        for (int s = 0; s < kSteps; ++s) x[s] = *reinterpret_cast<const U32x4*>(tile + lane % 16 * kRowBytes + lane / 16 * 16 + s * 64);
+    }
+};
+
+// Where key key0 + lane of a unit lies; of the last one past the end, and of any that is there where its page is not.
+__device__ __forceinline__ int64_t key_at(const Pages& cache, const Request& r, const Weigh& p, int key0, int keys) {
+    const int j = key0 + static_cast<int>(threadIdx.x % kWave) % keys, at = j < r.held ? j : r.held - 1;
+    const uint32_t cell = p.page_size(at);
+    const int page = r.table[cell];
+    const bool there = page >= 0 && page < p.pages;
+    return there ? page * cache.page_bytes + (at - static_cast<int>(cell * p.page_size.by)) * cache.token_bytes : 0;
+}
+
+// Adds a tile of rows' weights to the sums of the lane's keys; `row0` is the lane's first row of four, `base` their log-sums.
+template <typename T, int GROUPS, int STEPS>
+__device__ __forceinline__ void weigh(float (&sum)[GROUPS], const U32x4 (&a)[STEPS], const U32x4 (&k)[GROUPS][STEPS], F32x4 base, float c,
+                                      bool masked, const WeighArrays& arrays, const Request& request, const Weigh& p, int row0, int key0) {
+    Acc acc[GROUPS] = {};
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s)
-                    k[g][s] = load_chunk(key[g] + kv_head * key_cache.head_bytes, 4 * s + quarter, p.dim, there[g]);
-            for (int row0 = split * kRowsAtOnce; row0 < rows; row0 += p.splits * kRowsAtOnce) {
-                const int mine = row0 + column;
-                const int my_token = static_cast<int>(p.group(mine));
-                const char* q_row = q.at(begin + my_token, kv_head * group + mine - my_token * group);
-                U32x4 a[kSteps];
+    for (int s = 0; s < STEPS; ++s)
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s) a[s] = load_chunk(q_row, 4 * s + quarter, p.dim, mine < rows);
-                float base[4];
-                bool none[4];
-                int token[4];
+        for (int g = 0; g < GROUPS; ++g) acc[g] = product<T>(a[s], k[g][s], acc[g]);
+    if (!masked) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int row = row0 + 4 * quarter + r;
-                    token[r] = static_cast<int>(p.group(row));
-                    float l = -INFINITY;
-                    if (row < rows)
-                        l = lse[static_cast<int64_t>(kv_head * group + row - token[r] * group) * p.q_tokens + begin + token[r]];
-                    none[r] = l == -INFINITY;
-                    base[r] = none[r] ? INFINITY : l * kLog2e;  // rows that are not there, or see nothing, weigh nothing
-                }
-                Acc acc[kGroups] = {};
+        for (int g = 0; g < GROUPS; ++g)
 #pragma unroll
-                for (int s = 0; s < kSteps; ++s)
+            for (int r = 0; r < 4; ++r) sum[g] += exp2_fast(acc[g][r] * c - base[r]);
+        return;
+    }
 #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) acc[g] = product<T>(a[s], k[g][s], acc[g]);
-                if (!masked && row0 + kRowsAtOnce <= rows) {
+    for (int r = 0; r < 4; ++r) {
+        const int row = row0 + r, token = static_cast<int>(p.group(row));
+        const bool real = row < request.rows && base[r] != INFINITY;
+        const uint64_t word = real && arrays.tree != nullptr ? arrays.tree[request.begin + token] : 0;
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const int fresh = key0 + 16 * g + static_cast<int>(threadIdx.x % 16) - request.ahead;  // which of the new keys
+            const bool seen = arrays.tree == nullptr ? fresh <= token : fresh < 0 || (fresh < 64 && (word >> fresh & 1) != 0);
+            const float w = exp2_fast(acc[g][r] * c - base[r]);
+            sum[g] += real && seen ? w : 0.f;
+        }
+    }
+}
+
+// Four lanes have the sums of a key's rows.
+template <int GROUPS>
+__device__ __forceinline__ void meet(float (&sum)[GROUPS]) {
+#pragma unroll
+    for (int g = 0; g < GROUPS; ++g) {
+        sum[g] += __shfl_xor(sum[g], 16);
+        sum[g] += __shfl_xor(sum[g], 32);
+    }
+}
+
+// Requests of few rows: a wave goes through the key heads of 32 keys, a tile of 16 rows at a time, the next head's keys on their way
+// while it works on one.
+constexpr int kFewKeys = 16;
+constexpr int kFewHeads = 32;  // key heads whose log-sums lie in LDS at once
+
+template <typename T, int DP, bool EXACT>
+__global__ __launch_bounds__(kWeightBlock) void attention_weights_few_kernel(Rows q, Pages key_cache, WeighArrays arrays, Weigh p) {
+    using S = Stage<DP, EXACT>;
+    constexpr int kGroups = kFewKeys / 16;
+    __shared__ __attribute__((aligned(16))) char staged[kWeightWaves][kGroups * S::kBytes];
+    __shared__ __attribute__((aligned(16))) float bases[kFewHeads * kRowsAtOnce];
+    const Request request(arrays, p, static_cast<int>(blockIdx.x / p.parts));
+    const int part = static_cast<int>(blockIdx.x % p.parts), lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), column = lane % 16, quarter = lane / 16;
+    const int units = (request.held + kFewKeys - 1) / kFewKeys;
+    if (part * kWeightWaves >= units || request.rows > p.few) return;
+    const float c = p.scale * kLog2e;
+    char* tile = staged[wave];
+    bool first = true;
+    for (int row_base = 0; row_base < request.rows || first; row_base += kRowsAtOnce) {
+        // (Rows that are not there are the first one with a log-sum of infinity: they weigh nothing.)
+        const int mine = row_base + column < request.rows ? row_base + column : 0;
+        for (int head_base = 0; head_base < p.kv_heads; head_base += kFewHeads) {
+            const int heads = p.kv_heads - head_base < kFewHeads ? p.kv_heads - head_base : kFewHeads;
+            if (row_base + head_base > 0) __syncthreads();
+            for (int i = threadIdx.x; i < heads * kRowsAtOnce; i += kWeightBlock) {
+                const int row = row_base + i % kRowsAtOnce;
+                bases[i] = row < request.rows ? request.base_of(arrays, p, head_base + i / kRowsAtOnce, row) : INFINITY;
+            }
+            __syncthreads();
+            for (int unit = part * kWeightWaves + wave; unit < units; unit += static_cast<int>(p.parts) * kWeightWaves) {
+                const int key0 = unit * kFewKeys;
+                // Rows that see every key of the unit need no masks.
+                const bool masked = key0 + kFewKeys - 1 > (arrays.tree != nullptr ? request.ahead - 1 : request.ahead);
+                float sum[kGroups] = {};
+                if (request.rows > 0) {
+                    const int64_t own = key_at(key_cache, request, p, key0, kFewKeys);
+                    const char* from[kGroups][S::kLoads];
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) sum[g] += exp2_fast(acc[g][r] * c - base[r]);
-                } else {
+                        for (int i = 0; i < S::kLoads; ++i)
+                            from[g][i] = key_cache.data + head_base * key_cache.head_bytes + __shfl(own, 16 * g + S::row(i));
+                    typename S::Chunks keys[kGroups];
+                    typename S::Operand a, next;
+                    const auto load = [&](int local) {
+                        const char* row = request.row_at(q, p, head_base + local, mine);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const bool real = row0 + 4 * quarter + r < rows && !none[r];
-                        const uint64_t word = real && tree != nullptr ? tree[begin + token[r]] : 0;
-#pragma unroll
-                        for (int g = 0; g < kGroups; ++g) {
-                            const int fresh = key0 + 16 * g + column - ahead;  // which of the new keys
-                            const bool seen = tree == nullptr ? fresh <= token[r] : fresh < 0 || (fresh < 64 && (word >> fresh & 1) != 0);
-                            sum[g] += real && seen ? exp2_fast(acc[g][r] * c - base[r]) : 0.f;
+                        for (int s = 0; s < S::kSteps; ++s) {
+                            const int chunk = 4 * s + quarter;  // (past a row's items: any, the keys' are zeros)
+                            next[s] = *reinterpret_cast<const U32x4*>(row + (EXACT || chunk * 8 < p.dim ? chunk : 0) * 16);
                         }
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                            for (int i = 0; i < S::kLoads; ++i) keys[g][i] = S::load(from[g][i] + local * key_cache.head_bytes, p.dim);
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    load(0);
+                    for (int local = 0; local < heads; ++local) {
+                        wave_lds_order();
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g) S::write(tile + g * S::kBytes, keys[g], p.dim);
+#pragma unroll
+                        for (int s = 0; s < S::kSteps; ++s) a[s] = next[s];
+                        wave_lds_order();
+                        load(local + 1 < heads ? local + 1 : local);  // (the last one again: a load, but no branch)
+                        typename S::Operand k[kGroups];
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g) S::read(tile + g * S::kBytes, k[g]);
+                        const F32x4 base = *reinterpret_cast<const F32x4*>(&bases[local * kRowsAtOnce + 4 * quarter]);
+                        weigh<T>(sum, a, k, base, c, masked, arrays, request, p, row_base + 4 * quarter, key0);
                     }
                 }
+                meet(sum);
+                float total = sum[0];  // of group `quarter`
+#pragma unroll
+                for (int g = 1; g < kGroups; ++g) total = quarter == g ? sum[g] : total;
+                if (quarter < kGroups) request.put(arrays, p, key0 + lane, total, first);
             }
+            first = false;
         }
+    }
+}
+
+// Requests of more rows: a workgroup has 64 keys, its waves take the key heads in turn and go through their rows, the next tile on
+// its way while they work on one; the waves' sums meet in LDS.
+constexpr int kManyKeys = 64;
+constexpr int kTableHeads = 64;  // key heads that the table of rows holds at once
+constexpr int kTableRows = 2048;
+
+// Where each row of a few key heads lies, after the request's first, and its log-sum.  Rows that are not there are the first one,
+// with a log-sum of infinity.
+struct RowTable {
+    int64_t at[kTableRows];
+    __attribute__((aligned(16))) float base[kTableRows];
+};
+
+template <typename T, int DP, bool EXACT>
+__global__ __launch_bounds__(kWeightBlock) void attention_weights_many_kernel(Rows q, Pages key_cache, WeighArrays arrays, Weigh p) {
+    using S = Stage<DP, EXACT>;
+    constexpr int kGroups = kManyKeys / 16;
+    __shared__ RowTable table;
+    __shared__ __attribute__((aligned(16))) char staged[kWeightWaves][S::kBytes];
+    __shared__ float sums[kWeightWaves][kManyKeys];
+    const Request request(arrays, p, static_cast<int>(blockIdx.x / p.parts));
+    const int part = static_cast<int>(blockIdx.x % p.parts), lane = threadIdx.x % kWave;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), column = lane % 16, quarter = lane / 16;
+    const int units = (request.held + kManyKeys - 1) / kManyKeys;
+    if (part >= units || request.rows <= p.few) return;
+    const float c = p.scale * kLog2e;
+    const char* first_row = q.at(request.begin, 0);
+    char* stage = staged[wave];
+    // A few heads' rows at a time; what came before is in weights_out already.
+    const int heads_at_once = p.kv_heads < kTableHeads ? p.kv_heads : kTableHeads;
+    const int most_rows = kTableRows / heads_at_once / kRowsAtOnce * kRowsAtOnce;
+    bool first = true;
+    for (int row_base = 0; row_base < request.rows || first; row_base += most_rows) {
+        const int some = request.rows - row_base < most_rows ? request.rows - row_base : most_rows;
+        const int tiles = (some + kRowsAtOnce - 1) / kRowsAtOnce, table_rows = tiles * kRowsAtOnce;
+        for (int head_base = 0; head_base < p.kv_heads; head_base += heads_at_once) {
+            const int heads = p.kv_heads - head_base < heads_at_once ? p.kv_heads - head_base : heads_at_once;
+            __syncthreads();
+            for (int i = threadIdx.x; i < heads * table_rows; i += kWeightBlock) {
+                const int local = i / table_rows, row = i - local * table_rows;
+                const bool real = row < some;
+                const int at = real ? row_base + row : 0;
+                table.at[i] = request.row_at(q, p, head_base + local, at) - first_row;
+                table.base[i] = real ? request.base_of(arrays, p, head_base + local, at) : INFINITY;
+            }
+            __syncthreads();
+            for (int unit = part; unit < units; unit += static_cast<int>(p.parts)) {
+                const int key0 = unit * kManyKeys;
+                const bool masked = key0 + kManyKeys - 1 > (arrays.tree != nullptr ? request.ahead - 1 : request.ahead);
+                const int64_t own = key_at(key_cache, request, p, key0, kManyKeys);
+                float sum[kGroups] = {};
+                for (int local = wave; local < heads && tiles > 0; local += kWeightWaves) {
+                    typename S::Operand k[kGroups], a;
+                    typename S::Chunks rows;
+                    {
+                        typename S::Chunks keys[kGroups];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-            sum[g] += __shfl_xor(sum[g], 16);
-            sum[g] += __shfl_xor(sum[g], 32);
-            if (quarter == 0) sums[wave][16 * g + column] = sum[g];
-        }
-        __syncthreads();
-        if (threadIdx.x < kUnitKeys) {
-            const int j = key0 + static_cast<int>(threadIdx.x);
-            float total = 0.f;
+                        for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-            for (int w = 0; w < kWeightWaves; ++w) total += sums[w][threadIdx.x];
-            if (j < held) {
-                const uint32_t cell = p.page_size(j);
-                const int page = table[cell];
-                if (page >= 0 && page < p.pages) {
-                    const int64_t slot = static_cast<int64_t>(page) * p.page_size.by + (j - cell * p.page_size.by);
-                    weights_out[slot] = j < known && weights_in != nullptr ? weights_in[slot] * p.decay + total : total;
+                            for (int i = 0; i < S::kLoads; ++i)
+                                keys[g][i] = S::load(key_cache.at(0, 0, head_base + local) + __shfl(own, 16 * g + S::row(i)), p.dim);
+                        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                        for (int g = 0; g < kGroups; ++g) {
+                            wave_lds_order();
+                            S::write(stage, keys[g], p.dim);
+                            wave_lds_order();
+                            S::read(stage, k[g]);
+                        }
+                    }
+                    const auto load = [&](int tile) {
+#pragma unroll
+                        for (int i = 0; i < S::kLoads; ++i)
+                            rows[i] = S::load(first_row + table.at[local * table_rows + tile * kRowsAtOnce + S::row(i)], p.dim);
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    load(0);
+                    for (int tile = 0; tile < tiles; ++tile) {
+                        wave_lds_order();
+                        S::write(stage, rows, p.dim);
+                        wave_lds_order();
+                        load(tile + 1 < tiles ? tile + 1 : tile);
+                        S::read(stage, a);
+                        const int row0 = tile * kRowsAtOnce + 4 * quarter;
+                        const F32x4 base = *reinterpret_cast<const F32x4*>(&table.base[local * table_rows + row0]);
+                        weigh<T>(sum, a, k, base, c, masked, arrays, request, p, row_base + row0, key0);
+                    }
                 }
+                meet(sum);
+                if (quarter == 0)
+#pragma unroll
+                    for (int g = 0; g < kGroups; ++g) sums[wave][16 * g + column] = sum[g];
+                __syncthreads();
+                if (threadIdx.x < kManyKeys) {
+                    float total = 0.f;
+#pragma unroll
+                    for (int w = 0; w < kWeightWaves; ++w) total += sums[w][threadIdx.x];
+                    request.put(arrays, p, key0 + static_cast<int>(threadIdx.x), total, first);
+                }
+                __syncthreads();
             }
+            first = false;
         }
-        __syncthreads();
     }
 }
 
 // Workgroups wanted: a request's units are dealt out to so many that all requests make about this number.
-constexpr uint64_t kWeightGrid = 8192;
+constexpr uint64_t kFewGrid = 16384;
+constexpr uint64_t kManyGrid = 2048;
+// Rows of a key head up to which a request counts as one of few.
+constexpr int kFewRows = 16;
+
+template <typename T, int DP, bool EXACT>
+void launch_weights(const Rows& q, const Pages& key_cache, const WeighArrays& arrays, Weigh p, uint64_t max_kv_length, bool few, bool many,
+                    hipStream_t stream) {
+    const auto parts = [&](uint64_t keys, uint64_t grid) {
+        const uint64_t units = ceil_div(max_kv_length ? max_kv_length : 1, keys), wanted = ceil_div(grid, p.requests);
+        return static_cast<uint32_t>(units < wanted ? units : wanted);
+    };
+    if (few) {
+        p.parts = parts(kFewKeys * kWeightWaves, kFewGrid);
+        attention_weights_few_kernel<T, DP, EXACT><<<p.parts * p.requests, kWeightBlock, 0, stream>>>(q, key_cache, arrays, p);
+    }
+    if (many) {
+        p.parts = parts(kManyKeys, kManyGrid);
+        attention_weights_many_kernel<T, DP, EXACT><<<p.parts * p.requests, kWeightBlock, 0, stream>>>(q, key_cache, arrays, p);
+    }
+}
 
 template <typename T>
 int paged_weights(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const lcpp_hip_pages* key_cache, const int32_t* block_table,
@@ -199,19 +436,24 @@ int paged_weights(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const l
         return usable(q) ? set_error(kInvalidArgument, "%s: null lse", what) : unusable(what);
     const size_t needed = lcpp_hip_attention_paged_weights_temp_bytes(requests, q_tokens, max_kv_length, q_heads, kv_heads, dim);
     if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
-    const uint64_t units = ceil_div(max_kv_length ? max_kv_length : 1, kUnitKeys), wanted = ceil_div(kWeightGrid, requests);
-    const int splits = kv_heads >= kWeightWaves ? 1 : static_cast<int>(kWeightWaves / kv_heads);
+    // One token a request on average, or no more than a tile of rows in all: all requests count as ones of few rows.  More than
+    // that on average: all as ones of many.  Otherwise each goes by its own rows, in two launches.
+    const uint64_t group = q_heads / kv_heads, rows = q_tokens * group;
+    const bool all_few = (q_tokens <= requests && group <= kFewRows) || rows <= kFewRows, all_many = rows > uint64_t{requests} * kFewRows;
     const Weigh p{static_cast<int>(requests), static_cast<int>(q_tokens), static_cast<int>(q_heads), static_cast<int>(kv_heads),
                   static_cast<int>(dim), Divider(q_heads / kv_heads), Divider(page_size), static_cast<int>(pages),
-                  static_cast<int64_t>(table_stride), static_cast<int>(table_width),
-                  static_cast<uint32_t>(units < wanted ? units : wanted), splits, scale, decay};
+                  static_cast<int64_t>(table_stride), static_cast<int>(table_width), 0,
+                  all_few ? INT32_MAX : all_many ? -1 : kFewRows, scale, decay};
+    const WeighArrays arrays{block_table, q_offsets, kv_lengths, known_lengths, tree, lse, weights_in, weights_out};
     const Rows q_rows = q_tokens ? rows_of(q) : Rows{};
     LaunchScope scope(what, stream);
-    auto* kernel = dim <= 64   ? attention_weights_kernel<T, 64>
-                   : dim <= 96 ? attention_weights_kernel<T, 96>
-                               : attention_weights_kernel<T, 128>;
-    kernel<<<p.parts * requests, kWeightBlock, 0, stream>>>(
-        q_rows, pages_of(key_cache), block_table, q_offsets, kv_lengths, known_lengths, tree, lse, weights_in, weights_out, p);
+    auto* launch = dim == 64    ? launch_weights<T, 64, true>
+                   : dim < 64   ? launch_weights<T, 64, false>
+                   : dim == 96  ? launch_weights<T, 96, true>
+                   : dim < 96   ? launch_weights<T, 96, false>
+                   : dim == 128 ? launch_weights<T, 128, true>
+                                : launch_weights<T, 128, false>;
+    launch(q_rows, pages_of(key_cache), arrays, p, max_kv_length, !all_many, !all_few, stream);
     return check_hip(hipGetLastError(), "attention_paged_weights launch");
 }
 
