@@ -15,3 +15,4 @@
 #include "lcpp/device/device_segmented_sort.h"
 #include "lcpp/device/device_segmented_radix_sort.h"
 #include "lcpp/device/device_attention.h"
+#include "lcpp/device/device_recurrence.h"
