@@ -294,8 +294,8 @@ __device__ __forceinline__ float look_back(const Inputs& in, const Handed& h, co
     return value;
 }
 
-// Steps of serving: a lane walks its channels through a sequence of a token or two, kWalkRows at a time.
-constexpr int kWalkRows = 4;
+// Steps of serving: a lane walks its channels through a sequence of a token or a few, kWalkRows at a time.
+constexpr int kWalkRows = 8;
 
 template <typename T, int V, bool BACK>
 __global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape p, int blocks) {
@@ -497,12 +497,14 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void recurrence_kernel(Inputs in,
 // (A wave's rows lie within 2^30 bytes.)
 constexpr int64_t kMostStride = int64_t{1} << 24;
 
+constexpr uint64_t kWalkedMore = 64;
+
 // Waves of a chunk: one while sequences have no more than a wave's rows on average, else eight.
 constexpr int kLongWaves = 8;
 bool short_sequences(uint64_t sequences, uint64_t tokens) { return tokens <= sequences * kRows; }
 
-// Steps of serving, a token or two a sequence, are walked: no chunk hands anything on, and there is one launch.
-bool walked(uint64_t sequences, uint64_t tokens) { return tokens <= sequences * 2; }
+// Steps of serving, a token a sequence and a few more, are walked: no chunk hands anything on, and there is one launch.
+bool walked(uint64_t sequences, uint64_t tokens) { return tokens <= sequences + kWalkedMore; }
 
 uint64_t numbers_of(uint64_t sequences, uint64_t tokens) {
     return tokens / (short_sequences(sequences, tokens) ? kRows : kRows * kLongWaves) + sequences;

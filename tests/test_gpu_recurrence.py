@@ -74,6 +74,16 @@ def test_ragged(hip, dev, suffix):
     check(hip, suffix, [6000, 50, 50], 16, seed=7, span=3000.0)
 
 
+@pytest.mark.parametrize("suffix", ["bf16", "f16", "f32"])
+def test_steps_of_serving(hip, dev, suffix):
+    """Around a token a sequence, where a sequence is walked: among them ones of none and of many."""
+    for channels in (1, 33, 130, 260):
+        check(hip, suffix, [1] * 70 + [60], channels, seed=3)
+        check(hip, suffix, [0] * 200 + [240, 1, 0], channels, seed=4)
+        check(hip, suffix, [1, 2, 0, 7, 8, 9, 16, 17, 1], channels, seed=5, gap=3)
+    check(hip, suffix, [1] * 70 + [66], 64, seed=6)
+
+
 def test_no_tokens_and_no_sequences(hip, dev):
     none = torch.empty(0, 12, dtype=torch.bfloat16, device=dev)
     states = torch.randn(3, 12, device=dev)
