@@ -5,7 +5,11 @@
 // with the log-sums that attention over the same pages gave, and g the key head of h.  Scores, exponentials and sums are f32;
 // nothing is rounded to 16 bits.  Each key's sum has one owner and one order.
 //
-// Each key is read once; 2 * dim operations a row, head and key.  Matrix instruction: 16x16x32, rows of queries by keys: lane
+// Each key is read once, which bounds a decoding step: 256 requests of 200 to 4,000 keys (8 key heads of 128, 32 query heads), 669 MB in
+// 124 us, 5.4 TB/s, where reads alone reach 6.7.  The last 32 rows of three prompts of 9,000 to 60,000 keys: 22 GFLOP and 175 MB in
+// 62 us, bound by the latency of a tile: two or three waves a SIMD fit the registers.
+//
+// 2 * dim operations a row, head and key.  Matrix instruction: 16x16x32, rows of queries by keys: lane
 // l has key l % 16 of the result, rows 4 (l / 16) .. + 3, so that a key's weights of 16 rows lie in four lanes' registers and are
 // added up there; lanes meet once, at the end.
 #include "attention.hpp"
@@ -192,8 +196,9 @@ __device__ __forceinline__ void meet(float (&sum)[GROUPS]) {
     }
 }
 
-// Requests of few rows: a wave goes through the key heads of 32 keys, a tile of 16 rows at a time, the next head's keys on their way
-// while it works on one.
+// Requests of few rows: a wave goes through the key heads of 16 keys, a tile of 16 rows at a time, the next head's keys on their way
+// while it works on one.  (256 requests: 16 keys a wave 124 us, 32 keys 215, 64 keys 203, as more fit fewer waves; with lanes on a key each
+// instead of side by side on it 218.)
 constexpr int kFewKeys = 16;
 constexpr int kFewHeads = 32;  // key heads whose log-sums lie in LDS at once
 
@@ -277,9 +282,10 @@ __global__ __launch_bounds__(kWeightBlock) void attention_weights_few_kernel(Row
     }
 }
 
-// Requests of more rows: a workgroup has 64 keys, its waves take the key heads in turn and go through their rows, the next tile on
-// its way while they work on one; the waves' sums meet in LDS.
-constexpr int kManyKeys = 64;
+// Requests of more rows: a workgroup has 48 keys, its waves take the key heads in turn and go through their rows, the next tile on
+// its way while they work on one; the waves' sums meet in LDS.  (Three windows of 32 rows: 48 keys 59 us, 64 keys, which fill the
+// registers of two waves a SIMD, 62, 32 keys, which read the rows more often, 69.)
+constexpr int kManyKeys = 48;
 constexpr int kTableHeads = 64;  // key heads that the table of rows holds at once
 constexpr int kTableRows = 2048;
 
@@ -383,7 +389,9 @@ __global__ __launch_bounds__(kWeightBlock) void attention_weights_many_kernel(Ro
     }
 }
 
-// Workgroups wanted: a request's units are dealt out to so many that all requests make about this number.
+// Workgroups wanted at most: a request's units are dealt out to so many that all requests make about this number.  (Few rows, 256
+// requests: 4,096 149 us, 8,192 175, 16,384, a unit each, 123, 32,768 no better, and every one costs a look at its request's
+// length.  Many rows, which share a table of rows: 512 77 us, 2,048 62, 4,096 66.)
 constexpr uint64_t kFewGrid = 16384;
 constexpr uint64_t kManyGrid = 2048;
 // Rows of a key head up to which a request counts as one of few.

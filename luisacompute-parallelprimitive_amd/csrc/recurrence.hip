@@ -5,6 +5,11 @@
 //
 // States are f32; outputs are rounded once.  A state that remembers thousands of tokens adds up as many errors of exp(l): for
 // small l the step is h + (exp(l) - 1) h + x with exp(l) - 1 from its series, whose error is relative to l.
+//
+// Memory bounds the large calls: 3 items a channel and token forwards, 5 backwards, each once.  30,000 tokens of 4,096 channels in bf16:
+// forwards 738 MB in 213 us, 3.5 TB/s, backwards 1.23 GB in 276, 4.5, where the library's copy reaches 6.0.  A workgroup loads,
+// waits for its state and stores, and two of them on a compute unit do not cover each other's waits quite.  (One pass over the rows
+// by a thread a channel took 27.8 ms for both.)  2,000 tokens of 770 channels: 12 to 14 us a direction, the latency of one chunk.
 #include "common.hpp"
 #include "../../include/lcpp_hip.h"
 #include "attention.hpp"
@@ -76,7 +81,9 @@ __device__ __forceinline__ int64_t state_of(const int32_t* rows, int sequence, i
 
 // ---- chunks ------------------------------------------------------------------------------------------------------
 // A chunk of a sequence is waves of kRows tokens; a lane has V neighbouring channels of a token, 8 bytes of them where the
-// rows allow.  A chunk's effect on the state is h -> A h + B.  A workgroup reads its chunk into registers once, makes each wave's
+// rows allow.  (The two directions of 30,000 tokens: eight waves of 16 rows 466 us, four waves 479, eight of 8 rows 515, sixteen of 8
+// rows 554.  Sequences of a few hundred rows alone would take 26 us for 31 with eight waves of 8.)  A chunk's effect on the state
+// is h -> A h + B.  A workgroup reads its chunk into registers once, makes each wave's
 // (A, B) and the chunk's, hands that on, gets the state that enters the chunk, and goes through its rows again with it.  The
 // backward pass does the same towards the sequence's start, with c in the place of h.
 //
@@ -294,8 +301,39 @@ __device__ __forceinline__ float look_back(const Inputs& in, const Handed& h, co
     return value;
 }
 
-// Steps of serving: a lane walks its channels through a sequence of a token or a few, kWalkRows at a time.
+// Short sequences: a lane walks its channels through a sequence, kWalkRows tokens at a time, the next ones on their way while it
+// works on some.  256 states of 4,096 channels and a token each: 14.7 MB in 6 to 7 us, of which an empty launch takes 2 to 3.
 constexpr int kWalkRows = 8;
+
+template <typename T, int V, bool BACK>
+struct WalkRows {
+    using Vec = Items<typename T::Item, V>;
+    Vec x[kWalkRows], l[kWalkRows], h[BACK ? kWalkRows : 1];
+    // Tokens from `done` on (backwards, the sequence's last one first).
+    __device__ __forceinline__ void load(const Inputs& in, const Span& span, int64_t done, int row_bytes, uint32_t at) {
+        const int64_t left = span.size - done, token = BACK ? span.begin + left - kWalkRows : span.begin + done;
+        const int some = left < kWalkRows ? static_cast<int>(left) : kWalkRows;
+        // Backwards the last rows of the window are the sequence's next ones; a window that would begin before the sequence is short.
+        const int skip = BACK && left < kWalkRows ? kWalkRows - (left > 0 ? static_cast<int>(left) : 0) : 0;
+        const Window<Vec> first(in.first, token + skip, some, row_bytes), log_decay(in.log_decay, token + skip, some, row_bytes);
+#pragma unroll
+        for (int r = 0; r < kWalkRows; ++r) {
+            const int row = BACK ? kWalkRows - 1 - r - skip : r;  // (negative: nowhere)
+            const uint32_t from = BACK && row < 0 ? kNowhere : at;
+            x[r] = first.load(BACK && row < 0 ? 0 : row, from);
+            l[r] = log_decay.load(BACK && row < 0 ? 0 : row, from);
+        }
+        if constexpr (BACK) {
+            const int late = token + skip == span.begin;
+            const Window<Vec> out(in.out, token + skip - 1 + late, some - late, row_bytes);
+#pragma unroll
+            for (int r = 0; r < kWalkRows; ++r) {
+                const int row = kWalkRows - 1 - r - skip - late;
+                h[r] = out.load(row < 0 ? 0 : row, row < 0 ? kNowhere : at);
+            }
+        }
+    }
+};
 
 template <typename T, int V, bool BACK>
 __global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape p, int blocks) {
@@ -303,50 +341,58 @@ __global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape
     using Vec = Items<Item, V>;
     const int sequence = static_cast<int>(blockIdx.x / blocks);
     const int channel = (static_cast<int>(blockIdx.x % blocks) * kWave + static_cast<int>(threadIdx.x)) * V;
-    if (channel >= p.channels) return;
+    const bool active = channel < p.channels;
     const Span span = span_of(in.offsets, sequence, p.tokens);
     const int64_t held = BACK ? sequence : state_of(in.state_rows, sequence, p.num_states);
+    const int row_bytes = p.channels * static_cast<int>(sizeof(Item));
+    const uint32_t at = active ? static_cast<uint32_t>(channel) * sizeof(Item) : kNowhere;
+    WalkRows<T, V, BACK> even, odd;
+    even.load(in, span, 0, row_bytes, at);
     const float* from = BACK ? in.dfinal : in.initial;
-    float state[V];
+    float state[V], first[V];  // (backwards: the state before the first token)
 #pragma unroll
-    for (int v = 0; v < V; ++v) state[v] = from != nullptr && held >= 0 ? from[held * p.channels + channel + v] : 0.f;
-    const auto row = [&](const Steps& s, int64_t t) { return reinterpret_cast<Vec*>(s.template at<Item>(t) + channel); };
-    for (int64_t done = 0; done < span.size; done += kWalkRows) {
-        Vec x[kWalkRows], l[kWalkRows], h[kWalkRows];
+    for (int v = 0; v < V; ++v) {
+        state[v] = from != nullptr && held >= 0 && active ? from[held * p.channels + channel + v] : 0.f;
+        first[v] = BACK && in.initial != nullptr && active ? in.initial[held * p.channels + channel + v] : 0.f;
+    }
+    const auto work = [&](const WalkRows<T, V, BACK>& rows, int64_t done) {
+        const int64_t left = span.size - done;
+        const int some = left < kWalkRows ? static_cast<int>(left) : kWalkRows;
+        const int64_t token = BACK ? span.begin + left - some : span.begin + done;
+        const Window<Vec> a(BACK ? in.dx : in.out, token, some, row_bytes), b(BACK ? in.dlog_decay : in.out, token, BACK ? some : 0, row_bytes);
 #pragma unroll
-        for (int i = 0; i < kWalkRows; ++i) {
-            if (done + i >= span.size) continue;
-            const int64_t t = BACK ? span.begin + span.size - 1 - done - i : span.begin + done + i;
-            x[i] = *row(in.first, t);
-            l[i] = *row(in.log_decay, t);
-            if (BACK && t > span.begin) h[i] = *row(in.out, t - 1);
-        }
-#pragma unroll
-        for (int i = 0; i < kWalkRows; ++i) {
-            if (done + i >= span.size) continue;
-            const int64_t t = BACK ? span.begin + span.size - 1 - done - i : span.begin + done + i;
-            Vec a, b;
+        for (int r = 0; r < kWalkRows; ++r) {
+            if (r >= some) continue;
+            Vec g_row, l_row;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const Decay d(to_float<T>(l[i].at[v]));
-                const float input = to_float<T>(x[i].at[v]);
+                const Decay d(to_float<T>(rows.l[r].at[v]));
+                const float input = to_float<T>(rows.x[r].at[v]);
                 if constexpr (BACK) {
                     const float g = input + state[v];
                     state[v] = d.times(g);
-                    const float before = t > span.begin ? to_float<T>(h[i].at[v])
-                                         : in.initial != nullptr ? in.initial[held * p.channels + channel + v] : 0.f;
-                    a.at[v] = static_cast<Item>(g);
-                    b.at[v] = static_cast<Item>(state[v] * before);
+                    const float before = r + 1 < left ? to_float<T>(rows.h[r].at[v]) : first[v];
+                    g_row.at[v] = static_cast<Item>(g);
+                    l_row.at[v] = static_cast<Item>(state[v] * before);
                 } else {
                     state[v] = d.step(state[v], input);
-                    a.at[v] = static_cast<Item>(state[v]);
+                    g_row.at[v] = static_cast<Item>(state[v]);
                 }
             }
-            *row(BACK ? in.dx : in.out, t) = a;
-            if constexpr (BACK) *row(in.dlog_decay, t) = b;
+            a.store(BACK ? some - 1 - r : r, at, g_row);
+            if constexpr (BACK) b.store(some - 1 - r, at, l_row);
         }
+    };
+    for (int64_t done = 0; done < span.size; done += 2 * kWalkRows) {
+        odd.load(in, span, done + kWalkRows, row_bytes, at);
+        __builtin_amdgcn_sched_barrier(0);  // (sent before the rows in between are written, which they would wait for)
+        work(even, done);
+        if (done + kWalkRows >= span.size) break;
+        even.load(in, span, done + 2 * kWalkRows, row_bytes, at);
+        __builtin_amdgcn_sched_barrier(0);
+        work(odd, done + kWalkRows);
     }
-    if (in.last == nullptr || held < 0) return;
+    if (in.last == nullptr || held < 0 || !active) return;
 #pragma unroll
     for (int v = 0; v < V; ++v) in.last[held * p.channels + channel + v] = state[v];
 }
@@ -360,7 +406,7 @@ __global__ __launch_bounds__(kClearBlock) void recurrence_clear_kernel(Inputs in
     const int channel = static_cast<int>(blockIdx.x % blocks) * kClearBlock + static_cast<int>(threadIdx.x);
     Chunk chunk;
     const bool there = chunk.find<WAVES>(in.offsets, p, number);
-    if (!there || channel >= p.channels) return;
+    if (!there || chunk.chunks <= 1 || channel >= p.channels) return;  // (a chunk alone hands nothing on)
     uint32_t state = kNotYet;
     if (chunk.index == (BACK ? chunk.chunks - 1 : 0)) {
         if constexpr (BACK) {
@@ -497,14 +543,18 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void recurrence_kernel(Inputs in,
 // (A wave's rows lie within 2^30 bytes.)
 constexpr int64_t kMostStride = int64_t{1} << 24;
 
-constexpr uint64_t kWalkedMore = 64;
+constexpr uint64_t kWalkedEach = 2, kWalkedMore = 64;
 
-// Waves of a chunk: one while sequences have no more than a wave's rows on average, else eight.
+// Waves of a chunk: one while sequences have no more than 64 tokens on average, else eight (64 sequences of 32 tokens of 4,096 channels:
+// one 26 us, eight 34; of 100 tokens 62 and 54; 8 sequences of 1,000 tokens 94 and 52).
+constexpr uint64_t kShortEach = 64;
 constexpr int kLongWaves = 8;
-bool short_sequences(uint64_t sequences, uint64_t tokens) { return tokens <= sequences * kRows; }
+bool short_sequences(uint64_t sequences, uint64_t tokens) { return tokens <= sequences * kShortEach; }
 
-// Steps of serving, a token a sequence and a few more, are walked: no chunk hands anything on, and there is one launch.
-bool walked(uint64_t sequences, uint64_t tokens) { return tokens <= sequences + kWalkedMore; }
+// Sequences of a token or two on average are walked: no chunk hands anything on, and there is one launch (4,096 channels, 256 sequences of
+// one token 7 us, in chunks 17; of two 7.5 and 18).  The price is a batch of many short sequences and a long one, which a wave walks
+// at 0.2 us a token: 255 of one token and one of 300 take 66 us, in chunks 37.
+bool walked(uint64_t sequences, uint64_t tokens) { return tokens <= sequences * kWalkedEach + kWalkedMore; }
 
 uint64_t numbers_of(uint64_t sequences, uint64_t tokens) {
     return tokens / (short_sequences(sequences, tokens) ? kRows : kRows * kLongWaves) + sequences;

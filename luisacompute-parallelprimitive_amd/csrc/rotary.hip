@@ -8,6 +8,10 @@
 //
 // An angle of a far position has more bits than 32-bit floats hold: the turns, t / 2 pi, and what is left of them after whole
 // ones, are taken in 64 bits.  Turning is f32, rounded once.  A pair's sine and cosine serve all heads of a token.
+//
+// Memory bounds the large calls: each item is read and written once.  11,059 tokens of 32 + 8 heads of 128: 226 MB in 41.5 us,
+// 5.5 TB/s, where the library's copy of 1 GiB reaches 6.0; 32,749 tokens of 16 heads and 4 + 4 into pages: 403 MB in 74 us, 5.5.
+// A decoding step of 64 tokens takes 3.7 us, two or three dependent loads.
 #include "attention.hpp"
 
 #include <cmath>
@@ -80,7 +84,8 @@ struct TokenPlace {
 };
 
 // EACH units a thread of `group` tokens, or of a part of a token's (blockIdx.y).  Rows are loaded first; while they come, some
-// threads make the workgroup's table of cosines and sines and others look up the tokens' slots.
+// threads make the workgroup's table of cosines and sines and others look up the tokens' slots.  (With the slots looked up
+// before the rows were loaded, 32,749 tokens took 294 us.)
 template <typename T, Layout LAYOUT, bool PAGED, int EACH>
 __global__ __launch_bounds__(kTurnBlock) void rotary_kernel(TurnRows rows, const int32_t* __restrict__ positions,
                                                             const int32_t* __restrict__ requests, const int32_t* __restrict__ shifts,
@@ -217,7 +222,8 @@ __global__ __launch_bounds__(kTurnBlock) void rotary_kernel(TurnRows rows, const
     }
 }
 
-// Units a thread: four where that leaves a workgroup for every compute unit four times over, else one.
+// Units a thread: four where that leaves four workgroups for every compute unit, else one: fewer tables, and more bytes on their way
+// in each wave, against more waves for a few tokens.
 constexpr int kEach = 4;
 constexpr uint64_t kManyBlocks = 1024;
 constexpr uint64_t kMostPairs = 2048;  // of a workgroup's table, 16 KB

@@ -81,6 +81,7 @@ def test_steps_of_serving(hip, dev, suffix):
         check(hip, suffix, [1] * 70 + [60], channels, seed=3)
         check(hip, suffix, [0] * 200 + [240, 1, 0], channels, seed=4)
         check(hip, suffix, [1, 2, 0, 7, 8, 9, 16, 17, 1], channels, seed=5, gap=3)
+        check(hip, suffix, [4] * 50 + [63] + [0, 25, 24], channels, seed=7, states=False)
     check(hip, suffix, [1] * 70 + [66], 64, seed=6)
 
 
