@@ -5,7 +5,7 @@
 // with the log-sums that attention over the same pages gave, and g the key head of h.  Scores, exponentials and sums are f32;
 // nothing is rounded to 16 bits.  Each key's sum has one owner and one order.
 //
-// Each key is read once, which bounds a decoding step: 256 requests of 200 to 4,000 keys (8 key heads of 128, 32 query heads), 669 MB in
+// Each key is read once, and that bounds a decoding step: 256 requests of 200 to 4,000 keys (8 key heads of 128, 32 query heads), 669 MB in
 // 124 us, 5.4 TB/s, where reads alone reach 6.7.  The last 32 rows of three prompts of 9,000 to 60,000 keys: 22 GFLOP and 175 MB in
 // 62 us, bound by the latency of a tile: two or three waves a SIMD fit the registers.
 //

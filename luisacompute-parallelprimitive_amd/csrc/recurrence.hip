@@ -6,10 +6,11 @@
 // States are f32; outputs are rounded once.  A state that remembers thousands of tokens adds up as many errors of exp(l): for
 // small l the step is h + (exp(l) - 1) h + x with exp(l) - 1 from its series, whose error is relative to l.
 //
-// Memory bounds the large calls: 3 items a channel and token forwards, 5 backwards, each once.  30,000 tokens of 4,096 channels in bf16:
-// forwards 738 MB in 213 us, 3.5 TB/s, backwards 1.23 GB in 276, 4.5, where the library's copy reaches 6.0.  A workgroup loads,
-// waits for its state and stores, and two of them on a compute unit do not cover each other's waits quite.  (One pass over the rows
-// by a thread a channel took 27.8 ms for both.)  2,000 tokens of 770 channels: 12 to 14 us a direction, the latency of one chunk.
+// Memory bounds the large calls: 3 items a channel and token forwards, 5 backwards, each once, and 3% of what chunks hand on.
+// 34,222 tokens of 4,096 channels in bf16: forwards 0.84 GB in 213 us, 3.9 TB/s, backwards 1.40 GB in 276, 5.1, where the library's copy
+// reaches 6.0.  A workgroup loads, waits for its state and stores, and two of them on a compute unit do not quite cover each
+// other's waits (forwards without looking back, which is wrong, 183 us).  (One pass over the rows by a thread a channel took 27.8 ms
+// for both.)  1,900 tokens of 770 channels: 12 to 14 us a direction, the latency of one chunk.
 #include "common.hpp"
 #include "../../include/lcpp_hip.h"
 #include "attention.hpp"
@@ -81,7 +82,7 @@ __device__ __forceinline__ int64_t state_of(const int32_t* rows, int sequence, i
 
 // ---- chunks ------------------------------------------------------------------------------------------------------
 // A chunk of a sequence is waves of kRows tokens; a lane has V neighbouring channels of a token, 8 bytes of them where the
-// rows allow.  (The two directions of 30,000 tokens: eight waves of 16 rows 466 us, four waves 479, eight of 8 rows 515, sixteen of 8
+// rows allow.  (The two directions of 34,222 tokens: eight waves of 16 rows 466 us, four waves 479, eight of 8 rows 515, sixteen of 8
 // rows 554.  Sequences of a few hundred rows alone would take 26 us for 31 with eight waves of 8.)  A chunk's effect on the state
 // is h -> A h + B.  A workgroup reads its chunk into registers once, makes each wave's
 // (A, B) and the chunk's, hands that on, gets the state that enters the chunk, and goes through its rows again with it.  The
