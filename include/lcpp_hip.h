@@ -789,7 +789,8 @@ int lcpp_hip_page_release(const int32_t* kv_lengths, const int32_t* keep_lengths
  * key past the new end, move_from[r][i], goes to the i-th place of an evicted key before it, move_to[r][i], as slots (-1: the
  * page is not there); entries past the last move are -1.  A request makes at most min(K, n - K) moves; those past `width` are
  * left out (see page_release's most_moves).  positions (slots' positions) may be null where first and recent are 0, shifts where nothing
- * was evicted before.  kv_lengths are those before the eviction.  max_kv_length is the longest of them, or more. */
+ * was evicted before.  kv_lengths are those before the eviction.  max_kv_length is the longest of them, or more.  temp starts at a
+ * multiple of 16 bytes. */
 size_t lcpp_hip_evict_plan_temp_bytes(uint32_t requests, uint64_t max_kv_length);
 int lcpp_hip_evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_t* positions,
                         const int32_t* block_table, uint64_t table_stride, uint32_t table_width, const int32_t* kv_lengths,
@@ -822,7 +823,7 @@ LCPP_HIP_DECLARE_PAGED_MOVE(f16)
  * What is not finite stays in its channel and sequence.  Sums have one order: the same call gives the same bits.
  *
  * The backward pass takes dout, and dfinal [sequences][channels] f32 (null: 0), to dx, dlog_decay and dinitial [sequences][channels]
- * f32 (or null); `initial` is [sequences][channels].  dlog_decay = dh_t exp(log_decay_t) h_{t-1} takes h as `out` has it.
+ * f32 (or null); `initial` is [sequences][channels].  temp starts at a multiple of 8 bytes.  dlog_decay = dh_t exp(log_decay_t) h_{t-1} takes h as `out` has it.
  * ------------------------------------------------------------------------------------------- */
 
 /* [tokens][channels]: the channels contiguous, the tokens' stride in items. */

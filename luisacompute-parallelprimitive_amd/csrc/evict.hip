@@ -670,6 +670,8 @@ int evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_
         return check_hip(hipGetLastError(), "evict_plan launch");
     }
     if (requests * count > 0x7FFFFFFFull / kPartBlock) return set_error(kInvalidArgument, "%s: too many requests of such length", what);
+    if (reinterpret_cast<uintptr_t>(temp) % sizeof(PartCounts) != 0)
+        return set_error(kInvalidArgument, "%s: temp storage must be 16-byte aligned", what);
     const EvictArrays a{weights, positions, block_table, kv_lengths, kept_lengths, shifts};
     const Parts parts{static_cast<uint32_t*>(temp), reinterpret_cast<PartCounts*>(static_cast<char*>(temp) + bins_bytes(requests)),
                       static_cast<int>(count)};

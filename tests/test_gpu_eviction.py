@@ -270,6 +270,11 @@ def test_plan_of_long_requests(hip, dev):
     check_plan(hip, [140001], [4097], 128, values="signed")
 
 
+def test_plan_of_requests_longer_than_stated(hip, dev):
+    check_plan(hip, [140001, 30, 17000], [70000, 3, 1], 64, stated=20000, first=3, recent=9)
+    check_plan(hip, [20000, 16385, 100], [300, 16384, 99], 16, stated=16385, values="few")
+
+
 def test_plan_corners(hip, dev):
     check_plan(hip, [50, 50, 50], [10, 60, -4], 16)
     check_plan(hip, [50, 0], [10, 10], 16)

@@ -150,6 +150,20 @@ def test_token_by_token_is_the_scan(hip, dev):
         oracle.check("final", state, want["final"])
 
 
+def test_long_memories_that_decay_alike(hip, dev):
+    """Roundings of either sign add up like a random walk, 2^-24 times the square root of the 10,000 tokens that a state remembers: 6e-6.
+    One of the same sign in every token or chunk would be a hundred or ten times that."""
+    tokens, channels = 20000, 64
+    x = torch.randn(tokens, channels, generator=torch.Generator().manual_seed(1)).cuda()
+    l = -torch.logspace(-4, -1, channels).cuda().expand(tokens, channels).contiguous()
+    out, final = torch.empty_like(x), torch.empty(1, channels, device=dev)
+    hip.recurrence("f32", x, l, offsets_of([tokens]).cuda(), out, final=final)
+    state, decay = torch.zeros(channels, dtype=torch.float64, device=dev), l[0].double().exp()
+    for row in x.double():
+        state = decay * state + row
+    assert float((final[0].double() - state).norm()) <= 6e-6 * float(state.norm())
+
+
 def test_forgetting_and_growing(hip, dev):
     """-infinity forgets the state exactly; 0 keeps it; growth by a little is the formula's."""
     x, _, dout, initial, dfinal = made(5, "f32", [400, 70], 40)

@@ -171,6 +171,24 @@ def test_recurrence_refuses(hip):
             assert backward(hip, **{name: bad}) == hip.ERR_INVALID_ARGUMENT and "channels apart" in message(hip)
 
 
+def test_temporary_storage(hip):
+    """Enough of it, and aligned to the words that it holds."""
+    need = hip.recurrence_temp_bytes(2, 1000, 64)
+    r = hip.Steps(ALIGNED, 64)
+    call = lambda temp, size: hip.lib().lcpp_hip_recurrence_bf16(temp, size, r, r, ALIGNED, None, None, 0, r, None, 2, 1000, 64, None)
+    back = lambda temp, size: hip.lib().lcpp_hip_recurrence_backward_bf16(temp, size, r, r, r, ALIGNED, None, None, r, r, None, 2, 1000, 64, None)
+    for run in (call, back):
+        assert need > 0 and run(ALIGNED, need - 1) == hip.ERR_TEMP_TOO_SMALL and run(None, need) == hip.ERR_TEMP_TOO_SMALL
+        assert run(ALIGNED + 4, need) == hip.ERR_INVALID_ARGUMENT and "8-byte" in message(hip)
+    need = hip.evict_plan_temp_bytes(2, 100000)
+    run = lambda temp, size: hip.lib().lcpp_hip_evict_plan(temp, size, ALIGNED, None, ALIGNED, 4, 4, ALIGNED, ALIGNED, None, 2, 100000, 16, 9, 0,
+                                                           0, ALIGNED, ALIGNED, 8, None)
+    assert need > 0 and run(ALIGNED, need - 1) == hip.ERR_TEMP_TOO_SMALL and run(None, need) == hip.ERR_TEMP_TOO_SMALL
+    assert run(ALIGNED + 8, need) == hip.ERR_INVALID_ARGUMENT and "16-byte" in message(hip)
+    assert hip.recurrence_temp_bytes(0, 0, 64) == 0 and hip.recurrence_temp_bytes(256, 256, 4096) == 0
+    assert hip.evict_plan_temp_bytes(0, 100000) == 0 and hip.evict_plan_temp_bytes(256, 1040) == 0
+
+
 # ---- the binding ---------------------------------------------------------------------------------
 @pytest.fixture
 def never(hip, monkeypatch):
