@@ -604,8 +604,8 @@ __global__ __launch_bounds__(kMoveBlock) void paged_move_kernel(Pages key_cache,
 }
 
 // ---- host side ---------------------------------------------------------------------------------------------------
-// Workgroups of a request: one up to kLongRequest keys, then one for every kPartKeys.  (16 requests of up to 131,000 keys, the orders
-// read again in each of eight passes: one workgroup each 455 us.)
+// Workgroups of a request: one up to kLongRequest keys, then one for every kPartKeys.  (16 requests of 8,192 keys: one 18 us, parts 42; of
+// 16,384: 36 and 42; of 32,768: 55 and 43; of 65,536, more than registers hold: 224 and 48.)
 constexpr uint64_t kLongRequest = 16384;
 uint64_t parts_of(uint64_t max_kv_length) { return max_kv_length <= kLongRequest ? 1 : ceil_div(max_kv_length, kPartKeys); }
 size_t bins_bytes(uint64_t requests) { return align_up(requests * kDigits * kBins * sizeof(uint32_t), kViewAlign); }
@@ -686,10 +686,10 @@ int evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_
     return check_hip(hipGetLastError(), "evict_plan launch");
 }
 
-// Moves a thread: two where that leaves thirty-two workgroups for every compute unit, else one (moves of 16 long prompts: one 105 us,
-// two 77, four 103, eight 229; up to 16 moves of each of 256 requests: one 6.4, two 8.3).
+// Moves a thread: two where that leaves 64 workgroups for every compute unit, else one (rows of 8 heads of 128: 4,096 moves one 6.0 us,
+// two 7.6; 32,768: 43.0 and 45.4; 65,536: 114 and 86; the lists of 16 long prompts, most of them empty: 105 and 77, four 103, eight 229).
 constexpr int kMovesEach = 2;
-constexpr uint64_t kManyMoves = 16384;
+constexpr uint64_t kManyMoves = 32768;
 
 int paged_move(const int64_t* move_from, const int64_t* move_to, uint64_t moves, const lcpp_hip_pages* key_cache,
                const lcpp_hip_pages* value_cache, float* weights, int32_t* positions, uint32_t kv_heads, uint32_t dim, uint32_t page_size,
