@@ -757,7 +757,8 @@ LCPP_HIP_DECLARE_PAGED_WRITE_ROTARY(f16)
  * nothing is added).  Rows, pages, tree and the keys that a row sees are those of attention_paged, and lse [q_heads][q_tokens]
  * is what it gave; rows with an lse of -infinity give no weight.  weights_out may be weights_in.  Slots that hold no key of a
  * request are left as they are.  Requests share no slots.  max_kv_length, the longest request's length or more, only
- * says how a request is dealt out. */
+ * says how the work is dealt out.  temp, asked for with the call's own q_tokens and max_kv_length, holds the parts of sums
+ * whose rows several workgroups share (few keys, many rows; else no bytes); calls that may run at once need their own. */
 size_t lcpp_hip_attention_paged_weights_temp_bytes(uint32_t requests, uint64_t q_tokens, uint64_t max_kv_length,
                                                    uint32_t q_heads, uint32_t kv_heads, uint32_t head_dim);
 #define LCPP_HIP_DECLARE_ATTENTION_WEIGHTS(S)                                                                          \

@@ -45,8 +45,10 @@ struct Weigh {
     int pages;
     int64_t table_stride;
     int table_width;
-    uint32_t parts;  // workgroups of a request
-    int few;         // rows of a key head that make a request one of few
+    int few;      // rows of a key head that make a request one of few
+    int splits;   // workgroups that share the rows of a unit, if there are at most `units` units
+    int64_t units;
+    int each;     // workgroups of each request, where they are not dealt out over all
     float scale;
     float decay;
 };
@@ -98,12 +100,69 @@ struct Request {
         const int page = table[cell];
         return page < 0 || page >= p.pages ? -1 : static_cast<int64_t>(page) * p.page_size.by + (j - cell * p.page_size.by);
     }
-    __device__ __forceinline__ void put(const WeighArrays& a, const Weigh& p, int j, float total, bool first) const {
+    __device__ __forceinline__ void put(const WeighArrays& a, const Weigh& p, int j, float total) const {
         if (j >= held) return;
         const int64_t at = slot(p, j);
-        if (at < 0) return;
-        if (!first) a.weights_out[at] += total;
-        else a.weights_out[at] = j < known && a.weights_in != nullptr ? a.weights_in[at] * p.decay + total : total;
+        if (at >= 0) a.weights_out[at] = j < known && a.weights_in != nullptr ? a.weights_in[at] * p.decay + total : total;
+    }
+};
+
+// Units of KEYS keys of the requests of a kind: each request's by `each` workgroups of its own, or (FLAT) numbered over all requests.
+// Then a workgroup counts them for itself, kWeightBlock requests at a time, and takes every gridDim.x-th, so that long and short
+// requests fill the device alike.  f(request, its unit, the unit's number, which of the workgroups that share its rows, how many do).
+template <int KEYS, bool FEW, bool FLAT>
+struct Units {
+    template <typename F>
+    __device__ __forceinline__ void each(const WeighArrays& a, const Weigh& p, F f) {
+        const int r = blockIdx.x / p.each;
+        const Request request(a, p, r);
+        if ((request.rows <= p.few) != FEW) return;
+        const int all = (request.held + KEYS - 1) / KEYS;
+        for (int unit = blockIdx.x % p.each; unit < all; unit += p.each) f(r, unit, int64_t{0}, 0, 1);
+    }
+};
+template <int KEYS, bool FEW>
+struct Units<KEYS, FEW, true> {
+    int64_t sums[kWeightWaves];
+    int64_t begins[kWeightBlock];
+    template <typename F>
+    __device__ __forceinline__ void each(const WeighArrays& a, const Weigh& p, F f) {
+        const int wave = threadIdx.x / kWave;
+        int64_t before = 0, next = blockIdx.x;
+        for (int base = 0; base < p.requests; base += kWeightBlock) {
+            const int r = base + static_cast<int>(threadIdx.x);
+            int64_t mine = 0;
+            if (r < p.requests) {
+                const Request request(a, p, r);
+                if ((request.rows <= p.few) == FEW) mine = (request.held + KEYS - 1) / KEYS;
+            }
+            const int64_t inclusive = wave_inclusive_scan(mine, SumOp{});
+            __syncthreads();
+            if (threadIdx.x % kWave == kWave - 1) sums[wave] = inclusive;
+            __syncthreads();
+            int64_t begin = inclusive - mine, total = 0;
+#pragma unroll
+            for (int w = 0; w < kWeightWaves; ++w) {
+                begin += w < wave ? sums[w] : 0;
+                total += sums[w];
+            }
+            begins[threadIdx.x] = begin;
+            __syncthreads();
+            // (Splits are for a few requests alone, which are all counted here.)
+            const int splits = p.splits > 1 && total <= p.units ? p.splits : 1;
+            for (; next < before + total * splits; next += gridDim.x) {
+                const int64_t number = (next - before) / splits;
+                int low = 0, high = kWeightBlock;
+                while (high - low > 1) {
+                    const int middle = low + (high - low) / 2;
+                    if (begins[middle] <= number) low = middle;
+                    else high = middle;
+                }
+                low = __builtin_amdgcn_readfirstlane(low);
+                f(base + low, static_cast<int>(number - begins[low]), number, static_cast<int>((next - before) % splits), splits);
+            }
+            before += total * splits;
+        }
     }
 };
 
@@ -202,84 +261,81 @@ __device__ __forceinline__ void meet(float (&sum)[GROUPS]) {
 constexpr int kFewKeys = 16;
 constexpr int kFewHeads = 32;  // key heads whose log-sums lie in LDS at once
 
-template <typename T, int DP, bool EXACT>
+template <typename T, int DP, bool EXACT, bool FLAT>
 __global__ __launch_bounds__(kWeightBlock) void attention_weights_few_kernel(Rows q, Pages key_cache, WeighArrays arrays, Weigh p) {
     using S = Stage<DP, EXACT>;
     constexpr int kGroups = kFewKeys / 16;
     __shared__ __attribute__((aligned(16))) char staged[kWeightWaves][kGroups * S::kBytes];
     __shared__ __attribute__((aligned(16))) float bases[kFewHeads * kRowsAtOnce];
-    const Request request(arrays, p, static_cast<int>(blockIdx.x / p.parts));
-    const int part = static_cast<int>(blockIdx.x % p.parts), lane = threadIdx.x % kWave;
+    __shared__ Units<kFewKeys * kWeightWaves, true, FLAT> units;
+    const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), column = lane % 16, quarter = lane / 16;
-    const int units = (request.held + kFewKeys - 1) / kFewKeys;
-    if (part * kWeightWaves >= units || request.rows > p.few) return;
     const float c = p.scale * kLog2e;
     char* tile = staged[wave];
-    bool first = true;
-    for (int row_base = 0; row_base < request.rows || first; row_base += kRowsAtOnce) {
-        // (Rows that are not there are the first one with a log-sum of infinity: they weigh nothing.)
-        const int mine = row_base + column < request.rows ? row_base + column : 0;
-        for (int head_base = 0; head_base < p.kv_heads; head_base += kFewHeads) {
-            const int heads = p.kv_heads - head_base < kFewHeads ? p.kv_heads - head_base : kFewHeads;
-            if (row_base + head_base > 0) __syncthreads();
-            for (int i = threadIdx.x; i < heads * kRowsAtOnce; i += kWeightBlock) {
-                const int row = row_base + i % kRowsAtOnce;
-                bases[i] = row < request.rows ? request.base_of(arrays, p, head_base + i / kRowsAtOnce, row) : INFINITY;
-            }
-            __syncthreads();
-            for (int unit = part * kWeightWaves + wave; unit < units; unit += static_cast<int>(p.parts) * kWeightWaves) {
-                const int key0 = unit * kFewKeys;
-                // Rows that see every key of the unit need no masks.
-                const bool masked = key0 + kFewKeys - 1 > (arrays.tree != nullptr ? request.ahead - 1 : request.ahead);
-                float sum[kGroups] = {};
-                if (request.rows > 0) {
-                    const int64_t own = key_at(key_cache, request, p, key0, kFewKeys);
-                    const char* from[kGroups][S::kLoads];
+    units.each(arrays, p, [&](int index, int unit, int64_t, int, int) {
+        const Request request(arrays, p, index);
+        const int key0 = (unit * kWeightWaves + wave) * kFewKeys;
+        const bool some = key0 < request.held;
+        // Rows that see every key of the unit need no masks.
+        const bool masked = key0 + kFewKeys - 1 > (arrays.tree != nullptr ? request.ahead - 1 : request.ahead);
+        const int64_t own = key_at(key_cache, request, p, some ? key0 : 0, kFewKeys);
+        float sum[kGroups] = {};
+        for (int row_base = 0; row_base < request.rows; row_base += kRowsAtOnce) {
+            // (Rows that are not there are the first one with a log-sum of infinity: they weigh nothing.)
+            const int mine = row_base + column < request.rows ? row_base + column : 0;
+            for (int head_base = 0; head_base < p.kv_heads; head_base += kFewHeads) {
+                const int heads = p.kv_heads - head_base < kFewHeads ? p.kv_heads - head_base : kFewHeads;
+                __syncthreads();
+                for (int i = threadIdx.x; i < heads * kRowsAtOnce; i += kWeightBlock) {
+                    const int row = row_base + i % kRowsAtOnce;
+                    bases[i] = row < request.rows ? request.base_of(arrays, p, head_base + i / kRowsAtOnce, row) : INFINITY;
+                }
+                __syncthreads();
+                if (!some) continue;
+                const char* from[kGroups][S::kLoads];
+#pragma unroll
+                for (int g = 0; g < kGroups; ++g)
+#pragma unroll
+                    for (int i = 0; i < S::kLoads; ++i)
+                        from[g][i] = key_cache.data + head_base * key_cache.head_bytes + __shfl(own, 16 * g + S::row(i));
+                typename S::Chunks keys[kGroups];
+                typename S::Operand a, next;
+                const auto load = [&](int local) {
+                    const char* row = request.row_at(q, p, head_base + local, mine);
+#pragma unroll
+                    for (int s = 0; s < S::kSteps; ++s) {
+                        const int chunk = 4 * s + quarter;  // (past a row's items: any, the keys' are zeros)
+                        next[s] = *reinterpret_cast<const U32x4*>(row + (EXACT || chunk * 8 < p.dim ? chunk : 0) * 16);
+                    }
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g)
 #pragma unroll
-                        for (int i = 0; i < S::kLoads; ++i)
-                            from[g][i] = key_cache.data + head_base * key_cache.head_bytes + __shfl(own, 16 * g + S::row(i));
-                    typename S::Chunks keys[kGroups];
-                    typename S::Operand a, next;
-                    const auto load = [&](int local) {
-                        const char* row = request.row_at(q, p, head_base + local, mine);
+                        for (int i = 0; i < S::kLoads; ++i) keys[g][i] = S::load(from[g][i] + local * key_cache.head_bytes, p.dim);
+                    __builtin_amdgcn_sched_barrier(0);
+                };
+                load(0);
+                for (int local = 0; local < heads; ++local) {
+                    wave_lds_order();
 #pragma unroll
-                        for (int s = 0; s < S::kSteps; ++s) {
-                            const int chunk = 4 * s + quarter;  // (past a row's items: any, the keys' are zeros)
-                            next[s] = *reinterpret_cast<const U32x4*>(row + (EXACT || chunk * 8 < p.dim ? chunk : 0) * 16);
-                        }
+                    for (int g = 0; g < kGroups; ++g) S::write(tile + g * S::kBytes, keys[g], p.dim);
 #pragma unroll
-                        for (int g = 0; g < kGroups; ++g)
+                    for (int s = 0; s < S::kSteps; ++s) a[s] = next[s];
+                    wave_lds_order();
+                    load(local + 1 < heads ? local + 1 : local);  // (the last one again: a load, but no branch)
+                    typename S::Operand k[kGroups];
 #pragma unroll
-                            for (int i = 0; i < S::kLoads; ++i) keys[g][i] = S::load(from[g][i] + local * key_cache.head_bytes, p.dim);
-                        __builtin_amdgcn_sched_barrier(0);
-                    };
-                    load(0);
-                    for (int local = 0; local < heads; ++local) {
-                        wave_lds_order();
-#pragma unroll
-                        for (int g = 0; g < kGroups; ++g) S::write(tile + g * S::kBytes, keys[g], p.dim);
-#pragma unroll
-                        for (int s = 0; s < S::kSteps; ++s) a[s] = next[s];
-                        wave_lds_order();
-                        load(local + 1 < heads ? local + 1 : local);  // (the last one again: a load, but no branch)
-                        typename S::Operand k[kGroups];
-#pragma unroll
-                        for (int g = 0; g < kGroups; ++g) S::read(tile + g * S::kBytes, k[g]);
-                        const F32x4 base = *reinterpret_cast<const F32x4*>(&bases[local * kRowsAtOnce + 4 * quarter]);
-                        weigh<T>(sum, a, k, base, c, masked, arrays, request, p, row_base + 4 * quarter, key0);
-                    }
+                    for (int g = 0; g < kGroups; ++g) S::read(tile + g * S::kBytes, k[g]);
+                    const F32x4 base = *reinterpret_cast<const F32x4*>(&bases[local * kRowsAtOnce + 4 * quarter]);
+                    weigh<T>(sum, a, k, base, c, masked, arrays, request, p, row_base + 4 * quarter, key0);
                 }
-                meet(sum);
-                float total = sum[0];  // of group `quarter`
-#pragma unroll
-                for (int g = 1; g < kGroups; ++g) total = quarter == g ? sum[g] : total;
-                if (quarter < kGroups) request.put(arrays, p, key0 + lane, total, first);
             }
-            first = false;
         }
-    }
+        meet(sum);
+        float total = sum[0];  // of group `quarter`
+#pragma unroll
+        for (int g = 1; g < kGroups; ++g) total = quarter == g ? sum[g] : total;
+        if (quarter < kGroups) request.put(arrays, p, key0 + lane, total);
+    });
 }
 
 // Requests of more rows: a workgroup has 48 keys, its waves take the key heads in turn and go through their rows, the next tile on
@@ -296,45 +352,52 @@ struct RowTable {
     __attribute__((aligned(16))) float base[kTableRows];
 };
 
-template <typename T, int DP, bool EXACT>
-__global__ __launch_bounds__(kWeightBlock) void attention_weights_many_kernel(Rows q, Pages key_cache, WeighArrays arrays, Weigh p) {
+template <typename T, int DP, bool EXACT, bool FLAT>
+__global__ __launch_bounds__(kWeightBlock, 3) void attention_weights_many_kernel(Rows q, Pages key_cache, WeighArrays arrays, float* partial,
+                                                                              Weigh p) {
     using S = Stage<DP, EXACT>;
     constexpr int kGroups = kManyKeys / 16;
     __shared__ RowTable table;
     __shared__ __attribute__((aligned(16))) char staged[kWeightWaves][S::kBytes];
     __shared__ float sums[kWeightWaves][kManyKeys];
-    const Request request(arrays, p, static_cast<int>(blockIdx.x / p.parts));
-    const int part = static_cast<int>(blockIdx.x % p.parts), lane = threadIdx.x % kWave;
+    __shared__ Units<kManyKeys, false, FLAT> units;
+    const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), column = lane % 16, quarter = lane / 16;
-    const int units = (request.held + kManyKeys - 1) / kManyKeys;
-    if (part >= units || request.rows <= p.few) return;
     const float c = p.scale * kLog2e;
-    const char* first_row = q.at(request.begin, 0);
     char* stage = staged[wave];
-    // A few heads' rows at a time; what came before is in weights_out already.
     const int heads_at_once = p.kv_heads < kTableHeads ? p.kv_heads : kTableHeads;
     const int most_rows = kTableRows / heads_at_once / kRowsAtOnce * kRowsAtOnce;
-    bool first = true;
-    for (int row_base = 0; row_base < request.rows || first; row_base += most_rows) {
-        const int some = request.rows - row_base < most_rows ? request.rows - row_base : most_rows;
-        const int tiles = (some + kRowsAtOnce - 1) / kRowsAtOnce, table_rows = tiles * kRowsAtOnce;
-        for (int head_base = 0; head_base < p.kv_heads; head_base += heads_at_once) {
-            const int heads = p.kv_heads - head_base < heads_at_once ? p.kv_heads - head_base : heads_at_once;
-            __syncthreads();
-            for (int i = threadIdx.x; i < heads * table_rows; i += kWeightBlock) {
-                const int local = i / table_rows, row = i - local * table_rows;
-                const bool real = row < some;
-                const int at = real ? row_base + row : 0;
-                table.at[i] = request.row_at(q, p, head_base + local, at) - first_row;
-                table.base[i] = real ? request.base_of(arrays, p, head_base + local, at) : INFINITY;
-            }
-            __syncthreads();
-            for (int unit = part; unit < units; unit += static_cast<int>(p.parts)) {
-                const int key0 = unit * kManyKeys;
-                const bool masked = key0 + kManyKeys - 1 > (arrays.tree != nullptr ? request.ahead - 1 : request.ahead);
-                const int64_t own = key_at(key_cache, request, p, key0, kManyKeys);
-                float sum[kGroups] = {};
-                for (int local = wave; local < heads && tiles > 0; local += kWeightWaves) {
+    int held_request = -1;  // whose rows all lie in the table
+    units.each(arrays, p, [&](int index, int unit, int64_t number, int split, int splits) {
+        const Request request(arrays, p, index);
+        const char* first_row = q.at(request.begin, 0);
+        const int key0 = unit * kManyKeys;
+        const bool masked = key0 + kManyKeys - 1 > (arrays.tree != nullptr ? request.ahead - 1 : request.ahead);
+        const int64_t own = key_at(key_cache, request, p, key0, kManyKeys);
+        // The split's tiles of rows.
+        const int all_tiles = (request.rows + kRowsAtOnce - 1) / kRowsAtOnce, per = (all_tiles + splits - 1) / splits;
+        const int first_tile = split * per < all_tiles ? split * per : all_tiles;
+        const int tile_end = first_tile + per < all_tiles ? first_tile + per : all_tiles;
+        const int row_first = first_tile * kRowsAtOnce, row_end = tile_end < all_tiles ? tile_end * kRowsAtOnce : request.rows;
+        float sum[kGroups] = {};
+        for (int row_base = row_first; row_base < row_end; row_base += most_rows) {
+            const int some = row_end - row_base < most_rows ? row_end - row_base : most_rows;
+            const int tiles = (some + kRowsAtOnce - 1) / kRowsAtOnce, table_rows = tiles * kRowsAtOnce;
+            for (int head_base = 0; head_base < p.kv_heads; head_base += heads_at_once) {
+                const int heads = p.kv_heads - head_base < heads_at_once ? p.kv_heads - head_base : heads_at_once;
+                if (held_request != index) {
+                    __syncthreads();
+                    for (int i = threadIdx.x; i < heads * table_rows; i += kWeightBlock) {
+                        const int local = i / table_rows, row = i - local * table_rows;
+                        const bool real = row < some;
+                        const int at = real ? row_base + row : 0;
+                        table.at[i] = request.row_at(q, p, head_base + local, at) - first_row;
+                        table.base[i] = real ? request.base_of(arrays, p, head_base + local, at) : INFINITY;
+                    }
+                    __syncthreads();
+                    held_request = splits == 1 && some == request.rows && heads == p.kv_heads ? index : -1;
+                }
+                for (int local = wave; local < heads; local += kWeightWaves) {
                     typename S::Operand k[kGroups], a;
                     typename S::Chunks rows;
                     {
@@ -371,47 +434,92 @@ __global__ __launch_bounds__(kWeightBlock) void attention_weights_many_kernel(Ro
                         weigh<T>(sum, a, k, base, c, masked, arrays, request, p, row_base + row0, key0);
                     }
                 }
-                meet(sum);
-                if (quarter == 0)
-#pragma unroll
-                    for (int g = 0; g < kGroups; ++g) sums[wave][16 * g + column] = sum[g];
-                __syncthreads();
-                if (threadIdx.x < kManyKeys) {
-                    float total = 0.f;
-#pragma unroll
-                    for (int w = 0; w < kWeightWaves; ++w) total += sums[w][threadIdx.x];
-                    request.put(arrays, p, key0 + static_cast<int>(threadIdx.x), total, first);
-                }
-                __syncthreads();
             }
-            first = false;
         }
-    }
+        meet(sum);
+        __syncthreads();
+        if (quarter == 0)
+#pragma unroll
+            for (int g = 0; g < kGroups; ++g) sums[wave][16 * g + column] = sum[g];
+        __syncthreads();
+        if (threadIdx.x < kManyKeys) {
+            float total = 0.f;
+#pragma unroll
+            for (int w = 0; w < kWeightWaves; ++w) total += sums[w][threadIdx.x];
+            if (FLAT && splits > 1) partial[(split * p.units + number) * kManyKeys + threadIdx.x] = total;
+            else request.put(arrays, p, key0 + static_cast<int>(threadIdx.x), total);
+        }
+    });
 }
 
-// Workgroups wanted at most: a request's units are dealt out to so many that all requests make about this number.  (Few rows, 256
-// requests: 4,096 149 us, 8,192 175, 16,384, a unit each, 123, 32,768 no better, and every one costs a look at its request's
-// length.  Many rows, which share a table of rows: 512 77 us, 2,048 62, 4,096 66.)
-constexpr uint64_t kFewGrid = 16384;
-constexpr uint64_t kManyGrid = 2048;
+// Adds up the splits of each unit, in their order.
+__global__ __launch_bounds__(kWeightBlock) void attention_weights_join_kernel(const float* __restrict__ partial, WeighArrays arrays, Weigh p) {
+    __shared__ Units<kManyKeys, false, true> units;
+    units.each(arrays, p, [&](int index, int unit, int64_t number, int split, int splits) {
+        if (splits == 1 || split != 0 || threadIdx.x >= kManyKeys) return;
+        float total = 0.f;
+        for (int i = 0; i < splits; ++i) total += partial[(i * p.units + number) * kManyKeys + threadIdx.x];
+        const Request request(arrays, p, index);
+        request.put(arrays, p, unit * kManyKeys + static_cast<int>(threadIdx.x), total);
+    });
+}
+
+// Workgroups of each request: as many as it has units at the stated length, as long as all have so many together (256 requests of
+// one token and up to 4,000 keys: 124 us; three windows of 32 rows, 683 a request: 59).
+constexpr uint64_t kFewOwn = 16384;
+constexpr uint64_t kManyOwn = 2048;
+// Where that leaves a request fewer than it has units and than the device has compute units, the longest would decide, and all units
+// are dealt out to so many workgroups: twice and once what the device holds at a time (256 requests of a token: 138 us with 768, 132
+// with 1,536, 145 with 8,192; 64 of 16 tokens: 85 us with 512, 97 with 768, 89 with 2,048).  A request of 500 tokens over 8,000 keys
+// among 255 of one: 445 us, by request 2,891; 256 requests of one token over 1,300 keys each: 138 us, by request 130.
+constexpr uint64_t kFlatBelow = 256;
+constexpr uint64_t kFewGrid = 1536;
+constexpr uint64_t kManyGrid = 512;
+// Workgroups wanted where rows are split (one request of 4,096 tokens over 8,192 keys: 2,481 us unsplit, 1,344 with 512, 862 with
+// 1,024; at 867 us 240 TFLOP/s: each tile of 16 rows passes LDS for each 48 keys).
+constexpr uint64_t kSplitGrid = 1024;
 // Rows of a key head up to which a request counts as one of few.
 constexpr int kFewRows = 16;
 
+bool is_few(uint64_t requests, uint64_t q_tokens, uint64_t group) {
+    return (q_tokens <= requests && group <= kFewRows) || q_tokens * group <= kFewRows;
+}
+
+// Workgroups that share a unit's rows: as many as the grid has for each unit, where there are few units of many rows (in requests of
+// the stated length, at most kWeightBlock of them), and each has four tiles of rows at least.
+struct Split {
+    uint64_t splits, units;
+    Split(uint64_t requests, uint64_t q_tokens, uint64_t max_kv_length, uint64_t q_heads, uint64_t kv_heads) {
+        units = requests * ceil_div(max_kv_length ? max_kv_length : 1, kManyKeys);
+        const uint64_t rows = kv_heads ? q_tokens * (q_heads / kv_heads) : 0, tiles = rows / (4 * kRowsAtOnce);
+        splits = requests == 0 || requests > kWeightBlock || units > kSplitGrid / 2 ? 1 : kSplitGrid / units;
+        splits = splits < tiles ? splits : tiles ? tiles : 1;
+    }
+    size_t bytes() const { return splits > 1 ? align_up(splits * units * kManyKeys * sizeof(float), kViewAlign) : 0; }
+};
+
 template <typename T, int DP, bool EXACT>
-void launch_weights(const Rows& q, const Pages& key_cache, const WeighArrays& arrays, Weigh p, uint64_t max_kv_length, bool few, bool many,
-                    hipStream_t stream) {
-    const auto parts = [&](uint64_t keys, uint64_t grid) {
-        const uint64_t units = ceil_div(max_kv_length ? max_kv_length : 1, keys), wanted = ceil_div(grid, p.requests);
-        return static_cast<uint32_t>(units < wanted ? units : wanted);
+void launch_weights(const Rows& q, const Pages& key_cache, const WeighArrays& arrays, float* partial, const Weigh& p, uint64_t max_kv_length,
+                    bool few, bool many, hipStream_t stream) {
+    const auto launch = [&](auto own_kernel, auto flat_kernel, uint64_t keys, uint64_t most_own, uint64_t most, int splits, auto... arguments) {
+        const uint64_t each = ceil_div(max_kv_length ? max_kv_length : 1, keys), units = p.requests * each * splits;
+        const uint64_t share = ceil_div(most_own, uint64_t(p.requests)), parts = share < each ? share : each;
+        Weigh by = p;
+        by.splits = splits;
+        by.each = static_cast<int>(parts);
+        if (splits > 1 || (parts < each && parts < kFlatBelow))
+            flat_kernel<<<static_cast<unsigned>(splits > 1 || units < most ? units : most), kWeightBlock, 0, stream>>>(arguments..., by);
+        else
+            own_kernel<<<static_cast<unsigned>(parts * p.requests), kWeightBlock, 0, stream>>>(arguments..., by);
     };
-    if (few) {
-        p.parts = parts(kFewKeys * kWeightWaves, kFewGrid);
-        attention_weights_few_kernel<T, DP, EXACT><<<p.parts * p.requests, kWeightBlock, 0, stream>>>(q, key_cache, arrays, p);
-    }
-    if (many) {
-        p.parts = parts(kManyKeys, kManyGrid);
-        attention_weights_many_kernel<T, DP, EXACT><<<p.parts * p.requests, kWeightBlock, 0, stream>>>(q, key_cache, arrays, p);
-    }
+    if (few)
+        launch(attention_weights_few_kernel<T, DP, EXACT, false>, attention_weights_few_kernel<T, DP, EXACT, true>,
+               kFewKeys * kWeightWaves, kFewOwn, kFewGrid, 1, q, key_cache, arrays);
+    if (many)
+        launch(attention_weights_many_kernel<T, DP, EXACT, false>, attention_weights_many_kernel<T, DP, EXACT, true>, kManyKeys, kManyOwn,
+               kManyGrid, p.splits, q, key_cache, arrays, partial);
+    if (many && p.splits > 1)
+        launch(attention_weights_join_kernel, attention_weights_join_kernel, kManyKeys, kManyOwn, kManyGrid, p.splits, partial, arrays);
 }
 
 template <typename T>
@@ -444,14 +552,19 @@ int paged_weights(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const l
         return usable(q) ? set_error(kInvalidArgument, "%s: null lse", what) : unusable(what);
     const size_t needed = lcpp_hip_attention_paged_weights_temp_bytes(requests, q_tokens, max_kv_length, q_heads, kv_heads, dim);
     if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
+    if (needed && reinterpret_cast<uintptr_t>(temp) % alignof(float) != 0)
+        return set_error(kInvalidArgument, "%s: temp storage must be 4-byte aligned", what);
     // One token a request on average, or no more than a tile of rows in all: all requests count as ones of few rows.  More than
-    // that on average: all as ones of many.  Otherwise each goes by its own rows, in two launches.
-    const uint64_t group = q_heads / kv_heads, rows = q_tokens * group;
-    const bool all_few = (q_tokens <= requests && group <= kFewRows) || rows <= kFewRows, all_many = rows > uint64_t{requests} * kFewRows;
+    // that on average: all as ones of many.  Otherwise each goes by its own rows, in two launches.  (256 requests of one token: 130 us,
+    // 135 with the second launch; a request of 200 tokens over 8,000 keys among 255 of none: 320 us, 130 with it.)
+    const uint64_t group = q_heads / kv_heads;
+    const bool all_few = is_few(requests, q_tokens, group), all_many = q_tokens * group > uint64_t{requests} * kFewRows;
+    const Split split(requests, all_few ? 0 : q_tokens, max_kv_length, q_heads, kv_heads);
     const Weigh p{static_cast<int>(requests), static_cast<int>(q_tokens), static_cast<int>(q_heads), static_cast<int>(kv_heads),
                   static_cast<int>(dim), Divider(q_heads / kv_heads), Divider(page_size), static_cast<int>(pages),
-                  static_cast<int64_t>(table_stride), static_cast<int>(table_width), 0,
-                  all_few ? INT32_MAX : all_many ? -1 : kFewRows, scale, decay};
+                  static_cast<int64_t>(table_stride), static_cast<int>(table_width),
+                  all_few ? INT32_MAX : all_many ? -1 : kFewRows,
+                  static_cast<int>(split.splits), static_cast<int64_t>(split.units), 0, scale, decay};
     const WeighArrays arrays{block_table, q_offsets, kv_lengths, known_lengths, tree, lse, weights_in, weights_out};
     const Rows q_rows = q_tokens ? rows_of(q) : Rows{};
     LaunchScope scope(what, stream);
@@ -461,7 +574,7 @@ int paged_weights(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const l
                    : dim < 96   ? launch_weights<T, 96, false>
                    : dim == 128 ? launch_weights<T, 128, true>
                                 : launch_weights<T, 128, false>;
-    launch(q_rows, pages_of(key_cache), arrays, p, max_kv_length, !all_many, !all_few, stream);
+    launch(q_rows, pages_of(key_cache), arrays, static_cast<float*>(temp), p, max_kv_length, !all_many, !all_few, stream);
     return check_hip(hipGetLastError(), "attention_paged_weights launch");
 }
 
@@ -473,7 +586,10 @@ using namespace lcpp_hip;
 
 extern "C" {
 
-size_t lcpp_hip_attention_paged_weights_temp_bytes(uint32_t, uint64_t, uint64_t, uint32_t, uint32_t, uint32_t) { return 0; }
+size_t lcpp_hip_attention_paged_weights_temp_bytes(uint32_t requests, uint64_t q_tokens, uint64_t max_kv_length, uint32_t q_heads,
+                                                   uint32_t kv_heads, uint32_t) {
+    return kv_heads == 0 || attention::is_few(requests, q_tokens, q_heads / kv_heads) ? 0 : attention::Split(requests, q_tokens, max_kv_length, q_heads, kv_heads).bytes();
+}
 
 #define LCPP_HIP_DEFINE_ATTENTION_WEIGHTS(S, T)                                                                               \
     int lcpp_hip_attention_paged_weights_##S(                                                                                 \

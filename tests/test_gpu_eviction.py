@@ -112,6 +112,47 @@ def test_many_requests(hip, dev):
     check_weights(hip, "bf16", [rng.randrange(1, 40) for _ in range(300)], [1] * 300, 2, 1, 32, 16)
 
 
+@pytest.mark.parametrize("suffix", ["bf16", "f16"])
+def test_units_dealt_out_over_all_requests(hip, dev, suffix):
+    """Lengths stated long enough that a request's own workgroups would be few; more requests than are counted at once."""
+    rng = random.Random(5)
+    lengths = [rng.choice((0, 1, 17, rng.randrange(1, 90), 130)) for _ in range(299)]
+    few = [min(n, 1) for n in lengths]
+    check_weights(hip, suffix, lengths + [700], few + [1], 2, 1, 32, 16, stated=1 << 20)
+    check_weights(hip, suffix, [700] + lengths, [40] + few, 4, 2, 64, 16, stated=1 << 20)       # one of many rows
+    check_weights(hip, suffix, lengths + [700], few + [300], 4, 2, 72, 24, stated=1 << 20)
+    check_weights(hip, suffix, lengths + [300], [min(n, 20) for n in lengths] + [250], 4, 2, 32, 16, stated=1 << 20)
+    check_weights(hip, suffix, lengths + [300], [0] * 299 + [140], 4, 2, 32, 16, stated=1 << 20)  # no row but one request's
+
+
+@pytest.mark.parametrize("suffix,dim", [("bf16", 64), ("f16", 128), ("bf16", 40)])
+def test_rows_that_workgroups_share(hip, dev, suffix, dim):
+    check_weights(hip, suffix, [700], [600], 4, 2, dim, 16)
+    check_weights(hip, suffix, [1], [257], 4, 2, dim, 16)
+    check_weights(hip, suffix, [700, 90, 0, 50], [600, 3, 0, 0], 4, 2, dim, 24)
+    check_weights(hip, suffix, [700, 300], [600, 210], 4, 2, dim, 16, stated=1)   # more units than the partial sums have room for
+    check_weights(hip, suffix, [90, 2000], [1, 1000], 3, 1, dim, 64, known=[20, 999])
+
+
+def test_shared_rows_are_the_same_every_time_in_a_graph(hip, dev):
+    q, keys, table, q_offsets, lse, old, first = check_weights(hip, "bf16", [700, 90], [600, 3], 4, 2, 64, 16)
+    after = torch.full_like(first, -5.0)
+    arguments = ints(table), ints(q_offsets), ints([700, 90])
+    size = hip.attention_paged_weights_temp_bytes(2, 603, arguments[0].shape[1] * 16, 4, 2, 64)
+    assert size > 0
+    temp = torch.full((size,), 0x7F, dtype=torch.uint8, device=dev)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        hip.attention_paged_weights("bf16", q, keys, *arguments, lse, after, weights_in=old, decay=0.9, temp=temp)
+    for _ in range(3):
+        after.fill_(-5.0)
+        temp.fill_(0x7F)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(after, first)
+
+
 def test_orders_of_the_cache(hip, dev):
     for order in ((0, 1, 2, 3), (2, 0, 1, 3), (1, 0, 2, 3), (0, 2, 1, 3)):
         check_weights(hip, "bf16", [90, 40], [1, 2], 4, 2, 40, 16, order=order)

@@ -91,6 +91,23 @@ def test_weights_refuse(hip, change, word):
     assert word in message(hip)
 
 
+def test_weights_refuse_temp_storage(hip):
+    size = hip.attention_paged_weights_temp_bytes
+    # Decoding steps, steps of a tile of rows in all, and full grids share no rows; few units of many rows do.
+    assert size(256, 256, 4000, 32, 8, 128) == 0 and size(1, 4, 1 << 20, 32, 8, 128) == 0 and size(64, 4096, 8192, 32, 8, 128) == 0
+    assert size(0, 0, 0, 32, 8, 128) == 0 and size(1, 0, 64, 2, 1, 64) == 0
+    assert size(1, 4096, 8192, 32, 8, 128) > 0
+    def call(temp, given):
+        return hip.lib().lcpp_hip_attention_paged_weights_bf16(
+            temp, given, rows(hip), pages(hip), ALIGNED, 4, 4, ALIGNED, ALIGNED, None, None, ALIGNED, None, ALIGNED, 1, 600, 64, 2, 1, 64, 16, 9,
+            0.125, 1.0, None)
+    needed = size(1, 600, 64, 2, 1, 64)
+    assert needed > 0
+    for temp, given, word in ((None, 0, "small"), (None, needed, "small"), (ALIGNED, needed - 1, "small")):
+        assert call(temp, given) == hip.ERR_TEMP_TOO_SMALL and word in message(hip)
+    assert call(ALIGNED + 2, needed) == hip.ERR_INVALID_ARGUMENT and "aligned" in message(hip)
+
+
 def test_weights_refuse_rows_and_head_sizes(hip):
     for dim in (0, 4, 60, 136):
         assert weights(hip, dim=dim) == hip.ERR_UNSUPPORTED
