@@ -554,6 +554,8 @@ int paged_weights(void* temp, size_t temp_bytes, const lcpp_hip_rows* q, const l
     if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
     if (needed && reinterpret_cast<uintptr_t>(temp) % alignof(float) != 0)
         return set_error(kInvalidArgument, "%s: temp storage must be 4-byte aligned", what);
+    // A cache of no pages has no slot to add to, and not the first page that the kernels read in place of one that is not there.
+    if (pages == 0) return kOk;
     // One token a request on average, or no more than a tile of rows in all: all requests count as ones of few rows.  More than
     // that on average: all as ones of many.  Otherwise each goes by its own rows, in two launches.  (256 requests of one token: 130 us,
     // 135 with the second launch; a request of 200 tokens over 8,000 keys among 255 of none: 320 us, 130 with it.)

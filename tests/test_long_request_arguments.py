@@ -91,6 +91,13 @@ def test_weights_refuse(hip, change, word):
     assert word in message(hip)
 
 
+def test_weights_of_a_cache_without_pages(hip):
+    # No slot is there to add to, so that nothing is launched: the arguments name no memory.
+    assert weights(hip, n_pages=0) == hip.OK
+    assert weights(hip, n_pages=0, tokens=0) == hip.OK
+    assert weights(hip, n_pages=0, cache=pages(hip, None)) == hip.ERR_INVALID_ARGUMENT
+
+
 def test_weights_refuse_temp_storage(hip):
     size = hip.attention_paged_weights_temp_bytes
     # Decoding steps, steps of a tile of rows in all, and full grids share no rows; few units of many rows do.
