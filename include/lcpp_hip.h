@@ -822,6 +822,8 @@ LCPP_HIP_DECLARE_PAGED_MOVE(f16)
  * sequences share a row.  A sequence of no tokens hands its initial state on; one of a single token is a step of serving.
  * log_decay is at most 0 in use (-infinity forgets the state); growth is right as long as products over 128 steps stay finite.
  * What is not finite stays in its channel and sequence.  Sums have one order: the same call gives the same bits.
+ * Output rows share no memory with the rows that are read or with each other, in either direction: a call that writes over its
+ * inputs is refused where the arrays' rows are equally far apart, or their first rows share items.
  *
  * The backward pass takes dout, and dfinal [sequences][channels] f32 (null: 0), to dx, dlog_decay and dinitial [sequences][channels]
  * f32 (or null); `initial` is [sequences][channels].  temp starts at a multiple of 8 bytes.  dlog_decay = dh_t exp(log_decay_t) h_{t-1} takes h as `out` has it.

@@ -607,6 +607,30 @@ int width_of(uint32_t channels, std::initializer_list<const lcpp_hip_steps*> row
     return bits % kMost == 0 ? kMost : bits % 2 == 0 ? 2 : 1;
 }
 
+// Whether rows of two arrays share an item, of arrays whose rows are equally far apart (others: whether their first rows do).
+bool share(const Steps& a, const Steps& b, int64_t tokens, int64_t row_bytes) {
+    const int64_t ahead = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data) - reinterpret_cast<uintptr_t>(a.data));
+    const int64_t stride = a.token_bytes;
+    if (tokens == 1 || b.token_bytes != stride) return ahead < row_bytes && -ahead < row_bytes;
+    int64_t rows = ahead / stride, past = ahead % stride;  // b's first row begins `past` bytes after a's row `rows`
+    if (past < 0) {
+        --rows;
+        past += stride;
+    }
+    return (past < row_bytes && rows < tokens && -rows < tokens) || (stride - past < row_bytes && rows + 1 < tokens && -rows - 1 < tokens);
+}
+
+// A chunk's rows may be read again by the workgroups of later chunks: nothing is written where something is read.
+template <bool BACK>
+bool apart(const Inputs& in, const Shape& p, int64_t row_bytes) {
+    if (p.tokens == 0) return true;
+    for (const Steps& to : BACK ? std::initializer_list<Steps>{in.dx, in.dlog_decay} : std::initializer_list<Steps>{in.out}) {
+        if (share(to, in.first, p.tokens, row_bytes) || share(to, in.log_decay, p.tokens, row_bytes)) return false;
+        if (BACK && share(to, in.out, p.tokens, row_bytes)) return false;
+    }
+    return !BACK || !share(in.dx, in.dlog_decay, p.tokens, row_bytes);
+}
+
 template <typename T, int V, bool BACK, int WAVES>
 int run(const char* what, const Inputs& in, const Handed& h, const Shape& p, bool hands, hipStream_t stream) {
     const int numbers = static_cast<int>(numbers_of(p.sequences, p.tokens));
@@ -635,6 +659,8 @@ int launch(const char* what, void* temp, size_t temp_bytes, const Inputs& in, co
     if (temp_bytes < needed || (needed && !temp)) return set_error(kTempTooSmall, "%s: temp storage too small", what);
     if (needed && reinterpret_cast<uintptr_t>(temp) % sizeof(uint64_t) != 0)
         return set_error(kInvalidArgument, "%s: temp storage must be 8-byte aligned", what);
+    if (!apart<BACK>(in, p, static_cast<int64_t>(p.channels) * static_cast<int64_t>(sizeof(typename T::Item))))
+        return set_error(kInvalidArgument, "%s: rows that are written share no memory with others", what);
     Handed h{static_cast<uint64_t*>(temp), nullptr, static_cast<int64_t>(stride_of(p.channels))};
     if (needed) h.states = reinterpret_cast<uint32_t*>(static_cast<char*>(temp) + effects_bytes(p.sequences, p.tokens, p.channels));
     const bool few = short_sequences(p.sequences, p.tokens);

@@ -34,6 +34,7 @@ class DeviceRecurrence : public LuisaModule {
 
     // out[t] = exp(log_decay[t]) out[t - 1] + x[t] along each sequence, from the rows of `initial` [states][channels] to those of
     // `final`; either may be empty, and both may be the same view.  Sequence b's row is state_rows[b], or b where that is empty.
+    // `out` shares no memory with x or log_decay (the command throws).
     template <RecurrenceItemT T>
     void Scan(CommandList& cmdlist, BufferView<uint> temp_storage, RecurrenceRows<T> x, RecurrenceRows<T> log_decay,
               BufferView<int32_t> offsets, RecurrenceRows<T> out, BufferView<float> initial, BufferView<float> final,
@@ -57,6 +58,7 @@ class DeviceRecurrence : public LuisaModule {
     }
 
     // Gradients of Scan, from the out that it gave; states [sequences][channels], each view of them may be empty.
+    // dx and dlog_decay share no memory with each other or with what is read (the command throws).
     template <RecurrenceItemT T>
     void ScanBackward(CommandList& cmdlist, BufferView<uint> temp_storage, RecurrenceRows<T> log_decay, RecurrenceRows<T> out,
                       RecurrenceRows<T> dout, BufferView<int32_t> offsets, BufferView<float> initial, BufferView<float> dfinal,

@@ -1093,7 +1093,8 @@ def recurrence_temp_bytes(sequences: int, tokens: int, channels: int) -> int:
 
 def recurrence(suffix: str, x, log_decay, offsets, out, initial=None, final=None, rows=None, temp=None, stream=None) -> None:
     """out[t] = exp(log_decay[t]) out[t - 1] + x[t] along each sequence of a ragged batch, [tokens, channels], from the rows of
-    `initial` [states, channels] f32 to those of `final`, which may be the same tensor: sequence b's is rows[b] (int32), or b."""
+    `initial` [states, channels] f32 to those of `final`, which may be the same tensor: sequence b's is rows[b] (int32), or b.
+    out shares no memory with x or log_decay."""
     dt, f32, i32 = _step_types(suffix)
     tokens, channels = shape = _axes("x", x, 2)
     sequences = offsets.numel() - 1
@@ -1112,7 +1113,8 @@ def recurrence(suffix: str, x, log_decay, offsets, out, initial=None, final=None
 def recurrence_backward(suffix: str, log_decay, out, dout, offsets, dx, dlog_decay, initial=None, dfinal=None, dinitial=None,
                         temp=None, stream=None) -> None:
     """Gradients of recurrence: dx and dlog_decay, and dinitial [sequences, channels] f32 if given, from dout and dfinal, and
-    from the out that the forward call gave; states are in the sequences' order."""
+    from the out that the forward call gave; states are in the sequences' order.  dx and dlog_decay share no memory with each
+    other or with what is read."""
     dt, f32, i32 = _step_types(suffix)
     tokens, channels = shape = _axes("out", out, 2)
     sequences = offsets.numel() - 1

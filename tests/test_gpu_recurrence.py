@@ -293,3 +293,22 @@ def test_graphs_and_streams(hip, dev):
     hip.recurrence("bf16", x, l, offsets, other, initial=initial, stream=stream)
     stream.synchronize()
     assert torch.equal(other, want["out"])
+
+
+@pytest.mark.parametrize("suffix", ["bf16", "f32"])
+@pytest.mark.parametrize("lengths,channels", [([1], 40), ([40, 300], 33), ([700], 64)])
+def test_rows_side_by_side_in_one_array(hip, dev, suffix, lengths, channels):
+    """What is read and what is written as columns of one array: they share no item, and are not refused."""
+    x, l, dout, initial, dfinal = made(14, suffix, lengths, channels)
+    want = oracle.recurrence(x, l, lengths, initial, dout, dfinal)
+    wide = torch.full((x.shape[0], 6 * channels + 1), 7.0, dtype=x.dtype, device=dev)
+    columns = [wide[:, i * channels:(i + 1) * channels] for i in (4, 1, 5, 0, 3, 2)]
+    for column, rows in zip(columns, (x, l, dout)):
+        column.copy_(rows)
+    out, dx, dl = columns[3:]
+    offsets, final, dinitial = offsets_of(lengths).cuda(), torch.empty_like(initial), torch.empty_like(initial)
+    hip.recurrence(suffix, columns[0], columns[1], offsets, out, initial=initial, final=final)
+    hip.recurrence_backward(suffix, columns[1], out, columns[2], offsets, dx, dl, initial=initial, dfinal=dfinal, dinitial=dinitial)
+    for name, got in (("out", out), ("final", final), ("dx", dx), ("dlog_decay", dl), ("dinitial", dinitial)):
+        oracle.check(name, got, want[name])
+    assert torch.equal(columns[0], x) and torch.equal(columns[1], l) and torch.equal(columns[2], dout) and bool((wide[:, -1] == 7.0).all())

@@ -195,6 +195,32 @@ def test_recurrence_refuses(hip):
             assert backward(hip, **{name: bad}) == hip.ERR_INVALID_ARGUMENT and "channels apart" in message(hip)
 
 
+@pytest.mark.parametrize("tokens,channels,stride", [(4, 64, 64), (70, 64, 200), (1, 64, 64), (1000, 10, 24), (8, 1, 1)])
+def test_recurrence_refuses_rows_written_over_what_is_read(hip, tokens, channels, stride):
+    """A workgroup that does not wait for its neighbours reads their rows itself, which they may have written by then."""
+    need, sequences = hip.recurrence_temp_bytes(2, tokens, channels), 2
+    far = lambda i, shift=0, step=stride: hip.Steps(ALIGNED + (i << 24) + 2 * shift, step)
+
+    def forward(x, l, out):
+        return hip.lib().lcpp_hip_recurrence_bf16(ALIGNED, need, x, l, ALIGNED, None, None, 0, out, None, sequences, tokens, channels, None)
+
+    def backward(l, out, dout, dx, dl):
+        return hip.lib().lcpp_hip_recurrence_backward_bf16(ALIGNED, need, l, out, dout, ALIGNED, None, None, dx, dl, None, sequences, tokens,
+                                                           channels, None)
+
+    # The same rows; rows that begin in others; rows that others begin in; the last row that another's first one is.
+    shifts = [0, channels - 1, 1 - channels, (tokens - 1) * stride, (1 - tokens) * stride]
+    if tokens > 2:
+        shifts += [stride + channels - 1, 2 * stride - channels + 1, (2 - tokens) * stride + 1 - channels]
+    for shift in shifts:
+        for call in (lambda: forward(far(1), far(2), far(1, shift)), lambda: forward(far(1), far(2), far(2, shift)),
+                     *(lambda a=a, b=b: backward(*[far(b, shift) if i == a else far(i) for i in range(5)])
+                       for a, b in ((3, 0), (3, 1), (3, 2), (4, 0), (4, 1), (4, 2), (3, 4)))):
+            assert call() == hip.ERR_INVALID_ARGUMENT and "share no memory" in message(hip), shift
+    # First rows that share items, other rows further apart.
+    assert forward(far(1), far(2), far(1, 0, stride + 1)) == hip.ERR_INVALID_ARGUMENT and "share no memory" in message(hip)
+
+
 def test_temporary_storage(hip):
     """Enough of it, and aligned to the words that it holds."""
     need = hip.recurrence_temp_bytes(2, 1000, 64)
