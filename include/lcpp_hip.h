@@ -777,7 +777,7 @@ LCPP_HIP_DECLARE_ATTENTION_WEIGHTS(f16)
  * that no kept key is in, in the requests' order, to `released` (pages that were not there, negative entries, are left out).  A
  * request of n keys that would keep K of them and may need more than most_moves moves, min(K, n - K), keeps all n.  shifts_out [requests]
  * or null: shifts (null: 0) plus the number of keys evicted, what rotary adds to the positions of later tokens; it may be
- * `shifts`.  counts[0] pages released (those from max_released on are left out of the list), counts[1] keys kept.  The block
+ * `shifts` where no plan that protects the latest keys follows: evict_plan needs the shifts from before.  counts[0] pages released (those from max_released on are left out of the list), counts[1] keys kept.  The block
  * table is read alone: entries past a request's pages are not looked at by the other calls. */
 int lcpp_hip_page_release(const int32_t* kv_lengths, const int32_t* keep_lengths, uint32_t requests, uint32_t page_size,
                           const int32_t* block_table, uint64_t table_stride, uint32_t table_width, uint64_t most_moves,
@@ -790,7 +790,9 @@ int lcpp_hip_page_release(const int32_t* kv_lengths, const int32_t* keep_lengths
  * key past the new end, move_from[r][i], goes to the i-th place of an evicted key before it, move_to[r][i], as slots (-1: the
  * page is not there); entries past the last move are -1.  A request makes at most min(K, n - K) moves; those past `width` are
  * left out (see page_release's most_moves).  positions (slots' positions) may be null where first and recent are 0, shifts where nothing
- * was evicted before.  kv_lengths are those before the eviction.  max_kv_length is the longest of them, or more.  temp starts at a
+ * was evicted before.  kv_lengths and shifts are those before the eviction, what page_release read, not what it wrote: with its
+ * shifts_out in their place the latest keys would lose their protection, as many of them as keys go.  Every layer's plan needs
+ * them, so a program that protects the latest keys has two arrays of shifts by turns.  max_kv_length is the longest of them, or more.  temp starts at a
  * multiple of 16 bytes. */
 size_t lcpp_hip_evict_plan_temp_bytes(uint32_t requests, uint64_t max_kv_length);
 int lcpp_hip_evict_plan(void* temp, size_t temp_bytes, const float* weights, const int32_t* positions,

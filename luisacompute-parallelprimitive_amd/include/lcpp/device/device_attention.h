@@ -290,7 +290,8 @@ class DeviceAttention : public LuisaModule {
         };
     }
 
-    // Lengths after an eviction, the pages that come free, and with shifts_out (or empty) what later positions are ahead by.
+    // Lengths after an eviction, the pages that come free, and with shifts_out (or empty) what later positions are ahead by: another
+    // view than `shifts` where EvictPlan protects the latest keys.
     void PageRelease(CommandList& cmdlist, BufferView<int32_t> kv_lengths, BufferView<int32_t> keep_lengths, uint page_size, BlockTable table,
                      BufferView<int32_t> shifts, BufferView<int32_t> kept_lengths, BufferView<int32_t> shifts_out,
                      BufferView<int32_t> released, BufferView<int32_t> counts,
@@ -312,6 +313,7 @@ class DeviceAttention : public LuisaModule {
     }
 
     // The moves, requests times as many, that cut each request to its kept length; positions may be empty where no key is protected.
+    // kv_lengths and shifts are those before PageRelease.
     void EvictPlan(CommandList& cmdlist, BufferView<uint> temp_storage, BufferView<float> weights, BufferView<int32_t> positions,
                    BlockTable table, BufferView<int32_t> kv_lengths, BufferView<int32_t> kept_lengths, BufferView<int32_t> shifts,
                    BufferView<int64_t> move_from, BufferView<int64_t> move_to, size_t max_kv_length, PageShape page,

@@ -1008,8 +1008,9 @@ def attention_paged_weights(suffix: str, q, key_cache, block_table, q_offsets, k
 def page_release(kv_lengths, keep_lengths, page_size: int, block_table, kept_lengths, released, counts, shifts=None,
                  shifts_out=None, most_moves=None, stream=None) -> None:
     """kept_lengths of requests cut to keep_lengths, the pages that come free (released, counts[0] of them; counts[1] keys are
-    kept), and shifts_out: `shifts` plus the keys evicted.  Requests that may need more than most_moves moves (evict_plan's
-    width) are not cut.  All int32."""
+    kept), and shifts_out: `shifts` plus the keys evicted (another array than `shifts` where evict_plan protects the latest
+    keys: it takes the shifts from before).  Requests that may need more than most_moves moves (evict_plan's width) are not
+    cut.  All int32."""
     _, _, i32, _ = _row_types("bf16")
     requests = kv_lengths.numel()
     table, table_stride, width = _table(i32, block_table, requests)
@@ -1028,7 +1029,8 @@ def evict_plan(weights, positions, block_table, kv_lengths, kept_lengths, move_f
                shifts=None, max_kv_length=None, temp=None, stream=None) -> None:
     """The moves, slots move_from[r] to move_to[r] (int64 [requests, width], -1 past the last), that cut each request from
     kv_lengths to kept_lengths keys: the `first` positions and the latest `recent` ones stay, then the largest of
-    weights [pages, page size].  positions [pages, page size] int32, or None where first and recent are 0."""
+    weights [pages, page size].  positions [pages, page size] int32, or None where first and recent are 0.  kv_lengths and
+    shifts are those before page_release: with its shifts_out in their place the latest keys would not be protected."""
     _, f32, i32, i64 = _row_types("bf16")
     requests = kv_lengths.numel()
     pages, page_size = _axes("weights", weights, 2)

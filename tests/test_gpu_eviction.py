@@ -316,6 +316,36 @@ def test_plan_of_requests_longer_than_stated(hip, dev):
     check_plan(hip, [20000, 16385, 100], [300, 16384, 99], 16, stated=16385, values="few")
 
 
+def test_the_latest_keys_stay_when_requests_are_cut_again_and_again(hip, dev):
+    """Lengths, pages, plan and moves as a program makes them, in two arrays of shifts by turns and no copy: a plan takes the shifts
+    that page_release read.  (With what it wrote, each cut of more keys than are protected would protect none of the latest.)"""
+    page, recent, first, keep, new = 8, 6, 2, [30, 17], [25, 20]
+    table = torch.arange(2 * 12, dtype=torch.int32, device=dev).view(2, 12)
+    keys, values = (torch.zeros(24, page, 1, 8, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    weights, positions = torch.zeros(24, page, device=dev), torch.full((24, page), -1, dtype=torch.int32, device=dev)
+    shifts, later = torch.zeros(2, dtype=torch.int32, device=dev), torch.zeros(2, dtype=torch.int32, device=dev)
+    kept, released, counts = torch.zeros(2, dtype=torch.int32, device=dev), torch.zeros(24, dtype=torch.int32, device=dev), ints([0, 0])
+    moves = [torch.empty(2, 40, dtype=torch.int64, device=dev) for _ in range(2)]
+    seen = [0, 0]
+    for cut in range(5):
+        lengths = [int(k) + n for k, n in zip(kept.tolist(), new)]
+        for r, n in enumerate(lengths):
+            slots = table[r, 0].item() * page + torch.arange(n - new[r], n, device=dev)
+            positions.flatten()[slots] = torch.arange(seen[r], seen[r] + new[r], dtype=torch.int32, device=dev)
+            weights.flatten()[slots] = -1.0 - torch.arange(new[r], device=dev)  # the later, the lighter: without protection the latest go
+            seen[r] += new[r]
+        kv = ints(lengths)
+        hip.page_release(kv, ints(keep), page, table, kept, released, counts, shifts=shifts, shifts_out=later)
+        hip.evict_plan(weights, positions, table, kv, kept, *moves, first=first, recent=recent, shifts=shifts)
+        hip.paged_move("bf16", *moves, keys, values, weights=weights, positions=positions)
+        shifts, later = later, shifts
+        assert kept.tolist() == [min(n, k) for n, k in zip(lengths, keep)]
+        assert shifts.tolist() == [a - b for a, b in zip(seen, kept.tolist())]
+        for r, n in enumerate(kept.tolist()):
+            mine = positions[table[r].long()].flatten()[:n].tolist()
+            assert set(range(seen[r] - recent, seen[r])) | set(range(first)) <= set(mine) and len(set(mine)) == n, (cut, r, sorted(mine))
+
+
 def test_plan_corners(hip, dev):
     check_plan(hip, [50, 50, 50], [10, 60, -4], 16)
     check_plan(hip, [50, 0], [10, 10], 16)
