@@ -822,7 +822,8 @@ LCPP_HIP_DECLARE_PAGED_MOVE(f16)
  * whole number of items apart.  States are [num_states][channels] f32: sequence b has row state_rows[b] (null: b; a row
  * outside [0, num_states): starts from 0 and is not kept).  final_states (or null) may be the same memory as `initial`, and then no two
  * sequences share a row.  A sequence of no tokens hands its initial state on; one of a single token is a step of serving.
- * log_decay is at most 0 in use (-infinity forgets the state); growth is right as long as products over 128 steps stay finite.
+ * log_decay is at most 0 in use (-infinity forgets a finite state); growth is right as long as products over 128 steps stay finite.
+ * An infinite state stays infinite under any finite log_decay, however small exp of it is.
  * What is not finite stays in its channel and sequence.  Sums have one order: the same call gives the same bits.
  * Output rows share no memory with the rows that are read or with each other, in either direction: a call that writes over its
  * inputs is refused where the arrays' rows are equally far apart, or their first rows share items.

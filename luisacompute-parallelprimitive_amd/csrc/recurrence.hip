@@ -32,20 +32,35 @@ __device__ __forceinline__ float to_float(typename T::Item x) {
     return static_cast<float>(x);
 }
 
+// A number of 32 bits rounded to the items' type.  (In f16 a product or sum would be rounded to 16 bits in one step in one place and
+// in two in another, as the compiler finds, and rows that are gone through twice would not come out the same.)
+template <typename T>
+__device__ __forceinline__ typename T::Item rounded(float x) {
+    if constexpr (std::is_same_v<T, F16>) asm("" : "+v"(x));
+    return static_cast<typename T::Item>(x);
+}
+
 constexpr float kSmall = 0.0625f;
 
 // y -> exp(l) y + x, with what depends on l alone.
 struct Decay {
     float factor;  // exp(l), or exp(l) - 1 where l is small
     bool small;
+    bool keeps;    // l is above -infinity
     __device__ __forceinline__ explicit Decay(float l) {
         // (The first term left out is l^5 / 120, 1.3e-7 of l.)
         const float series = l * __builtin_fmaf(l, __builtin_fmaf(l, __builtin_fmaf(l, 1.f / 24.f, 1.f / 6.f), 0.5f), 1.f);
         small = __builtin_fabsf(l) < kSmall;
         factor = small ? series : attention::exp2_fast(l * attention::kLog2e);
+        keeps = l > -INFINITY;
     }
     __device__ __forceinline__ float step(float y, float x) const { return __builtin_fmaf(factor, y, small ? y + x : x); }
     __device__ __forceinline__ float times(float y) const { return __builtin_fmaf(factor, y, small ? y : 0.f); }
+    // The same of an infinite y too: any exp(l) above 0 leaves it what it is, where exp(l) - 1, or an exp(l) that is 0 in 32 bits,
+    // makes NaN of it.  Rows in registers go without this and are gone through again where a NaN comes out, which stays to their end.
+    // (Both directions of 34,222 tokens: 481 us, without any of it 470; with NaN looked for in the hand-over too 490.)
+    __device__ __forceinline__ float step_any(float y, float x) const { return __builtin_isinf(y) && keeps ? y + x : step(y, x); }
+    __device__ __forceinline__ float times_any(float y) const { return __builtin_isinf(y) && keeps ? y : times(y); }
 };
 
 struct Shape {
@@ -104,19 +119,24 @@ __device__ __forceinline__ uint32_t handed(float x) {
 // products.)
 struct Effect {
     float l, b;
-    // This one, then another.
+    // (ANY: where b, or the state, may be infinite.)  This one, then another.
+    template <bool ANY>
     __device__ __forceinline__ void then(Effect next) {
-        b = next.of(b);
+        b = next.of<ANY>(b);
         l += next.l;
     }
     // This one, then a row.
-    template <bool BACK>
+    template <bool BACK, bool ANY>
     __device__ __forceinline__ void row(float l_row, float x) {
         const Decay d(l_row);
-        b = BACK ? d.times(x + b) : d.step(b, x);
+        if constexpr (ANY) b = BACK ? d.times_any(x + b) : d.step_any(b, x);
+        else b = BACK ? d.times(x + b) : d.step(b, x);
         l += l_row;
     }
-    __device__ __forceinline__ float of(float h) const { return Decay(l).step(h, b); }
+    template <bool ANY>
+    __device__ __forceinline__ float of(float h) const {
+        return ANY ? Decay(l).step_any(h, b) : Decay(l).step(h, b);
+    }
 };
 
 __device__ __forceinline__ uint64_t handed(Effect e) { return static_cast<uint64_t>(handed(e.b)) << 32 | handed(e.l); }
@@ -203,9 +223,29 @@ struct WaveRows {
             const int r = BACK ? kRows - 1 - i : i;
             if (r < count)
 #pragma unroll
-                for (int v = 0; v < V; ++v) e[v].template row<BACK>(to_float<T>(l[r].at[v]), to_float<T>(x[r].at[v]));
+                for (int v = 0; v < V; ++v) e[v].template row<BACK, false>(to_float<T>(l[r].at[v]), to_float<T>(x[r].at[v]));
             __builtin_amdgcn_sched_barrier(0);  // (a row at a time: all decays at once would take the registers)
         }
+    }
+    // The same where states may be infinite, from memory, row by row.
+    __device__ __forceinline__ static void effect_any(Effect (&e)[V], int rows, const Window<Vec>& first, const Window<Vec>& log_decay, uint32_t at) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) e[v] = {0.f, 0.f};
+#pragma unroll 1
+        for (int i = 0; i < rows; ++i) {
+            const int r = BACK ? rows - 1 - i : i;
+            const Vec x_row = first.load(r, at), l_row = log_decay.load(r, at);
+#pragma unroll
+            for (int v = 0; v < V; ++v) e[v].template row<BACK, true>(to_float<T>(l_row.at[v]), to_float<T>(x_row.at[v]));
+        }
+    }
+    // Whether any of a wave's V values a lane is NaN.
+    template <typename F>
+    __device__ __forceinline__ static bool any_nan(F value) {
+        bool found = false;
+#pragma unroll
+        for (int v = 0; v < V; ++v) found |= value(v) != value(v);
+        return wave_ballot(found) != 0;
     }
 };
 
@@ -241,9 +281,9 @@ __device__ __forceinline__ Effect effect_of_chunk(const Inputs& in, int64_t toke
 #pragma unroll 1
         for (int k = 0; k < rows; ++k) {
             const int64_t t = token + w * kRows + (BACK ? rows - 1 - k : k);
-            part.row<BACK>(to_float<T>(in.log_decay.template at<Item>(t)[channel]), to_float<T>(in.first.template at<Item>(t)[channel]));
+            part.row<BACK, true>(to_float<T>(in.log_decay.template at<Item>(t)[channel]), to_float<T>(in.first.template at<Item>(t)[channel]));
         }
-        all.then(part);
+        all.then<true>(part);
     }
     return all;
 }
@@ -298,7 +338,7 @@ __device__ __forceinline__ float look_back(const Inputs& in, const Handed& h, co
             }
             const Effect e = {__builtin_bit_cast(float, static_cast<uint32_t>(words[i])),
                               __builtin_bit_cast(float, static_cast<uint32_t>(words[i] >> 32))};
-            value = e.of(value);
+            value = e.of<true>(value);
         }
     }
     return value;
@@ -373,13 +413,13 @@ __global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape
                 const float input = to_float<T>(rows.x[r].at[v]);
                 if constexpr (BACK) {
                     const float g = input + state[v];
-                    state[v] = d.times(g);
+                    state[v] = d.times_any(g);
                     const float before = r + 1 < left ? to_float<T>(rows.h[r].at[v]) : first[v];
-                    g_row.at[v] = static_cast<Item>(g);
-                    l_row.at[v] = static_cast<Item>(state[v] * before);
+                    g_row.at[v] = rounded<T>(g);
+                    l_row.at[v] = rounded<T>(state[v] * before);
                 } else {
-                    state[v] = d.step(state[v], input);
-                    g_row.at[v] = static_cast<Item>(state[v]);
+                    state[v] = d.step_any(state[v], input);
+                    g_row.at[v] = rounded<T>(state[v]);
                 }
             }
             a.store(BACK ? some - 1 - r : r, at, g_row);
@@ -447,19 +487,21 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void recurrence_kernel(Inputs in,
     WaveRows<T, V, BACK> rows;
     const int row_bytes = p.channels * static_cast<int>(sizeof(Item)), some = mine < kRows ? mine : kRows;
     const uint32_t at = active ? static_cast<uint32_t>(own) * sizeof(Item) : kNowhere;
-    rows.load(Window<Vec>(in.first, token, some, row_bytes), Window<Vec>(in.log_decay, token, some, row_bytes), at);
+    const auto rows_of = [&](const Steps& steps) { return Window<Vec>(steps, token, some, row_bytes); };
+    rows.load(rows_of(in.first), rows_of(in.log_decay), at);
     if (!alone || WAVES > 1) {
         Effect effect[V];
         rows.effect(effect, mine);
+        if (rows.any_nan([&](int v) { return effect[v].b; })) rows.effect_any(effect, some, rows_of(in.first), rows_of(in.log_decay), at);
 #pragma unroll
         for (int v = 0; v < V; ++v) parts[wave][lane * V + v] = effect[v];
     }
     // Backwards: the states before each token, as they were stored.
+    // (The window begins a row before the wave's, or where the sequence does: then it is read a row late.)
     Vec stored[BACK ? kRows : 1];
+    const int late = BACK && token == chunk.begin;
+    const Window<Vec> out(in.out, BACK ? token - 1 + late : token, some - late, row_bytes);
     if constexpr (BACK) {
-        // (The window begins a row before the wave's, or where the sequence does: then it is read a row late.)
-        const int late = token == chunk.begin;
-        const Window<Vec> out(in.out, token - 1 + late, some - late, row_bytes);
 #pragma unroll
         for (int r = 0; r < kRows; ++r)
             if (r >= late) stored[r] = out.load(r - late, at);
@@ -478,60 +520,66 @@ __global__ __launch_bounds__(WAVES * kWave, 4) void recurrence_kernel(Inputs in,
         } else {
             Effect all = {0.f, 0.f};
 #pragma unroll
-            for (int w = 0; w < WAVES; ++w) all.then(parts[BACK ? WAVES - 1 - w : w][at]);
+            for (int w = 0; w < WAVES; ++w) all.then<true>(parts[BACK ? WAVES - 1 - w : w][at]);
             if (after > 0 && there) atomic_store_agent(h.effects + number * h.stride + target, handed(all));
             state = look_back<T, BACK, WAVES>(in, h, chunk, number, before, target, there, patience);
-            if (after > 0 && there) atomic_store_agent(h.states + (BACK ? number - 1 : number + 1) * h.stride + target, handed(all.of(state)));
+            if (after > 0 && there) atomic_store_agent(h.states + (BACK ? number - 1 : number + 1) * h.stride + target, handed(all.of<true>(state)));
         }
-        entering[at] = state;
+        entering[at] = there ? state : 0.f;  // (a lane without a channel may have found a word that was not there yet, a NaN)
     }
     if constexpr (WAVES > 1) __syncthreads();
     else wave_lds_order();
     float state[V];
+    const auto enter = [&](auto any) {
+        constexpr bool kAny = decltype(any)::value;
 #pragma unroll
-    for (int v = 0; v < V; ++v) {
-        state[v] = entering[lane * V + v];
-        if constexpr (BACK) {
-            for (int w = WAVES - 1; w > wave; --w) state[v] = parts[w][lane * V + v].of(state[v]);
-        } else {
-            for (int w = 0; w < wave; ++w) state[v] = parts[w][lane * V + v].of(state[v]);
+        for (int v = 0; v < V; ++v) {
+            state[v] = entering[lane * V + v];
+            if constexpr (BACK) {
+                for (int w = WAVES - 1; w > wave; --w) state[v] = parts[w][lane * V + v].template of<kAny>(state[v]);
+            } else {
+                for (int w = 0; w < wave; ++w) state[v] = parts[w][lane * V + v].template of<kAny>(state[v]);
+            }
         }
-    }
+    };
+    // Row r of the wave with the state before it (backwards, after it); `h` is the stored state before a row.
+    const Window<Vec> dx(in.dx, token, BACK ? some : 0, row_bytes), dlog_decay(in.dlog_decay, token, BACK ? some : 0, row_bytes);
+    const auto work = [&](auto any, int r, const Vec& x, const Vec& l, const Vec& h_row) {
+        constexpr bool kAny = decltype(any)::value;
+        Vec row, l_row;
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            const Decay d(to_float<T>(l.at[v]));
+            if constexpr (BACK) {
+                const float g = to_float<T>(x.at[v]) + state[v];
+                state[v] = kAny ? d.times_any(g) : d.times(g);
+                float h = to_float<T>(h_row.at[v]);
+                if (r == 0 && late) h = in.initial != nullptr && active ? in.initial[static_cast<int64_t>(chunk.sequence) * p.channels + own + v] : 0.f;
+                row.at[v] = rounded<T>(g);
+                l_row.at[v] = rounded<T>(state[v] * h);
+            } else {
+                state[v] = kAny ? d.step_any(state[v], to_float<T>(x.at[v])) : d.step(state[v], to_float<T>(x.at[v]));
+                row.at[v] = rounded<T>(state[v]);
+            }
+        }
+        (BACK ? dx : out).store(r, at, row);
+        if constexpr (BACK) dlog_decay.store(r, at, l_row);
+    };
+    enter(std::false_type{});
     rows.forget();
-    if constexpr (BACK) {
-        const Window<Vec> dx(in.dx, token, some, row_bytes), dlog_decay(in.dlog_decay, token, some, row_bytes);
 #pragma unroll
-        for (int i = 0; i < kRows; ++i) {
-            const int r = kRows - 1 - i;
-            __builtin_amdgcn_sched_barrier(0);
-            if (r >= mine) continue;
-            Vec g_row, l_row;
-            const bool first = r == 0 && token == chunk.begin;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                const float g = to_float<T>(rows.x[r].at[v]) + state[v];
-                state[v] = Decay(to_float<T>(rows.l[r].at[v])).times(g);
-                float h = to_float<T>(stored[r].at[v]);
-                if (first) h = in.initial != nullptr && active ? in.initial[static_cast<int64_t>(chunk.sequence) * p.channels + own + v] : 0.f;
-                g_row.at[v] = static_cast<Item>(g);
-                l_row.at[v] = static_cast<Item>(state[v] * h);
-            }
-            dx.store(r, at, g_row);
-            dlog_decay.store(r, at, l_row);
-        }
-    } else {
-        const Window<Vec> out(in.out, token, some, row_bytes);
-#pragma unroll
-        for (int r = 0; r < kRows; ++r) {
-            __builtin_amdgcn_sched_barrier(0);
-            if (r >= mine) continue;
-            Vec row;
-#pragma unroll
-            for (int v = 0; v < V; ++v) {
-                state[v] = Decay(to_float<T>(rows.l[r].at[v])).step(state[v], to_float<T>(rows.x[r].at[v]));
-                row.at[v] = static_cast<Item>(state[v]);
-            }
-            out.store(r, at, row);
+    for (int i = 0; i < kRows; ++i) {
+        const int r = BACK ? kRows - 1 - i : i;
+        __builtin_amdgcn_sched_barrier(0);
+        if (r < mine) work(std::false_type{}, r, rows.x[r], rows.l[r], stored[BACK ? r : 0]);
+    }
+    if (rows.any_nan([&](int v) { return state[v]; })) {
+        enter(std::true_type{});
+        const Window<Vec> first = rows_of(in.first), log_decay = rows_of(in.log_decay);
+#pragma unroll 1
+        for (int i = 0; i < some; ++i) {
+            const int r = BACK ? some - 1 - i : i;
+            work(std::true_type{}, r, first.load(r, at), log_decay.load(r, at), BACK ? out.load(r < late ? 0 : r - late, at) : Vec{});
         }
     }
     // The last state: forwards of the wave that has the sequence's last token, backwards of the first.

@@ -312,3 +312,51 @@ def test_rows_side_by_side_in_one_array(hip, dev, suffix, lengths, channels):
     for name, got in (("out", out), ("final", final), ("dx", dx), ("dlog_decay", dl), ("dinitial", dinitial)):
         oracle.check(name, got, want[name])
     assert torch.equal(columns[0], x) and torch.equal(columns[1], l) and torch.equal(columns[2], dout) and bool((wide[:, -1] == 7.0).all())
+
+
+@pytest.mark.parametrize("suffix", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("lengths", [[3, 20, 1], [60, 50, 3], [700, 40], [2100]])  # walked, chunks of one wave, and of eight
+def test_infinite_states_are_the_formula_s(hip, dev, suffix, lengths):
+    """exp(l) times an infinity is one for every finite l: around 0, where exp(l) - 1 is taken, and far below, where a chunk's decay
+    is 0 in 32 bits.  An infinity of the other sign makes NaN, and only what the formulas make infinite or NaN differs from the same
+    call with finite items there."""
+    dtype, tokens = DTYPE[suffix], sum(lengths)
+    decays = [0.0, -2.0 ** -7, -0.0625, -0.5, -3.0, 2.0 ** -9]
+    places = ["initial", "below", "x", "x, then the other", "dout", "dfinal", "none"]
+    channels = len(decays) * len(places)
+    x, l, dout, initial, dfinal = made(21, suffix, lengths, channels)
+    l = torch.tensor(decays * len(places), dtype=dtype).cuda().expand(tokens, channels).contiguous()
+    clean = run(hip, suffix, lengths, x, l, dout, initial, dfinal)
+    begins = offsets_of(lengths).tolist()
+    for i, place in enumerate(places):
+        mine = slice(i * len(decays), (i + 1) * len(decays))
+        for b, n in enumerate(lengths):
+            if place in ("initial", "below"):
+                initial[b, mine] = math.inf if place == "initial" else -math.inf
+            if place.startswith("x"):
+                x[begins[b] + n // 3, mine] = math.inf
+            if place.endswith("other"):
+                x[begins[b] + n // 3 + n // 2, mine] = -math.inf
+            if place == "dout":
+                dout[begins[b] + n // 2, mine] = -math.inf
+            if place == "dfinal":
+                dfinal[b, mine] = math.inf
+    got = run(hip, suffix, lengths, x, l, dout, initial, dfinal)
+    want = {name: value for name, (value, _) in oracle.recurrence(x, l, lengths, initial, dout, dfinal).items()}
+    for name, value in want.items():
+        mine = got[name].cpu().double()
+        for what, a, b in (("NaN", mine.isnan(), value.isnan()), ("inf", mine == math.inf, value == math.inf),
+                           ("-inf", mine == -math.inf, value == -math.inf)):
+            assert torch.equal(a, b), f"{name}: {int((a != b).sum())} items are {what} or are not, in channels {(a != b).any(0).nonzero()[:, 0].tolist()}"
+        finite = value.isfinite().cuda()
+        assert torch.equal(got[name][finite], clean[name][finite]), name
+
+
+def test_infinite_states_without_waiting(hip, dev):
+    """As a workgroup makes them that reads its neighbours' rows itself."""
+    before = hip.lib().lcpp_hip_get_lookback_spin_limit()
+    try:
+        hip.check(hip.lib().lcpp_hip_set_lookback_spin_limit(0))
+        test_infinite_states_are_the_formula_s(hip, dev, "bf16", [2100])
+    finally:
+        hip.check(hip.lib().lcpp_hip_set_lookback_spin_limit(before))
