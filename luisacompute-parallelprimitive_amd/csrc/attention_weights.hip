@@ -214,6 +214,23 @@ __device__ __forceinline__ int64_t key_at(const Pages& cache, const Request& r, 
     return there ? page * cache.page_bytes + (at - static_cast<int>(cell * p.page_size.by)) * cache.token_bytes : 0;
 }
 
+// Whether a workgroup's rows have some without a log-sum among them: they give no weight whatever they hold, an infinity or NaN
+// too, and take the way of masked rows.  note: each thread's own, between the barriers that its log-sums are written between; any:
+// after them.
+struct Without {
+    int waves[kWeightWaves];
+    __device__ __forceinline__ void note(bool mine) {
+        const bool some = wave_ballot(mine) != 0;
+        if (threadIdx.x % kWave == 0) waves[threadIdx.x / kWave] = some;
+    }
+    __device__ __forceinline__ bool any() const {
+        int all = 0;
+#pragma unroll
+        for (int w = 0; w < kWeightWaves; ++w) all |= waves[w];
+        return __builtin_amdgcn_readfirstlane(all) != 0;
+    }
+};
+
 // Adds a tile of rows' weights to the sums of the lane's keys; `row0` is the lane's first row of four, `base` their log-sums.
 template <typename T, int GROUPS, int STEPS>
 __device__ __forceinline__ void weigh(float (&sum)[GROUPS], const U32x4 (&a)[STEPS], const U32x4 (&k)[GROUPS][STEPS], F32x4 base, float c,
@@ -267,6 +284,7 @@ __global__ __launch_bounds__(kWeightBlock) void attention_weights_few_kernel(Row
     constexpr int kGroups = kFewKeys / 16;
     __shared__ __attribute__((aligned(16))) char staged[kWeightWaves][kGroups * S::kBytes];
     __shared__ __attribute__((aligned(16))) float bases[kFewHeads * kRowsAtOnce];
+    __shared__ Without without;
     __shared__ Units<kFewKeys * kWeightWaves, true, FLAT> units;
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), column = lane % 16, quarter = lane / 16;
@@ -281,17 +299,21 @@ __global__ __launch_bounds__(kWeightBlock) void attention_weights_few_kernel(Row
         const int64_t own = key_at(key_cache, request, p, some ? key0 : 0, kFewKeys);
         float sum[kGroups] = {};
         for (int row_base = 0; row_base < request.rows; row_base += kRowsAtOnce) {
-            // (Rows that are not there are the first one with a log-sum of infinity: they weigh nothing.)
-            const int mine = row_base + column < request.rows ? row_base + column : 0;
+            // (Rows that are not there are the tile's first one with a log-sum of infinity: they weigh nothing.)
+            const int mine = row_base + column < request.rows ? row_base + column : row_base;
             for (int head_base = 0; head_base < p.kv_heads; head_base += kFewHeads) {
                 const int heads = p.kv_heads - head_base < kFewHeads ? p.kv_heads - head_base : kFewHeads;
                 __syncthreads();
+                bool out = false;
                 for (int i = threadIdx.x; i < heads * kRowsAtOnce; i += kWeightBlock) {
                     const int row = row_base + i % kRowsAtOnce;
                     bases[i] = row < request.rows ? request.base_of(arrays, p, head_base + i / kRowsAtOnce, row) : INFINITY;
+                    out |= row < request.rows && bases[i] == INFINITY;
                 }
+                without.note(out);
                 __syncthreads();
                 if (!some) continue;
+                const bool any_masked = masked || without.any();
                 const char* from[kGroups][S::kLoads];
 #pragma unroll
                 for (int g = 0; g < kGroups; ++g)
@@ -326,7 +348,7 @@ __global__ __launch_bounds__(kWeightBlock) void attention_weights_few_kernel(Row
 #pragma unroll
                     for (int g = 0; g < kGroups; ++g) S::read(tile + g * S::kBytes, k[g]);
                     const F32x4 base = *reinterpret_cast<const F32x4*>(&bases[local * kRowsAtOnce + 4 * quarter]);
-                    weigh<T>(sum, a, k, base, c, masked, arrays, request, p, row_base + 4 * quarter, key0);
+                    weigh<T>(sum, a, k, base, c, any_masked, arrays, request, p, row_base + 4 * quarter, key0);
                 }
             }
         }
@@ -345,8 +367,8 @@ constexpr int kManyKeys = 48;
 constexpr int kTableHeads = 64;  // key heads that the table of rows holds at once
 constexpr int kTableRows = 2048;
 
-// Where each row of a few key heads lies, after the request's first, and its log-sum.  Rows that are not there are the first one,
-// with a log-sum of infinity.
+// Where each row of a few key heads lies, after the request's first, and its log-sum.  Rows that are not there are the table's first
+// one, with a log-sum of infinity.
 struct RowTable {
     int64_t at[kTableRows];
     __attribute__((aligned(16))) float base[kTableRows];
@@ -360,6 +382,7 @@ __global__ __launch_bounds__(kWeightBlock, 3) void attention_weights_many_kernel
     __shared__ RowTable table;
     __shared__ __attribute__((aligned(16))) char staged[kWeightWaves][S::kBytes];
     __shared__ float sums[kWeightWaves][kManyKeys];
+    __shared__ Without without;
     __shared__ Units<kManyKeys, false, FLAT> units;
     const int lane = threadIdx.x % kWave;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), column = lane % 16, quarter = lane / 16;
@@ -368,6 +391,7 @@ __global__ __launch_bounds__(kWeightBlock, 3) void attention_weights_many_kernel
     const int heads_at_once = p.kv_heads < kTableHeads ? p.kv_heads : kTableHeads;
     const int most_rows = kTableRows / heads_at_once / kRowsAtOnce * kRowsAtOnce;
     int held_request = -1;  // whose rows all lie in the table
+    bool held_without = false;
     units.each(arrays, p, [&](int index, int unit, int64_t number, int split, int splits) {
         const Request request(arrays, p, index);
         const char* first_row = q.at(request.begin, 0);
@@ -387,14 +411,18 @@ __global__ __launch_bounds__(kWeightBlock, 3) void attention_weights_many_kernel
                 const int heads = p.kv_heads - head_base < heads_at_once ? p.kv_heads - head_base : heads_at_once;
                 if (held_request != index) {
                     __syncthreads();
+                    bool out = false;
                     for (int i = threadIdx.x; i < heads * table_rows; i += kWeightBlock) {
                         const int local = i / table_rows, row = i - local * table_rows;
                         const bool real = row < some;
-                        const int at = real ? row_base + row : 0;
+                        const int at = real ? row_base + row : row_base;
                         table.at[i] = request.row_at(q, p, head_base + local, at) - first_row;
                         table.base[i] = real ? request.base_of(arrays, p, head_base + local, at) : INFINITY;
+                        out |= real && table.base[i] == INFINITY;
                     }
+                    without.note(out);
                     __syncthreads();
+                    held_without = without.any();
                     held_request = splits == 1 && some == request.rows && heads == p.kv_heads ? index : -1;
                 }
                 for (int local = wave; local < heads; local += kWeightWaves) {
@@ -431,7 +459,7 @@ __global__ __launch_bounds__(kWeightBlock, 3) void attention_weights_many_kernel
                         S::read(stage, a);
                         const int row0 = tile * kRowsAtOnce + 4 * quarter;
                         const F32x4 base = *reinterpret_cast<const F32x4*>(&table.base[local * table_rows + row0]);
-                        weigh<T>(sum, a, k, base, c, masked, arrays, request, p, row_base + row0, key0);
+                        weigh<T>(sum, a, k, base, c, masked || held_without, arrays, request, p, row_base + row0, key0);
                     }
                 }
             }

@@ -206,6 +206,34 @@ def test_not_finite_stays_with_what_meets_it(hip, dev):
     assert bool(after.flatten()[mine.cuda()].isnan().all()) and torch.equal(after.flatten()[~mine.cuda()], clean.flatten()[~mine.cuda()])
 
 
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("lengths,new,tree,stated", [
+    ([90, 80], [3, 1], False, None),                # few rows
+    ([90, 80], [3, 1], True, None),
+    ([300, 50], [40, 9], False, None),              # many
+    ([300, 50], [40, 9], True, None),
+    ([700, 90], [600, 3], False, None),             # rows that workgroups share
+    ([700] + [20] * 299, [40] + [1] * 299, False, 1 << 20),  # units dealt out, of both kinds
+])
+def test_rows_without_a_log_sum_may_hold_anything(hip, dev, bad, lengths, new, tree, stated):
+    """They give no weight, to the keys before the new ones either, the first row of a request among them."""
+    words = [2 ** min(i + 1, 64) - 1 for n in new for i in range(n)] if tree else None
+    q, keys, table, q_offsets, lse, old, _ = check_weights(hip, "bf16", lengths, new, 4, 2, 64, 16, tree=words, stated=stated)
+    out_of_it = sorted({0, 2, q_offsets[1] - 1} | ({37, 301, 302} & set(range(q_offsets[1]))))
+    lse[:, out_of_it] = -math.inf
+    lse[1, q_offsets[1] - 2] = -math.inf  # one head of a row
+    results = []
+    for value in (0.0, bad):
+        q[out_of_it] = value
+        q[q_offsets[1] - 2, 1] = value
+        after = torch.full_like(old, -5.0)
+        hip.attention_paged_weights("bf16", q, keys, ints(table), ints(q_offsets), ints(lengths), lse, after, weights_in=old, decay=0.9,
+                                    tree=None if words is None else ints([w - (1 << 64) if w >> 63 else w for w in words], torch.int64),
+                                    max_kv_length=stated)
+        results.append(after)
+    assert torch.equal(*results)
+
+
 def test_weights_from_the_framework_s_attention(hip, dev):
     """With the lse that attention_paged gave, a step's weights add up to the number of its rows and heads."""
     lengths, new = [300, 77, 1000], [1, 3, 20]
