@@ -818,8 +818,8 @@ LCPP_HIP_DECLARE_PAGED_MOVE(f16)
  *     h_t = exp(log_decay_t) h_{t-1} + x_t,   out_t = h_t rounded,
  *
  * from the sequence's initial state (null: 0) to its final one.  Rows and offsets as for attention over packed sequences;
- * x, log_decay, out and their gradients are [tokens][channels] of one type, bf16, f16 or f32, any number of channels, rows any
- * whole number of items apart.  States are [num_states][channels] f32: sequence b has row state_rows[b] (null: b; a row
+ * x, log_decay, out and their gradients are [tokens][channels] of one type, bf16, f16 or f32, rows any whole number of items
+ * apart, with fewer than 2^24 items from row to row, 2^31 tokens and 2^27 sequences.  States are [num_states][channels] f32: sequence b has row state_rows[b] (null: b; a row
  * outside [0, num_states): starts from 0 and is not kept).  final_states (or null) may be the same memory as `initial`, and then no two
  * sequences share a row.  A sequence of no tokens hands its initial state on; one of a single token is a step of serving.
  * log_decay is at most 0 in use (-infinity forgets a finite state); growth is right as long as products over 128 steps stay finite.

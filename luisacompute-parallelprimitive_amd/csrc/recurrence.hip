@@ -379,10 +379,10 @@ struct WalkRows {
 };
 
 template <typename T, int V, bool BACK>
-__global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape p, int blocks) {
+__global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape p, int first_sequence, int blocks) {
     using Item = typename T::Item;
     using Vec = Items<Item, V>;
-    const int sequence = static_cast<int>(blockIdx.x / blocks);
+    const int sequence = first_sequence + static_cast<int>(blockIdx.x / blocks);
     const int channel = (static_cast<int>(blockIdx.x % blocks) * kWave + static_cast<int>(threadIdx.x)) * V;
     const bool active = channel < p.channels;
     const Span span = span_of(in.offsets, sequence, p.tokens);
@@ -444,8 +444,8 @@ __global__ __launch_bounds__(kWave) void recurrence_walk_kernel(Inputs in, Shape
 constexpr int kClearBlock = 256;
 
 template <bool BACK, int WAVES>
-__global__ __launch_bounds__(kClearBlock) void recurrence_clear_kernel(Inputs in, Handed h, Shape p, int blocks) {
-    const int number = static_cast<int>(blockIdx.x / blocks);
+__global__ __launch_bounds__(kClearBlock) void recurrence_clear_kernel(Inputs in, Handed h, Shape p, int first_number, int blocks) {
+    const int number = first_number + static_cast<int>(blockIdx.x / blocks);
     const int channel = static_cast<int>(blockIdx.x % blocks) * kClearBlock + static_cast<int>(threadIdx.x);
     Chunk chunk;
     const bool there = chunk.find<WAVES>(in.offsets, p, number);
@@ -464,14 +464,15 @@ __global__ __launch_bounds__(kClearBlock) void recurrence_clear_kernel(Inputs in
 }
 
 template <typename T, int V, bool BACK, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave, 4) void recurrence_kernel(Inputs in, Handed h, Shape p, int numbers, int blocks, uint32_t patience) {
+__global__ __launch_bounds__(WAVES * kWave, 4) void recurrence_kernel(Inputs in, Handed h, Shape p, int numbers, int first_ordinal, int blocks,
+                                                                  uint32_t patience) {
     using Item = typename T::Item;
     using Vec = Items<Item, V>;
     constexpr int kChunk = WAVES * kRows, kTile = kWave * V;
     __shared__ __attribute__((aligned(16))) Effect parts[WAVES][kTile];
     __shared__ __attribute__((aligned(16))) float entering[kTile];
     // Chunks in the order that states go through them, all channels of one together.
-    const int ordinal = static_cast<int>(blockIdx.x / blocks), number = BACK ? numbers - 1 - ordinal : ordinal;
+    const int ordinal = first_ordinal + static_cast<int>(blockIdx.x / blocks), number = BACK ? numbers - 1 - ordinal : ordinal;
     Chunk chunk;
     if (!chunk.find<WAVES>(in.offsets, p, number)) return;
     const int lane = threadIdx.x % kWave, wave = WAVES == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -640,8 +641,7 @@ int unusable(const char* what) {
 int check_sizes(const char* what, uint32_t sequences, uint64_t tokens, uint32_t channels) {
     if (channels == 0 || channels >= kMostStride) return set_error(kInvalidArgument, "%s: no channels, or too many", what);
     if (tokens > 0x7FFFFFFFull) return set_error(kInvalidArgument, "%s: too many tokens", what);
-    if (sequences > 0x7FFFFFFu || numbers_of(sequences, tokens) * ceil_div(channels, kWave) > 0x7FFFFFFFull / (kLongWaves * kWave))
-        return set_error(kInvalidArgument, "%s: too many sequences, tokens and channels", what);
+    if (sequences > 0x7FFFFFFu) return set_error(kInvalidArgument, "%s: too many sequences", what);
     return kOk;
 }
 
@@ -679,25 +679,40 @@ bool apart(const Inputs& in, const Shape& p, int64_t row_bytes) {
     return !BACK || !share(in.dx, in.dlog_decay, p.tokens, row_bytes);
 }
 
+// A launch holds fewer than 2^31 threads: units of `blocks` workgroups in as many launches as that takes, in their order (what a chunk
+// waits for is in its own launch or an earlier one).
+template <typename F>
+void in_launches(uint64_t units, uint64_t blocks, uint64_t threads, F launch) {
+    const uint64_t most = 0x7FFFFFFFull / (blocks * threads);
+    for (uint64_t first = 0; first < units; first += most) {
+        const uint64_t count = units - first < most ? units - first : most;
+        launch(static_cast<int>(first), static_cast<unsigned>(count * blocks));
+    }
+}
+
 template <typename T, int V, bool BACK, int WAVES>
 int run(const char* what, const Inputs& in, const Handed& h, const Shape& p, bool hands, hipStream_t stream) {
     const int numbers = static_cast<int>(numbers_of(p.sequences, p.tokens));
+    const int blocks = static_cast<int>(ceil_div(p.channels, kWave * V));
     if (walked(p.sequences, p.tokens)) {
         LaunchScope scope(what, stream);
-        const int blocks = static_cast<int>(ceil_div(p.channels, kWave * V));
-        recurrence_walk_kernel<T, V, BACK><<<static_cast<unsigned>(p.sequences * blocks), kWave, 0, stream>>>(in, p, blocks);
+        in_launches(p.sequences, blocks, kWave, [&](int first, unsigned grid) {
+            recurrence_walk_kernel<T, V, BACK><<<grid, kWave, 0, stream>>>(in, p, first, blocks);
+        });
         return check_hip(hipGetLastError(), what);
     }
     if (hands) {
         LaunchScope scope(BACK ? "recurrence_backward_clear" : "recurrence_clear", stream);
-        const int blocks = static_cast<int>(ceil_div(p.channels, kClearBlock));
-        recurrence_clear_kernel<BACK, WAVES><<<static_cast<unsigned>(numbers * blocks), kClearBlock, 0, stream>>>(in, h, p, blocks);
+        const int parts = static_cast<int>(ceil_div(p.channels, kClearBlock));
+        in_launches(numbers, parts, kClearBlock, [&](int first, unsigned grid) {
+            recurrence_clear_kernel<BACK, WAVES><<<grid, kClearBlock, 0, stream>>>(in, h, p, first, parts);
+        });
         if (int st = check_hip(hipGetLastError(), what); st != kOk) return st;
     }
     LaunchScope scope(what, stream);
-    const int blocks = static_cast<int>(ceil_div(p.channels, kWave * V));
-    recurrence_kernel<T, V, BACK, WAVES><<<static_cast<unsigned>(numbers * blocks), WAVES * kWave, 0, stream>>>(in, h, p, numbers, blocks,
-                                                                                                                lookback_spin_limit());
+    in_launches(numbers, blocks, WAVES * kWave, [&](int first, unsigned grid) {
+        recurrence_kernel<T, V, BACK, WAVES><<<grid, WAVES * kWave, 0, stream>>>(in, h, p, numbers, first, blocks, lookback_spin_limit());
+    });
     return check_hip(hipGetLastError(), what);
 }
 

@@ -360,3 +360,67 @@ def test_infinite_states_without_waiting(hip, dev):
         test_infinite_states_are_the_formula_s(hip, dev, "bf16", [2100])
     finally:
         hip.check(hip.lib().lcpp_hip_set_lookback_spin_limit(before))
+
+
+# ---- large batches -------------------------------------------------------------------------------
+def check_large(hip, lengths, sequences, channels, suffix="f32"):
+    """Both directions of `sequences` of the lengths, which repeat, against 64 bits on the GPU, with the bounds of the oracle."""
+    period, tokens = sum(lengths), sum(lengths) * (sequences // len(lengths))
+    log(f"{suffix} {sequences} sequences {tokens} tokens {channels} channels")
+    repeats, dtype, u, tiny = sequences // len(lengths), DTYPE[suffix], oracle.ROUNDOFF[DTYPE[suffix]], oracle.TINY[DTYPE[suffix]]
+    g = torch.Generator(device="cuda").manual_seed(5)
+    rows = lambda: torch.randn(tokens, channels, generator=g, device="cuda").to(dtype)
+    states = lambda: torch.randn(sequences, channels, generator=g, device="cuda")
+    x, dout, l = rows(), rows(), rows().abs_().mul_(-0.3)
+    initial, dfinal = states(), states()
+    count = torch.tensor([0] + lengths, device="cuda").cumsum(0)
+    offsets = (torch.arange(repeats, device="cuda")[:, None] * period + count[:-1]).flatten()
+    offsets = torch.cat([offsets, offsets.new_tensor([tokens])]).to(torch.int32)
+    got = {name: torch.full_like(x, 7.0) for name in ("out", "dx", "dlog_decay")} | {n: torch.full_like(initial, 7.0) for n in ("final", "dinitial")}
+    hip.recurrence(suffix, x, l, offsets, got["out"], initial=initial, final=got["final"])
+    hip.recurrence_backward(suffix, l, got["out"], dout, offsets, got["dx"], got["dlog_decay"], initial=initial, dfinal=dfinal,
+                            dinitial=got["dinitial"])
+    torch.cuda.synchronize()
+
+    def within(name, mine, value, bound):
+        over = ((mine.double() - value).abs() - bound).nan_to_num(nan=math.inf).amax()
+        assert float(over) <= 0, (name, float(over))
+
+    token = lambda t, i: t.view(repeats, period, channels)[:, i].double()
+    at = 0
+    for b, n in enumerate(lengths):
+        state = lambda t: t.view(repeats, len(lengths), channels)[:, b].double()
+        h, size, e = state(initial), state(initial).abs(), torch.zeros(repeats, channels, dtype=torch.float64, device="cuda")
+        before = []
+        for i in range(at, at + n):
+            before.append((h, e + u * h.abs() if i > at else e))
+            li, xi = token(l, i), token(x, i)
+            a = li.exp()
+            e = a * e + oracle._step_error(li, a, size, xi)
+            h, size = a * h + xi, a * size + xi.abs()
+            within("out", token(got["out"], i), h, e + u * h.abs() + tiny)
+        within("final", state(got["final"]), h, e + tiny)
+        c, size, e = state(dfinal), state(dfinal).abs(), torch.zeros_like(e)
+        for i in range(at + n - 1, at - 1, -1):
+            li, d = token(l, i), token(dout, i)
+            a = li.exp()
+            gr, g_size, g_off = d + c, d.abs() + size, e + 2.0 ** -22 * (d.abs() + size)
+            c, size, e = a * gr, a * g_size, a * g_off + oracle._step_error(li, a, g_size, torch.zeros_like(gr))
+            h, h_off = before[i - at]
+            within("dx", token(got["dx"], i), gr, g_off + u * gr.abs() + tiny)
+            within("dlog_decay", token(got["dlog_decay"], i), c * h, u * (c * h).abs() * (1 + u) + (c.abs() + e) * (h_off + tiny) + e * h.abs() + tiny)
+        within("dinitial", state(got["dinitial"]), c, e + tiny)
+        at += n
+
+
+# More workgroups of 64 channels than 2^31 threads of eight waves each are; those of one channel, more than one launch holds.
+@pytest.mark.parametrize("name,lengths,sequences,channels,suffix", [
+    ("walked, 4,096 channels", [1], 70_000, 4096, "bf16"),
+    ("walked", [1], 34_000_000, 1, "bf16"),
+    ("chunks of a wave, 4,096 channels", [1, 1, 1, 1, 1, 17, 2, 1], 60_000, 4096, "bf16"),
+    ("chunks of a wave", [2] * 63 + [40], 64 * 453_200, 1, "f32"),
+    ("chunks of eight waves", [130, 2, 66], 3 * 1_350_000, 1, "f32"),
+])
+def test_large_batches(hip, dev, name, lengths, sequences, channels, suffix):
+    check_large(hip, lengths, sequences, channels, suffix)
+    torch.cuda.empty_cache()
