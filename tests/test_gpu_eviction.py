@@ -234,6 +234,14 @@ def test_rows_without_a_log_sum_may_hold_anything(hip, dev, bad, lengths, new, t
     assert torch.equal(*results)
 
 
+@pytest.mark.parametrize("kv_heads", [31, 32, 33, 40, 63, 64, 65, 70, 130])
+def test_many_key_heads(hip, dev, kv_heads):
+    """More than have their log-sums (32) or the places of their rows (64) at hand at once; with as many rows as fit beside them, and more."""
+    check_weights(hip, "bf16", [40, 3, 17], [1, 1, 1], kv_heads, kv_heads, 16, 8)
+    check_weights(hip, "f16", [40, 30], [20, 9], kv_heads, kv_heads, 16, 8)
+    check_weights(hip, "bf16", [70, 9], [50, 1], kv_heads, kv_heads, 8, 16)
+
+
 def test_weights_from_the_framework_s_attention(hip, dev):
     """With the lse that attention_paged gave, a step's weights add up to the number of its rows and heads."""
     lengths, new = [300, 77, 1000], [1, 3, 20]
@@ -411,6 +419,28 @@ def test_move(hip, dev, suffix, kv_heads, dim, page, count):
     for w, got in zip(want, caches + [weights, positions]):
         assert torch.equal(got.cpu().reshape(w.shape), w)
     hip.paged_move(suffix, source[:0].cuda(), target[:0].cuda(), *caches)
+
+
+@pytest.mark.parametrize("suffix,kv_heads,dim,page,count", [("bf16", 8, 128, 16, 70_001), ("f16", 3, 80, 24, 280_007), ("bf16", 40, 128, 8, 14_003)])
+def test_many_moves(hip, dev, suffix, kv_heads, dim, page, count):
+    """Two moves a thread, and rows of less and of more than a workgroup's chunks."""
+    log(f"{suffix} {kv_heads} heads of {dim}, pages of {page}, {count} moves")
+    g = torch.Generator(device=dev).manual_seed(count)
+    pages = -(-2 * count // page) + 2
+    make = lambda: torch.randn(pages, page, kv_heads, dim, generator=g, device=dev).to(DTYPE[suffix])
+    caches = [make(), make()]
+    weights, positions = torch.randn(pages, page, generator=g, device=dev), torch.arange(pages * page, dtype=torch.int32, device=dev).view(pages, page)
+    slots = torch.randperm(2 * count, generator=g, device=dev)
+    source, target = slots[:count].clone(), slots[count:].clone()
+    source[::5], target[3::7] = -1, -1
+    source[11], target[12], source[-1], target[-3] = pages * page, 1 << 40, pages * page + 3, -7
+    real = (source >= 0) & (target >= 0) & (source < pages * page) & (target < pages * page)
+    want = [t.clone().flatten(0, 1) for t in caches + [weights, positions]]
+    for w in want:
+        w[target[real]] = w[source[real]].clone()
+    hip.paged_move(suffix, source, target, *caches, weights=weights, positions=positions)
+    for w, got in zip(want, caches + [weights, positions]):
+        assert torch.equal(got.flatten(0, 1), w)
 
 
 def test_graph(hip, dev):

@@ -186,6 +186,12 @@ def test_paged_write(hip, dev, suffix, interleaved, rotary, page, tokens):
     assert all(bool((c[free] == 3.0).all()) for c in flat)
 
 
+@pytest.mark.parametrize("suffix,interleaved,rotary,page", [("bf16", False, 128, 16), ("f16", True, 64, 24), ("bf16", False, 36, 8)])
+def test_many_rows_into_pages(hip, dev, suffix, interleaved, rotary, page):
+    """Four units a thread."""
+    test_paged_write(hip, dev, suffix, interleaved, rotary, page, 20011)
+
+
 def test_the_write_is_rotary_and_paged_write(hip, dev):
     """Bit for bit, on a stream of its own, replayed from a graph with other inputs."""
     tokens, f = 70, hip.rotary_frequencies(64)
