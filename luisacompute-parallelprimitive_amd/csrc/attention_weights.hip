@@ -7,7 +7,11 @@
 //
 // Each key is read once, and that bounds a decoding step: 256 requests of 200 to 4,000 keys (8 key heads of 128, 32 query heads), 669 MB in
 // 124 us, 5.4 TB/s, where reads alone reach 6.7.  The last 32 rows of three prompts of 9,000 to 60,000 keys: 22 GFLOP and 175 MB in
-// 62 us, bound by the latency of a tile: two or three waves a SIMD fit the registers.
+// 60 us, bound by the latency of a tile: two or three waves a SIMD fit the registers.
+//
+// Key heads are what waves share out (many rows) or go through with the next one's keys on their way (few): with fewer than four key
+// heads waves of the first have nothing to do (windows of 32 rows of one key head: 122 us for 107 MB), and with one the second waits
+// for each tile of keys (256 requests of one key head, 684 MB: 270 us where eight heads of the same bytes take 136).
 //
 // 2 * dim operations a row, head and key.  Matrix instruction: 16x16x32, rows of queries by keys: lane
 // l has key l % 16 of the result, rows 4 (l / 16) .. + 3, so that a key's weights of 16 rows lie in four lanes' registers and are

@@ -605,7 +605,9 @@ __global__ __launch_bounds__(kMoveBlock) void paged_move_kernel(Pages key_cache,
 
 // ---- host side ---------------------------------------------------------------------------------------------------
 // Workgroups of a request: one up to kLongRequest keys, then one for every kPartKeys.  (16 requests of 8,192 keys: one 18 us, parts 42; of
-// 16,384: 36 and 42; of 32,768: 55 and 43; of 65,536, more than registers hold: 224 and 48.)
+// 16,384: 36 and 42; of 32,768: 55 and 43; of 65,536, more than registers hold: 224 and 48.)  The stated length decides, so one far
+// above what requests hold costs time: 256 requests of 1,040 keys 8.1 us stated as such, 17.8 as 16,384, 55 as 16,385, 106 as 32,768
+// and 220 as 131,072.
 constexpr uint64_t kLongRequest = 16384;
 uint64_t parts_of(uint64_t max_kv_length) { return max_kv_length <= kLongRequest ? 1 : ceil_div(max_kv_length, kPartKeys); }
 size_t bins_bytes(uint64_t requests) { return align_up(requests * kDigits * kBins * sizeof(uint32_t), kViewAlign); }

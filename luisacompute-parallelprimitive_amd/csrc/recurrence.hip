@@ -7,10 +7,11 @@
 // small l the step is h + (exp(l) - 1) h + x with exp(l) - 1 from its series, whose error is relative to l.
 //
 // Memory bounds the large calls: 3 items a channel and token forwards, 5 backwards, each once, and 3% of what chunks hand on.
-// 34,222 tokens of 4,096 channels in bf16: forwards 0.84 GB in 213 us, 3.9 TB/s, backwards 1.40 GB in 276, 5.1, where the library's copy
-// reaches 6.0.  A workgroup loads, waits for its state and stores, and two of them on a compute unit do not quite cover each
+// 34,222 tokens of 4,096 channels in bf16: forwards 0.84 GB in 219 us, 3.8 TB/s, backwards 1.40 GB in 286, 4.9, where the library's copy
+// reaches 6.0; in f32 twice the bytes in 304 and 482, 5.5 and 5.8.  A workgroup loads, waits for its state and stores, and two of them on a compute unit do not quite cover each
 // other's waits (forwards without looking back, which is wrong, 183 us).  (One pass over the rows by a thread a channel took 27.8 ms
-// for both.)  1,900 tokens of 770 channels: 12 to 14 us a direction, the latency of one chunk.
+// for both.)  1,900 tokens of 770 channels: 14 us a direction, the latency of one chunk.  A wave has one sequence's channels: of 16 channels
+// it uses 4 lanes, and 34,222 tokens take 45 us a direction for 3 MB, as those of 64 do.
 #include "common.hpp"
 #include "../../include/lcpp_hip.h"
 #include "attention.hpp"
@@ -97,8 +98,8 @@ __device__ __forceinline__ int64_t state_of(const int32_t* rows, int sequence, i
 
 // ---- chunks ------------------------------------------------------------------------------------------------------
 // A chunk of a sequence is waves of kRows tokens; a lane has V neighbouring channels of a token, 8 bytes of them where the
-// rows allow.  (The two directions of 34,222 tokens: eight waves of 16 rows 466 us, four waves 479, eight of 8 rows 515, sixteen of 8
-// rows 554.  Sequences of a few hundred rows alone would take 26 us for 31 with eight waves of 8.)  A chunk's effect on the state
+// rows allow.  (The two directions of 34,222 tokens, measured before infinite states were kept, which added 11 us: eight waves of 16 rows
+// 466 us, four waves 479, eight of 8 rows 515, sixteen of 8 rows 554.  Sequences of a few hundred rows alone would take 26 us for 31 with eight waves of 8.)  A chunk's effect on the state
 // is h -> exp(L) h + B.  A workgroup reads its chunk into registers once, makes each wave's
 // (L, B) and the chunk's, hands that on, gets the state that enters the chunk, and goes through its rows again with it.  The
 // backward pass does the same towards the sequence's start, with c in the place of h.
@@ -168,7 +169,7 @@ struct Inputs {
 // Rows [token, token + count) of an array as a wave reads and writes them: what lies past them, or is asked for at kNowhere, reads
 // as zeros and is not written.  (Offsets are below 2^31, as strides are below 2^26 bytes.)
 constexpr uint32_t kNowhere = 0x7FFFFFFF;
-constexpr int kOnce = 2;  // (each row is read once and written once: they stay out of the caches, 466 us where 490 were taken)
+constexpr int kOnce = 2;  // (each row is read once and written once: they stay out of the caches, 466 us where 490 were taken then)
 
 template <typename Vec>
 struct Window {
@@ -345,7 +346,7 @@ __device__ __forceinline__ float look_back(const Inputs& in, const Handed& h, co
 }
 
 // Short sequences: a lane walks its channels through a sequence, kWalkRows tokens at a time, the next ones on their way while it
-// works on some.  256 states of 4,096 channels and a token each: 14.7 MB in 6 to 7 us, of which an empty launch takes 2 to 3.
+// works on some.  256 states of 4,096 channels and a token each: 14.7 MB in 6 to 8 us, of which an empty launch takes 2 to 3.
 constexpr int kWalkRows = 8;
 
 template <typename T, int V, bool BACK>

@@ -1030,7 +1030,8 @@ def evict_plan(weights, positions, block_table, kv_lengths, kept_lengths, move_f
     """The moves, slots move_from[r] to move_to[r] (int64 [requests, width], -1 past the last), that cut each request from
     kv_lengths to kept_lengths keys: the `first` positions and the latest `recent` ones stay, then the largest of
     weights [pages, page size].  positions [pages, page size] int32, or None where first and recent are 0.  kv_lengths and
-    shifts are those before page_release: with its shifts_out in their place the latest keys would not be protected."""
+    shifts are those before page_release: with its shifts_out in their place the latest keys would not be protected.
+    `max_kv_length` defaults to what the block table can hold; a plan of shorter requests is faster with their longest length."""
     _, f32, i32, i64 = _row_types("bf16")
     requests = kv_lengths.numel()
     pages, page_size = _axes("weights", weights, 2)
